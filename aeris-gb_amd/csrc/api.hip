@@ -43,6 +43,7 @@ int ensure_init(void* stream = nullptr, bool from_launch = false) {
     if (g_init_status == hipSuccess) g_init_status = aeris::attention_stream_configure_all();
     if (g_init_status == hipSuccess) g_init_status = aeris::input_stage_configure();
     if (g_init_status == hipSuccess) g_init_status = aeris::qkv_attention_configure();
+    if (g_init_status == hipSuccess) g_init_status = aeris::cross_attention_configure();
     g_init_done.store(true, std::memory_order_release);
   });
   if (g_init_status == hipSuccess && !from_launch) {
@@ -377,6 +378,91 @@ int aeris_gemm_heads_fwd(const void* A, const void* W, void* C, const void* bias
                                     plane_stride, q_planes > 0 ? q_scale : 1.0f, q_planes * head_dim,
                                     reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "aeris_gemm_heads_fwd launch");
+  return AERIS_OK;
+}
+
+int aeris_qk_norm_rope_fwd(const aeris_qk_part* parts, int n_parts, int64_t tokens, int head_dim, int x_dtype, int y_dtype, int gain_dtype,
+                           int normed, float eps, const float* rotation, int64_t P, int R, int interleaved, const int32_t* positions,
+                           int64_t n_positions, void* stream) {
+  const char* who = "aeris_qk_norm_rope_fwd";
+  if (!parts || n_parts < 1 || n_parts > 2) return fail(AERIS_EINVAL, "%s: one or two parts (got %d)", who, n_parts);
+  for (int dt : {x_dtype, y_dtype, gain_dtype})
+    if (dt != AERIS_BF16 && dt != AERIS_F32) return fail(AERIS_EINVAL, "%s: dtype must be AERIS_BF16 or AERIS_F32", who);
+  if (tokens <= 0) return fail(AERIS_EINVAL, "%s: tokens must be positive", who);
+  if (!(eps >= 0.f)) return fail(AERIS_EINVAL, "%s: eps must be non-negative", who);
+  if (!aeris::qk_norm_rope_supported(head_dim, R))
+    return fail(AERIS_EUNSUPPORTED, "%s: head_dim %d, %d rotated elements (need head_dim 32, 64 or 128, and a multiple of 16 up to it)", who, head_dim, R);
+  if (R > 0 && (!rotation || !aligned16(rotation) || P <= 0 || P > 0x7fffffffLL))
+    return fail(AERIS_EINVAL, "%s: the rotation table must be 16-byte aligned and have 1 .. 2^31-1 rows", who);
+  if (R > 0 && positions && (n_positions <= 0 || n_positions > 0x7fffffffLL || (reinterpret_cast<uintptr_t>(positions) & 3u)))
+    return fail(AERIS_EINVAL, "%s: positions must be 4-byte aligned, 1 .. 2^31-1 of them", who);
+  // (token numbers are formed in 32 bits, up to a block of them beyond the last; the grid's second dimension counts heads)
+  if (tokens > 0x7fffffffLL - 64) return fail(AERIS_EUNSUPPORTED, "%s: more than 2^31-65 tokens", who);
+  int64_t heads = 0;
+  for (int i = 0; i < n_parts; ++i) {
+    const aeris_qk_part& p = parts[i];
+    if (!p.x || !p.y || p.heads <= 0) return fail(AERIS_EINVAL, "%s: x/y is NULL or heads is not positive", who);
+    const int ex = x_dtype == AERIS_F32 ? 4 : 8, ey = y_dtype == AERIS_F32 ? 4 : 8, eg = gain_dtype == AERIS_F32 ? 4 : 8;
+    if (!aligned16(p.x) || !aligned16(p.y) || (p.gain && !aligned16(p.gain)) || p.x_token_stride % ex || p.x_head_stride % ex ||
+        p.y_token_stride % ey || p.y_head_stride % ey || p.gain_head_stride % eg)
+      return fail(AERIS_EINVAL, "%s: x, y and gain must be 16-byte aligned, their strides multiples of 16 bytes", who);
+    if (p.heads > 32767) return fail(AERIS_EUNSUPPORTED, "%s: more than 32767 heads", who);
+    heads += p.heads;
+  }
+  if (heads > 65535) return fail(AERIS_EUNSUPPORTED, "%s: more than 65535 heads", who);
+  hipError_t e = aeris::qk_norm_rope_launch(parts, n_parts, (int)tokens, head_dim, x_dtype, y_dtype, gain_dtype, normed ? 1 : 0, eps, rotation,
+                                            (int)P, R, interleaved ? 1 : 0, R > 0 ? positions : nullptr, (int)n_positions,
+                                            reinterpret_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "aeris_qk_norm_rope_fwd launch");
+  return AERIS_OK;
+}
+
+namespace {
+// sizes of a cross attention call, for the workspace's size and the call
+int check_cross_sizes(const char* who, const aeris_cross_attention* a) {
+  if (!a) return fail(AERIS_EINVAL, "%s: NULL", who);
+  if (a->B <= 0 || a->Nq <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->Nk < 0 || a->Np < 0)
+    return fail(AERIS_EINVAL, "%s: B, Nq, heads, kv_heads must be positive, Nk and Np not negative", who);
+  if (a->heads % a->kv_heads) return fail(AERIS_EINVAL, "%s: %lld heads do not divide among %lld key heads", who, (long long)a->heads, (long long)a->kv_heads);
+  if (!aeris::cross_attention_supported((int)a->head_dim) || a->head_dim > 128)
+    return fail(AERIS_EUNSUPPORTED, "%s: head_dim %lld (need 32, 64 or 128)", who, (long long)a->head_dim);
+  const int64_t most = 0x7fffffffLL;
+  if (a->B > most || a->Nq > most || a->heads > 65535 || a->Nk > most - 4096 || a->Np > most - 4096 || a->B * a->Nq > most ||
+      a->B * a->Nq * a->heads > most / 2)
+    return fail(AERIS_EUNSUPPORTED, "%s: more than 2^30 rows (B * Nq * heads), 2^31-4097 keys or 65535 heads", who);
+  return AERIS_OK;
+}
+}  // namespace
+
+int64_t aeris_cross_attention_workspace_bytes(const aeris_cross_attention* a) {
+  if (check_cross_sizes("aeris_cross_attention_workspace_bytes", a)) return 0;
+  return aeris::cross_attention_workspace_bytes(*a);
+}
+
+int aeris_cross_attention_fwd(const aeris_cross_attention* a, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* who = "aeris_cross_attention_fwd";
+  if (int rc = check_cross_sizes(who, a)) return rc;
+  if (!a->q || !a->out || (a->Nk > 0 && (!a->k || !a->v)) || (a->Np > 0 && (!a->prefix_k || !a->prefix_v)))
+    return fail(AERIS_EINVAL, "%s: q, k, v, prefix or out is NULL", who);
+  const int64_t strides[] = {a->q_batch_stride, a->q_row_stride, a->q_head_stride, a->k_batch_stride, a->k_row_stride, a->k_head_stride,
+                             a->v_batch_stride, a->v_row_stride, a->v_head_stride, a->prefix_k_row_stride, a->prefix_k_head_stride,
+                             a->prefix_v_row_stride, a->prefix_v_head_stride};
+  for (int64_t s : strides)
+    if (s < 0 || s % 8) return fail(AERIS_EINVAL, "%s: strides must be multiples of 8 elements and not negative", who);
+  if (!aligned16(a->q) || !aligned16(a->out) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->prefix_k) || !aligned16(a->prefix_v))
+    return fail(AERIS_EINVAL, "%s: q, k, v, prefix and out must be 16-byte aligned", who);
+  for (int64_t s : {a->k_row_stride, a->v_row_stride, a->prefix_k_row_stride, a->prefix_v_row_stride})
+    if (s >= (1 << 23)) return fail(AERIS_EUNSUPPORTED, "%s: rows of k and v 2^23 elements apart or more", who);
+  if (a->lengths && ((a->lengths_stride != 0 && a->lengths_stride != 1) || (reinterpret_cast<uintptr_t>(a->lengths) & 3u)))
+    return fail(AERIS_EINVAL, "%s: lengths must be 4-byte aligned, its stride 0 or 1", who);
+  if (a->key_mask && a->mask_batch_stride < 0) return fail(AERIS_EINVAL, "%s: mask_batch_stride must not be negative", who);
+  if (!a->q_prescaled && !(a->scale > 0.0 && a->scale < 1e30)) return fail(AERIS_EINVAL, "%s: scale must be positive", who);
+  const int64_t need = aeris::cross_attention_workspace_bytes(*a);
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
+    return fail(AERIS_EINVAL, "%s: workspace must be 16-byte aligned and hold %lld bytes (got %lld)", who, (long long)need, (long long)workspace_bytes);
+  if (int rc = ensure_init(stream, true)) return rc;
+  hipError_t e = aeris::cross_attention_launch(*a, workspace, reinterpret_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "aeris_cross_attention_fwd launch");
   return AERIS_OK;
 }
 

@@ -110,6 +110,7 @@ __device__ __forceinline__ u32x2 lds_read_tr16_b64(uint32_t lds_address) {
   return r;
 }
 struct TrFrag { u32x2 lo, hi; };  // two transposing reads = the 8 k slots of one MFMA operand
+__device__ __forceinline__ void lds_tr_wait(TrFrag& a) { asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a.lo), "+v"(a.hi)); }
 __device__ __forceinline__ void lds_tr_wait(TrFrag& a, TrFrag& b) {
   asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a.lo), "+v"(a.hi), "+v"(b.lo), "+v"(b.hi));
 }

@@ -64,6 +64,18 @@ hipError_t output_stage_launch(const void* x, int x_dtype, const void* gamma, co
                                float* out, int64_t B, int64_t rows_per_batch, int N, int d, int kind, float eps,
                                void* workspace, hipStream_t stream);
 
+// norm and rotation of query and key heads (qk_norm_rope.hip)
+bool qk_norm_rope_supported(int head_dim, int rotated);
+hipError_t qk_norm_rope_launch(const aeris_qk_part* parts, int n_parts, int T, int head_dim, int x_dtype, int y_dtype, int gain_dtype, int normed,
+                               float eps, const float* rotation, int P, int R, int interleaved, const int32_t* positions, int n_pos,
+                               hipStream_t stream);
+
+// attention to an encoder's states (cross_attention.hip)
+bool cross_attention_supported(int head_dim);
+hipError_t cross_attention_configure();
+int64_t cross_attention_workspace_bytes(const aeris_cross_attention& a);
+hipError_t cross_attention_launch(const aeris_cross_attention& a, void* workspace, hipStream_t stream);
+
 hipError_t modulation_linear_launch(const aeris_modulation_layer* layers, int n, int B, int K, int w_dtype, int act, hipStream_t stream);
 hipError_t heun_update_launch(const float* x, const float* f0, const float* f1, const float* t, float sigma_data, float* out, int64_t n,
                               hipStream_t stream);
