@@ -8,6 +8,8 @@ from ._lib import AerisError, LIB_PATH  # noqa: F401
 from .model import (  # noqa: F401
     Attention,
     BlockOptions,
+    ContextKV,
+    CrossAttention,
     FeedForward,
     InputStage,
     LocalAERIS,

@@ -44,6 +44,10 @@ class BlockOptions:
     rel_pos_bias: bool = False
     shift_mask: bool = False
     eps: Optional[float] = None
+    qk_norm: bool = False  # RMS norm of every query and key head
+    rope: bool = False  # queries and keys rotated by their place in the window (RoPE2D)
+    context_dim: int = 0  # channels of an encoder's states that the tokens attend to (CrossAttention); 0: none
+    context_kv_heads: int = 0  # its key heads; 0: as many as heads
 
     @staticmethod
     def make(preset: str = "ref", **overrides) -> "BlockOptions":
@@ -156,8 +160,10 @@ class PositionalEncoding2D(nn.Module):
 
 
 class RoPE2D(nn.Module):
-    """Accepted for constructor parity only: the reference builds it but never applies it
-    (the call is commented out at model.py:304) and its buffers are not part of the state_dict."""
+    """Axial rotation of queries and keys by their row and column in the window: ``rope_dim`` elements turn with each, neighbouring
+    elements by the angle place * rope_base^(-2j / rope_dim).  The reference builds it but never applies it (model.py:198-260, the
+    call is commented out at model.py:304) and its buffers are not part of the state_dict; here ``Attention(rope=True)`` applies it, in
+    the pass that norms the heads (ops.qk_norm_rope)."""
 
     def __init__(self, window_size=None, rope_dim=None, rope_base=10_000):
         super().__init__()
@@ -165,6 +171,41 @@ class RoPE2D(nn.Module):
 
     def forward(self, x):
         raise NotImplementedError("RoPE2D is not on the executed path of the reference")
+
+    def table(self, device):
+        """cos | sin for every place of a window, f32 [ws_y * ws_x, 2 * rope_dim], from angles in 64 bits."""
+        wy, wx = self.window_size
+
+        def make():
+            freq = float(self.rope_base) ** (-torch.arange(0, self.rope_dim, 2, dtype=torch.float64, device=device) / self.rope_dim)
+            y = torch.arange(wy, dtype=torch.float64, device=device)[:, None, None] * freq
+            x = torch.arange(wx, dtype=torch.float64, device=device)[None, :, None] * freq
+            angle = torch.cat([y.expand(wy, wx, -1), x.expand(wy, wx, -1)], dim=-1).flatten(0, 1)
+            return torch.cat([angle.cos(), angle.sin()], dim=1).float()
+        return _made_once(("table", wy, wx, self.rope_dim, self.rope_base, device), make)
+
+    def positions(self, image_shape, shift, device):
+        """The place in its window, int32 [H * W], of every token of the grid whose windows are cut ``shift`` further on."""
+        (H, W), (wy, wx) = image_shape, self.window_size
+
+        def make():
+            y = (torch.arange(H, device=device) - shift[0]) % H % wy
+            x = (torch.arange(W, device=device) - shift[1]) % W % wx
+            return (y[:, None] * wx + x[None]).flatten().int()
+        return _made_once(("positions", H, W, wy, wx, *shift, device), make)
+
+
+_MADE = {}  # tables that follow from geometry alone, shared by the blocks of every model
+
+
+def _made_once(key, make):
+    """A table made at its first use and kept.  One that is first asked for while a stream is being captured is made by the graph, at
+    every replay, and not kept: it has no values yet."""
+    if key not in _MADE:
+        if key[-1].type == "cuda" and torch._C._cuda_isCurrentStreamCapturing():
+            return make()
+        _MADE[key] = make()
+    return _MADE[key]
 
 
 # Whether ``Attention`` runs the to_qkv projection inside the attention kernel where that kernel exists (16x16 windows,
@@ -180,7 +221,7 @@ class Attention(nn.Module):
     (model.py:265-309).  ``forward(x, shift=(sy, sx))`` folds a cyclic shift into the kernel."""
 
     def __init__(self, dim, heads, head_dim, window_size, image_shape, device_mesh=None, wp_dims=(1, 1), *,
-                 bias=False, rel_pos_bias=False, shift_mask=False, **rope_kwargs):
+                 bias=False, rel_pos_bias=False, shift_mask=False, qk_norm=False, rope=False, **rope_kwargs):
         super().__init__()
         if tuple(wp_dims) != (1, 1):
             raise NotImplementedError("window parallelism across devices is not part of this build")
@@ -191,7 +232,11 @@ class Attention(nn.Module):
         self.fuse_qkv = FUSE_QKV_ATTENTION  # per module; see FUSE_QKV_ATTENTION
         self._b4cache = None
         inner = heads * head_dim
-        self.rope = RoPE2D(**{k: v for k, v in rope_kwargs.items() if k in ("window_size", "rope_dim", "rope_base")})
+        self.rope = RoPE2D(self.window_size, **{"rope_dim": head_dim // 2, **{k: v for k, v in rope_kwargs.items() if k in ("rope_dim", "rope_base")}})
+        self.rotates = bool(rope)
+        self.qk_norm = bool(qk_norm)
+        if self.qk_norm:
+            self.q_norm, self.k_norm = nn.RMSNorm(head_dim), nn.RMSNorm(head_dim)
         self.to_qkv = nn.Linear(dim, inner * 3, bias=bias)
         self.wo = nn.Linear(inner, dim, bias=bias)
         if rel_pos_bias:
@@ -215,6 +260,8 @@ class Attention(nn.Module):
         """y bf16 [b, n, d] -> attention output before ``wo`` (bf16 [b*n, inner])."""
         b, n, _ = y.shape
         use_mask = self.shift_mask and (shift[0] > 0 or shift[1] > 0)
+        if self.qk_norm or self.rotates:
+            return self._normed_core(y, shift, use_mask, out)
         if self.fuse_qkv and ops.qkv_attention_supported(y.shape[-1], self.heads, self.head_dim, self.window_size,
                                                          self.image_shape):
             # projection and attention in one kernel: q, k, v stay on the chip (same arithmetic, bit-identical result)
@@ -232,10 +279,95 @@ class Attention(nn.Module):
                                     self.window_size, shift, self.relative_position_bias_table, use_mask, self.scale, out=out,
                                     head_planes=True, q_prescaled=True)
 
+    def prepare(self, device, shift):
+        """Make the tables that ``core`` reads, ahead of a capture."""
+        if self.rotates:
+            self.rope.table(device)
+            self.rope.positions(self.image_shape, shift, device)
+
+    def _normed_core(self, y, shift, use_mask, out):
+        """``core`` with the heads normed and rotated: one pass over the q and k planes between projection and attention, in place."""
+        b, n, _ = y.shape
+        qkv = ops.gemm_heads(y, self.to_qkv.weight, self.to_qkv.bias, self.head_dim,
+                             out=ops.workspace("qkv", (3 * self.heads, b * n, self.head_dim), torch.bfloat16, y.device))
+        q, k = (qkv[i * self.heads:(i + 1) * self.heads].permute(1, 0, 2) for i in range(2))
+        q_gain, k_gain = (self.q_norm.weight, self.k_norm.weight) if self.qk_norm else (None, None)
+        rotation = positions = None
+        if self.rotates:
+            rotation, positions = self.rope.table(y.device), self.rope.positions(self.image_shape, shift, y.device)
+        ops.qk_norm_rope(q, k, q_gain, k_gain, rotation=rotation, positions=positions, interleaved=True, normed=self.qk_norm, eps=_FP32_EPS,
+                         q_scale=self.scale * ops.LOG2E, q_out=q, k_out=k)
+        return ops.window_attention(qkv, b, self.image_shape, self.heads, self.head_dim, self.window_size, shift,
+                                    self.relative_position_bias_table, use_mask, self.scale, out=out, head_planes=True, q_prescaled=True)
+
     def forward(self, x, shift=(0, 0)):
         b, n, d = x.shape
         o = self.core(x, shift)
         return ops.gemm(o, self.wo.weight, self.wo.bias).view(b, n, d)
+
+
+class ContextKV(NamedTuple):
+    """What one block's cross attention reads of a context: its keys and values, made once for all denoiser calls of a draw (they
+    do not depend on the noise level)."""
+    k: torch.Tensor  # [b | 1, n, key heads, head_dim]
+    v: torch.Tensor
+    lengths: Optional[torch.Tensor] = None  # int32 [b | 1]: states that each member has
+    key_mask: Optional[torch.Tensor] = None  # bool [b | 1, n]: which of them take part
+    prefix: Optional[Tuple[torch.Tensor, torch.Tensor]] = None  # keys and values of states that all members share
+
+
+class CrossAttention(nn.Module):
+    """Tokens attend to an encoder's states of another length (observations, another model's tokens); no reference counterpart.
+    to_q and to_kv GEMMs -> norm of the heads -> ops.cross_attention -> wo GEMM; ``kv_heads`` divides ``heads``."""
+
+    def __init__(self, dim, heads, head_dim, context_dim, *, kv_heads=None, bias=False, qk_norm=True):
+        super().__init__()
+        self.heads, self.head_dim, self.kv_heads = heads, head_dim, kv_heads or heads
+        if heads % self.kv_heads:
+            raise ValueError(f"{heads} heads do not divide among {self.kv_heads} key heads")
+        self.scale = head_dim ** -0.5
+        self.qk_norm = bool(qk_norm)
+        self.to_q = nn.Linear(dim, heads * head_dim, bias=bias)
+        self.to_kv = nn.Linear(context_dim, 2 * self.kv_heads * head_dim, bias=bias)
+        self.wo = nn.Linear(heads * head_dim, dim, bias=bias)
+        if self.qk_norm:
+            self.q_norm, self.k_norm = nn.RMSNorm(head_dim), nn.RMSNorm(head_dim)
+
+    def keys_values(self, states):
+        """states bf16 [b, n, context_dim] -> k, v [b, n, key heads, head_dim]."""
+        b, n, c = states.shape
+        if b * n == 0:
+            none = torch.empty(b, n, self.kv_heads, self.head_dim, dtype=torch.bfloat16, device=states.device)
+            return none, none
+        kv = ops.gemm(states.contiguous(), self.to_kv.weight, self.to_kv.bias).view(b * n, 2, self.kv_heads, self.head_dim)
+        if self.qk_norm:
+            ops.qk_norm_rope(kv[:, 0], None, self.k_norm.weight, eps=_FP32_EPS, q_out=kv[:, 0])
+        kv = kv.view(b, n, 2, self.kv_heads, self.head_dim)
+        return kv[:, :, 0], kv[:, :, 1]
+
+    def encode(self, states, lengths=None, key_mask=None, prefix=None) -> ContextKV:
+        """states bf16 [b | 1, n, context_dim], prefix bf16 [np, context_dim] (states that all members share): see ``ContextKV``."""
+        if prefix is not None:
+            prefix = tuple(t[0] for t in self.keys_values(prefix[None]))
+        return ContextKV(*self.keys_values(states), lengths, key_mask, prefix)
+
+    def core(self, y, context: ContextKV, out=None):
+        """y bf16 [b, n, d] -> attention output before ``wo`` (bf16 [b, n, heads, head_dim])."""
+        b, n, _ = y.shape
+        q_scale = self.scale * ops.LOG2E
+        planes = ops.gemm_heads(y, self.to_q.weight, self.to_q.bias, self.head_dim,
+                                out=ops.workspace("cross_q", (self.heads, b * n, self.head_dim), torch.bfloat16, y.device),
+                                q_scale=1.0 if self.qk_norm else q_scale, q_planes=0 if self.qk_norm else self.heads)
+        if self.qk_norm:
+            q = planes.permute(1, 0, 2)
+            ops.qk_norm_rope(q, None, self.q_norm.weight, eps=_FP32_EPS, q_scale=q_scale, q_out=q)
+        return ops.cross_attention(planes.view(self.heads, b, n, self.head_dim).permute(1, 2, 0, 3), context.k, context.v, lengths=context.lengths,
+                                   key_mask=context.key_mask, prefix=context.prefix, q_prescaled=True, out=out)
+
+    def forward(self, x, context: ContextKV):
+        b, n, d = x.shape
+        o = self.core(x, context)
+        return ops.gemm(o.view(b * n, -1), self.wo.weight, self.wo.bias).view(b, n, d)
 
 
 class ModulationLinear(nn.Module):
@@ -361,8 +493,11 @@ def _modulation_vectors(modules, dt, extra=()):
 
 
 def _own_block(block):
-    """Whether the native call does what the block's modules say: attention's ``core`` is a method that a caller may override."""
+    """Whether the native call does what the block's modules say: attention's ``core`` is a method that a caller may override, and one
+    that norms or rotates heads has a pass of its own between projection and attention."""
     attn = block._modules["1"]
+    if attn.__dict__.get("qk_norm") or attn.__dict__.get("rotates"):
+        return False
     return getattr(type(attn), "core", None) is _AS_DEFINED[Attention] and "core" not in attn.__dict__
 
 
@@ -370,6 +505,8 @@ def _own_blocks(layer):
     """Whether all of the layer's blocks can go in native calls, their modulation vectors computed ahead of the first: a caller
     may have replaced ``block_forward`` or a modulation module, or hooked one (which is then called when its block is due)."""
     if getattr(type(layer), "block_forward", None) is not _AS_DEFINED[SwinLayer] or "block_forward" in layer.__dict__:
+        return False
+    if layer.opts.context_dim:
         return False
     modulated = layer.opts.mod_ways
     for block in layer._modules["modulelist"]._modules.values():
@@ -385,6 +522,9 @@ class SwinLayer(nn.Module):
     With preset="ref" the layer, like the reference's, does not shift on its own (the reference
     shifts at model level, model.py:471-475); ``LocalAERIS`` passes ``shift=`` for odd layers.
     With preset="spec" ``shifted_grid=True`` shifts by half a window inside the attention kernel.
+
+    ``qk_norm`` / ``rope``: see ``Attention``.  ``context_dim``: behind its window attention every block attends to an encoder's states
+    (norm -> CrossAttention -> residual, modules in ``contextlist``); ``forward`` then takes ``context=layer.encode_context(states)``.
     """
 
     def __init__(self, device_mesh, dim, heads, head_dim, mlp_dim, window_size, image_shape, shifted_grid, rope_base,
@@ -402,7 +542,7 @@ class SwinLayer(nn.Module):
             mods = [
                 _norm_module(o, dim),
                 Attention(dim, heads, head_dim, image_shape=image_shape, device_mesh=device_mesh, wp_dims=wp_dims,
-                          bias=o.bias, rel_pos_bias=o.rel_pos_bias, shift_mask=o.shift_mask, **rope_kwargs),
+                          bias=o.bias, rel_pos_bias=o.rel_pos_bias, shift_mask=o.shift_mask, qk_norm=o.qk_norm, rope=o.rope, **rope_kwargs),
                 _norm_module(o, dim),
                 FeedForward(dim, mlp_dim) if o.mlp == "swiglu" else Mlp(dim, mlp_dim, bias=o.bias),
             ]
@@ -410,6 +550,16 @@ class SwinLayer(nn.Module):
                 mods.append(ModulationLinear(dim, 2 * o.mod_ways * dim, bias=True))
             blocks.append(nn.ModuleList(mods))
         self.modulelist = nn.ModuleList(blocks)
+        if o.context_dim:
+            self.contextlist = nn.ModuleList(
+                nn.ModuleList([_norm_module(o, dim), CrossAttention(dim, heads, head_dim, o.context_dim, kv_heads=o.context_kv_heads or None, bias=o.bias)])
+                for _ in range(sublayers))
+
+    def encode_context(self, states, lengths=None, key_mask=None, prefix=None):
+        """The keys and values of an encoder's states for each block (arguments: ``CrossAttention.encode``)."""
+        if not self.opts.context_dim:
+            raise ValueError("this layer does not attend to a context (context_dim)")
+        return [cross.encode(states, lengths, key_mask, prefix) for _, cross in self.contextlist]
 
     def default_shift(self):
         if self.own_shift and self.shifted_grid:
@@ -472,8 +622,9 @@ class SwinLayer(nn.Module):
         keep = (n1_w, n1_b, n2_w, n2_b, qkv_w, qkv_b, wo_w, wo_b, up_w, up_b, dn_w, dn_b)
         return BlockCall(rec, fused, config, (keep, table, m), not _STORED.issuperset(map(type, keep)))
 
-    def _block_by_ops(self, block, x, m, shift, out, tap):
-        """One block from the single operations, in the order of aeris_blocks_fwd."""
+    def _block_by_ops(self, block, x, m, shift, out, tap, cross=None):
+        """One block from the single operations, in the order of aeris_blocks_fwd; ``cross``: norm, CrossAttention and ContextKV of what
+        stands between attention and MLP."""
         o = self.opts
         n1, attn, n2, ff = list(block._modules.values())[:4]
         b, n, d = x.shape
@@ -495,6 +646,11 @@ class SwinLayer(nn.Module):
         if out is None:
             out = torch.empty_like(x)
         ops.gemm(a, attn.wo.weight, attn.wo.bias, gate=g1, residual=x, rows_per_batch=n, out=out)
+        if cross is not None:
+            n3, attn3, context = cross
+            a = attn3.core(norm(n3, out, None, None, y), context,
+                           out=ops.workspace("attn", (b, n, attn3.heads, attn3.head_dim), torch.bfloat16, x.device))
+            ops.gemm(a.view(b * n, -1), attn3.wo.weight, attn3.wo.bias, residual=out, out=out)
         z = norm(n2, out, s2, c2, y)
         swiglu = o.mlp == "swiglu"
         if swiglu:  # no biases, whatever its Linears hold (FeedForward)
@@ -508,16 +664,23 @@ class SwinLayer(nn.Module):
         ops.gemm(h, w_dn, bias_dn, gate=g2, residual=out, rows_per_batch=n, out=out)  # in place: out += gate * mlp
         return out
 
-    def block_forward(self, j, x, dt, shift, out=None, tap=None):
+    def block_forward(self, j, x, dt, shift, out=None, tap=None, context=None):
         """One block.  x is not modified; the result is written to ``out`` (allocated if None; may be x; bf16 or f32, whatever
         x is).
 
         ``tap(name, tensor, block)``, if given, is shown the two intermediates the block holds anyway before they are
         consumed: "attn" (attention output ahead of the wo projection) and "hidden" (activated MLP hidden ahead of the
-        down projection), both as views of shared scratch that the next kernel overwrites.
+        down projection), both as views of shared scratch that the next kernel overwrites.  ``context``: one entry per block, as
+        ``encode_context`` returns it.
         """
         block = self.modulelist[j]
         m = block[4](dt) if self.opts.mod_ways else None  # f32 [1|b, 2*ways*d]
+        if self.opts.context_dim:
+            if context is None:
+                raise ValueError("this layer attends to a context: context=layer.encode_context(states) is required")
+            return self._block_by_ops(block, x, m, shift, out, tap, (*self.contextlist[j], context[j]))
+        if context is not None:
+            raise ValueError("this layer does not attend to a context (context_dim)")
         if tap is not None or not _own_block(block) or (out is not None and out.dtype != x.dtype):
             return self._block_by_ops(block, x, m, shift, out, tap)
         call = self._block_call(block, x, m, shift)
@@ -526,16 +689,17 @@ class SwinLayer(nn.Module):
         _run_blocks([call], x, out)
         return out
 
-    def forward(self, x, dt=None, shift=None, tap=None):
+    def forward(self, x, dt=None, shift=None, tap=None, context=None):
         if self.opts.mod_ways and dt is None:
             raise ValueError("this layer is modulated: dt (noise-level embedding [1|b, d]) is required")
         shift = self.default_shift() if shift is None else shift
         if x.dtype not in (torch.bfloat16, torch.float32):
             raise TypeError("x must be bf16 or f32")
         x = x.contiguous()
-        if tap is not None or not _own_blocks(self):
+        with_context = {} if context is None else {"context": context}
+        if tap is not None or with_context or not _own_blocks(self):
             for j in range(self.sublayers):
-                x = self.block_forward(j, x, dt, shift, tap=tap)
+                x = self.block_forward(j, x, dt, shift, tap=tap, **with_context)
             return x
         if self.sublayers == 0:
             return x
@@ -701,8 +865,21 @@ class LocalAERIS(nn.Module):
         self.input_stage.ape_generated = pe.permute(0, 2, 3, 1).reshape(1, H * W, c).contiguous()
         return self.input_stage.ape_generated
 
-    def forward(self, x, dt, return_hidden=False, cond=None, x_div=1.0, block_hook=None):
+    def prepare(self, device):
+        """Make what the blocks' rotations read, ahead of a capture."""
+        half = (self.window_size[0] // 2, self.window_size[1] // 2)
+        for i, layer in enumerate(self.layers):
+            for block in getattr(layer, "modulelist", ()):
+                if isinstance(block[1], Attention):
+                    block[1].prepare(device, half if i % 2 == 1 else (0, 0))
+
+    def encode_context(self, states, lengths=None, key_mask=None, prefix=None):
+        """What ``forward(context=...)`` takes, for all its calls with the same states (arguments: ``CrossAttention.encode``)."""
+        return [layer.encode_context(states, lengths, key_mask, prefix) for layer in self.layers]
+
+    def forward(self, x, dt, return_hidden=False, cond=None, x_div=1.0, block_hook=None, context=None):
         """``cond`` / ``x_div``: see InputStage.forward (the sampler's concatenation folded into the embedding).
+        ``context``: keys and values of an encoder's states (``encode_context``), of a model built with ``context_dim``.
         ``block_hook(k, hidden)`` is called with the residual stream after the embedding (k = 0) and after every
         block (k = 1..); the tensor is reused by later blocks, so a hook that keeps it must copy it."""
         tok, t = self.input_stage(x, dt, out_dtype=self.residual_dtype, cond=cond, x_div=x_div)
@@ -711,7 +888,7 @@ class LocalAERIS(nn.Module):
         layers = list(self.layers)
         half = (self.window_size[0] // 2, self.window_size[1] // 2)
         shifts = [half if i % 2 == 1 else (0, 0) for i in range(len(layers))]  # model.py:471-475, folded into the attention kernel
-        if block_hook is None and all(map(_own_blocks, layers)):
+        if block_hook is None and context is None and all(map(_own_blocks, layers)):
             # every modulation MLP of the model depends on the noise level alone: two launches for all of them
             modules = [layer.modulations() for layer in layers]
             own_end = _plain(self.output_stage, OutputStage)
@@ -729,11 +906,12 @@ class LocalAERIS(nn.Module):
         else:
             # block by block between two buffers: a hook may bring in the next block's weights, and looks at the stream
             k, spare = 0, None
-            for layer, shift in zip(layers, shifts):
+            for i, (layer, shift) in enumerate(zip(layers, shifts)):
+                with_context = {} if context is None else {"context": context[i]}
                 for j in range(layer.sublayers):
                     if spare is None:
                         spare = torch.empty_like(tok)
-                    res = layer.block_forward(j, tok, t, shift, out=spare)
+                    res = layer.block_forward(j, tok, t, shift, out=spare, **with_context)
                     tok, spare = res, tok
                     k += 1
                     if block_hook is not None:

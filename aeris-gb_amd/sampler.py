@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 
 from . import _lib as L, ops
-from .model import calls_ahead
+from .model import LocalAERIS, calls_ahead
 
 
 def sigma_schedule(n_steps, sigma_min=0.2, sigma_max=500.0, sigma_data=1.0, rho=10, device="cpu"):
@@ -66,6 +66,7 @@ class _Rollout:
             self.latents = latents.to(dev, torch.float32).contiguous()
         self.B = B
         self.graph, self.step = None, None
+        self.context = None  # keys and values of an encoder's states, the same for every forecast step
         self.steps_per_replay = 1  # forecast steps recorded in ``graph``
         self._done = 0
         self.reset()
@@ -119,10 +120,11 @@ class TrigFlowSampler:
         self.t_steps = sigma_schedule(n_steps, sigma_min, sigma_max, sigma_data, device=device)
         self._graph = None
 
-    def _denoise(self, x, cond, t):
+    def _denoise(self, x, cond, t, context=None):
         # the condition channels follow the state channels (inference.py:160); the division by sigma_data and the
         # concatenation happen inside the embedding's operand preparation
-        return self.model(x, t, cond=cond, x_div=self.sigma_data)
+        with_context = {} if context is None else {"context": context}
+        return self.model(x, t, cond=cond, x_div=self.sigma_data, **with_context)
 
     def _advance(self, x, F_s, F_t, i):
         """x + h F_s, or x + (h / 2) (F_s + F_t), h = (t[i + 1] - t[i]) sigma_data  (inference.py:160-178)."""
@@ -139,15 +141,17 @@ class TrigFlowSampler:
             TrigFlowSampler._denoise, TrigFlowSampler._advance)
 
     @torch.no_grad()
-    def sample(self, cond: torch.Tensor, latents: torch.Tensor) -> torch.Tensor:
-        """cond [B, S, C_cond], latents [B, S, C] ~ N(0,1) -> sample [B, S, C]; 2*n_steps-1 denoiser calls."""
+    def sample(self, cond: torch.Tensor, latents: torch.Tensor, context=None) -> torch.Tensor:
+        """cond [B, S, C_cond], latents [B, S, C] ~ N(0,1) -> sample [B, S, C]; 2*n_steps-1 denoiser calls.  ``context``: what the
+        model's ``encode_context`` made of an encoder's states, the same for all of them."""
         sd, n = self.sigma_data, self.n_steps
         x = latents * sd
-        ahead = calls_ahead(self.model, self.t_steps[:n]) if self._own_steps() else None
+        ahead = calls_ahead(self.model, self.t_steps[:n]) if self._own_steps() and context is None else None
+        with_context = {} if context is None else {"context": context}
         levels = self.t_steps.split(1)
 
         def denoise(x, i):
-            return self._denoise(x, cond, levels[i]) if ahead is None else ahead(x, cond, sd, i)
+            return self._denoise(x, cond, levels[i], **with_context) if ahead is None else ahead(x, cond, sd, i)
 
         for i in range(n):
             F_s = denoise(x, i)
@@ -160,11 +164,13 @@ class TrigFlowSampler:
         return x
 
     # ---- HIP-graph replay of one sampling pass ---------------------------------------------------
-    def capture(self, cond_example: torch.Tensor, latents_example: torch.Tensor, warmup: int = 1):
-        """Capture ``sample`` into a HIP graph with static input/output buffers."""
+    def capture(self, cond_example: torch.Tensor, latents_example: torch.Tensor, warmup: int = 1, context=None):
+        """Capture ``sample`` into a HIP graph with static input/output buffers; ``context``'s tensors are read where they are."""
         self._cond = cond_example.clone()
         self._lat = latents_example.clone()
-        self._graph = self._capture(lambda: self.sample(self._cond, self._lat), warmup)
+        self._context = context
+        with_context = {} if context is None else {"context": context}
+        self._graph = self._capture(lambda: self.sample(self._cond, self._lat, **with_context), warmup)
         self._out = self._captured
         return self
 
@@ -187,6 +193,8 @@ class TrigFlowSampler:
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
         torch.cuda.empty_cache()  # the warm-up's cached blocks would sit next to the graph's own pool
+        if isinstance(self.model, LocalAERIS):
+            self.model.prepare(torch.device("cuda", torch.cuda.current_device()))
         graph = torch.cuda.CUDAGraph()
         if generator is not None:
             graph.register_generator_state(generator)
@@ -210,7 +218,7 @@ class TrigFlowSampler:
             lat = ro.latents.index_select(0, ro.k)[0]
         else:
             lat = torch.randn(ro.cond.shape, generator=generator, device=ro.cond.device)  # inference.py:135
-        y = self.sample(c, lat)
+        y = self.sample(c, lat) if ro.context is None else self.sample(c, lat, context=ro.context)
         ro.x_un.add_(y * ro.t_std + ro.t_mean)  # X <- X + unstandardize_t(Y)   (inference.py:180-183, era5.py:107-114)
         torch.div(ro.x_un - ro.x_mean, ro.x_std, out=ro.cond)  # standardize_x  (inference.py:186, era5.py:95-99)
         ro.states.index_copy_(0, ro.k, ro.cond.unsqueeze(0))
@@ -219,7 +227,7 @@ class TrigFlowSampler:
     @torch.no_grad()
     def begin_rollout(self, state0: torch.Tensor, n_forecast: int, generator: Optional[torch.Generator] = None,
                       x_mean=None, x_std=None, t_mean=None, t_std=None, forcing=None, static=None, extra_cond=None,
-                      latents=None, use_graph=False, graph_warmup: int = 0, graph_steps: int = 1) -> "_Rollout":
+                      latents=None, use_graph=False, graph_warmup: int = 0, graph_steps: int = 1, context=None) -> "_Rollout":
         """Set up an autoregressive forecast (arguments: see ``rollout``) and, with ``use_graph``, capture
         ``graph_steps`` consecutive forecast steps as one HIP graph (1: the graph is one forecast step and is replayed
         per step; n_forecast: the whole rollout is one graph and one replay), after ``graph_warmup`` eager steps whose
@@ -231,6 +239,7 @@ class TrigFlowSampler:
         if graph_steps < 1 or n_forecast % graph_steps:
             raise ValueError(f"graph_steps must divide n_forecast = {n_forecast}")
         ro = _Rollout(state0, n_forecast, x_mean, x_std, t_mean, t_std, forcing, static, extra_cond, latents)
+        ro.context = context
         if use_graph and generator is None and latents is None:
             generator = torch.cuda.default_generators[state0.device.index or 0]
         gen = generator if latents is None else None
@@ -271,7 +280,8 @@ class TrigFlowSampler:
         (identity when omitted); ``forcing`` [n_forecast + 1, 1|B, S, Cf]; ``static`` [1|B, S, Cs]; ``extra_cond``
         [1|B, S, Ce] or one per step [n_forecast, 1|B, S, Ce]; ``latents`` [n_forecast, B, S, C] replaces the draw
         from ``generator``.  ``use_graph``: the forecast step is captured once and replayed n_forecast times
-        (``graph_steps=n_forecast``: the whole rollout is captured as one graph and replayed once).
+        (``graph_steps=n_forecast``: the whole rollout is captured as one graph and replayed once).  ``context``: the model's
+        ``encode_context`` of an encoder's states, read in every step.
         Returns the standardised state after every forecast step, [n_forecast, B, S, C].
         """
         ro = self.begin_rollout(state0, n_forecast, generator, **kw)

@@ -1,0 +1,228 @@
+"""Blocks whose heads are normed and rotated and whose tokens attend to an encoder's states, against fp32 evaluations with the same
+weights, up to the sampler.  Tolerances are those of the other block and denoiser tests: 1e-2 of the 2-norm (bf16 weights and operands)."""
+import importlib
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from helpers import rel_l2
+
+EPS = torch.finfo(torch.float32).eps
+
+
+def rms(x, w):
+    return x * torch.rsqrt(x.square().mean(-1, keepdim=True) + EPS) * w
+
+
+def heads_of(x, w, bias, heads):
+    y = F.linear(x, w.float(), None if bias is None else bias.float())
+    return y.unflatten(-1, (heads, -1))
+
+
+def rotate(x, places, base):
+    """x [.., n, heads, d], places [n, 2]: pairs (2j, 2j + 1), the first half of them by the row, the others by the column."""
+    d = x.shape[-1]
+    freq = float(base) ** (-torch.arange(0, d // 2, 2, dtype=torch.float64, device=x.device) / (d // 2))
+    angle = torch.cat([places[:, :1].double() * freq, places[:, 1:].double() * freq], dim=1)[:, None]
+    z = torch.view_as_complex(x.double().unflatten(-1, (-1, 2)).contiguous()) * torch.polar(torch.ones_like(angle), angle)
+    return torch.view_as_real(z).flatten(-2).float()
+
+
+def window_attention(attn, y, shift):
+    """y [b, H * W, d] -> attention output ahead of wo, [b, H * W, inner]."""
+    (H, W), (wy, wx), b = attn.image_shape, attn.window_size, y.shape[0]
+    q, k, v = F.linear(y, attn.to_qkv.weight.float(), None if attn.to_qkv.bias is None else attn.to_qkv.bias.float()).unflatten(-1, (3, attn.heads, -1)).unbind(2)
+    if attn.qk_norm:
+        q, k = rms(q, attn.q_norm.weight.float()), rms(k, attn.k_norm.weight.float())
+
+    def windows(t):
+        t = torch.roll(t.unflatten(1, (H, W)), (-shift[0], -shift[1]), (1, 2))
+        t = t.unflatten(2, (W // wx, wx)).unflatten(1, (H // wy, wy)).transpose(2, 3)  # b ny nx wy wx h d
+        return t.flatten(3, 4).flatten(0, 2)
+    q, k, v = windows(q), windows(k), windows(v)
+    if attn.rotates:
+        i = torch.arange(wy * wx, device=y.device)
+        places = torch.stack([i // wx, i % wx], 1)
+        q, k = rotate(q, places, attn.rope.rope_base), rotate(k, places, attn.rope.rope_base)
+    p = torch.softmax(torch.einsum("wqhd,wkhd->whqk", q, k) * attn.scale, -1)
+    o = torch.einsum("whqk,wkhd->wqhd", p, v).flatten(-2)
+    o = o.unflatten(0, (b, H // wy, W // wx)).unflatten(3, (wy, wx)).transpose(2, 3).flatten(3, 4).flatten(1, 2)
+    return torch.roll(o, shift, (1, 2)).flatten(1, 2)
+
+
+def cross_attention(cross, y, states, lengths, mask, prefix):
+    """-> output of wo; states [b | 1, n, c]."""
+    q = heads_of(y, cross.to_q.weight, cross.to_q.bias, cross.heads)
+
+    def kv(s):
+        k, v = heads_of(s, cross.to_kv.weight, cross.to_kv.bias, 2 * cross.kv_heads).chunk(2, dim=-2)
+        return (rms(k, cross.k_norm.weight.float()) if cross.qk_norm else k), v
+    if cross.qk_norm:
+        q = rms(q, cross.q_norm.weight.float())
+    out = []
+    for b in range(y.shape[0]):
+        s = states[b if states.shape[0] > 1 else 0].float()
+        keep = torch.arange(s.shape[0], device=y.device)
+        if lengths is not None:
+            keep = keep[:int(lengths[b if lengths.numel() > 1 else 0])]
+        if mask is not None:
+            keep = keep[mask[b if mask.shape[0] > 1 else 0][keep]]
+        s = s[keep] if prefix is None else torch.cat([prefix.float(), s[keep]])
+        k, v = (t.repeat_interleave(cross.heads // cross.kv_heads, dim=-2) for t in kv(s))
+        p = torch.softmax(torch.einsum("qhd,khd->hqk", q[b], k) * cross.scale, -1)
+        out.append(torch.einsum("hqk,khd->qhd", p, v).flatten(-2))
+    return F.linear(torch.stack(out), cross.wo.weight.float(), None if cross.wo.bias is None else cross.wo.bias.float())
+
+
+def layer_forward(layer, x, shift, context=None):
+    """The un-modulated blocks of a layer in fp32."""
+    x = x.float()
+    for j, (n1, attn, n2, ff) in enumerate(layer.modulelist):
+        def norm(n, t):
+            if layer.opts.norm == "layernorm":
+                return F.layer_norm(t, t.shape[-1:], n.weight.float(), n.bias.float(), layer.opts.norm_eps)
+            return rms(t, n.weight.float())
+
+        def lin(m, t):
+            return F.linear(t, m.weight.float(), None if m.bias is None else m.bias.float())
+        x = x + lin(attn.wo, window_attention(attn, norm(n1, x), shift))
+        if context is not None:
+            n3, cross = layer.contextlist[j]
+            x = x + cross_attention(cross, norm(n3, x), *context)
+        h = norm(n2, x)
+        if layer.opts.mlp == "swiglu":
+            gate, up = lin(ff.w1, h).chunk(2, -1)
+            x = x + lin(ff.w2, F.silu(gate) * up)
+        else:
+            x = x + lin(ff.fc2, F.gelu(lin(ff.fc1, h)))
+    return x
+
+
+def fill(module, seed):
+    g = torch.Generator().manual_seed(seed)
+    with torch.no_grad():
+        for p in module.parameters():
+            r = torch.randn(p.shape, generator=g)
+            p.copy_(r * p.shape[1] ** -0.5 if p.dim() >= 2 else 0.1 * r + (1.0 if p is not None and p.dim() == 1 else 0.0))
+    return module
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("preset,qk_norm,rope,head_dim,window", [("spec", True, True, 32, (8, 8)), ("ref", True, True, 64, (12, 8)), ("spec", False, True, 64, (16, 16)),
+                                                                 ("ref", True, False, 128, (8, 4))])
+@pytest.mark.parametrize("shift", [(0, 0), (4, 2)])
+def test_window_blocks_with_normed_and_rotated_heads(pkg, cuda, preset, qk_norm, rope, head_dim, window, shift):
+    layer = pkg.SwinLayer(None, 2 * head_dim, 2, head_dim, 256, window, (window[0] * 3, window[1] * 4), False, 10_000, sublayers=2, preset=preset, mod_ways=0,
+                          rel_pos_bias=False, shift_mask=False, qk_norm=qk_norm, rope=rope)
+    layer = fill(layer, 1).to(torch.bfloat16).to(cuda)
+    x = torch.randn(2, 12 * window[0] * window[1], 2 * head_dim, generator=torch.Generator().manual_seed(2)).to(cuda)
+    got, want = layer(x, shift=shift), layer_forward(layer, x, shift)
+    assert rel_l2(got, want) <= 1e-2
+    # what is switched on is felt
+    plain = pkg.SwinLayer(None, 2 * head_dim, 2, head_dim, 256, window, layer.image_shape, False, 10_000, sublayers=2, preset=preset, mod_ways=0,
+                          rel_pos_bias=False, shift_mask=False).to(torch.bfloat16).to(cuda)
+    plain.load_state_dict({k: v for k, v in layer.state_dict().items() if "q_norm" not in k and "k_norm" not in k})
+    assert rel_l2(plain(x, shift=shift), want) > 2e-2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv_heads,head_dim,stream", [(0, 64, torch.float32), (2, 64, torch.bfloat16), (1, 128, torch.float32)])
+@pytest.mark.parametrize("kind", ["plain", "ragged", "shared", "prefix"])
+def test_blocks_that_attend_to_a_context(pkg, cuda, kv_heads, head_dim, stream, kind):
+    B, dim, heads, cdim = 3, 256, 256 // head_dim, 192
+    layer = pkg.SwinLayer(None, dim, heads, head_dim, 512, (8, 8), (16, 24), False, 10_000, sublayers=2, preset="ref", mod_ways=0, context_dim=cdim,
+                          context_kv_heads=kv_heads)
+    layer = fill(layer, 3).to(torch.bfloat16).to(cuda)
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(B, 384, dim, generator=g).to(cuda).to(stream)
+    states = torch.randn(1 if kind == "shared" else B, 70, cdim, generator=g).bfloat16().to(cuda)
+    lengths = mask = prefix = None
+    if kind == "ragged":
+        lengths, mask = torch.tensor([70, 9, 33], dtype=torch.int32, device=cuda), (torch.rand(B, 70, generator=g) < 0.7).to(cuda)
+    if kind == "prefix":
+        prefix = torch.randn(200, cdim, generator=g).bfloat16().to(cuda)
+    context = layer.encode_context(states, lengths, mask, prefix)
+    assert len(context) == 2 and context[0].k.shape == (states.shape[0], 70, kv_heads or heads, head_dim)
+    want = layer_forward(layer, x, (0, 0), (states, lengths, mask, prefix))
+    assert rel_l2(layer(x, context=context), want) <= 1e-2
+    assert rel_l2(layer_forward(layer, x, (0, 0)), want) > 2e-2
+    # the module alone
+    cross, y = layer.contextlist[0][1], torch.randn(B, 384, dim, generator=g).bfloat16().to(cuda)
+    assert rel_l2(cross(y, context[0]), cross_attention(cross, y.float(), states, lengths, mask, prefix)) <= 1e-2
+    with pytest.raises(ValueError, match="context"):
+        layer(x)
+
+
+def _model(pkg, cuda, **kw):
+    m = pkg.LocalAERIS(heads=4, dim=256, head_dim=64, mlp_dim=512, window_size=(8, 8), image_shape=(16, 32), rope_base=10_000, sublayers=1,
+                       sinusoidal_emb_max_period=10_000, n_layers=4, model_in_channels=12, model_out_channels=5, **kw)
+    return fill(m, 5).to(cuda)
+
+
+@pytest.mark.gpu
+def test_denoiser_and_sampler_with_a_context(pkg, cuda):
+    """All of them together, as a draw uses them: normed and rotated heads, a context whose keys and values are made once, members that share
+    a prefix; the captured draw gives the eager one's bits, and no context is an error, as is one that the model does not take."""
+    m = _model(pkg, cuda, qk_norm=True, rope=True, context_dim=128, context_kv_heads=2)
+    g = torch.Generator().manual_seed(6)
+    B = 3
+    context = m.encode_context(torch.randn(B, 40, 128, generator=g).bfloat16().to(cuda), torch.tensor([40, 1, 17], dtype=torch.int32, device=cuda), None,
+                               torch.randn(300, 128, generator=g).bfloat16().to(cuda))
+    cond, latents = torch.randn(B, 512, 7, generator=g).to(cuda), torch.randn(B, 512, 5, generator=g).to(cuda)
+    sampler = pkg.TrigFlowSampler(m, n_steps=3, device=cuda)
+    sampler.capture(cond, latents, warmup=0, context=context)
+    want = sampler.sample_graph(cond, latents).clone()  # (a first replay also makes the packed weights that a capture without warm-up recorded)
+    assert bool(torch.isfinite(want).all())
+    for _ in range(3):
+        got = sampler.sample_graph(cond, latents)
+        torch.cuda.synchronize()
+        again = sampler.sample(cond, latents, context=context)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(again, want)
+    # each member alone, with its own states: the same draw
+    one = sampler.sample(cond[1:2], latents[1:2], context=[[pkg.ContextKV(c.k[1:2, :1], c.v[1:2, :1], None, None, c.prefix) for c in layer] for layer in context])
+    assert rel_l2(one, want[1:2]) <= 1e-2
+    states = sampler.rollout(cond[..., :5], 2, static=cond[..., 5:], latents=torch.stack([latents, latents]), context=context, use_graph=True)
+    assert bool(torch.isfinite(states).all())
+    eager = sampler.rollout(cond[..., :5], 2, static=cond[..., 5:], latents=torch.stack([latents, latents]), context=context)
+    assert torch.equal(states, eager)
+    with pytest.raises(ValueError, match="context"):
+        sampler.sample(cond, latents)
+    with pytest.raises(ValueError, match="context"):
+        _model(pkg, cuda)(torch.randn(B, 512, 12).to(cuda), torch.tensor([0.5], device=cuda), context=context)
+
+
+@pytest.mark.gpu
+def test_denoiser_with_normed_heads_in_one_step(pkg, cuda):
+    """Every block of a modulated model runs its own forward: the layers one by one give the model's bits."""
+    m = _model(pkg, cuda, qk_norm=True, rope=True)
+    x, t = torch.randn(2, 512, 12, generator=torch.Generator().manual_seed(8)).to(cuda), torch.tensor([0.7], device=cuda)
+    seen = []
+    want = m(x, t, block_hook=lambda k, h: seen.append(h.clone()))
+    assert torch.equal(m(x, t), want) and len(seen) == 3
+    tok, dt = m.input_stage(x, t, out_dtype=torch.float32)
+    assert torch.equal(m.layers[0](tok, dt), seen[1]) and torch.equal(m.layers[1](seen[1], dt, shift=(4, 4)), seen[2])
+
+
+def test_options_and_state_dict(pkg):
+    """The options change no model that does not ask for them; what they add is named beside the rest."""
+    kw = dict(device_mesh=None, dim=128, heads=2, head_dim=64, mlp_dim=256, window_size=(8, 8), image_shape=(16, 16), shifted_grid=False, rope_base=10_000)
+    plain, full = pkg.SwinLayer(**kw), pkg.SwinLayer(**kw, qk_norm=True, rope=True, context_dim=64)
+    new = full.state_dict().keys() - plain.state_dict().keys()
+    assert plain.state_dict().keys() < full.state_dict().keys()
+    assert new == {"modulelist.0.1.q_norm.weight", "modulelist.0.1.k_norm.weight", "contextlist.0.0.weight", "contextlist.0.1.to_q.weight",
+                   "contextlist.0.1.to_kv.weight", "contextlist.0.1.wo.weight", "contextlist.0.1.q_norm.weight", "contextlist.0.1.k_norm.weight"}
+    model = importlib.import_module("aeris-gb_amd.model")
+    assert model._own_blocks(plain) and not model._own_blocks(full)
+    assert not model._own_blocks(pkg.SwinLayer(**kw, rope=True)) and not model._own_blocks(pkg.SwinLayer(**kw, context_dim=64))
+    with pytest.raises(ValueError):
+        pkg.CrossAttention(128, 3, 32, 64, kv_heads=2)
+    with pytest.raises(ValueError):
+        plain.encode_context(torch.zeros(1, 4, 64))
+    rope = pkg.RoPE2D((3, 5), 32, 10_000)
+    assert rope.table(torch.device("cpu")).shape == (15, 64)
+    got = rope.positions((6, 10), (1, 2), torch.device("cpu")).view(6, 10)
+    for Y in range(6):
+        for X in range(10):
+            assert int(got[Y, X]) == (Y - 1) % 6 % 3 * 5 + (X - 2) % 10 % 5
