@@ -45,8 +45,7 @@ SIGNATURES = {
                                 _c_int, _c_int, _c_i64, _c_i64, _c_vp]),
     "aeris_gemm_heads_fwd": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_int, _c_int, _c_int, _c_i64, _c_f32, _c_int,
                                       _c_vp]),
-    "aeris_qk_norm_rope_fwd": (_c_int, [_c_vp, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_f32, _c_vp, _c_i64, _c_int, _c_int,
-                                        _c_vp, _c_i64, _c_vp]),
+    "aeris_qk_norm_rope_fwd": (_c_int, [_c_vp, _c_vp]),
     "aeris_cross_attention_workspace_bytes": (_c_i64, [_c_vp]),
     "aeris_cross_attention_fwd": (_c_int, [_c_vp, _c_vp, _c_i64, _c_vp]),
     "aeris_modulation_linear_fwd": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp]),

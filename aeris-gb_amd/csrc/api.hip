@@ -381,28 +381,27 @@ int aeris_gemm_heads_fwd(const void* A, const void* W, void* C, const void* bias
   return AERIS_OK;
 }
 
-int aeris_qk_norm_rope_fwd(const aeris_qk_part* parts, int n_parts, int64_t tokens, int head_dim, int x_dtype, int y_dtype, int gain_dtype,
-                           int normed, float eps, const float* rotation, int64_t P, int R, int interleaved, const int32_t* positions,
-                           int64_t n_positions, void* stream) {
+int aeris_qk_norm_rope_fwd(const aeris_qk_norm_rope* a, void* stream) {
   const char* who = "aeris_qk_norm_rope_fwd";
-  if (!parts || n_parts < 1 || n_parts > 2) return fail(AERIS_EINVAL, "%s: one or two parts (got %d)", who, n_parts);
-  for (int dt : {x_dtype, y_dtype, gain_dtype})
+  if (!a || a->n_parts < 1 || a->n_parts > 2) return fail(AERIS_EINVAL, "%s: one or two parts", who);
+  for (int64_t dt : {a->x_dtype, a->y_dtype, a->gain_dtype})
     if (dt != AERIS_BF16 && dt != AERIS_F32) return fail(AERIS_EINVAL, "%s: dtype must be AERIS_BF16 or AERIS_F32", who);
-  if (tokens <= 0) return fail(AERIS_EINVAL, "%s: tokens must be positive", who);
-  if (!(eps >= 0.f)) return fail(AERIS_EINVAL, "%s: eps must be non-negative", who);
-  if (!aeris::qk_norm_rope_supported(head_dim, R))
-    return fail(AERIS_EUNSUPPORTED, "%s: head_dim %d, %d rotated elements (need head_dim 32, 64 or 128, and a multiple of 16 up to it)", who, head_dim, R);
-  if (R > 0 && (!rotation || !aligned16(rotation) || P <= 0 || P > 0x7fffffffLL))
+  if (a->tokens <= 0) return fail(AERIS_EINVAL, "%s: tokens must be positive", who);
+  if (!(a->eps >= 0.0)) return fail(AERIS_EINVAL, "%s: eps must be non-negative", who);
+  if (!aeris::qk_norm_rope_supported(a->head_dim, a->R))
+    return fail(AERIS_EUNSUPPORTED, "%s: head_dim %lld, %lld rotated elements (need head_dim 32, 64 or 128, and a multiple of 16 up to it)", who,
+                (long long)a->head_dim, (long long)a->R);
+  if (a->R > 0 && (!a->rotation || !aligned16(a->rotation) || a->P <= 0 || a->P > 0x7fffffffLL))
     return fail(AERIS_EINVAL, "%s: the rotation table must be 16-byte aligned and have 1 .. 2^31-1 rows", who);
-  if (R > 0 && positions && (n_positions <= 0 || n_positions > 0x7fffffffLL || (reinterpret_cast<uintptr_t>(positions) & 3u)))
+  if (a->R > 0 && a->positions && (a->n_positions <= 0 || a->n_positions > 0x7fffffffLL || (reinterpret_cast<uintptr_t>(a->positions) & 3u)))
     return fail(AERIS_EINVAL, "%s: positions must be 4-byte aligned, 1 .. 2^31-1 of them", who);
   // (token numbers are formed in 32 bits, up to a block of them beyond the last; the grid's second dimension counts heads)
-  if (tokens > 0x7fffffffLL - 64) return fail(AERIS_EUNSUPPORTED, "%s: more than 2^31-65 tokens", who);
+  if (a->tokens > 0x7fffffffLL - 64) return fail(AERIS_EUNSUPPORTED, "%s: more than 2^31-65 tokens", who);
   int64_t heads = 0;
-  for (int i = 0; i < n_parts; ++i) {
-    const aeris_qk_part& p = parts[i];
+  for (int i = 0; i < (int)a->n_parts; ++i) {
+    const aeris_qk_part& p = a->parts[i];
     if (!p.x || !p.y || p.heads <= 0) return fail(AERIS_EINVAL, "%s: x/y is NULL or heads is not positive", who);
-    const int ex = x_dtype == AERIS_F32 ? 4 : 8, ey = y_dtype == AERIS_F32 ? 4 : 8, eg = gain_dtype == AERIS_F32 ? 4 : 8;
+    const int ex = a->x_dtype == AERIS_F32 ? 4 : 8, ey = a->y_dtype == AERIS_F32 ? 4 : 8, eg = a->gain_dtype == AERIS_F32 ? 4 : 8;
     if (!aligned16(p.x) || !aligned16(p.y) || (p.gain && !aligned16(p.gain)) || p.x_token_stride % ex || p.x_head_stride % ex ||
         p.y_token_stride % ey || p.y_head_stride % ey || p.gain_head_stride % eg)
       return fail(AERIS_EINVAL, "%s: x, y and gain must be 16-byte aligned, their strides multiples of 16 bytes", who);
@@ -410,9 +409,7 @@ int aeris_qk_norm_rope_fwd(const aeris_qk_part* parts, int n_parts, int64_t toke
     heads += p.heads;
   }
   if (heads > 65535) return fail(AERIS_EUNSUPPORTED, "%s: more than 65535 heads", who);
-  hipError_t e = aeris::qk_norm_rope_launch(parts, n_parts, (int)tokens, head_dim, x_dtype, y_dtype, gain_dtype, normed ? 1 : 0, eps, rotation,
-                                            (int)P, R, interleaved ? 1 : 0, R > 0 ? positions : nullptr, (int)n_positions,
-                                            reinterpret_cast<hipStream_t>(stream));
+  hipError_t e = aeris::qk_norm_rope_launch(*a, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "aeris_qk_norm_rope_fwd launch");
   return AERIS_OK;
 }
@@ -424,7 +421,7 @@ int check_cross_sizes(const char* who, const aeris_cross_attention* a) {
   if (a->B <= 0 || a->Nq <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->Nk < 0 || a->Np < 0)
     return fail(AERIS_EINVAL, "%s: B, Nq, heads, kv_heads must be positive, Nk and Np not negative", who);
   if (a->heads % a->kv_heads) return fail(AERIS_EINVAL, "%s: %lld heads do not divide among %lld key heads", who, (long long)a->heads, (long long)a->kv_heads);
-  if (!aeris::cross_attention_supported((int)a->head_dim) || a->head_dim > 128)
+  if (!aeris::cross_attention_supported(a->head_dim))
     return fail(AERIS_EUNSUPPORTED, "%s: head_dim %lld (need 32, 64 or 128)", who, (long long)a->head_dim);
   const int64_t most = 0x7fffffffLL;
   if (a->B > most || a->Nq > most || a->heads > 65535 || a->Nk > most - 4096 || a->Np > most - 4096 || a->B * a->Nq > most ||

@@ -65,13 +65,11 @@ hipError_t output_stage_launch(const void* x, int x_dtype, const void* gamma, co
                                void* workspace, hipStream_t stream);
 
 // norm and rotation of query and key heads (qk_norm_rope.hip)
-bool qk_norm_rope_supported(int head_dim, int rotated);
-hipError_t qk_norm_rope_launch(const aeris_qk_part* parts, int n_parts, int T, int head_dim, int x_dtype, int y_dtype, int gain_dtype, int normed,
-                               float eps, const float* rotation, int P, int R, int interleaved, const int32_t* positions, int n_pos,
-                               hipStream_t stream);
+bool qk_norm_rope_supported(int64_t head_dim, int64_t rotated);
+hipError_t qk_norm_rope_launch(const aeris_qk_norm_rope& a, hipStream_t stream);
 
 // attention to an encoder's states (cross_attention.hip)
-bool cross_attention_supported(int head_dim);
+bool cross_attention_supported(int64_t head_dim);
 hipError_t cross_attention_configure();
 int64_t cross_attention_workspace_bytes(const aeris_cross_attention& a);
 hipError_t cross_attention_launch(const aeris_cross_attention& a, void* workspace, hipStream_t stream);

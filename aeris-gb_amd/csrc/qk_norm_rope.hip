@@ -197,23 +197,22 @@ hipError_t launch_types(const QkParams& p, bool x_f32, bool y_f32, hipStream_t s
 
 }  // namespace
 
-bool qk_norm_rope_supported(int head_dim, int rotated) {
+bool qk_norm_rope_supported(int64_t head_dim, int64_t rotated) {
   return (head_dim == 32 || head_dim == 64 || head_dim == 128) && rotated >= 0 && rotated <= head_dim && rotated % 16 == 0;
 }
 
-hipError_t qk_norm_rope_launch(const aeris_qk_part* parts, int n_parts, int T, int head_dim, int x_dtype, int y_dtype, int gain_dtype, int normed,
-                               float eps, const float* rotation, int P, int R, int interleaved, const int32_t* positions, int n_pos,
-                               hipStream_t stream) {
+hipError_t qk_norm_rope_launch(const aeris_qk_norm_rope& a, hipStream_t stream) {
   QkParams p{};
-  p.part[0] = parts[0];
-  if (n_parts > 1) p.part[1] = parts[1];
-  p.T = T; p.P = P; p.R = R; p.normed = normed; p.interleaved = interleaved; p.gain_f32 = gain_dtype == AERIS_F32; p.eps = eps;
-  p.rotation = rotation; p.positions = positions;
-  p.n_pos = positions ? n_pos : P > 0 ? P : 1;
-  const bool xf = x_dtype == AERIS_F32, yf = y_dtype == AERIS_F32;
-  const bool many = (int64_t)T * head_dim >= 32768 * 8;
-  if (head_dim == 32) return many ? launch_types<32, 4>(p, xf, yf, stream) : launch_types<32, 1>(p, xf, yf, stream);
-  if (head_dim == 64) return many ? launch_types<64, 4>(p, xf, yf, stream) : launch_types<64, 1>(p, xf, yf, stream);
+  p.part[0] = a.parts[0];
+  if (a.n_parts > 1) p.part[1] = a.parts[1];
+  p.T = (int)a.tokens; p.P = (int)a.P; p.R = (int)a.R; p.normed = a.normed != 0; p.interleaved = a.interleaved != 0;
+  p.gain_f32 = a.gain_dtype == AERIS_F32; p.eps = (float)a.eps;
+  p.rotation = a.rotation; p.positions = a.R > 0 ? a.positions : nullptr;
+  p.n_pos = p.positions ? (int)a.n_positions : a.P > 0 ? (int)a.P : 1;
+  const bool xf = a.x_dtype == AERIS_F32, yf = a.y_dtype == AERIS_F32;
+  const bool many = a.tokens * a.head_dim >= 32768 * 8;
+  if (a.head_dim == 32) return many ? launch_types<32, 4>(p, xf, yf, stream) : launch_types<32, 1>(p, xf, yf, stream);
+  if (a.head_dim == 64) return many ? launch_types<64, 4>(p, xf, yf, stream) : launch_types<64, 1>(p, xf, yf, stream);
   return many ? launch_types<128, 4>(p, xf, yf, stream) : launch_types<128, 1>(p, xf, yf, stream);
 }
 

@@ -414,24 +414,19 @@ def gemm_heads(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], h
 
 def _on_current_device(t: torch.Tensor, name: str, device):
     """Whose stream the call goes to: every tensor of it lives on the current GPU."""
-    if not t.is_cuda:
-        raise RuntimeError(f"{name} must live on the GPU (the HIP kernels have no CPU fallback)")
     if t.device != device or device.index != torch._C._cuda_getDevice():
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} must live on the GPU (the HIP kernels have no CPU fallback)")
         raise RuntimeError(f"{name} is on {t.device}; every tensor of the call must be on the current device (cuda:{torch._C._cuda_getDevice()})")
 
 
-def _head_strides(t: torch.Tensor, name: str, dims: int):
-    """Strides, in elements, of a tensor whose last dimension is the elements of a head (contiguous, 16-byte pieces); 0 where a
-    dimension has one entry."""
-    shape, stride = t.shape, t.stride()
-    if len(shape) != dims:
-        raise RuntimeError(f"{name} must have {dims} dimensions, got {tuple(shape)}")
-    piece = 16 // t.element_size()
-    strides = tuple(0 if n <= 1 else s for n, s in zip(shape[:-1], stride[:-1]))
-    if stride[-1] != 1 or any(s % piece for s in strides) or t.data_ptr() % 16:
-        raise RuntimeError(f"{name} must be 16-byte aligned, the elements of a head contiguous and the other strides multiples of {piece} "
-                           f"(strides {stride})")
-    return strides
+def _head_strides(t: torch.Tensor, name: str):
+    """Strides, in elements, of [.., heads, head_dim]; 0 where a dimension has one entry.  (That they are multiples of 16 bytes, and the
+    address too, is for the library to say.)"""
+    stride = t.stride()
+    if stride[-1] != 1:
+        raise RuntimeError(f"{name}: the elements of a head must be contiguous (strides {stride})")
+    return [s if n > 1 else 0 for s, n in zip(stride[:-1], t.shape)]
 
 
 def _written_once(t: torch.Tensor, name: str):
@@ -444,7 +439,32 @@ def _written_once(t: torch.Tensor, name: str):
             span = s * (n - 1) + span
 
 
-QK_PART = struct.Struct("=3Q6qd")  # struct aeris_qk_part of include/aeris_hip.h
+QK_NORM_ROPE = struct.Struct("=3Q6qd3Q6qd2Q11qd")  # struct aeris_qk_norm_rope of include/aeris_hip.h
+_NO_PART = (0,) * 9 + (0.0,)
+
+
+def _qk_part(x, gain, out, scale, name, q, device, y_dtype):
+    """One part's fields of the call's struct, and its output."""
+    heads, D = x.shape[1:]
+    if out is None:
+        out = torch.empty_like(x, dtype=y_dtype)
+    else:
+        _on_current_device(out, f"{name}_out", device)
+        if out.shape != x.shape or out.dtype != y_dtype:
+            raise RuntimeError(f"{name}_out must be {y_dtype} {tuple(x.shape)}, got {out.dtype} {tuple(out.shape)}")
+        _written_once(out, f"{name}_out")
+    gain_ptr = per_head = 0
+    if gain is not None:
+        _on_current_device(gain, f"{name}_gain", device)
+        shape = tuple(gain.shape)
+        if shape == (heads, D):
+            per_head = D
+        elif shape != (D,):
+            raise RuntimeError(f"{name}_gain must be [{D}] or [{heads}, {D}], got {shape}")
+        if not gain.is_contiguous():
+            raise RuntimeError(f"{name}_gain must be contiguous")
+        gain_ptr = gain.data_ptr()
+    return (x.data_ptr(), out.data_ptr(), gain_ptr, heads, *_head_strides(x, name), *_head_strides(out, f"{name}_out"), per_head, scale), out
 
 
 def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_gain: Optional[torch.Tensor] = None,
@@ -461,64 +481,57 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_gain: Opti
     q is multiplied by q_scale ahead of its rounding (``scale * LOG2E`` for the attention calls' ``q_prescaled``).
     The outputs (out_dtype) may be given; q_out may be q and k_out may be k.  Otherwise an output shares no memory with an input."""
     device = q.device
-    parts = [(q, q_gain, q_out, float(q_scale), "q")]
-    if k is not None:
-        parts.append((k, k_gain, k_out, 1.0, "k"))
-    elif k_gain is not None or k_out is not None:
-        raise RuntimeError("k_gain and k_out need k")
-    if q.dtype not in _DT or out_dtype not in _DT:
-        raise RuntimeError("q and the outputs must be bf16 or f32")
-    given = [o.dtype for o in (q_out, k_out) if o is not None]
-    y_dtype = given[0] if given else out_dtype
-    gains = [g.dtype for g in (q_gain, k_gain) if g is not None]
-    gain_dtype = gains[0] if gains else torch.float32
-    if y_dtype not in _DT or any(d != y_dtype for d in given) or gain_dtype not in _DT or any(d != gain_dtype for d in gains):
-        raise RuntimeError("the outputs must be of one type, the gains must be of one type, bf16 or f32")
-    records, outs, moved = [], [], 0
-    for x, gain, out, scale, name in parts:
-        _on_current_device(x, name, device)
-        xs = _head_strides(x, name, 3)
-        T, heads, D = x.shape
-        if x.dtype != q.dtype or T != q.shape[0] or D != q.shape[2]:
-            raise RuntimeError(f"k must be {q.dtype} [{q.shape[0]}, key heads, {q.shape[2]}], got {x.dtype} {tuple(x.shape)}")
-        if out is None:
-            out = torch.empty_like(x, dtype=y_dtype)
-        else:
-            _on_current_device(out, f"{name}_out", device)
-            if out.shape != x.shape:
-                raise RuntimeError(f"{name}_out must be {tuple(x.shape)}, got {tuple(out.shape)}")
-            _written_once(out, f"{name}_out")
-        ys = _head_strides(out, f"{name}_out", 3)
-        per_head = 0
-        if gain is not None:
-            _on_current_device(gain, f"{name}_gain", device)
-            if not gain.is_contiguous() or tuple(gain.shape) not in ((D,), (heads, D)):
-                raise RuntimeError(f"{name}_gain must be contiguous, [{D}] or [{heads}, {D}], got {tuple(gain.shape)}")
-            per_head = D if gain.dim() == 2 else 0
-        records.append(QK_PART.pack(x.data_ptr(), out.data_ptr(), _ptr(gain) or 0, heads, *xs, *ys, per_head, scale))
-        outs.append(out)
-        moved += x.numel() * (x.element_size() + out.element_size())
-    P = R = n_pos = 0
+    _on_current_device(q, "q", device)
+    if q.dim() != 3:
+        raise RuntimeError(f"q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
+    T, _, D = q.shape
+    given = q_out if q_out is not None else k_out
+    y_dtype = out_dtype if given is None else given.dtype
+    some_gain = q_gain if q_gain is not None else k_gain
+    gain_type = _DT.get(some_gain.dtype) if some_gain is not None else 0
+    if q.dtype not in _DT or y_dtype not in _DT or gain_type is None:
+        raise RuntimeError("q, k, the gains and the outputs must be bf16 or f32")
+    q_part, yq = _qk_part(q, q_gain, q_out, q_scale, "q", q, device, y_dtype)
+    if k is None:
+        if k_gain is not None or k_out is not None:
+            raise RuntimeError("k_gain and k_out need k")
+        k_part, yk, empty = _NO_PART, None, yq.numel() == 0
+    else:
+        _on_current_device(k, "k", device)
+        if k.dtype != q.dtype or k.dim() != 3 or k.shape[0] != T or k.shape[2] != D:
+            raise RuntimeError(f"k must be {q.dtype} [{T}, key heads, {D}], got {k.dtype} {tuple(k.shape)}")
+        if q_gain is not None and k_gain is not None and q_gain.dtype != k_gain.dtype:
+            raise RuntimeError("q_gain and k_gain must be of one type")
+        k_part, yk = _qk_part(k, k_gain, k_out, 1.0, "k", q, device, y_dtype)
+        empty = yq.numel() == 0 or yk.numel() == 0
+        if empty and T:
+            raise RuntimeError("q and k must both have heads")
+    table_ptr = P = R = positions_ptr = n_pos = 0
     if rotation is not None:
         _on_current_device(rotation, "rotation", device)
         if rotation.dtype != torch.float32 or rotation.dim() != 2 or not rotation.is_contiguous():
             raise RuntimeError("rotation must be contiguous f32 [positions, rotated elements]")
         P, R = rotation.shape
+        table_ptr = rotation.data_ptr()
         if P == 0:
             raise RuntimeError("rotation has no rows")
     if positions is not None:
         _on_current_device(positions, "positions", device)
-        if rotation is None or positions.dtype != torch.int32 or positions.dim() != 1 or not positions.is_contiguous() or positions.numel() == 0:
-            raise RuntimeError("positions must be a contiguous int32 vector, and need rotation")
         n_pos = positions.numel()
-    if all(o.numel() for o in outs):
+        if rotation is None or positions.dtype != torch.int32 or positions.dim() != 1 or not positions.is_contiguous() or not n_pos:
+            raise RuntimeError("positions must be a contiguous int32 vector, and need rotation")
+        positions_ptr = positions.data_ptr()
+    if empty:
+        return yq, yk
+    call = QK_NORM_ROPE.pack(*q_part, *k_part, table_ptr, positions_ptr, T, D, _DT[q.dtype], _DT[y_dtype], gain_type, normed, interleaved, P, R, n_pos,
+                             1 if k is None else 2, eps)
+    if _profile is None:
+        L.call("aeris_qk_norm_rope_fwd", call, _stream())
+    else:
+        moved = sum(y.numel() * (q.element_size() + y.element_size()) for y in (yq, yk) if y is not None)
         with _timed("qk_norm_rope", float(moved), "byte"):
-            L.call("aeris_qk_norm_rope_fwd", b"".join(records), len(records), q.shape[0], q.shape[2], _DT[q.dtype], _DT[y_dtype],
-                   _DT[gain_dtype], int(bool(normed)), float(eps), _ptr(rotation) if R else None, P, R, int(bool(interleaved)),
-                   _ptr(positions), n_pos, _stream())
-    elif outs[0].numel() or outs[-1].numel():
-        raise RuntimeError("q and k must both have heads")
-    return outs[0], (outs[1] if k is not None else None)
+            L.call("aeris_qk_norm_rope_fwd", call, _stream())
+    return yq, yk
 
 
 CROSS_ATTENTION = struct.Struct("=8Q23qd")  # struct aeris_cross_attention of include/aeris_hip.h
@@ -534,61 +547,63 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, length
     lengths int32 [B | 1]: how many of the Nk keys a member has; key_mask bool | uint8 [B | 1, Nk]: which of those take part.  What k and v
     hold elsewhere is not looked at.  prefix = (k, v), [Np, key heads, head_dim]: states that all members see ahead of their own, read once
     for all of them where a member has few queries.  A query without any key gives zeros.
-    scale: head_dim^-0.5 unless given; ``q_prescaled``: q already holds q * scale * log2(e) (``qk_norm_rope(q_scale=scale * LOG2E)``),
-    rounded once; otherwise the product is rounded to bf16 once more.  out shares no memory with the inputs."""
-    device = q.device
+    scale: head_dim^-0.5 unless given; ``q_prescaled``: q already holds q * scale * log2(e) (``qk_norm_rope(q_scale=scale * LOG2E)``).  out shares
+    no memory with the inputs."""
+    device, shape, kv_shape = q.device, q.shape, k.shape
     _on_current_device(q, "q", device)
-    qs = _head_strides(q, "q", 4)
-    B, Nq, heads, D = q.shape
-    kv, prefix_strides, prefix_ptrs, Np = [], (0, 0, 0, 0), (0, 0), 0
-    for t, name in ((k, "k"), (v, "v")):
-        _on_current_device(t, name, device)
-        s = _head_strides(t, name, 4)
-        kv.append((0 if t.shape[0] == 1 else s[0], *s[1:]))
-    if k.shape != v.shape or k.shape[3] != D or k.shape[0] not in (1, B) or k.shape[2] == 0 or heads % k.shape[2]:
-        raise RuntimeError(f"k and v must be [1 | {B}, keys, divisor of {heads}, {D}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    Nk, kv_heads = k.shape[1], k.shape[2]
-    tensors = [q, k, v]
+    _on_current_device(k, "k", device)
+    _on_current_device(v, "v", device)
+    if len(shape) != 4 or len(kv_shape) != 4:
+        raise RuntimeError(f"q, k and v must have 4 dimensions, got {tuple(shape)} and {tuple(kv_shape)}")
+    B, Nq, heads, D = shape
+    Bk, Nk, kv_heads, Dk = kv_shape
+    if v.shape != kv_shape or Dk != D or (Bk != B and Bk != 1) or kv_heads == 0 or heads % kv_heads:
+        raise RuntimeError(f"k and v must be [1 | {B}, keys, divisor of {heads}, {D}], got {tuple(kv_shape)} and {tuple(v.shape)}")
+    bf16 = torch.bfloat16
+    if q.dtype is not bf16 or k.dtype is not bf16 or v.dtype is not bf16:
+        raise RuntimeError("q, k and v must be bf16")
+    prefix_ptrs, Np, prefix_strides = (0, 0), 0, (0, 0, 0, 0)
     if prefix is not None:
         pk, pv = prefix
-        for t, name in ((pk, "prefix k"), (pv, "prefix v")):
-            _on_current_device(t, name, device)
-        prefix_strides = _head_strides(pk, "prefix k", 3) + _head_strides(pv, "prefix v", 3)
-        if pk.shape != pv.shape or tuple(pk.shape[1:]) != (kv_heads, D):
-            raise RuntimeError(f"prefix must be two [keys, {kv_heads}, {D}], got {tuple(pk.shape)} and {tuple(pv.shape)}")
+        _on_current_device(pk, "prefix k", device)
+        _on_current_device(pv, "prefix v", device)
+        if pk.shape != pv.shape or pk.dim() != 3 or pk.shape[1] != kv_heads or pk.shape[2] != D or pk.dtype is not bf16 or pv.dtype is not bf16:
+            raise RuntimeError(f"prefix must be two bf16 [keys, {kv_heads}, {D}], got {pk.dtype} {tuple(pk.shape)} and {pv.dtype} {tuple(pv.shape)}")
         Np = pk.shape[0]
         prefix_ptrs = (pk.data_ptr(), pv.data_ptr())
-        tensors += [pk, pv]
-    if any(t.dtype != torch.bfloat16 for t in tensors):
-        raise RuntimeError("q, k, v and prefix must be bf16")
-    lengths_stride = mask_stride = 0
+        prefix_strides = (*_head_strides(pk, "prefix k"), *_head_strides(pv, "prefix v"))
+    lengths_ptr = lengths_stride = mask_ptr = mask_stride = 0
     if lengths is not None:
         _on_current_device(lengths, "lengths", device)
-        if lengths.dtype != torch.int32 or lengths.dim() != 1 or lengths.shape[0] not in (1, B) or not lengths.is_contiguous():
+        n = lengths.numel()
+        if lengths.dtype is not torch.int32 or lengths.dim() != 1 or (n != B and n != 1) or not lengths.is_contiguous():
             raise RuntimeError(f"lengths must be contiguous int32 [1 | {B}], got {lengths.dtype} {tuple(lengths.shape)}")
-        lengths_stride = int(lengths.shape[0] > 1)
+        lengths_ptr, lengths_stride = lengths.data_ptr(), int(n > 1)
     if key_mask is not None:
         _on_current_device(key_mask, "key_mask", device)
         if (key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.dim() != 2 or key_mask.shape[0] not in (1, B) or key_mask.shape[1] != Nk or
                 (Nk > 1 and key_mask.stride(1) != 1)):
             raise RuntimeError(f"key_mask must be bool or uint8 [1 | {B}, {Nk}] with contiguous rows, got {key_mask.dtype} {tuple(key_mask.shape)}")
-        mask_stride = key_mask.stride(0) if key_mask.shape[0] > 1 else 0
+        mask_ptr, mask_stride = key_mask.data_ptr(), key_mask.stride(0) if key_mask.shape[0] > 1 else 0
     if out is None:
-        out = torch.empty(B, Nq, heads, D, dtype=torch.bfloat16, device=device)
+        out = torch.empty(shape, dtype=bf16, device=device)
     else:
         _on_current_device(out, "out", device)
-        _dev(out, "out", torch.bfloat16)
-        if out.shape != q.shape:
-            raise RuntimeError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+        _dev(out, "out", bf16)
+        if out.shape != shape:
+            raise RuntimeError(f"out must be {tuple(shape)}, got {tuple(out.shape)}")
     if out.numel() == 0:
         return out
-    call = CROSS_ATTENTION.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), *prefix_ptrs, out.data_ptr(), _ptr(lengths) or 0, _ptr(key_mask) or 0,
-                                B, Nq, heads, kv_heads, D, Nk, Np, *qs, *kv[0], *kv[1], *prefix_strides, lengths_stride, mask_stride,
-                                int(bool(q_prescaled)), float(D ** -0.5 if scale is None else scale))
+    call = CROSS_ATTENTION.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), *prefix_ptrs, out.data_ptr(), lengths_ptr, mask_ptr, B, Nq, heads, kv_heads, D,
+                                Nk, Np, *_head_strides(q, "q"), *_head_strides(k, "k"), *_head_strides(v, "v"), *prefix_strides, lengths_stride,
+                                mask_stride, q_prescaled, D ** -0.5 if scale is None else scale)
     need = L.lib().aeris_cross_attention_workspace_bytes(call)
-    ws = workspace("cross_attention", (need,), torch.uint8, device) if need else None
-    with _timed("cross_attention", 4.0 * B * Nq * heads * D * (Np + Nk), "flop"):
-        L.call("aeris_cross_attention_fwd", call, _ptr(ws), need, _stream())
+    ws = workspace("cross_attention", (need,), torch.uint8, device).data_ptr() if need else None
+    if _profile is None:
+        L.call("aeris_cross_attention_fwd", call, ws, need, _stream())
+    else:
+        with _timed("cross_attention", 4.0 * B * Nq * heads * D * (Np + Nk), "flop"):
+            L.call("aeris_cross_attention_fwd", call, ws, need, _stream())
     return out
 
 

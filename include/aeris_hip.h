@@ -195,7 +195,7 @@ int aeris_gemm_heads_fwd(const void* A, const void* W, void* C, const void* bias
  *   n = x * rsqrt(mean(x^2) + eps) * gain  per (token, head) over the head_dim elements (normed == 0: n = x * gain)
  *   the pairs (a, b) of the first R elements become (a cos - b sin, a sin + b cos); interleaved: pairs (2j, 2j + 1), else (j, j + R/2)
  *   y = n * scale
- * in fp32, rounded once.  parts: one, or two that share tokens and positions (queries, keys).  Of each: x and y start at token 0, head 0,
+ * in fp32, rounded once.  parts: one (n_parts 1), or two that share tokens and positions (queries, keys).  Of each: x and y start at token 0, head 0,
  * strides in elements, the head_dim elements of a head are contiguous; y may be x (same strides and type) and may otherwise not overlap it;
  * gain [head_dim] (gain_head_stride 0) or one row per head, or NULL.  Addresses 16-byte aligned, strides multiples of 16 bytes.
  *   rotation f32 [P, R]: cos of the R/2 pairs, then sin (NULL with R = 0: no rotation); a token's row is positions[t % n_positions]
@@ -208,9 +208,14 @@ typedef struct aeris_qk_part {
   int64_t heads, x_token_stride, x_head_stride, y_token_stride, y_head_stride, gain_head_stride;
   double scale;
 } aeris_qk_part;
-int aeris_qk_norm_rope_fwd(const aeris_qk_part* parts, int n_parts, int64_t tokens, int head_dim, int x_dtype, int y_dtype, int gain_dtype,
-                           int normed, float eps, const float* rotation, int64_t P, int R, int interleaved, const int32_t* positions,
-                           int64_t n_positions, void* stream);
+typedef struct aeris_qk_norm_rope {
+  aeris_qk_part parts[2];
+  const float* rotation;
+  const int32_t* positions;
+  int64_t tokens, head_dim, x_dtype, y_dtype, gain_dtype, normed, interleaved, P, R, n_positions, n_parts;
+  double eps;
+} aeris_qk_norm_rope;
+int aeris_qk_norm_rope_fwd(const aeris_qk_norm_rope* a, void* stream);
 
 /* Attention to states of another length (an encoder's, observations', a whole grid's): per member b, query n, head h
  *   out = softmax(scale * q k^T) v  over the prefix's Np keys, then those of the member's Nk keys that lie before lengths[b] (held to [0, Nk])

@@ -4,7 +4,6 @@ Tolerance: an output is rounded once, by at most half a step (bf16 2^-8 of the v
 D <= 128 squares (partial sums of 8, then up to 4 levels: 12 roundings at most), the reciprocal root (2 units), the products with
 factor, gain, cosine / sine and scale and one sum: 20 roundings of 2^-24 at most, of values up to the pair's length - below 2^-19 of it.
 """
-import ctypes
 import math
 
 import pytest
@@ -204,23 +203,24 @@ def test_refusals_on_the_gpu(pkg, cuda):
 def test_refusals_without_a_gpu(pkg):
     """The entry point looks at everything on the host before anything touches a GPU."""
     L, at = pkg._lib, 1 << 20
-    P = pkg.ops.QK_PART
+    S = pkg.ops.QK_NORM_ROPE
 
-    def call(part=(), n=1, tokens=4, D=64, xd=L.BF16, yd=L.BF16, gd=L.F32, eps=1e-6, rot=at, rows=4, R=64, pos=None, n_pos=0, records=None):
+    def call(part=(), n=1, tokens=4, D=64, xd=L.BF16, yd=L.BF16, gd=L.F32, eps=1e-6, rot=at, rows=4, R=64, pos=0, n_pos=0):
         f = dict(x=at, y=at, gain=0, heads=2, xt=128, xh=64, yt=128, yh=64, gh=0, scale=1.0)
         f.update(part)
-        return L.lib().aeris_qk_norm_rope_fwd(P.pack(*f.values()) * n if records is None else records, n, tokens, D, xd, yd, gd, 1, eps, rot, rows, R, 0,
-                                              pos, n_pos, None)
+        a = S.pack(*f.values(), *f.values(), rot, pos, tokens, D, xd, yd, gd, 1, 0, rows, R, n_pos, n, eps)
+        return L.lib().aeris_qk_norm_rope_fwd(a, None)
 
     for kw in [dict(part={"x": 0}), dict(part={"y": 0}), dict(part={"x": at + 8}), dict(part={"gain": at + 4}), dict(part={"xt": 129}),
                dict(part={"yh": 4}), dict(part={"gain": at, "gh": 2}), dict(part={"heads": 0}), dict(tokens=0), dict(tokens=-1), dict(xd=2), dict(yd=-1),
-               dict(gd=5), dict(eps=-1.0), dict(eps=float("nan")), dict(rot=None), dict(rot=at + 4), dict(rows=0), dict(rows=2 ** 31),
+               dict(gd=5), dict(eps=-1.0), dict(eps=float("nan")), dict(rot=0), dict(rot=at + 4), dict(rows=0), dict(rows=2 ** 31),
                dict(pos=at, n_pos=0), dict(pos=at + 2, n_pos=4), dict(n=0), dict(n=3)]:
         assert call(**kw) == L.EINVAL, kw
         assert "aeris_qk_norm_rope_fwd" in L.last_error()
-    for kw in [dict(D=48), dict(D=256), dict(R=8), dict(R=80), dict(R=-16), dict(tokens=2 ** 31 - 1), dict(part={"heads": 40000}), dict(part={"heads": 32767}, n=3)]:
-        assert call(**kw) in (L.EUNSUPPORTED, L.EINVAL), kw
-    assert L.lib().aeris_qk_norm_rope_fwd(None, 1, 4, 64, 0, 0, 0, 1, 1e-6, None, 0, 0, 0, None, 0, None) == L.EINVAL
+    for kw in [dict(D=48), dict(D=256), dict(D=2 ** 32 + 64), dict(R=8), dict(R=80), dict(R=-16), dict(R=2 ** 32), dict(tokens=2 ** 31 - 1),
+               dict(part={"heads": 40000}), dict(part={"heads": 32768}, n=2)]:
+        assert call(**kw) == L.EUNSUPPORTED, kw
+    assert L.lib().aeris_qk_norm_rope_fwd(None, None) == L.EINVAL
     with pytest.raises(RuntimeError, match="GPU"):
         pkg.ops.qk_norm_rope(torch.zeros(4, 2, 64, dtype=torch.bfloat16))
-    assert ctypes.sizeof(ctypes.c_void_p) == 8 and P.size == 80
+    assert S.size == 272
