@@ -402,9 +402,11 @@ int aeris_qk_norm_rope_fwd(const aeris_qk_norm_rope* a, void* stream) {
     const aeris_qk_part& p = a->parts[i];
     if (!p.x || !p.y || p.heads <= 0) return fail(AERIS_EINVAL, "%s: x/y is NULL or heads is not positive", who);
     const int ex = a->x_dtype == AERIS_F32 ? 4 : 8, ey = a->y_dtype == AERIS_F32 ? 4 : 8, eg = a->gain_dtype == AERIS_F32 ? 4 : 8;
-    if (!aligned16(p.x) || !aligned16(p.y) || (p.gain && !aligned16(p.gain)) || p.x_token_stride % ex || p.x_head_stride % ex ||
-        p.y_token_stride % ey || p.y_head_stride % ey || p.gain_head_stride % eg)
-      return fail(AERIS_EINVAL, "%s: x, y and gain must be 16-byte aligned, their strides multiples of 16 bytes", who);
+    const int64_t n[2] = {a->tokens, p.heads};
+    bool ok = p.x_stride[2] == 1 && p.y_stride[2] == 1;
+    for (int d = 0; d < 2; ++d) ok = ok && (n[d] == 1 || (p.x_stride[d] % ex == 0 && p.y_stride[d] % ey == 0));
+    if (!ok || !aligned16(p.x) || !aligned16(p.y) || (p.gain && !aligned16(p.gain)) || p.gain_head_stride % eg)
+      return fail(AERIS_EINVAL, "%s: x, y and gain must be 16-byte aligned, the elements of a head contiguous and the other strides multiples of 16 bytes", who);
     if (p.heads > 32767) return fail(AERIS_EUNSUPPORTED, "%s: more than 32767 heads", who);
     heads += p.heads;
   }
@@ -415,50 +417,66 @@ int aeris_qk_norm_rope_fwd(const aeris_qk_norm_rope* a, void* stream) {
 }
 
 namespace {
-// sizes of a cross attention call, for the workspace's size and the call
-int check_cross_sizes(const char* who, const aeris_cross_attention* a) {
+// sizes of a cross attention call, for the workspace's size and the call; c: what the launch takes, strides of dimensions with one entry 0
+int check_cross_sizes(const char* who, const aeris_cross_attention* a, aeris::CrossArgs* c) {
   if (!a) return fail(AERIS_EINVAL, "%s: NULL", who);
   if (a->B <= 0 || a->Nq <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->Nk < 0 || a->Np < 0)
     return fail(AERIS_EINVAL, "%s: B, Nq, heads, kv_heads must be positive, Nk and Np not negative", who);
   if (a->heads % a->kv_heads) return fail(AERIS_EINVAL, "%s: %lld heads do not divide among %lld key heads", who, (long long)a->heads, (long long)a->kv_heads);
-  if (!aeris::cross_attention_supported(a->head_dim))
-    return fail(AERIS_EUNSUPPORTED, "%s: head_dim %lld (need 32, 64 or 128)", who, (long long)a->head_dim);
+  if ((a->kv_batch != 1 && a->kv_batch != a->B) || (a->lengths && a->n_lengths != 1 && a->n_lengths != a->B) ||
+      (a->key_mask && a->mask_batch != 1 && a->mask_batch != a->B))
+    return fail(AERIS_EINVAL, "%s: kv_batch, n_lengths and mask_batch must be 1 or B", who);
+  if (!aeris::cross_attention_supported(a->head_dim)) return fail(AERIS_EUNSUPPORTED, "%s: head_dim %lld (need 32, 64 or 128)", who, (long long)a->head_dim);
   const int64_t most = 0x7fffffffLL;
   if (a->B > most || a->Nq > most || a->heads > 65535 || a->Nk > most - 4096 || a->Np > most - 4096 || a->B * a->Nq > most ||
       a->B * a->Nq * a->heads > most / 2)
     return fail(AERIS_EUNSUPPORTED, "%s: more than 2^30 rows (B * Nq * heads), 2^31-4097 keys or 65535 heads", who);
+  aeris::CrossArgs r{};
+  r.q = a->q; r.k = a->k; r.v = a->v; r.prefix_k = a->prefix_k; r.prefix_v = a->prefix_v; r.out = a->out; r.lengths = a->lengths; r.key_mask = a->key_mask;
+  r.B = a->B; r.Nq = a->Nq; r.heads = a->heads; r.kv_heads = a->kv_heads; r.head_dim = a->head_dim; r.Nk = a->Nk; r.Np = a->Np;
+  auto stride = [](int64_t n, int64_t s) { return n > 1 ? s : 0; };
+  r.q_batch_stride = stride(a->B, a->q_stride[0]); r.q_row_stride = stride(a->Nq, a->q_stride[1]); r.q_head_stride = stride(a->heads, a->q_stride[2]);
+  r.k_batch_stride = stride(a->kv_batch, a->k_stride[0]); r.k_row_stride = stride(a->Nk, a->k_stride[1]); r.k_head_stride = stride(a->kv_heads, a->k_stride[2]);
+  r.v_batch_stride = stride(a->kv_batch, a->v_stride[0]); r.v_row_stride = stride(a->Nk, a->v_stride[1]); r.v_head_stride = stride(a->kv_heads, a->v_stride[2]);
+  r.prefix_k_row_stride = stride(a->Np, a->prefix_k_stride[0]); r.prefix_k_head_stride = stride(a->kv_heads, a->prefix_k_stride[1]);
+  r.prefix_v_row_stride = stride(a->Np, a->prefix_v_stride[0]); r.prefix_v_head_stride = stride(a->kv_heads, a->prefix_v_stride[1]);
+  r.lengths_stride = a->n_lengths > 1 ? 1 : 0; r.mask_batch_stride = stride(a->mask_batch, a->mask_stride);
+  r.q_prescaled = a->q_prescaled; r.scale = a->scale;
+  *c = r;
   return AERIS_OK;
 }
 }  // namespace
 
 int64_t aeris_cross_attention_workspace_bytes(const aeris_cross_attention* a) {
-  if (check_cross_sizes("aeris_cross_attention_workspace_bytes", a)) return 0;
-  return aeris::cross_attention_workspace_bytes(*a);
+  aeris::CrossArgs c;
+  if (check_cross_sizes("aeris_cross_attention_workspace_bytes", a, &c)) return 0;
+  return aeris::cross_attention_workspace_bytes(c);
 }
 
 int aeris_cross_attention_fwd(const aeris_cross_attention* a, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* who = "aeris_cross_attention_fwd";
-  if (int rc = check_cross_sizes(who, a)) return rc;
-  if (!a->q || !a->out || (a->Nk > 0 && (!a->k || !a->v)) || (a->Np > 0 && (!a->prefix_k || !a->prefix_v)))
+  aeris::CrossArgs c;
+  if (int rc = check_cross_sizes(who, a, &c)) return rc;
+  if (!c.q || !c.out || (c.Nk > 0 && (!c.k || !c.v)) || (c.Np > 0 && (!c.prefix_k || !c.prefix_v)))
     return fail(AERIS_EINVAL, "%s: q, k, v, prefix or out is NULL", who);
-  const int64_t strides[] = {a->q_batch_stride, a->q_row_stride, a->q_head_stride, a->k_batch_stride, a->k_row_stride, a->k_head_stride,
-                             a->v_batch_stride, a->v_row_stride, a->v_head_stride, a->prefix_k_row_stride, a->prefix_k_head_stride,
-                             a->prefix_v_row_stride, a->prefix_v_head_stride};
-  for (int64_t s : strides)
-    if (s < 0 || s % 8) return fail(AERIS_EINVAL, "%s: strides must be multiples of 8 elements and not negative", who);
-  if (!aligned16(a->q) || !aligned16(a->out) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->prefix_k) || !aligned16(a->prefix_v))
-    return fail(AERIS_EINVAL, "%s: q, k, v, prefix and out must be 16-byte aligned", who);
-  for (int64_t s : {a->k_row_stride, a->v_row_stride, a->prefix_k_row_stride, a->prefix_v_row_stride})
+  bool ok = a->q_stride[3] == 1 && a->k_stride[3] == 1 && a->v_stride[3] == 1 && (c.Np == 0 || (a->prefix_k_stride[2] == 1 && a->prefix_v_stride[2] == 1));
+  for (int64_t s : {c.q_batch_stride, c.q_row_stride, c.q_head_stride, c.k_batch_stride, c.k_row_stride, c.k_head_stride, c.v_batch_stride, c.v_row_stride,
+                    c.v_head_stride, c.prefix_k_row_stride, c.prefix_k_head_stride, c.prefix_v_row_stride, c.prefix_v_head_stride})
+    ok = ok && s >= 0 && s % 8 == 0;
+  for (const void* p : {c.q, c.k, c.v, c.prefix_k, c.prefix_v, (const void*)c.out}) ok = ok && aligned16(p);
+  if (!ok)
+    return fail(AERIS_EINVAL, "%s: q, k, v, prefix and out must be 16-byte aligned, the elements of a head contiguous and the other strides multiples of 8, "
+                              "not negative", who);
+  for (int64_t s : {c.k_row_stride, c.v_row_stride, c.prefix_k_row_stride, c.prefix_v_row_stride})
     if (s >= (1 << 23)) return fail(AERIS_EUNSUPPORTED, "%s: rows of k and v 2^23 elements apart or more", who);
-  if (a->lengths && ((a->lengths_stride != 0 && a->lengths_stride != 1) || (reinterpret_cast<uintptr_t>(a->lengths) & 3u)))
-    return fail(AERIS_EINVAL, "%s: lengths must be 4-byte aligned, its stride 0 or 1", who);
-  if (a->key_mask && a->mask_batch_stride < 0) return fail(AERIS_EINVAL, "%s: mask_batch_stride must not be negative", who);
-  if (!a->q_prescaled && !(a->scale > 0.0 && a->scale < 1e30)) return fail(AERIS_EINVAL, "%s: scale must be positive", who);
-  const int64_t need = aeris::cross_attention_workspace_bytes(*a);
+  if (c.lengths && (reinterpret_cast<uintptr_t>(c.lengths) & 3u)) return fail(AERIS_EINVAL, "%s: lengths must be 4-byte aligned", who);
+  if (c.key_mask && c.mask_batch_stride < 0) return fail(AERIS_EINVAL, "%s: mask_stride must not be negative", who);
+  if (!c.q_prescaled && !(c.scale > 0.0 && c.scale < 1e30)) return fail(AERIS_EINVAL, "%s: scale must be positive", who);
+  const int64_t need = aeris::cross_attention_workspace_bytes(c);
   if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
     return fail(AERIS_EINVAL, "%s: workspace must be 16-byte aligned and hold %lld bytes (got %lld)", who, (long long)need, (long long)workspace_bytes);
   if (int rc = ensure_init(stream, true)) return rc;
-  hipError_t e = aeris::cross_attention_launch(*a, workspace, reinterpret_cast<hipStream_t>(stream));
+  hipError_t e = aeris::cross_attention_launch(c, workspace, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "aeris_cross_attention_fwd launch");
   return AERIS_OK;
 }

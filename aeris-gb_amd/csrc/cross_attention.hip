@@ -64,7 +64,8 @@ __device__ __forceinline__ int v_swizzle(int row) { return HD == 128 ? 2 * (row 
 __device__ __forceinline__ uint64_t first_keys(int n) { return n >= KC ? ~0ull : (1ull << n) - 1; }
 
 // A wave's 16 QN rows: queries, sums, and what a chunk in LDS does to them.
-template <int HD, int QN, bool SCALED>
+// SUM: the row sums by the matrix cores too (a product with ones), four VALU operations fewer per 8 weights and one MFMA more per 4 to 8.
+template <int HD, int QN, bool SCALED, bool SUM>
 struct Rows {
   static constexpr int KS = HD / 32;  // k32 steps of K Q^T
   static constexpr int KB = KC / 16;  // blocks of 16 keys per chunk
@@ -72,9 +73,8 @@ struct Rows {
   typedef __attribute__((address_space(3))) const unsigned char* lds_cptr;
 
   bf16x8 qf[QN][KS];  // B operand: lane = row, 8 consecutive elements per k32 step
-  bool valid[QN];
-  int64_t out_row[QN];
   float m[QN], l[QN];
+  f32x4 lv[QN];     // SUM: the row sum so far, in each of the four
   f32x4 o[QN][DB];  // o[n][db][i] = O[row 16 n + l15][16 db + 4 q4 + i]
   lds_cptr k_lane[KS];
   uint32_t v_tr[DB];
@@ -98,16 +98,21 @@ struct Rows {
     }
   }
 
-  __device__ __forceinline__ void load_q(const CrossParams& p, int rows, int member, int hk, int row0, int lane, bf16x8 (&f)[QN][KS]) {
+  // the rows from row0 of a unit: where their results go (in units of a head's row), and their queries into `f`
+  __device__ __forceinline__ void load_q(const CrossParams& p, int rows, int member, int hk, int row0, int lane, int64_t (&to)[QN], bf16x8 (&f)[QN][KS]) const {
 #pragma unroll
     for (int n = 0; n < QN; ++n) {
       int r = row0 + n * 16 + (lane & 15);
-      valid[n] = r < rows;
-      if (!valid[n]) r = rows - 1;
-      const int bb = r / p.rows_m, rm = r - bb * p.rows_m;
-      const int query = rm / p.group, head = hk * p.group + rm - query * p.group;
-      const int64_t b = member + bb;
-      out_row[n] = (b * p.Nq + query) * p.heads + head;
+      if (r >= rows) r = rows - 1;
+      int query = r, head = hk;
+      int64_t b = member;
+      if (p.group != 1 || rows != p.rows_m) {  // (uniform; two divisions)
+        const int bb = r / p.rows_m, rm = r - bb * p.rows_m;
+        query = rm / p.group;
+        head = hk * p.group + rm - query * p.group;
+        b += bb;
+      }
+      to[n] = (b * p.Nq + query) * p.heads + head;
       const uint16_t* qp = p.q + b * p.q_batch + query * p.q_row + head * p.q_head + q4 * 8;
 #pragma unroll
       for (int s = 0; s < KS; ++s) f[n][s] = *reinterpret_cast<const bf16x8*>(qp + s * 32);
@@ -119,6 +124,7 @@ struct Rows {
     for (int n = 0; n < QN; ++n) {
       m[n] = -3.0e38f;  // (finite: a chunk all of whose logits are -infinity leaves it where it is)
       l[n] = 0.f;
+      lv[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[n][db] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -128,6 +134,30 @@ struct Rows {
   // m, accumulated output and sum rescaled whenever a maximum moves.
   template <bool FAST>
   __device__ __forceinline__ void chunk(uint32_t at, uint64_t keys) {
+    // PV step of 32 keys: k slots 0-3 <-> keys 32 step + 4 q4 + (0..3), slots 4-7 <-> 16 more.  The fragments of half of the row
+    // blocks are read ahead of the MFMAs of the half before.
+    constexpr int DH = DB / 2, PARTS = KC / 32 * 2;
+    bf16x8 vfb[2][DH];
+    TrFrag vtr[2][DH];
+    auto load_v = [&](int part, int slot) {
+#pragma unroll
+      for (int d = 0; d < DH; ++d) {
+        const uint32_t a0 = v_tr[(part & 1) * DH + d] + at + (part >> 1) * 32 * (HD * 2);
+        vtr[slot][d].lo = lds_read_tr16_b64<0>(a0);
+        vtr[slot][d].hi = lds_read_tr16_b64<16 * (HD * 2)>(a0);
+      }
+    };
+    auto v_ready = [&](int slot) {
+      if constexpr (DH == 4) lds_tr_wait(vtr[slot][0], vtr[slot][1 % DH], vtr[slot][2 % DH], vtr[slot][3 % DH]);
+      else if constexpr (DH == 2) lds_tr_wait(vtr[slot][0], vtr[slot][1 % DH]);
+      else lds_tr_wait(vtr[slot][0]);
+#pragma unroll
+      for (int d = 0; d < DH; ++d) vfb[slot][d] = tr_frag_value(vtr[slot][d]);
+    };
+    // (ahead of the MFMAs: behind them the reads could return into registers that the first of an accumulator's MFMAs is still writing)
+    load_v(0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+
     f32x4 acc[QN][KB];
     // ---- S^T: acc[n][kb][i] = logit of key 16 kb + 4 q4 + i, row 16 n + l15; K fragments are read two ahead of their MFMAs
     {
@@ -150,7 +180,9 @@ struct Rows {
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if (keys != ~0ull) {  // keys that do not take part
+    // Keys that do not take part: their rows of K and V are zeros, so that FAST, where P is then 1, has them in the sum alone (sums() takes
+    // them out again)
+    if (!FAST && keys != ~0ull) {
       const uint64_t mine = keys >> (4 * q4);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
@@ -161,28 +193,6 @@ struct Rows {
             for (int n = 0; n < QN; ++n) acc[n][kb][i] = -INFINITY;
           }
     }
-
-    // PV step of 32 keys: k slots 0-3 <-> keys 32 step + 4 q4 + (0..3), slots 4-7 <-> 16 more.  The fragments of half of the row
-    // blocks are read ahead of the MFMAs of the half before.
-    constexpr int DH = DB / 2, PARTS = KC / 32 * 2;
-    bf16x8 vfb[2][DH];
-    TrFrag vtr[2][DH];
-    auto load_v = [&](int part, int slot) {
-#pragma unroll
-      for (int d = 0; d < DH; ++d) {
-        const uint32_t a0 = v_tr[(part & 1) * DH + d] + at + (part >> 1) * 32 * (HD * 2);
-        vtr[slot][d].lo = lds_read_tr16_b64<0>(a0);
-        vtr[slot][d].hi = lds_read_tr16_b64<16 * (HD * 2)>(a0);
-      }
-    };
-    auto v_ready = [&](int slot) {
-      if constexpr (DH == 4) lds_tr_wait(vtr[slot][0], vtr[slot][1 % DH], vtr[slot][2 % DH], vtr[slot][3 % DH]);
-      else if constexpr (DH == 2) lds_tr_wait(vtr[slot][0], vtr[slot][1 % DH]);
-      else lds_tr_wait(vtr[slot][0]);
-#pragma unroll
-      for (int d = 0; d < DH; ++d) vfb[slot][d] = tr_frag_value(vtr[slot][d]);
-    };
-    load_v(0, 0);
 
     if (!FAST) {
 #pragma unroll
@@ -199,6 +209,7 @@ struct Rows {
         if (__builtin_amdgcn_ballot_w64(m_new > m[n]) != 0) {
           const float alpha = __builtin_amdgcn_exp2f(m[n] - m_new);
           l[n] *= alpha;
+          if (SUM) lv[n] *= alpha;
 #pragma unroll
           for (int db = 0; db < DB; ++db) o[n][db] *= alpha;
           m[n] = m_new;
@@ -206,6 +217,7 @@ struct Rows {
       }
     }
 
+    const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
     uint32_t pkb[2][QN][4];
     auto p_of = [&](float a, int n) {
       return __builtin_amdgcn_exp2f(SCALED ? (FAST ? a * q_mul : fmaf(a, q_mul, -m[n])) : FAST ? a : a - m[n]);
@@ -215,7 +227,7 @@ struct Rows {
       for (int h = 0; h < 4; ++h) {
         const f32x4& a = acc[n][2 * step + (h >> 1)];
         pkb[step & 1][n][h] = pack_bf16x2(p_of(a[2 * (h & 1)], n), p_of(a[2 * (h & 1) + 1], n));
-        l[n] = dot2_ones(pkb[step & 1][n][h], l[n]);
+        if (!SUM) l[n] = dot2_ones(pkb[step & 1][n][h], l[n]);
       }
     };
 #pragma unroll
@@ -237,35 +249,42 @@ struct Rows {
           const bf16x8 pf = __builtin_bit_cast(bf16x8, u32x4{pkb[step & 1][n][0], pkb[step & 1][n][1], pkb[step & 1][n][2], pkb[step & 1][n][3]});
           f32x4& od = o[n][(part & 1) * DH + d];
           od = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vfb[part & 1][d], pf, od, 0, 0, 0);
+          if (SUM && (part & 1) && d == 0) lv[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf, lv[n], 0, 0, 0);
         }
     }
     __builtin_amdgcn_sched_barrier(0);
   }
 
-  // the sums over a row's four lanes; whether any row's left the range in which exp2 needs no maximum (or is not a number)
-  __device__ __forceinline__ bool out_of_range() {
+  // The rows' sums, `idle` keys of the chunks that did not take part taken out of them.  Whether any row's left the range in which exp2 needs no
+  // maximum (or is not a number), or is so small beside the idle keys' ones that their difference says little.
+  __device__ __forceinline__ bool sums(int idle) {
     bool bad = false;
 #pragma unroll
     for (int n = 0; n < QN; ++n) {
-      l[n] += __shfl_xor(l[n], 16, 64);
-      l[n] += __shfl_xor(l[n], 32, 64);
-      bad = bad || !(l[n] >= 0x1p-40f && l[n] <= 0x1p100f);
+      if (SUM) {
+        l[n] = lv[n][0];
+      } else {
+        l[n] += __shfl_xor(l[n], 16, 64);
+        l[n] += __shfl_xor(l[n], 32, 64);
+      }
+      l[n] -= (float)idle;
+      bad = bad || !(l[n] >= 0x1p-40f && l[n] >= 0x1p-10f * (float)idle && l[n] <= 0x1p100f);
     }
     return __builtin_amdgcn_ballot_w64(bad) != 0;
   }
 
   // normalise (a row without any key is zeros), 8 consecutive elements a lane and store
-  __device__ __forceinline__ void store(uint16_t* out) const {
+  __device__ __forceinline__ void store(uint16_t* out, const int64_t (&to)[QN], int row0, int rows, int lane) const {
 #pragma unroll
     for (int n = 0; n < QN; ++n) {
       const float inv = l[n] == 0.f ? 0.f : __builtin_amdgcn_rcpf(l[n]);
-      uint16_t* op = out + out_row[n] * HD + 16 * (q4 & 1) + 8 * (q4 >> 1);
+      uint16_t* op = out + to[n] * HD + 16 * (q4 & 1) + 8 * (q4 >> 1);
 #pragma unroll
       for (int m2 = 0; m2 < DB / 2; ++m2) {
         const f32x4 a = o[n][2 * m2] * inv, c = o[n][2 * m2 + 1] * inv;
         const auto rx = __builtin_amdgcn_permlane16_swap(pack_bf16x2(a[0], a[1]), pack_bf16x2(c[0], c[1]), false, false);
         const auto ry = __builtin_amdgcn_permlane16_swap(pack_bf16x2(a[2], a[3]), pack_bf16x2(c[2], c[3]), false, false);
-        if (valid[n]) *reinterpret_cast<u32x4*>(op + m2 * 32) = u32x4{rx[0], ry[0], rx[1], ry[1]};
+        if (row0 + n * 16 + (lane & 15) < rows) *reinterpret_cast<u32x4*>(op + m2 * 32) = u32x4{rx[0], ry[0], rx[1], ry[1]};
       }
     }
   }
@@ -372,21 +391,18 @@ __device__ __forceinline__ uint64_t uniform64(uint64_t x) {
   return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)x);
 }
 
-template <int N>
-__device__ __forceinline__ void wait_loads_and_barrier() {  // all but the wave's N youngest loads have landed, and so they have in every wave
-  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
-}
-
 }  // namespace
 
-template <int HD, int NWAVE, int NBUF, int QN, bool SPLIT, bool SCALED>
+// K and V in two buffers: a chunk is loaded while the one before is worked on.  (Three and four buffers: the same times, with a row block alone on its
+// CU too - a chunk takes a wave longer, 0.5 us and more, than its load.)
+template <int HD, int NWAVE, int QN, bool SPLIT, bool SCALED, bool SUM>
 __global__ void __launch_bounds__(64 * NWAVE) __attribute__((amdgpu_waves_per_eu(2)))
 cross_attention_kernel(CrossParams p) {
   using Load = Loader<HD, NWAVE>;
-  constexpr int BYTES = Load::BYTES, V_BASE = NBUF * BYTES;
+  constexpr int BYTES = Load::BYTES, V_BASE = 2 * BYTES;
   constexpr int QW = 16 * QN, QB = QW * NWAVE;  // rows per wave and workgroup
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  uint64_t* const words = reinterpret_cast<uint64_t*>(smem + 2 * NBUF * BYTES);
+  uint64_t* const words = reinterpret_cast<uint64_t*>(smem + 4 * BYTES);
   const uint32_t smem_addr = lds_byte_address(smem);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
@@ -410,15 +426,17 @@ cross_attention_kernel(CrossParams p) {
   Keys keys(p, t, member, hk);
   int c0 = 0, c1 = keys.chunks;
   if (SPLIT) {
-    c0 = (int)((int64_t)keys.chunks * split / t.splits);
-    c1 = (int)((int64_t)keys.chunks * (split + 1) / t.splits);
+    const int all = (t.Np + KC - 1) / KC + (t.Nk + KC - 1) / KC, each = (all + t.splits - 1) / t.splits;  // (the same for members of any length)
+    c0 = each * split < keys.chunks ? each * split : keys.chunks;
+    c1 = c0 + each < keys.chunks ? c0 + each : keys.chunks;
   }
   const int nch = c1 - c0;
 
   const int row0 = qb * QB + wave * QW;
   const bool wave_active = row0 < t.rows;  // wave-uniform: a wave without rows only loads and keeps the barriers
-  Rows<HD, QN, SCALED> rows(smem, V_BASE, lane, p.q_mul);
+  Rows<HD, QN, SCALED, SUM> rows(smem, V_BASE, lane, p.q_mul);
   Load load(lane, wave);
+  int64_t to[QN];
 
   const bool masked = p.mask && t.Nk > 0;
   if (masked) {
@@ -430,36 +448,34 @@ cross_attention_kernel(CrossParams p) {
     if (masked) w &= uniform64(words[j]);
     return w;
   };
-  uint64_t kk[NBUF];  // of the chunks in the buffers
+  uint64_t kk[2];  // of the chunks in the buffers
   auto issue = [&](int j, int buf) {
     kk[buf] = word_of(j);
     load.issue(p, t, hk, lane, keys, c0 + j, kk[buf], smem_addr + buf * BYTES, smem_addr + V_BASE + buf * BYTES);
   };
   bool any = false;  // whether any key took part (uniform)
+  int idle = 0;      // keys that did not, of chunks with keys that did
 
   auto sweep = [&](auto fast_tag) {
     constexpr bool FAST = decltype(fast_tag)::value;
     keys.seek(p, t, hk, c0);
     load.rows(lane, keys);
-#pragma unroll
-    for (int u = 0; u < NBUF - 1; ++u)
-      if (u < nch) issue(u, u);
-    if (FAST) rows.load_q(p, t.rows, member, hk, row0, lane, rows.qf);  // (behind the first chunks' loads, which take longer)
+    if (nch > 0) issue(0, 0);
+    if (FAST) rows.load_q(p, t.rows, member, hk, row0, lane, to, rows.qf);
     rows.reset();
-    // vmcnt(0), in a form that the compiler takes into account: a wait of its own for the queries inside the loop would be one for all chunks
-    if (FAST) __builtin_amdgcn_s_waitcnt(0x0F70);
-    for (int j0 = 0; j0 < nch; j0 += NBUF) {
+    if (FAST) __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the compiler knows the queries to be there (inside the loop it would wait for the chunks too)
+    for (int j0 = 0; j0 < nch; j0 += 2) {
 #pragma unroll
-      for (int u = 0; u < NBUF; ++u) {
+      for (int u = 0; u < 2; ++u) {
         const int j = j0 + u;
         if (j >= nch) break;
-        // chunk j has landed; younger ones, up to NBUF - 2 of them, may be on their way.  The barrier says so for every wave's part of it, and
-        // that every wave is done with chunk j - 1, whose buffer chunk j + NBUF - 1 goes to
-        if (NBUF > 2 && j + NBUF - 2 < nch) wait_loads_and_barrier<(NBUF - 2) * 2 * Load::LOADS>();
-        else wait_loads_and_barrier<0>();
-        if (j + NBUF - 1 < nch) issue(j + NBUF - 1, (u + NBUF - 1) % NBUF);
+        // this wave's part of chunk j has landed; behind the barrier every wave's has, and every wave is done with chunk j - 1, whose
+        // buffer chunk j + 1 goes to
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        if (j + 1 < nch) issue(j + 1, u ^ 1);
         if (kk[u] != 0) {
           any = true;
+          if (FAST) idle += KC - __builtin_popcountll(kk[u]);
           if (wave_active) rows.template chunk<FAST>(u * BYTES, kk[u]);
         }
       }
@@ -472,29 +488,100 @@ cross_attention_kernel(CrossParams p) {
     int* const redo = reinterpret_cast<int*>(smem);
     if (tid == 0) *redo = 0;
     __syncthreads();
-    if (rows.out_of_range() && any && wave_active && lane == 0) *redo = 1;
+    if (rows.sums(idle) && any && wave_active && lane == 0) *redo = 1;
     __syncthreads();
     online = __builtin_amdgcn_readfirstlane(*redo) != 0;
     if (online) {
       __syncthreads();
       sweep(std::false_type{});
-      rows.out_of_range();
+      rows.sums(0);
     }
   }
   if (!SPLIT) {
-    rows.store(p.out);
+    rows.store(p.out, to, row0, t.rows, lane);
     return;
   }
 #pragma unroll
   for (int n = 0; n < QN; ++n) {
-    const int64_t at = ((int64_t)split * t.members * p.kv_heads + bh) * t.rows + row0 + n * 16 + (lane & 15);
-    if (!rows.valid[n]) continue;
+    const int row = row0 + n * 16 + (lane & 15);
+    const int64_t at = ((int64_t)split * t.members * p.kv_heads + bh) * t.rows + row;
+    if (row >= t.rows) continue;
     if (rows.q4 == 0) {
       t.ml[2 * at] = online ? rows.m[n] : 0.f;
       t.ml[2 * at + 1] = rows.l[n];
     }
 #pragma unroll
-    for (int db = 0; db < HD / 16; ++db) *reinterpret_cast<f32x4*>(t.o + at * HD + 16 * db + 4 * rows.q4) = rows.o[n][db];
+    for (int db = 0; db < HD / 16; ++db)  // (not to be held in L2, which a kernel's end empties: 18.2 -> 15.2 us where the parts are 16 MB)
+      __builtin_nontemporal_store(rows.o[n][db], reinterpret_cast<f32x4*>(t.o + at * HD + 16 * db + 4 * rows.q4));
+  }
+}
+
+// Few keys, many rows: the workgroup's unit stays in LDS, its waves walk down the row blocks, each at its own pace: no barrier behind the
+// first, a block's queries are fetched while the one before is worked on.  Task::qblks is the number of workgroups of a unit.
+template <int HD, int NWAVE, int QN, bool SCALED, bool SUM>
+__global__ void __launch_bounds__(64 * NWAVE) __attribute__((amdgpu_waves_per_eu(2)))
+cross_attention_resident_kernel(CrossParams p, int max_chunks) {
+  using Load = Loader<HD, NWAVE>;
+  constexpr int BYTES = Load::BYTES, QW = 16 * QN;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const uint32_t v_base = (uint32_t)max_chunks * BYTES, smem_addr = lds_byte_address(smem);
+  uint64_t* const words = reinterpret_cast<uint64_t*>(smem + 2 * v_base);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Task& t = p.task[0];
+  const int unit = blockIdx.x % t.units, part = blockIdx.x / t.units;
+  const int member = unit / p.kv_heads, hk = unit - member * p.kv_heads;
+  Keys keys(p, t, member, hk);
+  const int nch = keys.chunks;
+  if (p.mask && t.Nk > 0) {
+    mask_words<NWAVE>(p.mask + member * p.mask_batch, keys, 0, nch, words, lane, wave);
+    __syncthreads();
+  }
+  Rows<HD, QN, SCALED, SUM> rows(smem, v_base, lane, p.q_mul);
+  Load load(lane, wave);
+  const int step = t.qblks * NWAVE * QW;
+  int row0 = (part * NWAVE + wave) * QW;
+  int64_t to[QN], to_next[QN];
+  bf16x8 next[QN][HD / 32];
+  if (row0 < t.rows) rows.load_q(p, t.rows, member, hk, row0, lane, to_next, next);
+  keys.seek(p, t, hk, 0);
+  load.rows(lane, keys);
+  int idle = 0;
+  auto word_of = [&](int c) {
+    const int n = c < keys.prefix_chunks ? t.Np - c * KC : keys.own - (c - keys.prefix_chunks) * KC;
+    uint64_t w = first_keys(n);
+    if (p.mask && t.Nk > 0) w &= uniform64(words[c]);
+    return w;
+  };
+  for (int c = 0; c < nch; ++c) {
+    const uint64_t w = word_of(c);
+    idle += KC - __builtin_popcountll(w);
+    load.issue(p, t, hk, lane, keys, c, w, smem_addr + c * BYTES, smem_addr + v_base + c * BYTES);
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __syncthreads();
+  const bool any = idle < nch * KC;
+
+  for (; row0 < t.rows; row0 += step) {
+#pragma unroll
+    for (int n = 0; n < QN; ++n) {
+      to[n] = to_next[n];
+#pragma unroll
+      for (int s = 0; s < HD / 32; ++s) rows.qf[n][s] = next[n][s];
+    }
+    if (row0 + step < t.rows) rows.load_q(p, t.rows, member, hk, row0 + step, lane, to_next, next);
+    rows.reset();
+    if (any) {
+      for (int c = 0; c < nch; ++c) rows.template chunk<true>(c * BYTES, ~0ull);
+      if (rows.sums(idle)) {
+        rows.reset();
+        for (int c = 0; c < nch; ++c) {
+          const uint64_t w = word_of(c);
+          if (w != 0) rows.template chunk<false>(c * BYTES, w);
+        }
+        rows.sums(0);
+      }
+    }
+    rows.store(p.out, to, row0, t.rows, lane);
   }
 }
 
@@ -506,58 +593,88 @@ namespace {
 struct JoinParams {
   Task task[2];
   uint16_t* out;
+  int64_t rows;  // (member, query, head)
   int Nq, heads, kv_heads, group, rows_m;
 };
 
 }  // namespace
 
-// out[row] = sum over the parts of 2^(m - max m) o / sum of 2^(m - max m) l.  A thread has 4 elements and every SPth part.
-template <int HD>
-__global__ void __launch_bounds__(256) cross_attention_join_kernel(JoinParams p) {
-  constexpr int CT = HD / 4, SP = 256 / CT;
-  __shared__ f32x4 so[SP][CT];
-  __shared__ float sm[SP], sl[SP];
-  const int c = threadIdx.x % CT, sp = threadIdx.x / CT;
-  const int64_t row = blockIdx.x;  // (member, query, head)
-  const int head = (int)(row % p.heads);
-  const int64_t bq = row / p.heads;
-  const int query = (int)(bq % p.Nq), b = (int)(bq / p.Nq);
-  const int hk = head / p.group, rm = query * p.group + head - hk * p.group;
+// out[row] = sum over the parts of 2^(m - max m) o / sum of 2^(m - max m) l.  WPR waves do a row, each every WPR-th part: lane i looks at part i's
+// maximum and sum, the weights then go round by lane exchange, and HD / 4 lanes read a part's row, 64 / (HD / 4) parts at a time.  What it costs is the
+// latency of two reads behind one another.
+template <int HD, int WPR>
+__global__ void __launch_bounds__(WPR > 4 ? 64 * WPR : 256) cross_attention_join_kernel(JoinParams p) {
+  constexpr int CT = HD / 4, SUB = 64 / CT, NW = WPR > 4 ? WPR : 4;  // waves of a workgroup
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane % CT, sub = lane / CT, first_part = wave % WPR;
+  const int64_t row = (int64_t)blockIdx.x * (NW / WPR) + wave / WPR;
   float m = -3.0e38f, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  if (row < p.rows) {  // (wave-uniform)
+    const int head = (int)(row % p.heads);
+    const int64_t bq = row / p.heads;
+    const int query = (int)(bq % p.Nq), b = (int)(bq / p.Nq);
+    const int hk = head / p.group, rm = query * p.group + head - hk * p.group;
 #pragma unroll
-  for (int set = 0; set < 2; ++set) {
-    const Task& t = p.task[set];
-    const bool all = t.members == 1;  // a unit's rows are those of all members
-    const int64_t first = ((int64_t)(all ? 0 : b) * p.kv_heads + hk) * t.rows + (all ? b * p.rows_m : 0) + rm;
-    const int64_t step = (int64_t)t.members * p.kv_heads * t.rows;
-    for (int s = sp; s < t.splits; s += SP) {
-      const int64_t at = first + s * step;
-      const float pm = t.ml[2 * at], pl = t.ml[2 * at + 1];
-      const f32x4 po = *reinterpret_cast<const f32x4*>(t.o + at * HD + 4 * c);
-      if (pl == 0.f) continue;  // no key of this part
-      const float mn = fmaxf(m, pm), a0 = __builtin_amdgcn_exp2f(m - mn), a1 = __builtin_amdgcn_exp2f(pm - mn);
-      o = o * a0 + po * a1;
-      l = l * a0 + pl * a1;
-      m = mn;
+    for (int set = 0; set < 2; ++set) {
+      const Task& t = p.task[set];
+      const bool all = t.members == 1;  // a unit's rows are those of all members
+      const int64_t first = ((int64_t)(all ? 0 : b) * p.kv_heads + hk) * t.rows + (all ? b * p.rows_m : 0) + rm;
+      const int64_t step = (int64_t)t.members * p.kv_heads * t.rows;
+      for (int s0 = first_part; s0 < t.splits; s0 += 64 * WPR) {
+        const int n = (t.splits - s0 + WPR - 1) / WPR < 64 ? (t.splits - s0 + WPR - 1) / WPR : 64;
+        float pm = -3.0e38f, pl = 0.f;
+        if (lane < n) {
+          const float* at = t.ml + 2 * (first + (s0 + lane * WPR) * step);
+          pm = at[0];
+          pl = at[1];
+          if (pl == 0.f) pm = -3.0e38f;  // no key of this part
+        }
+        float mx = pm;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
+        const float mn = fmaxf(m, mx), a0 = __builtin_amdgcn_exp2f(m - mn), w = pl == 0.f ? 0.f : __builtin_amdgcn_exp2f(pm - mn);
+        m = mn;
+        l = l * a0 + wave_sum(w * pl);
+        o *= a0;
+#pragma unroll 4
+        for (int i = sub; i < 64; i += SUB) {
+          if (i - sub >= n) break;
+          const float wi = __shfl(w, i, 64);
+          const int64_t at = first + (s0 + (i < n ? i : n - 1) * WPR) * step;
+          const f32x4 po = *reinterpret_cast<const f32x4*>(t.o + at * HD + 4 * c);
+          // (a part without keys has written nothing)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] += wi == 0.f ? 0.f : po[e] * wi;
+        }
+      }
+    }
+#pragma unroll
+    for (int d = CT; d < 64; d *= 2)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], d, 64);
+  }
+  if (WPR > 1) {
+    __shared__ f32x4 so[NW][CT];
+    __shared__ float sm[NW], sl[NW];
+    if (sub == 0) so[wave][c] = o;
+    if (lane == 0) {
+      sm[wave] = m;
+      sl[wave] = l;
+    }
+    __syncthreads();
+    if (first_part != 0) return;
+    float mx = m;
+    for (int w = 1; w < WPR; ++w) mx = fmaxf(mx, sm[wave + w]);
+    const float a0 = __builtin_amdgcn_exp2f(m - mx);
+    o *= a0;
+    l *= a0;
+    for (int w = 1; w < WPR; ++w) {
+      const float a = __builtin_amdgcn_exp2f(sm[wave + w] - mx);
+      o += so[wave + w][c] * a;
+      l += sl[wave + w] * a;
     }
   }
-  so[sp][c] = o;
-  if (c == 0) {
-    sm[sp] = m;
-    sl[sp] = l;
-  }
-  __syncthreads();
-  if (sp == 0) {
-    float mx = sm[0];
-    for (int s = 1; s < SP; ++s) mx = fmaxf(mx, sm[s]);
-    o = f32x4{0.f, 0.f, 0.f, 0.f};
-    l = 0.f;
-    for (int s = 0; s < SP; ++s) {
-      const float a = __builtin_amdgcn_exp2f(sm[s] - mx);
-      o += so[s][c] * a;
-      l += sl[s] * a;
-    }
+  if (sub == 0 && row < p.rows) {
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     *reinterpret_cast<u32x2*>(p.out + row * HD + 4 * c) = u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
   }
@@ -568,18 +685,40 @@ __global__ void __launch_bounds__(256) cross_attention_join_kernel(JoinParams p)
 namespace {
 
 constexpr int NWAVE = 4;
-constexpr int STREAM_BUF = 2, SPLIT_BUF = 4;
+// Blocks of 16 rows per wave.  More of them read a K / V fragment from LDS for more rows; fewer leave registers for more waves.
+constexpr int resident_qn(int64_t head_dim) { return head_dim == 64 ? 3 : 2; }
+constexpr int64_t RESIDENT_LDS = 80 * 1024;  // two workgroups per CU
 
 struct Plan {
   Task task[2];
   int n, qn;
   bool split;
+  int resident;  // chunks that a workgroup keeps in LDS (0: they are streamed)
   int64_t grid, words, bytes;  // workgroups; mask words of a workgroup; of the workspace
 };
 
 int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-Plan plan_of(const aeris_cross_attention& a) {
+// Microseconds of a launch, fitted to measurements (60 to 8000 queries, 300 to 4000 keys, 4 and 8 heads): what a chunk takes a workgroup alone on
+// its CU, and one of several; the start; and for parts of the keys the joining kernel and what the parts' sums cost to write and read.
+struct Times {
+  float alone[2], among[2];  // 16 and 32 rows per wave
+  float chunk(int64_t wgs, int qn) const {
+    const float several = among[qn - 1] * div_up(wgs, 256);
+    return several > alone[qn - 1] ? several : alone[qn - 1];
+  }
+  float whole(int64_t units, int rows, int64_t chunks, int qn) const { return 4.2f + chunks * chunk(units * div_up(rows, 64 * qn), qn); }
+  float in_parts(int64_t units, int rows, int64_t chunks, int qn, int s, int head_dim) const {
+    const float mb = 4e-6f * units * rows * s * head_dim;
+    return 4.2f + div_up(chunks, s) * chunk(units * div_up(rows, 64 * qn) * s, qn) + (s > 1 ? 6.0f + 0.55f * mb : 0.f);
+  }
+};
+const Times& times_of(int64_t head_dim) {
+  static const Times t32 = {{0.48f, 0.56f}, {0.25f, 0.40f}}, t64 = {{0.56f, 0.75f}, {0.40f, 0.55f}}, t128 = {{0.84f, 1.12f}, {0.65f, 0.95f}};
+  return head_dim == 32 ? t32 : head_dim == 64 ? t64 : t128;
+}
+
+Plan plan_of(const CrossArgs& a) {
   const int B = (int)a.B, Hk = (int)a.kv_heads, rows_m = (int)(a.Nq * (a.heads / a.kv_heads));
   const bool own = a.Nk > 0, masked = a.key_mask && own;
   // every member sees the same keys: its rows are further rows of one unit
@@ -604,21 +743,44 @@ Plan plan_of(const aeris_cross_attention& a) {
     add(false, a.Nk, a.Np);
   }
   auto chunks = [](const Task& t) { return (int64_t)div_up(t.Np, KC) + div_up(t.Nk, KC); };
-  // Parts of the keys: two workgroups per CU, four chunks at least are worth a workgroup of their own; and no more than a mask's words cover
+  // Rows per wave and parts of the keys, by the time that a launch of them takes (see Times)
+  const Times& tm = times_of(a.head_dim);
   plan.qn = 2;
-  for (int i = 0; i < plan.n; ++i) {
-    Task& t = plan.task[i];
-    const int64_t wgs = (int64_t)t.members * Hk * div_up(t.rows, 64 * plan.qn);
-    int64_t s = 512 / wgs;
-    if (s > chunks(t) / 4) s = chunks(t) / 4;
-    if (masked && t.Nk > 0 && s * MAX_WORDS < chunks(t)) s = div_up(chunks(t), MAX_WORDS);
-    t.splits = s < 1 ? 1 : (int)s;
-    if (t.splits > 1) plan.split = true;
+  float best = 1e30f;
+  for (int qn = 1; qn <= 2 && !plan.split; ++qn) {  // whole
+    const float t = tm.whole(plan.task[0].members * Hk, plan.task[0].rows, chunks(plan.task[0]), qn);
+    if (t < best) {
+      best = t;
+      plan.qn = qn;
+    }
   }
+  int parts[2] = {1, 1}, split_qn = 1;
+  for (int i = 0; i < plan.n; ++i)
+    if (plan.task[i].rows > 64) split_qn = 2;
+  float in_parts = 0;
+  for (int i = 0; i < plan.n; ++i) {
+    const Task& t = plan.task[i];
+    const int64_t wgs = (int64_t)t.members * Hk * div_up(t.rows, 64 * split_qn);
+    float least = 1e30f;
+    for (int slots = 256; slots <= (a.head_dim == 128 ? 512 : 1024); slots += 256) {  // (head_dim 128: 64 KB of LDS each)
+      int64_t s = slots / wgs;
+      if (s > div_up(chunks(t), 3)) s = div_up(chunks(t), 3);
+      if (s < 1) s = 1;
+      const float x = tm.in_parts(t.members * Hk, t.rows, chunks(t), split_qn, (int)s, (int)a.head_dim);
+      if (x < least) {
+        least = x;
+        parts[i] = (int)s;
+      }
+    }
+    if (masked && t.Nk > 0 && (int64_t)parts[i] * MAX_WORDS < chunks(t)) parts[i] = div_up(chunks(t), MAX_WORDS);
+    in_parts = least > in_parts ? least : in_parts;
+  }
+  if (plan.n == 1 && (in_parts < best || (masked && chunks(plan.task[0]) > MAX_WORDS))) plan.split = true;
   if (plan.split) {
-    plan.qn = 1;
-    for (int i = 0; i < plan.n; ++i)
-      if (plan.task[i].rows > 64) plan.qn = 2;
+    plan.qn = split_qn;
+    for (int i = 0; i < plan.n; ++i) plan.task[i].splits = parts[i];
+  } else if (a.head_dim == 64 && chunks(plan.task[0]) >= 12 && (int64_t)plan.task[0].members * Hk * div_up(plan.task[0].rows, 256) >= 500) {
+    plan.qn = 4;  // long key ranges for many rows: 129 600 x 4000 keys, one head, 144 -> 132 us; 400 keys 69.5 -> 74.8, 500 workgroups on the mark
   }
   for (int i = 0; i < plan.n; ++i) {
     Task& t = plan.task[i];
@@ -634,22 +796,38 @@ Plan plan_of(const aeris_cross_attention& a) {
     if (plan.split) plan.bytes += ((int64_t)t.units * t.rows * (a.head_dim + 2) * 4 + 255) / 256 * 256;
   }
   if (plan.n < 2) plan.task[1].first = 0x7fffffff;
+  if (!plan.split) {
+    Task& t = plan.task[0];
+    const int64_t c = chunks(t), lds = c * (4 * KC * a.head_dim + 8);
+    const int64_t per = (lds <= RESIDENT_LDS / 2 ? 1024 : 512) / t.units, blocks = div_up(t.rows, 16 * resident_qn(a.head_dim) * NWAVE);
+    if (c > 0 && lds <= RESIDENT_LDS && per > 0 && blocks >= 2 * per) {
+      plan.resident = (int)c;
+      t.qblks = (int)per;
+      plan.grid = per * t.units;
+    }
+  }
   return plan;
 }
 
 // the kernel for (parts of the keys, scaled here, blocks of 16 rows per wave), handed to `f` with its LDS bytes
 template <int HD, class F>
 hipError_t with_kernel(bool split, bool scaled, int qn, const F& f) {
-  constexpr int CH = 2 * KC * HD * 2;
-  if (split)
-    return qn == 1 ? f(cross_attention_kernel<HD, NWAVE, SPLIT_BUF, 1, true, true>, SPLIT_BUF * CH)
-                   : f(cross_attention_kernel<HD, NWAVE, SPLIT_BUF, 2, true, true>, SPLIT_BUF * CH);
-  return scaled ? f(cross_attention_kernel<HD, NWAVE, STREAM_BUF, 2, false, true>, STREAM_BUF * CH)
-                : f(cross_attention_kernel<HD, NWAVE, STREAM_BUF, 2, false, false>, STREAM_BUF * CH);
+  constexpr int LDS = 8 * KC * HD;
+  constexpr bool SUM = HD == 32;
+  if (split) return qn == 1 ? f(cross_attention_kernel<HD, NWAVE, 1, true, true, false>, LDS) : f(cross_attention_kernel<HD, NWAVE, 2, true, true, false>, LDS);
+  if constexpr (HD == 64)
+    if (qn == 4) return scaled ? f(cross_attention_kernel<HD, NWAVE, 4, false, true, true>, LDS) : f(cross_attention_kernel<HD, NWAVE, 4, false, false, true>, LDS);
+  if (qn == 1) return scaled ? f(cross_attention_kernel<HD, NWAVE, 1, false, true, SUM>, LDS) : f(cross_attention_kernel<HD, NWAVE, 1, false, false, SUM>, LDS);
+  return scaled ? f(cross_attention_kernel<HD, NWAVE, 2, false, true, SUM>, LDS) : f(cross_attention_kernel<HD, NWAVE, 2, false, false, SUM>, LDS);
+}
+template <int HD, class F>
+hipError_t with_resident_kernel(bool scaled, const F& f) {
+  return scaled ? f(cross_attention_resident_kernel<HD, NWAVE, resident_qn(HD), true, HD <= 64>)
+                : f(cross_attention_resident_kernel<HD, NWAVE, resident_qn(HD), false, HD <= 64>);
 }
 
 template <int HD>
-hipError_t launch_dim(const aeris_cross_attention& a, Plan& plan, void* workspace, hipStream_t stream) {
+hipError_t launch_dim(const CrossArgs& a, Plan& plan, void* workspace, hipStream_t stream) {
   CrossParams p{};
   p.q = (const uint16_t*)a.q; p.k = (const uint16_t*)a.k; p.v = (const uint16_t*)a.v;
   p.prefix_k = (const uint16_t*)a.prefix_k; p.prefix_v = (const uint16_t*)a.prefix_v;
@@ -675,6 +853,11 @@ hipError_t launch_dim(const aeris_cross_attention& a, Plan& plan, void* workspac
   }
   p.task[0] = plan.task[0];
   p.task[1] = plan.task[1];
+  if (plan.resident)
+    return with_resident_kernel<HD>(!a.q_prescaled, [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)plan.grid), dim3(64 * NWAVE), (uint32_t)(plan.resident * (4 * KC * HD + 8)), stream, p, plan.resident);
+      return hipGetLastError();
+    });
   const hipError_t e = with_kernel<HD>(plan.split, !a.q_prescaled, plan.qn, [&](auto kernel, int lds) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)plan.grid), dim3(64 * NWAVE), (uint32_t)(lds + plan.words * 8), stream, p);
     return hipGetLastError();
@@ -684,16 +867,24 @@ hipError_t launch_dim(const aeris_cross_attention& a, Plan& plan, void* workspac
   j.task[0] = plan.task[0];
   if (plan.n > 1) j.task[1] = plan.task[1];
   j.out = p.out; j.Nq = p.Nq; j.heads = p.heads; j.kv_heads = p.kv_heads; j.group = p.group; j.rows_m = p.rows_m;
-  hipLaunchKernelGGL((cross_attention_join_kernel<HD>), dim3((unsigned)(a.B * a.Nq * a.heads)), dim3(256), 0, stream, j);
+  j.rows = a.B * a.Nq * a.heads;
+  const int parts = plan.task[0].splits + plan.task[1].splits;
+  if (parts <= 16) hipLaunchKernelGGL((cross_attention_join_kernel<HD, 1>), dim3((unsigned)((j.rows + 3) / 4)), dim3(256), 0, stream, j);
+  else if (parts <= 64) hipLaunchKernelGGL((cross_attention_join_kernel<HD, 4>), dim3((unsigned)j.rows), dim3(256), 0, stream, j);
+  else hipLaunchKernelGGL((cross_attention_join_kernel<HD, 16>), dim3((unsigned)j.rows), dim3(1024), 0, stream, j);
   return hipGetLastError();
 }
 
 template <int HD>
 hipError_t configure_dim() {
   hipError_t e = hipSuccess;
-  for (int i = 0; i < 8 && e == hipSuccess; ++i)
-    e = with_kernel<HD>(i & 1, i & 2, i & 4 ? 1 : 2, [](auto kernel, int lds) {
+  for (int i = 0; i < 12 && e == hipSuccess; ++i)
+    e = with_kernel<HD>(i & 1, i & 2, i >> 2 == 2 ? 4 : 1 + (i >> 2), [](auto kernel, int lds) {
       return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds + MAX_WORDS * 8);
+    });
+  for (int i = 0; i < 2 && e == hipSuccess; ++i)
+    e = with_resident_kernel<HD>(i, [](auto kernel) {
+      return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)RESIDENT_LDS);
     });
   return e;
 }
@@ -709,9 +900,9 @@ hipError_t cross_attention_configure() {
   return e;
 }
 
-int64_t cross_attention_workspace_bytes(const aeris_cross_attention& a) { return plan_of(a).bytes; }
+int64_t cross_attention_workspace_bytes(const CrossArgs& a) { return plan_of(a).bytes; }
 
-hipError_t cross_attention_launch(const aeris_cross_attention& a, void* workspace, hipStream_t stream) {
+hipError_t cross_attention_launch(const CrossArgs& a, void* workspace, hipStream_t stream) {
   Plan plan = plan_of(a);
   if (a.head_dim == 32) return launch_dim<32>(a, plan, workspace, stream);
   if (a.head_dim == 64) return launch_dim<64>(a, plan, workspace, stream);

@@ -68,11 +68,22 @@ hipError_t output_stage_launch(const void* x, int x_dtype, const void* gamma, co
 bool qk_norm_rope_supported(int64_t head_dim, int64_t rotated);
 hipError_t qk_norm_rope_launch(const aeris_qk_norm_rope& a, hipStream_t stream);
 
-// attention to an encoder's states (cross_attention.hip)
+// attention to an encoder's states (cross_attention.hip): aeris_cross_attention with the strides of dimensions with one entry 0
+struct CrossArgs {
+  const void *q, *k, *v, *prefix_k, *prefix_v;
+  void* out;
+  const int32_t* lengths;
+  const uint8_t* key_mask;
+  int64_t B, Nq, heads, kv_heads, head_dim, Nk, Np;
+  int64_t q_batch_stride, q_row_stride, q_head_stride, k_batch_stride, k_row_stride, k_head_stride, v_batch_stride, v_row_stride, v_head_stride;
+  int64_t prefix_k_row_stride, prefix_k_head_stride, prefix_v_row_stride, prefix_v_head_stride;
+  int64_t lengths_stride, mask_batch_stride, q_prescaled;
+  double scale;
+};
 bool cross_attention_supported(int64_t head_dim);
 hipError_t cross_attention_configure();
-int64_t cross_attention_workspace_bytes(const aeris_cross_attention& a);
-hipError_t cross_attention_launch(const aeris_cross_attention& a, void* workspace, hipStream_t stream);
+int64_t cross_attention_workspace_bytes(const CrossArgs& a);
+hipError_t cross_attention_launch(const CrossArgs& a, void* workspace, hipStream_t stream);
 
 hipError_t modulation_linear_launch(const aeris_modulation_layer* layers, int n, int B, int K, int w_dtype, int act, hipStream_t stream);
 hipError_t heun_update_launch(const float* x, const float* f0, const float* f1, const float* t, float sigma_data, float* out, int64_t n,

@@ -42,17 +42,18 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkParams p) {
   const int h0 = ((int)blockIdx.y - (second ? p.groups0 : 0)) * HPT;
   const int heads = (int)part.heads;
   const float mul = (float)part.scale;
+  const int64_t xt = part.x_stride[0], xh = part.x_stride[1], yt = part.y_stride[0], yh = part.y_stride[1];  // (of one token, one head: times 0)
 
   u32x4 raw[HPT][XF32 ? 2 : 1];
 #pragma unroll
   for (int i = 0; i < HPT; ++i) {
     const int64_t h = h0 + i < heads ? h0 + i : heads - 1;
     if constexpr (XF32) {
-      const float* x = reinterpret_cast<const float*>(part.x) + tt * part.x_token_stride + h * part.x_head_stride + c * 8;
+      const float* x = reinterpret_cast<const float*>(part.x) + tt * xt + h * xh + c * 8;
       raw[i][0] = *reinterpret_cast<const u32x4*>(x);
       raw[i][1] = *reinterpret_cast<const u32x4*>(x + 4);
     } else {
-      raw[i][0] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(part.x) + tt * part.x_token_stride + h * part.x_head_stride + c * 8);
+      raw[i][0] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(part.x) + tt * xt + h * xh + c * 8);
     }
   }
 
@@ -169,11 +170,11 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkParams p) {
     for (int e = 0; e < 8; ++e) y[e] *= mul;
     if (!ok) continue;
     if constexpr (YF32) {
-      float* o = reinterpret_cast<float*>(part.y) + tt * part.y_token_stride + h * part.y_head_stride + c * 8;
+      float* o = reinterpret_cast<float*>(part.y) + tt * yt + h * yh + c * 8;
       *reinterpret_cast<f32x4*>(o) = f32x4{y[0], y[1], y[2], y[3]};
       *reinterpret_cast<f32x4*>(o + 4) = f32x4{y[4], y[5], y[6], y[7]};
     } else {
-      uint16_t* o = reinterpret_cast<uint16_t*>(part.y) + tt * part.y_token_stride + h * part.y_head_stride + c * 8;
+      uint16_t* o = reinterpret_cast<uint16_t*>(part.y) + tt * yt + h * yh + c * 8;
       *reinterpret_cast<u32x4*>(o) = u32x4{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7])};
     }
   }

@@ -109,6 +109,16 @@ def workspaces(device, *requests):
     return got
 
 
+def _workspace_ptr(tag: str, nbytes: int, device) -> int:
+    """``workspace`` for a call that needs its address alone: the buffer that it last used on this stream, without a tensor around it."""
+    key = (tag, device, torch.uint8)
+    buf = _WORKSPACE.get(key)
+    if (buf is None or buf.numel() < nbytes or torch._C._cuda_isCurrentStreamCapturing() or
+            _WS_OWNER[key][0] != torch._C._cuda_getCurrentRawStream(device.index)):
+        return workspace(tag, (nbytes,), torch.uint8, device).data_ptr()
+    return buf.data_ptr()
+
+
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
@@ -412,21 +422,14 @@ def gemm_heads(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], h
     return out
 
 
-def _on_current_device(t: torch.Tensor, name: str, device):
-    """Whose stream the call goes to: every tensor of it lives on the current GPU."""
-    if t.device != device or device.index != torch._C._cuda_getDevice():
-        if not t.is_cuda:
+def _on_current_device(device, tensors):
+    """Whose stream the call goes to: every tensor of it (names and tensors) lives on the current GPU."""
+    for name, t in tensors.items():
+        if t is not None and not t.is_cuda:
             raise RuntimeError(f"{name} must live on the GPU (the HIP kernels have no CPU fallback)")
-        raise RuntimeError(f"{name} is on {t.device}; every tensor of the call must be on the current device (cuda:{torch._C._cuda_getDevice()})")
-
-
-def _head_strides(t: torch.Tensor, name: str):
-    """Strides, in elements, of [.., heads, head_dim]; 0 where a dimension has one entry.  (That they are multiples of 16 bytes, and the
-    address too, is for the library to say.)"""
-    stride = t.stride()
-    if stride[-1] != 1:
-        raise RuntimeError(f"{name}: the elements of a head must be contiguous (strides {stride})")
-    return [s if n > 1 else 0 for s, n in zip(stride[:-1], t.shape)]
+    for name, t in tensors.items():
+        if t is not None and (t.device != device or device.index != torch._C._cuda_getDevice()):
+            raise RuntimeError(f"{name} is on {t.device}; every tensor of the call must be on the current device (cuda:{torch._C._cuda_getDevice()})")
 
 
 def _written_once(t: torch.Tensor, name: str):
@@ -439,32 +442,30 @@ def _written_once(t: torch.Tensor, name: str):
             span = s * (n - 1) + span
 
 
-QK_NORM_ROPE = struct.Struct("=3Q6qd3Q6qd2Q11qd")  # struct aeris_qk_norm_rope of include/aeris_hip.h
-_NO_PART = (0,) * 9 + (0.0,)
+QK_NORM_ROPE = struct.Struct("=3Q8qd3Q8qd2Q11qd")  # struct aeris_qk_norm_rope of include/aeris_hip.h
+_NO_PART = (0,) * 11 + (0.0,)
 
 
-def _qk_part(x, gain, out, scale, name, q, device, y_dtype):
+def _qk_part(x, shape, gain, out, scale, name, y_dtype):
     """One part's fields of the call's struct, and its output."""
-    heads, D = x.shape[1:]
+    _, heads, D = shape
     if out is None:
         out = torch.empty_like(x, dtype=y_dtype)
     else:
-        _on_current_device(out, f"{name}_out", device)
-        if out.shape != x.shape or out.dtype != y_dtype:
-            raise RuntimeError(f"{name}_out must be {y_dtype} {tuple(x.shape)}, got {out.dtype} {tuple(out.shape)}")
+        if out.shape != shape or out.dtype is not y_dtype:
+            raise RuntimeError(f"{name}_out must be {y_dtype} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
         _written_once(out, f"{name}_out")
     gain_ptr = per_head = 0
     if gain is not None:
-        _on_current_device(gain, f"{name}_gain", device)
-        shape = tuple(gain.shape)
-        if shape == (heads, D):
+        gain_shape = gain.shape
+        if gain_shape == (heads, D):
             per_head = D
-        elif shape != (D,):
-            raise RuntimeError(f"{name}_gain must be [{D}] or [{heads}, {D}], got {shape}")
+        elif gain_shape != (D,):
+            raise RuntimeError(f"{name}_gain must be [{D}] or [{heads}, {D}], got {tuple(gain_shape)}")
         if not gain.is_contiguous():
             raise RuntimeError(f"{name}_gain must be contiguous")
         gain_ptr = gain.data_ptr()
-    return (x.data_ptr(), out.data_ptr(), gain_ptr, heads, *_head_strides(x, name), *_head_strides(out, f"{name}_out"), per_head, scale), out
+    return (x.data_ptr(), out.data_ptr(), gain_ptr, heads, *x.stride(), *out.stride(), per_head, scale), out
 
 
 def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_gain: Optional[torch.Tensor] = None,
@@ -481,50 +482,50 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_gain: Opti
     q is multiplied by q_scale ahead of its rounding (``scale * LOG2E`` for the attention calls' ``q_prescaled``).
     The outputs (out_dtype) may be given; q_out may be q and k_out may be k.  Otherwise an output shares no memory with an input."""
     device = q.device
-    _on_current_device(q, "q", device)
-    if q.dim() != 3:
-        raise RuntimeError(f"q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
-    T, _, D = q.shape
+    if (device.index != torch._C._cuda_getDevice() or (k is not None and k.device != device) or (q_gain is not None and q_gain.device != device) or
+            (k_gain is not None and k_gain.device != device) or (rotation is not None and rotation.device != device) or
+            (positions is not None and positions.device != device) or (q_out is not None and q_out.device != device) or
+            (k_out is not None and k_out.device != device)):
+        _on_current_device(device, dict(q=q, k=k, q_gain=q_gain, k_gain=k_gain, rotation=rotation, positions=positions, q_out=q_out, k_out=k_out))
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 3:
+        raise RuntimeError(f"q must be [tokens, heads, head_dim], got {tuple(shape)}")
+    T, _, D = shape
     given = q_out if q_out is not None else k_out
     y_dtype = out_dtype if given is None else given.dtype
     some_gain = q_gain if q_gain is not None else k_gain
-    gain_type = _DT.get(some_gain.dtype) if some_gain is not None else 0
-    if q.dtype not in _DT or y_dtype not in _DT or gain_type is None:
+    x_type, y_type, gain_type = _DT.get(dtype), _DT.get(y_dtype), 0 if some_gain is None else _DT.get(some_gain.dtype)
+    if x_type is None or y_type is None or gain_type is None:
         raise RuntimeError("q, k, the gains and the outputs must be bf16 or f32")
-    q_part, yq = _qk_part(q, q_gain, q_out, q_scale, "q", q, device, y_dtype)
+    q_part, yq = _qk_part(q, shape, q_gain, q_out, q_scale, "q", y_dtype)
     if k is None:
         if k_gain is not None or k_out is not None:
             raise RuntimeError("k_gain and k_out need k")
-        k_part, yk, empty = _NO_PART, None, yq.numel() == 0
+        k_part, yk, n_parts = _NO_PART, None, 1
     else:
-        _on_current_device(k, "k", device)
-        if k.dtype != q.dtype or k.dim() != 3 or k.shape[0] != T or k.shape[2] != D:
-            raise RuntimeError(f"k must be {q.dtype} [{T}, key heads, {D}], got {k.dtype} {tuple(k.shape)}")
-        if q_gain is not None and k_gain is not None and q_gain.dtype != k_gain.dtype:
+        k_shape = k.shape
+        if k.dtype is not dtype or len(k_shape) != 3 or k_shape[0] != T or k_shape[2] != D:
+            raise RuntimeError(f"k must be {dtype} [{T}, key heads, {D}], got {k.dtype} {tuple(k_shape)}")
+        if q_gain is not None and k_gain is not None and q_gain.dtype is not k_gain.dtype:
             raise RuntimeError("q_gain and k_gain must be of one type")
-        k_part, yk = _qk_part(k, k_gain, k_out, 1.0, "k", q, device, y_dtype)
-        empty = yq.numel() == 0 or yk.numel() == 0
-        if empty and T:
-            raise RuntimeError("q and k must both have heads")
+        k_part, yk = _qk_part(k, k_shape, k_gain, k_out, 1.0, "k", y_dtype)
+        n_parts = 2
     table_ptr = P = R = positions_ptr = n_pos = 0
     if rotation is not None:
-        _on_current_device(rotation, "rotation", device)
-        if rotation.dtype != torch.float32 or rotation.dim() != 2 or not rotation.is_contiguous():
+        if rotation.dtype is not torch.float32 or rotation.dim() != 2 or not rotation.is_contiguous():
             raise RuntimeError("rotation must be contiguous f32 [positions, rotated elements]")
         P, R = rotation.shape
         table_ptr = rotation.data_ptr()
         if P == 0:
             raise RuntimeError("rotation has no rows")
     if positions is not None:
-        _on_current_device(positions, "positions", device)
         n_pos = positions.numel()
-        if rotation is None or positions.dtype != torch.int32 or positions.dim() != 1 or not positions.is_contiguous() or not n_pos:
+        if rotation is None or positions.dtype is not torch.int32 or positions.dim() != 1 or not positions.is_contiguous() or not n_pos:
             raise RuntimeError("positions must be a contiguous int32 vector, and need rotation")
         positions_ptr = positions.data_ptr()
-    if empty:
+    if T == 0:
         return yq, yk
-    call = QK_NORM_ROPE.pack(*q_part, *k_part, table_ptr, positions_ptr, T, D, _DT[q.dtype], _DT[y_dtype], gain_type, normed, interleaved, P, R, n_pos,
-                             1 if k is None else 2, eps)
+    call = QK_NORM_ROPE.pack(*q_part, *k_part, table_ptr, positions_ptr, T, D, x_type, y_type, gain_type, normed, interleaved, P, R, n_pos, n_parts, eps)
     if _profile is None:
         L.call("aeris_qk_norm_rope_fwd", call, _stream())
     else:
@@ -534,7 +535,7 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_gain: Opti
     return yq, yk
 
 
-CROSS_ATTENTION = struct.Struct("=8Q23qd")  # struct aeris_cross_attention of include/aeris_hip.h
+CROSS_ATTENTION = struct.Struct("=8Q30qd")  # struct aeris_cross_attention of include/aeris_hip.h
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths: Optional[torch.Tensor] = None,
@@ -549,56 +550,53 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, length
     for all of them where a member has few queries.  A query without any key gives zeros.
     scale: head_dim^-0.5 unless given; ``q_prescaled``: q already holds q * scale * log2(e) (``qk_norm_rope(q_scale=scale * LOG2E)``).  out shares
     no memory with the inputs."""
-    device, shape, kv_shape = q.device, q.shape, k.shape
-    _on_current_device(q, "q", device)
-    _on_current_device(k, "k", device)
-    _on_current_device(v, "v", device)
+    device, shape, kv_shape, bf16 = q.device, q.shape, k.shape, torch.bfloat16
+    if device.index != torch._C._cuda_getDevice() or k.device != device or v.device != device:
+        _on_current_device(device, dict(q=q, k=k, v=v))
     if len(shape) != 4 or len(kv_shape) != 4:
         raise RuntimeError(f"q, k and v must have 4 dimensions, got {tuple(shape)} and {tuple(kv_shape)}")
     B, Nq, heads, D = shape
     Bk, Nk, kv_heads, Dk = kv_shape
     if v.shape != kv_shape or Dk != D or (Bk != B and Bk != 1) or kv_heads == 0 or heads % kv_heads:
         raise RuntimeError(f"k and v must be [1 | {B}, keys, divisor of {heads}, {D}], got {tuple(kv_shape)} and {tuple(v.shape)}")
-    bf16 = torch.bfloat16
     if q.dtype is not bf16 or k.dtype is not bf16 or v.dtype is not bf16:
         raise RuntimeError("q, k and v must be bf16")
-    prefix_ptrs, Np, prefix_strides = (0, 0), 0, (0, 0, 0, 0)
+    pk_ptr = pv_ptr = Np = lengths_ptr = n_lengths = mask_ptr = mask_batch = mask_stride = 0
+    prefix_strides = (0, 0, 0, 0, 0, 0)
     if prefix is not None:
         pk, pv = prefix
-        _on_current_device(pk, "prefix k", device)
-        _on_current_device(pv, "prefix v", device)
+        if pk.device != device or pv.device != device:
+            _on_current_device(device, {"prefix k": pk, "prefix v": pv})
         if pk.shape != pv.shape or pk.dim() != 3 or pk.shape[1] != kv_heads or pk.shape[2] != D or pk.dtype is not bf16 or pv.dtype is not bf16:
             raise RuntimeError(f"prefix must be two bf16 [keys, {kv_heads}, {D}], got {pk.dtype} {tuple(pk.shape)} and {pv.dtype} {tuple(pv.shape)}")
-        Np = pk.shape[0]
-        prefix_ptrs = (pk.data_ptr(), pv.data_ptr())
-        prefix_strides = (*_head_strides(pk, "prefix k"), *_head_strides(pv, "prefix v"))
-    lengths_ptr = lengths_stride = mask_ptr = mask_stride = 0
+        Np, pk_ptr, pv_ptr, prefix_strides = pk.shape[0], pk.data_ptr(), pv.data_ptr(), (*pk.stride(), *pv.stride())
     if lengths is not None:
-        _on_current_device(lengths, "lengths", device)
-        n = lengths.numel()
-        if lengths.dtype is not torch.int32 or lengths.dim() != 1 or (n != B and n != 1) or not lengths.is_contiguous():
+        if lengths.device != device:
+            _on_current_device(device, dict(lengths=lengths))
+        n_lengths, lengths_ptr = lengths.numel(), lengths.data_ptr()
+        if lengths.dtype is not torch.int32 or lengths.dim() != 1 or (n_lengths != B and n_lengths != 1) or not lengths.is_contiguous():
             raise RuntimeError(f"lengths must be contiguous int32 [1 | {B}], got {lengths.dtype} {tuple(lengths.shape)}")
-        lengths_ptr, lengths_stride = lengths.data_ptr(), int(n > 1)
     if key_mask is not None:
-        _on_current_device(key_mask, "key_mask", device)
+        if key_mask.device != device:
+            _on_current_device(device, dict(key_mask=key_mask))
         if (key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.dim() != 2 or key_mask.shape[0] not in (1, B) or key_mask.shape[1] != Nk or
                 (Nk > 1 and key_mask.stride(1) != 1)):
             raise RuntimeError(f"key_mask must be bool or uint8 [1 | {B}, {Nk}] with contiguous rows, got {key_mask.dtype} {tuple(key_mask.shape)}")
-        mask_ptr, mask_stride = key_mask.data_ptr(), key_mask.stride(0) if key_mask.shape[0] > 1 else 0
+        mask_ptr, mask_batch, mask_stride = key_mask.data_ptr(), key_mask.shape[0], key_mask.stride(0)
     if out is None:
         out = torch.empty(shape, dtype=bf16, device=device)
     else:
-        _on_current_device(out, "out", device)
-        _dev(out, "out", bf16)
-        if out.shape != shape:
-            raise RuntimeError(f"out must be {tuple(shape)}, got {tuple(out.shape)}")
-    if out.numel() == 0:
+        if out.device != device:
+            _on_current_device(device, dict(out=out))
+        if out.shape != shape or out.dtype is not bf16 or not out.is_contiguous():
+            raise RuntimeError(f"out must be contiguous bf16 {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
+    if B == 0 or Nq == 0 or heads == 0:
         return out
-    call = CROSS_ATTENTION.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), *prefix_ptrs, out.data_ptr(), lengths_ptr, mask_ptr, B, Nq, heads, kv_heads, D,
-                                Nk, Np, *_head_strides(q, "q"), *_head_strides(k, "k"), *_head_strides(v, "v"), *prefix_strides, lengths_stride,
-                                mask_stride, q_prescaled, D ** -0.5 if scale is None else scale)
+    call = CROSS_ATTENTION.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), pk_ptr, pv_ptr, out.data_ptr(), lengths_ptr, mask_ptr, B, Nq, heads, D, Bk, Nk,
+                                kv_heads, Np, n_lengths, mask_batch, *q.stride(), *k.stride(), *v.stride(), *prefix_strides, mask_stride, q_prescaled,
+                                D ** -0.5 if scale is None else scale)
     need = L.lib().aeris_cross_attention_workspace_bytes(call)
-    ws = workspace("cross_attention", (need,), torch.uint8, device).data_ptr() if need else None
+    ws = _workspace_ptr("cross_attention", need, device) if need else None
     if _profile is None:
         L.call("aeris_cross_attention_fwd", call, ws, need, _stream())
     else:

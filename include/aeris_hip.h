@@ -195,9 +195,10 @@ int aeris_gemm_heads_fwd(const void* A, const void* W, void* C, const void* bias
  *   n = x * rsqrt(mean(x^2) + eps) * gain  per (token, head) over the head_dim elements (normed == 0: n = x * gain)
  *   the pairs (a, b) of the first R elements become (a cos - b sin, a sin + b cos); interleaved: pairs (2j, 2j + 1), else (j, j + R/2)
  *   y = n * scale
- * in fp32, rounded once.  parts: one (n_parts 1), or two that share tokens and positions (queries, keys).  Of each: x and y start at token 0, head 0,
- * strides in elements, the head_dim elements of a head are contiguous; y may be x (same strides and type) and may otherwise not overlap it;
- * gain [head_dim] (gain_head_stride 0) or one row per head, or NULL.  Addresses 16-byte aligned, strides multiples of 16 bytes.
+ * in fp32, rounded once.  parts: one (n_parts 1), or two that share tokens and positions (queries, keys).  Of each: x [tokens, heads, head_dim]
+ * and y of the same shape by their strides (elements, one per dimension; that of a dimension with one entry does not count; the last is 1);
+ * y may be x (same strides and type) and may otherwise not overlap it; gain [head_dim] (gain_head_stride 0) or one row per head, or NULL.
+ * Addresses 16-byte aligned, strides multiples of 16 bytes.
  *   rotation f32 [P, R]: cos of the R/2 pairs, then sin (NULL with R = 0: no rotation); a token's row is positions[t % n_positions]
  *   (positions int32, on the device), or t % P where positions is NULL; a token whose position is not in [0, P) is not rotated.
  * Supported: head_dim 32, 64, 128; R a multiple of 16 up to head_dim. */
@@ -205,7 +206,7 @@ typedef struct aeris_qk_part {
   const void* x;    /* x_dtype */
   void* y;          /* y_dtype */
   const void* gain; /* gain_dtype, or NULL */
-  int64_t heads, x_token_stride, x_head_stride, y_token_stride, y_head_stride, gain_head_stride;
+  int64_t heads, x_stride[3], y_stride[3], gain_head_stride;
   double scale;
 } aeris_qk_part;
 typedef struct aeris_qk_norm_rope {
@@ -220,23 +221,24 @@ int aeris_qk_norm_rope_fwd(const aeris_qk_norm_rope* a, void* stream);
 /* Attention to states of another length (an encoder's, observations', a whole grid's): per member b, query n, head h
  *   out = softmax(scale * q k^T) v  over the prefix's Np keys, then those of the member's Nk keys that lie before lengths[b] (held to [0, Nk])
  *   and whose key_mask byte is not 0; zeros where that leaves no key.  What lies in rows of k and v that take no part is not looked at.
- *   q bf16 [B, Nq, heads, head_dim], k, v bf16 [B, Nk, kv_heads, head_dim], prefix_k, prefix_v bf16 [Np, kv_heads, head_dim] (the same for
- *   all members), by the strides below (elements; 0 where something is shared; a head's elements are contiguous; 16-byte aligned, strides
- *   multiples of 8, row strides of k and v below 2^23); head h uses key head h / (heads / kv_heads).
+ *   q bf16 [B, Nq, heads, head_dim], k, v bf16 [kv_batch, Nk, kv_heads, head_dim] (kv_batch 1: the same for all members, or B), prefix_k, prefix_v
+ *   bf16 [Np, kv_heads, head_dim] (the same for all members), by their strides (elements, one per dimension; 0 where entries are shared; that of
+ *   a dimension with one entry does not count; the last is 1); addresses 16-byte aligned, the other strides multiples of 8, those between keys below
+ *   2^23.  head h uses key head h / (heads / kv_heads).
  *   out bf16 [B, Nq, heads, head_dim], contiguous.
- *   lengths int32 [B] (lengths_stride 1) or one for all (0), on the device, or NULL; key_mask uint8, its rows contiguous, or NULL.
- *   q_prescaled != 0: q already holds q * scale * log2(e) (scale is ignored); otherwise q is multiplied and rounded to bf16 once more.
- * workspace: device memory of aeris_cross_attention_workspace_bytes(a) bytes (a's sizes and strides alone count; 0: none is needed), 16-byte
- * aligned, borrowed for the call.  Supported: head_dim 32, 64, 128. */
+ *   lengths int32 [n_lengths] (B, or one for all), on the device, or NULL; key_mask uint8 [mask_batch, Nk] (mask_batch B or 1), keys contiguous,
+ *   members mask_stride apart, or NULL.
+ *   q_prescaled != 0: q already holds q * scale * log2(e) (scale is ignored); otherwise the fp32 logits are multiplied.
+ * workspace: device memory of aeris_cross_attention_workspace_bytes(a) bytes (a's addresses do not count but for being NULL; 0: none is needed),
+ * 16-byte aligned, borrowed for the call.  Supported: head_dim 32, 64, 128. */
 typedef struct aeris_cross_attention {
   const void *q, *k, *v, *prefix_k, *prefix_v;
   void* out;
   const int32_t* lengths;
   const uint8_t* key_mask;
-  int64_t B, Nq, heads, kv_heads, head_dim, Nk, Np;
-  int64_t q_batch_stride, q_row_stride, q_head_stride, k_batch_stride, k_row_stride, k_head_stride, v_batch_stride, v_row_stride, v_head_stride;
-  int64_t prefix_k_row_stride, prefix_k_head_stride, prefix_v_row_stride, prefix_v_head_stride;
-  int64_t lengths_stride, mask_batch_stride, q_prescaled;
+  int64_t B, Nq, heads, head_dim, kv_batch, Nk, kv_heads, Np, n_lengths, mask_batch;
+  int64_t q_stride[4], k_stride[4], v_stride[4], prefix_k_stride[3], prefix_v_stride[3], mask_stride;
+  int64_t q_prescaled;
   double scale;
 } aeris_cross_attention;
 int64_t aeris_cross_attention_workspace_bytes(const aeris_cross_attention* a);

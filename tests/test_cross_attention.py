@@ -313,19 +313,22 @@ def test_refusals_on_the_gpu(pkg, cuda):
 def test_refusals_without_a_gpu(pkg):
     L, at = pkg._lib, 1 << 20
     S = pkg.ops.CROSS_ATTENTION
-    names = ("q k v pk pv out lengths mask B Nq heads kv_heads D Nk Np qb qr qh kb kr kh vb vr vh pkr pkh pvr pvh ls ms pre scale").split()
-    base = dict(zip(names, [at, at, at, 0, 0, at, 0, 0, 2, 5, 4, 2, 64, 9, 0, 1280, 256, 64, 1152, 128, 64, 1152, 128, 64, 0, 0, 0, 0, 0, 0, 0, 0.125]))
+    names = ("q k v pk pv out lengths mask B Nq heads D Bk Nk kv_heads Np n_lengths mask_batch qb qr qh qe kb kr kh ke vb vr vh ve pkr pkh pke pvr pvh pve "
+             "ms pre scale").split()
+    base = dict(zip(names, [at, at, at, 0, 0, at, 0, 0, 2, 5, 4, 64, 2, 9, 2, 0, 0, 0, 1280, 256, 64, 1, 1152, 128, 64, 1, 1152, 128, 64, 1, 0, 0, 0, 0, 0, 0, 0, 0,
+                            0.125]))
 
     def call(ws=at, ws_bytes=1 << 40, **kw):
         a = S.pack(*{**base, **kw}.values())
         return L.lib().aeris_cross_attention_fwd(a, ws, ws_bytes, None)
 
     for kw in [dict(q=0), dict(k=0), dict(v=0), dict(out=0), dict(Np=4), dict(q=at + 8), dict(out=at + 2), dict(k=at + 4), dict(B=0), dict(Nq=0), dict(heads=0),
-               dict(kv_heads=0), dict(heads=5), dict(Nk=-1), dict(Np=-1), dict(qr=4), dict(kb=-8), dict(vh=63), dict(pkr=1), dict(lengths=at, ls=2),
-               dict(lengths=at + 2), dict(mask=at, ms=-1), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf"))]:
+               dict(kv_heads=0), dict(heads=5), dict(Nk=-1), dict(Np=-1), dict(qr=4), dict(kb=-8), dict(vh=63), dict(qe=2), dict(ve=0),
+               dict(Np=4, pk=at, pv=at, pkr=1, pke=1, pve=1), dict(Np=4, pk=at, pv=at), dict(Bk=3), dict(lengths=at, n_lengths=3), dict(lengths=at + 2, n_lengths=2),
+               dict(mask=at, mask_batch=2, ms=-1), dict(mask=at, mask_batch=4), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf"))]:
         assert call(**kw) == L.EINVAL, kw
         assert "aeris_cross_attention_fwd" in L.last_error()
-    for kw in [dict(D=48), dict(D=256), dict(kr=1 << 23), dict(vr=1 << 23), dict(Nq=1 << 30), dict(B=1 << 40), dict(Nk=1 << 31), dict(Np=1 << 31, pk=at, pv=at),
+    for kw in [dict(D=48), dict(D=256), dict(kr=1 << 23), dict(vr=1 << 23), dict(Nq=1 << 30), dict(B=1 << 40, Bk=1), dict(Nk=1 << 31), dict(Np=1 << 31, pk=at, pv=at),
                dict(heads=1 << 17, kv_heads=1)]:
         assert call(**kw) == L.EUNSUPPORTED, kw
     assert L.lib().aeris_cross_attention_fwd(None, at, 0, None) == L.EINVAL
@@ -336,7 +339,7 @@ def test_refusals_without_a_gpu(pkg):
     for kw in (dict(ws=None), dict(ws_bytes=need - 1), dict(ws=at + 8)):
         assert call(**long, **kw) == L.EINVAL and "workspace" in L.last_error()
     assert L.lib().aeris_cross_attention_workspace_bytes(S.pack(*{**base, "B": 0}.values())) == 0
-    assert S.size == 256
+    assert S.size == 312
     t = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="GPU"):
         pkg.ops.cross_attention(t, t, t)

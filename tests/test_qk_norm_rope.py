@@ -206,13 +206,13 @@ def test_refusals_without_a_gpu(pkg):
     S = pkg.ops.QK_NORM_ROPE
 
     def call(part=(), n=1, tokens=4, D=64, xd=L.BF16, yd=L.BF16, gd=L.F32, eps=1e-6, rot=at, rows=4, R=64, pos=0, n_pos=0):
-        f = dict(x=at, y=at, gain=0, heads=2, xt=128, xh=64, yt=128, yh=64, gh=0, scale=1.0)
+        f = dict(x=at, y=at, gain=0, heads=2, xt=128, xh=64, xe=1, yt=128, yh=64, ye=1, gh=0, scale=1.0)
         f.update(part)
         a = S.pack(*f.values(), *f.values(), rot, pos, tokens, D, xd, yd, gd, 1, 0, rows, R, n_pos, n, eps)
         return L.lib().aeris_qk_norm_rope_fwd(a, None)
 
     for kw in [dict(part={"x": 0}), dict(part={"y": 0}), dict(part={"x": at + 8}), dict(part={"gain": at + 4}), dict(part={"xt": 129}),
-               dict(part={"yh": 4}), dict(part={"gain": at, "gh": 2}), dict(part={"heads": 0}), dict(tokens=0), dict(tokens=-1), dict(xd=2), dict(yd=-1),
+               dict(part={"yh": 4}), dict(part={"xe": 2}), dict(part={"ye": 0}), dict(part={"gain": at, "gh": 2}), dict(part={"heads": 0}), dict(tokens=0), dict(tokens=-1), dict(xd=2), dict(yd=-1),
                dict(gd=5), dict(eps=-1.0), dict(eps=float("nan")), dict(rot=0), dict(rot=at + 4), dict(rows=0), dict(rows=2 ** 31),
                dict(pos=at, n_pos=0), dict(pos=at + 2, n_pos=4), dict(n=0), dict(n=3)]:
         assert call(**kw) == L.EINVAL, kw
@@ -223,4 +223,4 @@ def test_refusals_without_a_gpu(pkg):
     assert L.lib().aeris_qk_norm_rope_fwd(None, None) == L.EINVAL
     with pytest.raises(RuntimeError, match="GPU"):
         pkg.ops.qk_norm_rope(torch.zeros(4, 2, 64, dtype=torch.bfloat16))
-    assert S.size == 272
+    assert S.size == 304
