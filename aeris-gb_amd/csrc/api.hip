@@ -395,7 +395,7 @@ int aeris_qk_norm_rope_fwd(const aeris_qk_norm_rope* a, void* stream) {
     return fail(AERIS_EINVAL, "%s: the rotation table must be 16-byte aligned and have 1 .. 2^31-1 rows", who);
   if (a->R > 0 && a->positions && (a->n_positions <= 0 || a->n_positions > 0x7fffffffLL || (reinterpret_cast<uintptr_t>(a->positions) & 3u)))
     return fail(AERIS_EINVAL, "%s: positions must be 4-byte aligned, 1 .. 2^31-1 of them", who);
-  // (token numbers are formed in 32 bits, up to a block of them beyond the last; the grid's second dimension counts heads)
+  // (token numbers are formed in 32 bits, up to a block of them beyond the last)
   if (a->tokens > 0x7fffffffLL - 64) return fail(AERIS_EUNSUPPORTED, "%s: more than 2^31-65 tokens", who);
   int64_t heads = 0;
   for (int i = 0; i < (int)a->n_parts; ++i) {
@@ -410,7 +410,8 @@ int aeris_qk_norm_rope_fwd(const aeris_qk_norm_rope* a, void* stream) {
     if (p.heads > 32767) return fail(AERIS_EUNSUPPORTED, "%s: more than 32767 heads", who);
     heads += p.heads;
   }
-  if (heads > 65535) return fail(AERIS_EUNSUPPORTED, "%s: more than 65535 heads", who);
+  // (workgroups of 2048 / head_dim tokens and a head at least)
+  if ((a->tokens * a->head_dim / 2048 + 1) * heads > 0x7fffffffLL) return fail(AERIS_EUNSUPPORTED, "%s: more than 2^31-1 workgroups", who);
   hipError_t e = aeris::qk_norm_rope_launch(*a, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "aeris_qk_norm_rope_fwd launch");
   return AERIS_OK;

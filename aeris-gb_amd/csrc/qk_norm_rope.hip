@@ -3,8 +3,13 @@
 //   n = x * rsqrt(mean(x^2) + eps) * gain          per (token, head), fp32
 //   (n_a, n_b) -> (n_a cos - n_b sin, n_a sin + n_b cos)    for the pairs (a, b) of the first R elements, angles by the token's position
 //   y = n * scale                                  (q: scale * log2 e, so that q is rounded to its type once, here)
-// Bound by HBM: every element is read once and written once.  D / 8 lanes hold a head's row, 16 bytes of bf16 each; a thread does a
-// few heads of one token, so that the token's row of the rotation table is read once for them, and their loads are in flight together.
+// Bound by HBM: every element is read once and written once.  D / 8 lanes hold a head's row, 16 bytes of bf16 each; a thread does four heads
+// of one token (one, where there are few tokens: latency), so that the token's row of the rotation table is read once for them and their loads are in
+// flight together (two: 5.3 TB/s, one 4.2, eight 5.4, all sixteen heads in rounds of four with the next round's loads ahead 5.1; four 5.6).  Head
+// planes: a group of heads walks through all tokens, stores that leave no line behind in the caches (1573 -> 1512 us).  Rows of heads side by
+// side: the groups of a block of tokens are neighbours, so that the parts of a row are fetched together (1811 -> 1477 us), ordinary stores
+// (1573 with the others).
+// 720 x 1440 tokens, 16 + 16 heads of 64: planes 1512 us, rows 1477 us, 5.6 - 5.75 TB/s (an element-wise multiplication of this size: 6.26 TB/s).
 #include "common.h"
 #include "kernels.h"
 
@@ -14,7 +19,9 @@ namespace {
 
 struct QkParams {
   aeris_qk_part part[2];
-  int groups0;  // groups of heads of the first part; the second part's follow
+  int groups0, groups;  // groups of heads: of the first part; of both
+  int blocks;           // of tokens
+  int heads_first;      // the groups of a block of tokens are neighbouring workgroups (else: the blocks of a group)
   int T, n_pos, P, R, normed, interleaved, gain_f32;
   float eps;
   const float* rotation;
@@ -30,16 +37,17 @@ __device__ __forceinline__ float row_sum(float v) {  // over the LPR neighbourin
   return v;
 }
 
-template <int D, bool XF32, bool YF32, int HPT>
+template <int D, bool XF32, bool YF32, int HPT, bool STREAM>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkParams p) {
   constexpr int LPR = D / 8, TPB = 256 / LPR;
   const int c = threadIdx.x % LPR;
-  const int t = blockIdx.x * TPB + threadIdx.x / LPR;
+  const int group = p.heads_first ? blockIdx.x % p.groups : blockIdx.x / p.blocks;
+  const int t = (int)(p.heads_first ? blockIdx.x / p.groups : blockIdx.x % p.blocks) * TPB + threadIdx.x / LPR;
   const bool ok = t < p.T;
   const int64_t tt = ok ? t : p.T - 1;
-  const bool second = (int)blockIdx.y >= p.groups0;
+  const bool second = group >= p.groups0;
   const aeris_qk_part& part = p.part[second ? 1 : 0];
-  const int h0 = ((int)blockIdx.y - (second ? p.groups0 : 0)) * HPT;
+  const int h0 = (group - (second ? p.groups0 : 0)) * HPT;
   const int heads = (int)part.heads;
   const float mul = (float)part.scale;
   const int64_t xt = part.x_stride[0], xh = part.x_stride[1], yt = part.y_stride[0], yh = part.y_stride[1];  // (of one token, one head: times 0)
@@ -174,8 +182,10 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkParams p) {
       *reinterpret_cast<f32x4*>(o) = f32x4{y[0], y[1], y[2], y[3]};
       *reinterpret_cast<f32x4*>(o + 4) = f32x4{y[4], y[5], y[6], y[7]};
     } else {
-      uint16_t* o = reinterpret_cast<uint16_t*>(part.y) + tt * yt + h * yh + c * 8;
-      *reinterpret_cast<u32x4*>(o) = u32x4{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7])};
+      u32x4* o = reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(part.y) + tt * yt + h * yh + c * 8);
+      const u32x4 w = {pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7])};
+      if (STREAM) __builtin_nontemporal_store(w, o);
+      else *o = w;
     }
   }
 }
@@ -183,10 +193,14 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkParams p) {
 template <int D, bool XF32, bool YF32, int HPT>
 hipError_t launch(const QkParams& p0, hipStream_t stream) {
   QkParams p = p0;
-  p.groups0 = (int)((p.part[0].heads + HPT - 1) / HPT);
-  const int groups = p.groups0 + (int)((p.part[1].heads + HPT - 1) / HPT);
   constexpr int TPB = 256 / (D / 8);
-  hipLaunchKernelGGL((qk_norm_rope_kernel<D, XF32, YF32, HPT>), dim3((unsigned)((p.T + TPB - 1) / TPB), (unsigned)groups), dim3(256), 0, stream, p);
+  p.groups0 = (int)((p.part[0].heads + HPT - 1) / HPT);
+  p.groups = p.groups0 + (int)((p.part[1].heads + HPT - 1) / HPT);
+  p.blocks = (p.T + TPB - 1) / TPB;
+  p.heads_first = p.part[0].x_stride[1] < p.part[0].x_stride[0];
+  const dim3 grid((unsigned)((int64_t)p.blocks * p.groups));
+  if (HPT == 1 || YF32 || p.heads_first) hipLaunchKernelGGL((qk_norm_rope_kernel<D, XF32, YF32, HPT, false>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((qk_norm_rope_kernel<D, XF32, YF32, HPT, (HPT > 1 && !YF32)>), grid, dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 
@@ -211,7 +225,10 @@ hipError_t qk_norm_rope_launch(const aeris_qk_norm_rope& a, hipStream_t stream) 
   p.rotation = a.rotation; p.positions = a.R > 0 ? a.positions : nullptr;
   p.n_pos = p.positions ? (int)a.n_positions : a.P > 0 ? (int)a.P : 1;
   const bool xf = a.x_dtype == AERIS_F32, yf = a.y_dtype == AERIS_F32;
-  const bool many = a.tokens * a.head_dim >= 32768 * 8;
+  // one head a thread up to 1600 workgroups of that kind: 4096 tokens, 4 + 4 heads of 64 4.2 us, with four 4.8; 8192 6.2, 5.7; 2048 tokens, 3 + 3 of
+  // 128 3.8, 4.4; 4096 5.3, 5.0
+  const int64_t heads = a.parts[0].heads + (a.n_parts > 1 ? a.parts[1].heads : 0);
+  const bool many = a.tokens * a.head_dim / 2048 * heads >= 1600;
   if (a.head_dim == 32) return many ? launch_types<32, 4>(p, xf, yf, stream) : launch_types<32, 1>(p, xf, yf, stream);
   if (a.head_dim == 64) return many ? launch_types<64, 4>(p, xf, yf, stream) : launch_types<64, 1>(p, xf, yf, stream);
   return many ? launch_types<128, 4>(p, xf, yf, stream) : launch_types<128, 1>(p, xf, yf, stream);

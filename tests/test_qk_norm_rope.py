@@ -218,7 +218,7 @@ def test_refusals_without_a_gpu(pkg):
         assert call(**kw) == L.EINVAL, kw
         assert "aeris_qk_norm_rope_fwd" in L.last_error()
     for kw in [dict(D=48), dict(D=256), dict(D=2 ** 32 + 64), dict(R=8), dict(R=80), dict(R=-16), dict(R=2 ** 32), dict(tokens=2 ** 31 - 1),
-               dict(part={"heads": 40000}), dict(part={"heads": 32768}, n=2)]:
+               dict(part={"heads": 40000}), dict(part={"heads": 32768}, n=2), dict(part={"heads": 32767}, tokens=2 ** 31 - 100)]:
         assert call(**kw) == L.EUNSUPPORTED, kw
     assert L.lib().aeris_qk_norm_rope_fwd(None, None) == L.EINVAL
     with pytest.raises(RuntimeError, match="GPU"):
