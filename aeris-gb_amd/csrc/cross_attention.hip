@@ -11,11 +11,13 @@
 //                        multiplies the fp32 logits: q is not rounded again
 //   O^T += V^T P^T       V^T by the transposing LDS read, P^T straight from the accumulators of S^T, rounded to bf16; the row sum adds the
 //                        rounded values
-// Three ways to run that:
-//   cross_attention_kernel<.., SPLIT = false>  a workgroup = a block of a unit's rows, the unit's keys streamed past it
-//   cross_attention_kernel<.., SPLIT = true>   few rows: the chunks divided among workgroups, each leaves its sums in the workspace in fp32 and
-//                                              cross_attention_join_kernel adds them up, in their order
-//   cross_attention_resident_kernel            few keys and many rows: a workgroup keeps the unit's keys in LDS and walks down the rows
+// Three ways to run that, and parts:
+//   cross_attention_rows_kernel      many rows: a workgroup = a block of a unit's rows, the unit's keys streamed past its waves
+//   cross_attention_keys_kernel      few rows: the waves of a workgroup divide the keys among them for the same rows
+//   cross_attention_resident_kernel  few keys and many rows: a workgroup keeps the unit's keys in LDS and walks down the rows
+//   PARTS of the first two           fewer rows still: the keys divided among workgroups too, each leaves its sums in the workspace in fp32 and
+//                                    cross_attention_join_kernel adds them up, in their order
+// plan_of() chooses, by what each would cost.  1000 queries x 1000 keys, eight heads of 64: rows kernel 13.1 us, keys kernel 9.2; 4000 x 77: 6.1 and 9.4.
 #include "common.h"
 #include "kernels.h"
 #include <type_traits>
@@ -34,9 +36,10 @@ struct Task {
   int rows;          // of a unit
   int qblks, splits; // workgroups of a unit: row blocks, parts of the keys
   int units;         // splits * members * key heads
+  int together;      // key heads that an XCD takes at a time: one or all
   int by_rows;       // workgroups of an XCD: all units in turn, an eighth of the row blocks (else: an eighth of the units)
   int first;         // its first workgroup
-  float *o, *ml;     // SPLIT: [split][member][key head][row][HD], [..][2] = maximum, sum
+  float *o, *ml;     // PARTS: [split][member][key head][row][HD], [..][2] = maximum, sum
 };
 
 struct CrossParams {
@@ -61,7 +64,7 @@ template <int HD>
 __device__ __forceinline__ int v_swizzle(int row) { return HD == 128 ? 2 * (row & 7) : HD == 64 ? 2 * ((row >> 1) & 3) : 2 * ((row >> 2) & 1); }
 
 // The first `n` of 64 keys, n >= 0
-__device__ __forceinline__ uint64_t first_keys(int n) { return n >= KC ? ~0ull : (1ull << n) - 1; }
+__device__ __forceinline__ uint64_t first_keys(int n) { return n >= 64 ? ~0ull : (1ull << n) - 1; }
 
 // A wave's 16 QN rows: queries, sums, and what a chunk in LDS does to them.
 // SUM: the row sums by the matrix cores too (a product with ones), four VALU operations fewer per 8 weights and one MFMA more per 4 to 8.
@@ -255,6 +258,79 @@ struct Rows {
     __builtin_amdgcn_sched_barrier(0);
   }
 
+  // 32 keys, whose 64 or fewer rows of K and V lie `at` bytes behind the first: as chunk(), for waves that divide the keys among them
+  template <bool FAST>
+  __device__ __forceinline__ void step(uint32_t at, uint32_t keys) {
+    TrFrag vt[DB];
+    f32x4 acc[QN][2];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {  // (ahead of the MFMAs, see chunk())
+      vt[d].lo = lds_read_tr16_b64<0>(v_tr[d] + at);
+      vt[d].hi = lds_read_tr16_b64<16 * (HD * 2)>(v_tr[d] + at);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    {
+      const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
+      typedef __attribute__((address_space(3))) const bf16x8* frag_ptr;
+      bf16x8 kf[2][KS];
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) kf[b][s] = *(frag_ptr)(k_lane[s] + at + b * 16 * (HD * 2));
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int n = 0; n < QN; ++n) acc[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[b][s], qf[n][s], s == 0 ? zero4 : acc[n][b], 0, 0, 0);
+    }
+    if (!FAST) {
+      const uint32_t mine = keys >> (4 * q4);
+#pragma unroll
+      for (int n = 0; n < QN; ++n) {
+        float cm = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (!((mine >> (b * 16 + i)) & 1)) acc[n][b][i] = -INFINITY;
+            cm = fmaxf(cm, acc[n][b][i]);
+          }
+        cm = fmaxf(cm, __shfl_xor(cm, 16, 64));
+        cm = fmaxf(cm, __shfl_xor(cm, 32, 64));
+        if (SCALED) cm *= q_mul;
+        const float m_new = fmaxf(m[n], cm), alpha = __builtin_amdgcn_exp2f(m[n] - m_new);
+        l[n] *= alpha;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[n][db] *= alpha;
+        m[n] = m_new;
+      }
+    }
+    uint32_t pk[QN][4];
+#pragma unroll
+    for (int n = 0; n < QN; ++n)
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const f32x4& a = acc[n][h >> 1];
+        auto p_of = [&](float x) { return __builtin_amdgcn_exp2f(SCALED ? (FAST ? x * q_mul : fmaf(x, q_mul, -m[n])) : FAST ? x : x - m[n]); };
+        pk[n][h] = pack_bf16x2(p_of(a[2 * (h & 1)]), p_of(a[2 * (h & 1) + 1]));
+        l[n] = dot2_ones(pk[n][h], l[n]);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (DB == 2) {
+      lds_tr_wait(vt[0], vt[1 % DB]);
+    } else {
+      lds_tr_wait(vt[0], vt[1 % DB], vt[2 % DB], vt[3 % DB]);
+      if constexpr (DB == 8) lds_tr_wait(vt[4 % DB], vt[5 % DB], vt[6 % DB], vt[7 % DB]);
+    }
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int n = 0; n < QN; ++n)
+        o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(tr_frag_value(vt[d]), __builtin_bit_cast(bf16x8, u32x4{pk[n][0], pk[n][1], pk[n][2], pk[n][3]}), o[n][d], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
   // The rows' sums, `idle` keys of the chunks that did not take part taken out of them.  Whether any row's left the range in which exp2 needs no
   // maximum (or is not a number), or is so small beside the idle keys' ones that their difference says little.
   __device__ __forceinline__ bool sums(int idle) {
@@ -290,7 +366,8 @@ struct Rows {
   }
 };
 
-// A unit's keys, chunk by chunk: the prefix, then the member's own.
+// A unit's keys in chunks of U: the prefix, then the member's own.
+template <int U>
 struct Keys {
   const unsigned char *k, *v;          // of the chunk that is loaded next
   const unsigned char *k_own, *v_own;  // of the member's first key
@@ -305,42 +382,48 @@ struct Keys {
       own = __builtin_amdgcn_readfirstlane(p.lengths[member * p.lengths_step]);
       own = own < 0 ? 0 : own < t.Nk ? own : t.Nk;
     }
-    prefix_chunks = (t.Np + KC - 1) / KC;
-    chunks = prefix_chunks + (own + KC - 1) / KC;
+    prefix_chunks = (t.Np + U - 1) / U;
+    chunks = prefix_chunks + (own + U - 1) / U;
     k_own = reinterpret_cast<const unsigned char*>(p.k + member * p.k_batch + hk * p.k_head);
     v_own = reinterpret_cast<const unsigned char*>(p.v + member * p.v_batch + hk * p.v_head);
+  }
+  // the chunks of one part: as many for each, the same for members of any length
+  __device__ __forceinline__ void part(const Task& t, int split, int& c0, int& c1) const {
+    const int all = (t.Np + U - 1) / U + (t.Nk + U - 1) / U, each = (all + t.splits - 1) / t.splits;
+    c0 = each * split < chunks ? each * split : chunks;
+    c1 = c0 + each < chunks ? c0 + each : chunks;
   }
   __device__ __forceinline__ void seek(const CrossParams& p, const Task& t, int hk, int c) {
     if (c < prefix_chunks) {
       k_row = p.prefix_k_row;
       v_row = p.prefix_v_row;
-      k = reinterpret_cast<const unsigned char*>(p.prefix_k + hk * p.prefix_k_head) + (int64_t)c * KC * k_row;
-      v = reinterpret_cast<const unsigned char*>(p.prefix_v + hk * p.prefix_v_head) + (int64_t)c * KC * v_row;
-      left = t.Np - c * KC;
+      k = reinterpret_cast<const unsigned char*>(p.prefix_k + hk * p.prefix_k_head) + (int64_t)c * U * k_row;
+      v = reinterpret_cast<const unsigned char*>(p.prefix_v + hk * p.prefix_v_head) + (int64_t)c * U * v_row;
+      left = t.Np - c * U;
     } else {
       c -= prefix_chunks;
       k_row = p.k_row;
       v_row = p.v_row;
-      k = k_own + (int64_t)c * KC * k_row;
-      v = v_own + (int64_t)c * KC * v_row;
-      left = own - c * KC;
+      k = k_own + (int64_t)c * U * k_row;
+      v = v_own + (int64_t)c * U * v_row;
+      left = own - c * U;
     }
   }
 };
 
-// Loads of a chunk into LDS: instruction i of wave w fills the rows RPI * (w + NWAVE * i) .., lane = (row, 16-byte slot).
-template <int HD, int NWAVE>
+// Loads of a chunk of U keys into LDS by NWAVE waves: instruction i of wave w fills the rows RPI * (w + NWAVE * i) .., lane = (row, 16-byte slot).
+template <int HD, int NWAVE, int U>
 struct Loader {
-  static constexpr int BYTES = KC * HD * 2;  // of a chunk of K or of V
-  static constexpr int PPR = HD / 8;         // 16-byte pieces per row
-  static constexpr int RPI = 64 / PPR;       // rows that one load instruction of a wave fills
-  static constexpr int LOADS = KC / (RPI * NWAVE);
-  static_assert(KC % (RPI * NWAVE) == 0, "a chunk is a whole number of instructions of each wave");
-  int row0, wave;               // the lane's row of instruction 0
+  static constexpr int BYTES = U * HD * 2;  // of a chunk of K or of V
+  static constexpr int PPR = HD / 8;        // 16-byte pieces per row
+  static constexpr int RPI = 64 / PPR;      // rows that one load instruction of a wave fills
+  static constexpr int LOADS = U / (RPI * NWAVE);
+  static_assert(U % (RPI * NWAVE) == 0, "a chunk is a whole number of instructions of each wave");
+  int row0, wave;  // the lane's row of instruction 0
   uint32_t off_k[LOADS], off_v[LOADS];
 
   __device__ __forceinline__ Loader(int lane, int w) : row0(RPI * w + lane / PPR), wave(w) {}
-  __device__ __forceinline__ void rows(int lane, const Keys& keys) {  // where the lane's pieces lie in a chunk, for the rows' present strides
+  __device__ __forceinline__ void rows(int lane, const Keys<U>& keys) {  // where the lane's pieces lie in a chunk, for the rows' present strides
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int row = row0 + RPI * NWAVE * i, slot = lane % PPR;
@@ -348,11 +431,10 @@ struct Loader {
       off_v[i] = __umul24(row, keys.v_row) + (uint32_t)((slot ^ v_swizzle<HD>(row)) << 4);
     }
   }
-  // the chunk that `keys` stands at, into LDS at k_lds and v_lds; then on to the next one.  Bit i of `word`: key i takes part.
-  __device__ __forceinline__ void issue(const CrossParams& p, const Task& t, int hk, int lane, Keys& keys, int c, uint64_t word, uint32_t k_lds,
-                                        uint32_t v_lds) {
+  // the chunk that `keys` stands at, into LDS at k_lds and v_lds.  Bit i of `word`: key i takes part.
+  __device__ __forceinline__ void issue(const Keys<U>& keys, uint64_t word, uint32_t k_lds, uint32_t v_lds) const {
     const lds_dma_rsrc rk = make_lds_dma_rsrc(keys.k, 0x80000000u), rv = make_lds_dma_rsrc(keys.v, 0x80000000u);
-    if (word == ~0ull) {
+    if (word == (U == 64 ? ~0ull : 0xffffffffull)) {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         lds_dma_load16(rk, k_lds + (uint32_t)(wave + NWAVE * i) * 1024, off_k[i], 0);
@@ -366,22 +448,27 @@ struct Loader {
         lds_dma_load16(rv, v_lds + (uint32_t)(wave + NWAVE * i) * 1024, on ? off_v[i] : 0xFFFFF000u, 0);
       }
     }
+  }
+  // the same, then on to the next chunk (number c + 1)
+  __device__ __forceinline__ void issue_next(const CrossParams& p, const Task& t, int hk, int lane, Keys<U>& keys, int c, uint64_t word, uint32_t k_lds,
+                                             uint32_t v_lds) {
+    issue(keys, word, k_lds, v_lds);
     if (c + 1 == keys.prefix_chunks) {
       keys.seek(p, t, hk, c + 1);
       rows(lane, keys);
     } else {
-      keys.k += (int64_t)KC * keys.k_row;
-      keys.v += (int64_t)KC * keys.v_row;
-      keys.left -= KC;
+      keys.k += (int64_t)U * keys.k_row;
+      keys.v += (int64_t)U * keys.v_row;
+      keys.left -= U;
     }
   }
 };
 
-// The key mask of a workgroup's chunks c0 .. c1 as words of 64 bits in LDS (of the prefix: all ones)
-template <int NWAVE>
-__device__ __forceinline__ void mask_words(const uint8_t* mask, const Keys& keys, int c0, int c1, uint64_t* words, int lane, int wave) {
+// The key mask of a workgroup's chunks c0 .. c1 as words of 64 bits in LDS (of the prefix: all ones; of chunks of 32 keys the low half counts)
+template <int NWAVE, int U>
+__device__ __forceinline__ void mask_words(const uint8_t* mask, const Keys<U>& keys, int c0, int c1, uint64_t* words, int lane, int wave) {
   for (int c = c0 + wave; c < c1; c += NWAVE) {
-    const int key = (c - keys.prefix_chunks) * KC + lane;
+    const int key = (c - keys.prefix_chunks) * U + lane;
     const bool on = key < 0 || (key < keys.own && mask[key < keys.own ? key : 0] != 0);
     const uint64_t word = c < keys.prefix_chunks ? ~0ull : __builtin_amdgcn_ballot_w64(on);
     if (lane == 0) words[c - c0] = word;
@@ -393,12 +480,37 @@ __device__ __forceinline__ uint64_t uniform64(uint64_t x) {
 
 }  // namespace
 
+// The workgroup's unit (part of the keys, member, key head) and row block, and whether there is work for it.  XCDs take units in turn, or all heads of a
+// member's part at a time (`together`): rows of heads that lie side by side share lines of memory and its pages (64 members of 8000 keys, four heads of
+// 32: 80 -> 41 us against heads on XCDs in turn; 256 of 500 keys, eight of 64: 42 -> 40.5).  Each turn starts one XCD further: lengths, and with them
+// work, fall along members and parts, and none of them always goes to the same XCD.
+__device__ __forceinline__ bool place(const CrossParams& p, const Task& t, int block, int& split, int& member, int& hk, int& qb) {
+  const int at = block - t.first, xcd = at & 7, s = at >> 3;  // (a task's first workgroup is a multiple of 8)
+  int unit;
+  if (t.by_rows) {
+    const int per = (t.qblks + 7) / 8;
+    unit = s / per;
+    qb = xcd * per + s % per;
+  } else {
+    const int i = s / t.qblks, turn = i / t.together;
+    unit = (8 * turn + ((xcd + turn) & 7)) * t.together + i - turn * t.together;
+    qb = s % t.qblks;
+  }
+  if (unit >= t.units || qb >= t.qblks) return false;
+  const int bm = unit / p.kv_heads;
+  hk = unit - bm * p.kv_heads;
+  split = bm / t.members;
+  member = bm - split * t.members;
+  return true;
+}
+
 // K and V in two buffers: a chunk is loaded while the one before is worked on.  (Three and four buffers: the same times, with a row block alone on its
 // CU too - a chunk takes a wave longer, 0.5 us and more, than its load.)
-template <int HD, int NWAVE, int QN, bool SPLIT, bool SCALED, bool SUM>
+// PARTS: the keys are divided among workgroups, which leave their sums in the workspace.
+template <int HD, int NWAVE, int QN, bool PARTS, bool SCALED, bool SUM>
 __global__ void __launch_bounds__(64 * NWAVE) __attribute__((amdgpu_waves_per_eu(2)))
-cross_attention_kernel(CrossParams p) {
-  using Load = Loader<HD, NWAVE>;
+cross_attention_rows_kernel(CrossParams p) {
+  using Load = Loader<HD, NWAVE, KC>;
   constexpr int BYTES = Load::BYTES, V_BASE = 2 * BYTES;
   constexpr int QW = 16 * QN, QB = QW * NWAVE;  // rows per wave and workgroup
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -406,30 +518,12 @@ cross_attention_kernel(CrossParams p) {
   const uint32_t smem_addr = lds_byte_address(smem);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  const Task& t = p.task[SPLIT && (int)blockIdx.x >= p.task[1].first ? 1 : 0];
-  int unit, qb;
-  {
-    const int at = blockIdx.x - t.first, xcd = at & 7, s = at >> 3;  // (a task's first workgroup is a multiple of 8)
-    if (t.by_rows) {
-      const int per = (t.qblks + 7) / 8;
-      unit = s / per;
-      qb = xcd * per + s % per;
-    } else {
-      unit = xcd + 8 * (s / t.qblks);
-      qb = s % t.qblks;
-    }
-    if (unit >= t.units || qb >= t.qblks) return;
-  }
-  const int split = unit / (t.members * p.kv_heads);
-  const int bh = unit - split * (t.members * p.kv_heads);
-  const int member = bh / p.kv_heads, hk = bh - member * p.kv_heads;
-  Keys keys(p, t, member, hk);
+  const Task& t = p.task[PARTS && (int)blockIdx.x >= p.task[1].first ? 1 : 0];
+  int split, member, hk, qb;
+  if (!place(p, t, blockIdx.x, split, member, hk, qb)) return;
+  Keys<KC> keys(p, t, member, hk);
   int c0 = 0, c1 = keys.chunks;
-  if (SPLIT) {
-    const int all = (t.Np + KC - 1) / KC + (t.Nk + KC - 1) / KC, each = (all + t.splits - 1) / t.splits;  // (the same for members of any length)
-    c0 = each * split < keys.chunks ? each * split : keys.chunks;
-    c1 = c0 + each < keys.chunks ? c0 + each : keys.chunks;
-  }
+  if (PARTS) keys.part(t, split, c0, c1);
   const int nch = c1 - c0;
 
   const int row0 = qb * QB + wave * QW;
@@ -440,18 +534,14 @@ cross_attention_kernel(CrossParams p) {
 
   const bool masked = p.mask && t.Nk > 0;
   if (masked) {
-    mask_words<NWAVE>(p.mask + member * p.mask_batch, keys, c0, c1, words, lane, wave);
+    mask_words<NWAVE, KC>(p.mask + member * p.mask_batch, keys, c0, c1, words, lane, wave);
     __syncthreads();
   }
-  auto word_of = [&](int j) {  // of chunk c0 + j, which `keys` stands at
-    uint64_t w = first_keys(keys.left);
-    if (masked) w &= uniform64(words[j]);
-    return w;
-  };
-  uint64_t kk[2];  // of the chunks in the buffers
+  uint64_t kk[2];  // which keys of the chunks in the buffers take part
   auto issue = [&](int j, int buf) {
-    kk[buf] = word_of(j);
-    load.issue(p, t, hk, lane, keys, c0 + j, kk[buf], smem_addr + buf * BYTES, smem_addr + V_BASE + buf * BYTES);
+    kk[buf] = first_keys(keys.left);
+    if (masked) kk[buf] &= uniform64(words[j]);
+    load.issue_next(p, t, hk, lane, keys, c0 + j, kk[buf], smem_addr + buf * BYTES, smem_addr + V_BASE + buf * BYTES);
   };
   bool any = false;  // whether any key took part (uniform)
   int idle = 0;      // keys that did not, of chunks with keys that did
@@ -482,7 +572,7 @@ cross_attention_kernel(CrossParams p) {
     }
   };
   sweep(std::true_type{});
-  bool online = false;
+  bool online;
   {
     __syncthreads();  // every wave is done with the chunks: a flag in their place
     int* const redo = reinterpret_cast<int*>(smem);
@@ -497,15 +587,15 @@ cross_attention_kernel(CrossParams p) {
       rows.sums(0);
     }
   }
-  if (!SPLIT) {
+  if (!PARTS) {
     rows.store(p.out, to, row0, t.rows, lane);
     return;
   }
 #pragma unroll
   for (int n = 0; n < QN; ++n) {
     const int row = row0 + n * 16 + (lane & 15);
-    const int64_t at = ((int64_t)split * t.members * p.kv_heads + bh) * t.rows + row;
     if (row >= t.rows) continue;
+    const int64_t at = (((int64_t)split * t.members + member) * p.kv_heads + hk) * t.rows + row;
     if (rows.q4 == 0) {
       t.ml[2 * at] = online ? rows.m[n] : 0.f;
       t.ml[2 * at + 1] = rows.l[n];
@@ -516,12 +606,141 @@ cross_attention_kernel(CrossParams p) {
   }
 }
 
+// Few rows: the waves of a workgroup divide the keys among them, 32 at a time in turn, for the same 16 QN rows; each has its own buffers, RB of them, and
+// keeps its own pace.  Their sums meet in LDS.  PARTS: the keys are divided among workgroups too, which leave theirs in the workspace.
+template <int HD, int NWAVE, int QN, int RB, bool PARTS>
+__global__ void __launch_bounds__(64 * NWAVE) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 1 : 2)))
+cross_attention_keys_kernel(CrossParams p) {
+  constexpr int U = 32, QB = 16 * QN;
+  using Load = Loader<HD, 1, U>;
+  constexpr int BYTES = Load::BYTES, RING = RB * 2 * BYTES;  // of K or V of a step; of a wave's buffers
+  constexpr int LPS = 2 * Load::LOADS;                       // load instructions per step
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  uint64_t* const words = reinterpret_cast<uint64_t*>(smem + NWAVE * RING);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  unsigned char* const ring = smem + wave * RING;
+  const uint32_t ring_addr = lds_byte_address(ring);
+
+  const Task& t = p.task[PARTS && (int)blockIdx.x >= p.task[1].first ? 1 : 0];
+  int split, member, hk, qb;
+  if (!place(p, t, blockIdx.x, split, member, hk, qb)) return;
+  Keys<U> keys(p, t, member, hk);
+  int c0 = 0, c1 = keys.chunks;
+  if (PARTS) keys.part(t, split, c0, c1);
+  const int row0 = qb * QB;
+  Rows<HD, QN, true, false> rows(ring, BYTES, lane, p.q_mul);
+  Load load(lane, 0);
+  const bool masked = p.mask && t.Nk > 0;
+  if (masked) {
+    mask_words<NWAVE, U>(p.mask + member * p.mask_batch, keys, c0, c1, words, lane, wave);
+    __syncthreads();
+  }
+  const int steps = (c1 - c0 - wave + NWAVE - 1) / NWAVE;  // of this wave: c0 + wave, c0 + wave + NWAVE, ..
+  uint32_t kk[RB];
+  int part_of = -1;  // whose rows' strides the loader has: 0 the prefix's, 1 the member's own
+  auto issue = [&](int j, int buf) {
+    const int c = c0 + wave + j * NWAVE;
+    keys.seek(p, t, hk, c);
+    if (part_of != (c >= keys.prefix_chunks)) {
+      part_of = c >= keys.prefix_chunks;
+      load.rows(lane, keys);
+    }
+    uint64_t w = first_keys(keys.left < U ? keys.left : U);
+    if (masked) w &= uniform64(words[c - c0]);
+    kk[buf] = (uint32_t)w;
+    load.issue(keys, w & 0xffffffffull, ring_addr + buf * 2 * BYTES, ring_addr + buf * 2 * BYTES + BYTES);
+  };
+  bool any = false;
+  int idle = 0;
+  auto sweep = [&](auto fast_tag) {
+    constexpr bool FAST = decltype(fast_tag)::value;
+#pragma unroll
+    for (int u = 0; u < RB - 1; ++u)
+      if (u < steps) issue(u, u);
+    if (FAST) {
+      int64_t to[QN];
+      rows.load_q(p, t.rows, member, hk, row0, lane, to, rows.qf);
+    }
+    rows.reset();
+    if (FAST) __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0), see the kernel above
+    for (int j0 = 0; j0 < steps; j0 += RB) {
+#pragma unroll
+      for (int u = 0; u < RB; ++u) {
+        const int j = j0 + u;
+        if (j >= steps) break;
+        // step j's buffers are filled (younger loads: those of the steps behind it); then the buffers that step j - 1 was done with are loaded again
+        if (RB > 2 && j + RB - 2 < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((RB - 2) * LPS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (j + RB - 1 < steps) issue(j + RB - 1, (u + RB - 1) % RB);
+        if (kk[u] != 0) {
+          any = true;
+          if (FAST) idle += U - __builtin_popcount(kk[u]);
+          rows.template step<FAST>(u * 2 * BYTES, kk[u]);
+        }
+      }
+    }
+  };
+  sweep(std::true_type{});
+  const bool online = rows.sums(idle) && any;
+  if (online) {
+    sweep(std::false_type{});
+    rows.sums(0);
+  }
+
+  // ---- the waves' sums: [wave][row][HD] fp32, 16-byte pieces XOR-swizzled by the row, and [wave][row] maximum, sum
+  __syncthreads();
+  f32x4* const so = reinterpret_cast<f32x4*>(smem);
+  float* const sm = reinterpret_cast<float*>(smem + NWAVE * QB * HD * 4);
+  constexpr int PIECES = HD / 4, SWZ = PIECES < 16 ? PIECES - 1 : 15;
+  auto piece = [](int w, int row, int c) { return (w * QB + row) * PIECES + (c ^ (row & SWZ)); };
+#pragma unroll
+  for (int n = 0; n < QN; ++n) {
+    const int row = 16 * n + (lane & 15);
+    if (rows.q4 == 0) {
+      sm[2 * (wave * QB + row)] = online ? rows.m[n] : any ? 0.f : -3.0e38f;
+      sm[2 * (wave * QB + row) + 1] = any ? rows.l[n] : 0.f;
+    }
+#pragma unroll
+    for (int db = 0; db < HD / 16; ++db) so[piece(wave, row, 4 * db + rows.q4)] = rows.o[n][db];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < (QB * PIECES + 64 * NWAVE - 1) / (64 * NWAVE); ++i) {
+    const int at = i * 64 * NWAVE + tid, row = at / PIECES, c = at % PIECES;
+    const int r = row0 + row;
+    if (row >= QB || r >= t.rows) continue;
+    float m = -3.0e38f, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NWAVE; ++w) m = fmaxf(m, sm[2 * (w * QB + row)]);
+#pragma unroll
+    for (int w = 0; w < NWAVE; ++w) {
+      const float a = __builtin_amdgcn_exp2f(sm[2 * (w * QB + row)] - m);
+      l += a * sm[2 * (w * QB + row) + 1];
+      o += a * so[piece(w, row, c)];
+    }
+    if (PARTS) {
+      const int64_t dst = (((int64_t)split * t.members + member) * p.kv_heads + hk) * t.rows + r;
+      if (c == 0) {
+        t.ml[2 * dst] = m;
+        t.ml[2 * dst + 1] = l;
+      }
+      __builtin_nontemporal_store(o, reinterpret_cast<f32x4*>(t.o + dst * HD + 4 * c));
+    } else {
+      const int bb = r / p.rows_m, rm = r - bb * p.rows_m, query = rm / p.group, head = hk * p.group + rm - query * p.group;
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      *reinterpret_cast<u32x2*>(p.out + (((int64_t)(member + bb) * p.Nq + query) * p.heads + head) * HD + 4 * c) =
+          u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
+    }
+  }
+}
+
 // Few keys, many rows: the workgroup's unit stays in LDS, its waves walk down the row blocks, each at its own pace: no barrier behind the
 // first, a block's queries are fetched while the one before is worked on.  Task::qblks is the number of workgroups of a unit.
 template <int HD, int NWAVE, int QN, bool SCALED, bool SUM>
 __global__ void __launch_bounds__(64 * NWAVE) __attribute__((amdgpu_waves_per_eu(2)))
 cross_attention_resident_kernel(CrossParams p, int max_chunks) {
-  using Load = Loader<HD, NWAVE>;
+  using Load = Loader<HD, NWAVE, KC>;
   constexpr int BYTES = Load::BYTES, QW = 16 * QN;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const uint32_t v_base = (uint32_t)max_chunks * BYTES, smem_addr = lds_byte_address(smem);
@@ -530,10 +749,10 @@ cross_attention_resident_kernel(CrossParams p, int max_chunks) {
   const Task& t = p.task[0];
   const int unit = blockIdx.x % t.units, part = blockIdx.x / t.units;
   const int member = unit / p.kv_heads, hk = unit - member * p.kv_heads;
-  Keys keys(p, t, member, hk);
+  Keys<KC> keys(p, t, member, hk);
   const int nch = keys.chunks;
   if (p.mask && t.Nk > 0) {
-    mask_words<NWAVE>(p.mask + member * p.mask_batch, keys, 0, nch, words, lane, wave);
+    mask_words<NWAVE, KC>(p.mask + member * p.mask_batch, keys, 0, nch, words, lane, wave);
     __syncthreads();
   }
   Rows<HD, QN, SCALED, SUM> rows(smem, v_base, lane, p.q_mul);
@@ -555,7 +774,7 @@ cross_attention_resident_kernel(CrossParams p, int max_chunks) {
   for (int c = 0; c < nch; ++c) {
     const uint64_t w = word_of(c);
     idle += KC - __builtin_popcountll(w);
-    load.issue(p, t, hk, lane, keys, c, w, smem_addr + c * BYTES, smem_addr + v_base + c * BYTES);
+    load.issue_next(p, t, hk, lane, keys, c, w, smem_addr + c * BYTES, smem_addr + v_base + c * BYTES);
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   __syncthreads();
@@ -600,10 +819,11 @@ struct JoinParams {
 }  // namespace
 
 // out[row] = sum over the parts of 2^(m - max m) o / sum of 2^(m - max m) l.  WPR waves do a row, each every WPR-th part: lane i looks at part i's
-// maximum and sum, the weights then go round by lane exchange, and HD / 4 lanes read a part's row, 64 / (HD / 4) parts at a time.  What it costs is the
-// latency of two reads behind one another.
+// maximum and sum, the weights then go round by lane exchange, and HD / 4 lanes read a part's row, 16 parts on the way at a time.  What it costs, 4 to 5 us,
+// is the latency of two reads behind one another (a part at a time: 8 us for 16 of head size 128).
 template <int HD, int WPR>
 __global__ void __launch_bounds__(WPR > 4 ? 64 * WPR : 256) cross_attention_join_kernel(JoinParams p) {
+  constexpr int AT_ONCE = 16;  // parts (8 and 32: half a microsecond more at 16 and at 64 parts)
   constexpr int CT = HD / 4, SUB = 64 / CT, NW = WPR > 4 ? WPR : 4;  // waves of a workgroup
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane % CT, sub = lane / CT, first_part = wave % WPR;
   const int64_t row = (int64_t)blockIdx.x * (NW / WPR) + wave / WPR;
@@ -636,15 +856,20 @@ __global__ void __launch_bounds__(WPR > 4 ? 64 * WPR : 256) cross_attention_join
         m = mn;
         l = l * a0 + wave_sum(w * pl);
         o *= a0;
-#pragma unroll 4
-        for (int i = sub; i < 64; i += SUB) {
-          if (i - sub >= n) break;
-          const float wi = __shfl(w, i, 64);
-          const int64_t at = first + (s0 + (i < n ? i : n - 1) * WPR) * step;
-          const f32x4 po = *reinterpret_cast<const f32x4*>(t.o + at * HD + 4 * c);
-          // (a part without keys has written nothing)
+        for (int i0 = 0; i0 < n; i0 += AT_ONCE) {
+          float wi[AT_ONCE / SUB];
+          f32x4 po[AT_ONCE / SUB];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] += wi == 0.f ? 0.f : po[e] * wi;
+          for (int u = 0; u < AT_ONCE / SUB; ++u) {
+            const int i = i0 + u * SUB + sub;
+            wi[u] = __shfl(w, i, 64);
+            const int64_t at = first + (s0 + (i < n ? i : n - 1) * WPR) * step;
+            po[u] = *reinterpret_cast<const f32x4*>(t.o + at * HD + 4 * c);
+          }
+#pragma unroll
+          for (int u = 0; u < AT_ONCE / SUB; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += wi[u] == 0.f ? 0.f : po[u][e] * wi[u];  // (a part without keys has written nothing)
         }
       }
     }
@@ -689,37 +914,62 @@ constexpr int NWAVE = 4;
 constexpr int resident_qn(int64_t head_dim) { return head_dim == 64 ? 3 : 2; }
 constexpr int64_t RESIDENT_LDS = 80 * 1024;  // two workgroups per CU
 
+// How a call is run
+enum class Form { rows, keys, resident };
 struct Plan {
   Task task[2];
-  int n, qn;
-  bool split;
-  int resident;  // chunks that a workgroup keeps in LDS (0: they are streamed)
+  Form form;
+  int n, qn;    // tasks; blocks of 16 rows per wave
+  bool parts;   // sums go through the workspace
+  int resident; // chunks that a workgroup keeps in LDS
   int64_t grid, words, bytes;  // workgroups; mask words of a workgroup; of the workspace
 };
 
 int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// Microseconds of a launch, fitted to measurements (60 to 8000 queries, 300 to 4000 keys, 4 and 8 heads): what a chunk takes a workgroup alone on
-// its CU, and one of several; the start; and for parts of the keys the joining kernel and what the parts' sums cost to write and read.
-struct Times {
-  float alone[2], among[2];  // 16 and 32 rows per wave
-  float chunk(int64_t wgs, int qn) const {
-    const float several = among[qn - 1] * div_up(wgs, 256);
-    return several > alone[qn - 1] ? several : alone[qn - 1];
-  }
-  float whole(int64_t units, int rows, int64_t chunks, int qn) const { return 4.2f + chunks * chunk(units * div_up(rows, 64 * qn), qn); }
-  float in_parts(int64_t units, int rows, int64_t chunks, int qn, int s, int head_dim) const {
-    const float mb = 4e-6f * units * rows * s * head_dim;
-    return 4.2f + div_up(chunks, s) * chunk(units * div_up(rows, 64 * qn) * s, qn) + (s > 1 ? 6.0f + 0.55f * mb : 0.f);
-  }
+// Microseconds of a launch, fitted to measurements (1 to 8000 queries, 77 to 4000 keys, 4 and 8 heads): a workgroup's step - a chunk of 64 keys, or 32
+// keys for each of its waves - alone on its CU, and one of several there; what a round of workgroups costs besides; how many a CU holds.
+struct Cost { float alone, among, round; };
+struct Costs {
+  Cost rows[2], keys[3];  // 16 and 32 rows per wave; 16, 32 and 64 per workgroup
+  int rows_per_cu, keys_per_cu;
 };
-const Times& times_of(int64_t head_dim) {
-  static const Times t32 = {{0.48f, 0.56f}, {0.25f, 0.40f}}, t64 = {{0.56f, 0.75f}, {0.40f, 0.55f}}, t128 = {{0.84f, 1.12f}, {0.65f, 0.95f}};
-  return head_dim == 32 ? t32 : head_dim == 64 ? t64 : t128;
+const Costs& costs_of(int64_t head_dim) {
+  static const Costs c32 = {{{0.48f, 0.25f, 1.6f}, {0.56f, 0.40f, 1.9f}}, {{0.32f, 0.27f, 1.2f}, {0.41f, 0.30f, 1.6f}, {0.57f, 0.45f, 2.4f}}, 4, 4};
+  static const Costs c64 = {{{0.56f, 0.40f, 1.8f}, {0.75f, 0.55f, 2.2f}}, {{0.40f, 0.30f, 1.7f}, {0.48f, 0.39f, 2.4f}, {0.70f, 0.65f, 3.6f}}, 3, 2};
+  static const Costs c128 = {{{0.86f, 0.65f, 1.9f}, {1.12f, 0.95f, 2.3f}}, {{0.60f, 0.68f, 2.0f}, {0.75f, 0.85f, 3.2f}, {1.05f, 1.20f, 5.5f}}, 2, 1};
+  return head_dim == 32 ? c32 : head_dim == 64 ? c64 : c128;
+}
+
+// One way to run a task: kernel, rows, parts of the keys, and what it costs
+struct Way {
+  Form form;
+  int qn, splits;
+  float us;
+};
+int rows_of(Form form, int qn) { return 16 * qn * (form == Form::rows ? NWAVE : 1); }
+int keys_of(Form form) { return form == Form::rows ? KC : 32; }
+int64_t chunks_of(const Task& t, int u) { return (int64_t)div_up(t.Np, u) + div_up(t.Nk, u); }
+Way way_of(const Task& t, int Hk, int head_dim, Form form, int qn, int splits) {
+  const Costs& c = costs_of(head_dim);
+  const Cost& one = form == Form::rows ? c.rows[qn - 1] : c.keys[qn / 2];
+  const int64_t wgs = (int64_t)t.members * Hk * div_up(t.rows, rows_of(form, qn)) * splits;
+  const int64_t chunks = div_up(chunks_of(t, keys_of(form)), splits), steps = form == Form::rows ? chunks : div_up(chunks, NWAVE);
+  const int rounds = div_up(wgs, 256 * (form == Form::rows ? c.rows_per_cu : c.keys_per_cu));
+  const float several = one.among * div_up(wgs, 256), step = several > one.alone ? several : one.alone;
+  float us = 2.4f + rounds * one.round + steps * step;
+  // reading the keys, at a rate that grows with what a CU has on its way (32 KB 5.1 TB/s, 64 KB 5.7), longer where the last round leaves part of the chip idle
+  const float slots = 256.f * (form == Form::rows ? c.rows_per_cu : c.keys_per_cu);
+  const float on_way = (wgs < slots ? wgs : slots) / 256.f * (form == Form::rows ? KC : 32 * NWAVE) * head_dim * 4;
+  const float read = 4e-6f * t.members * Hk * head_dim * ((float)t.Np + t.Nk) / 6.4f * (1.f + 8192.f / on_way) * (rounds > 1 ? rounds * slots / wgs : 1.f);
+  us = us > read ? us : read;
+  // the joining kernel, and what the parts' sums cost to write and read
+  if (splits > 1) us += 6.0f + 0.55f * 4e-6f * t.members * Hk * (float)t.rows * splits * head_dim;
+  return {form, qn, splits, us};
 }
 
 Plan plan_of(const CrossArgs& a) {
-  const int B = (int)a.B, Hk = (int)a.kv_heads, rows_m = (int)(a.Nq * (a.heads / a.kv_heads));
+  const int B = (int)a.B, Hk = (int)a.kv_heads, rows_m = (int)(a.Nq * (a.heads / a.kv_heads)), D = (int)a.head_dim;
   const bool own = a.Nk > 0, masked = a.key_mask && own;
   // every member sees the same keys: its rows are further rows of one unit
   const bool shared = !own || (a.k_batch_stride == 0 && a.v_batch_stride == 0 && (!a.lengths || a.lengths_stride == 0) &&
@@ -735,90 +985,117 @@ Plan plan_of(const CrossArgs& a) {
   };
   if (B == 1 || (shared && rows_m % 128 != 0)) {
     add(true, a.Nk, a.Np);
-  } else if (a.Np > 0 && own && rows_m < 128) {
+  } else if (a.Np > 0 && own && rows_m < 128) {  // the prefix once for all members
     add(true, 0, a.Np);
     add(false, a.Nk, 0);
-    plan.split = true;
+    plan.parts = true;
   } else {
     add(false, a.Nk, a.Np);
   }
-  auto chunks = [](const Task& t) { return (int64_t)div_up(t.Np, KC) + div_up(t.Nk, KC); };
-  // Rows per wave and parts of the keys, by the time that a launch of them takes (see Times)
-  const Times& tm = times_of(a.head_dim);
-  plan.qn = 2;
-  float best = 1e30f;
-  for (int qn = 1; qn <= 2 && !plan.split; ++qn) {  // whole
-    const float t = tm.whole(plan.task[0].members * Hk, plan.task[0].rows, chunks(plan.task[0]), qn);
-    if (t < best) {
-      best = t;
-      plan.qn = qn;
+  auto setup = [&](Form form, int qn) {
+    plan.form = form;
+    plan.qn = qn;
+    plan.grid = plan.words = plan.bytes = 0;
+    for (int i = 0; i < plan.n; ++i) {
+      Task& t = plan.task[i];
+      t.qblks = div_up(t.rows, rows_of(form, qn));
+      t.units = t.splits * t.members * Hk;
+      // an eighth of the units per XCD, whose L2 then holds their keys for all row blocks; all units on every XCD, one after the other, an eighth of
+      // the row blocks each, where the units do not divide among the XCDs and the row blocks do better.  Heads together where there are turns enough
+      // to even out lengths (two members of 1000 and 600 keys on four XCDs each: 245 -> 280 us), and as many on each XCD as one by one (528 workgroups for
+      // 504, where 512 fit, cost 12 per cent; lines of 128 bytes shared by heads of 32 are worth a sixteenth more)
+      const int64_t eighth = div_up(t.units, 8), together = div_up(t.units / Hk, 8) * (int64_t)Hk;
+      t.together = t.units / Hk >= 64 && 16 * together <= (D == 32 ? 17 : 16) * eighth ? Hk : 1;
+      const int64_t by_units = (t.together > 1 ? together : eighth) * t.qblks, by_rows = div_up(t.qblks, 8) * (int64_t)t.units;
+      t.by_rows = by_rows < by_units;
+      t.first = (int)plan.grid;
+      plan.grid += 8 * (t.by_rows ? by_rows : by_units);
+      const int64_t words = div_up(chunks_of(t, keys_of(form)), t.splits);
+      if (masked && t.Nk > 0 && words > plan.words) plan.words = words;
+      if (plan.parts) plan.bytes += ((int64_t)t.units * t.rows * (D + 2) * 4 + 255) / 256 * 256;
     }
-  }
-  int parts[2] = {1, 1}, split_qn = 1;
-  for (int i = 0; i < plan.n; ++i)
-    if (plan.task[i].rows > 64) split_qn = 2;
-  float in_parts = 0;
-  for (int i = 0; i < plan.n; ++i) {
-    const Task& t = plan.task[i];
-    const int64_t wgs = (int64_t)t.members * Hk * div_up(t.rows, 64 * split_qn);
-    float least = 1e30f;
-    for (int slots = 256; slots <= (a.head_dim == 128 ? 512 : 1024); slots += 256) {  // (head_dim 128: 64 KB of LDS each)
-      int64_t s = slots / wgs;
-      if (s > div_up(chunks(t), 3)) s = div_up(chunks(t), 3);
-      if (s < 1) s = 1;
-      const float x = tm.in_parts(t.members * Hk, t.rows, chunks(t), split_qn, (int)s, (int)a.head_dim);
-      if (x < least) {
-        least = x;
-        parts[i] = (int)s;
-      }
-    }
-    if (masked && t.Nk > 0 && (int64_t)parts[i] * MAX_WORDS < chunks(t)) parts[i] = div_up(chunks(t), MAX_WORDS);
-    in_parts = least > in_parts ? least : in_parts;
-  }
-  if (plan.n == 1 && (in_parts < best || (masked && chunks(plan.task[0]) > MAX_WORDS))) plan.split = true;
-  if (plan.split) {
-    plan.qn = split_qn;
-    for (int i = 0; i < plan.n; ++i) plan.task[i].splits = parts[i];
-  } else if (a.head_dim == 64 && chunks(plan.task[0]) >= 12 && (int64_t)plan.task[0].members * Hk * div_up(plan.task[0].rows, 256) >= 500) {
-    plan.qn = 4;  // long key ranges for many rows: 129 600 x 4000 keys, one head, 144 -> 132 us; 400 keys 69.5 -> 74.8, 500 workgroups on the mark
-  }
-  for (int i = 0; i < plan.n; ++i) {
-    Task& t = plan.task[i];
-    t.qblks = div_up(t.rows, 64 * plan.qn);
-    t.units = t.splits * t.members * Hk;
-    // an eighth of the units per XCD, whose L2 then holds their keys for all row blocks; all units on every XCD, one after the other, an
-    // eighth of the row blocks each, where the units do not divide among the XCDs and the row blocks do better
-    const int64_t by_units = div_up(t.units, 8) * (int64_t)t.qblks, by_rows = div_up(t.qblks, 8) * (int64_t)t.units;
-    t.by_rows = by_rows < by_units;
-    t.first = (int)plan.grid;
-    plan.grid += 8 * (t.by_rows ? by_rows : by_units);
-    if (masked && t.Nk > 0 && div_up(chunks(t), t.splits) > plan.words) plan.words = div_up(chunks(t), t.splits);
-    if (plan.split) plan.bytes += ((int64_t)t.units * t.rows * (a.head_dim + 2) * 4 + 255) / 256 * 256;
-  }
-  if (plan.n < 2) plan.task[1].first = 0x7fffffff;
-  if (!plan.split) {
+    if (plan.n < 2) plan.task[1].first = 0x7fffffff;
+  };
+
+  // Few keys and many rows: a workgroup's keys stay (at least two row blocks for each of its waves)
+  if (!plan.parts) {
     Task& t = plan.task[0];
-    const int64_t c = chunks(t), lds = c * (4 * KC * a.head_dim + 8);
-    const int64_t per = (lds <= RESIDENT_LDS / 2 ? 1024 : 512) / t.units, blocks = div_up(t.rows, 16 * resident_qn(a.head_dim) * NWAVE);
+    const int64_t c = chunks_of(t, KC), lds = c * (4 * KC * D + 8), units = (int64_t)t.members * Hk;
+    const int64_t per = (lds <= RESIDENT_LDS / 2 ? 1024 : 512) / units, blocks = div_up(t.rows, 16 * resident_qn(D) * NWAVE);
     if (c > 0 && lds <= RESIDENT_LDS && per > 0 && blocks >= 2 * per) {
+      plan.form = Form::resident;
       plan.resident = (int)c;
       t.qblks = (int)per;
-      plan.grid = per * t.units;
+      t.units = (int)units;
+      plan.grid = per * units;
+      return plan;
     }
   }
+  // Otherwise the way that costs least.  Parts of the keys: what fills the chip once, twice, ..; no more chunks in one than a mask's words cover
+  Way best{Form::rows, 1, 1, 1e30f};
+  int splits[2] = {1, 1};
+  for (int f = 0; f < 5; ++f) {
+    const Form form = f < 2 ? Form::rows : Form::keys;
+    const int qn = f < 2 ? f + 1 : 1 << (f - 2);
+    if (form == Form::rows && plan.parts && qn == 1) continue;
+    float us = 0.f;
+    int s[2] = {1, 1};
+    bool whole = true;
+    for (int i = 0; i < plan.n; ++i) {
+      const Task& t = plan.task[i];
+      const int64_t one = (int64_t)t.members * Hk * div_up(t.rows, rows_of(form, qn)), chunks = chunks_of(t, keys_of(form));
+      const int least = masked && t.Nk > 0 ? div_up(chunks, MAX_WORDS) : 1;
+      Way w = way_of(t, Hk, D, form, qn, least > 1 ? least : 1);
+      for (int slots = 256; slots <= 1024 && !(form == Form::rows && qn == 1); slots += 256) {
+        const int64_t n = slots / one < div_up(chunks, NWAVE) ? slots / one : div_up(chunks, NWAVE);
+        if (n <= 1 || n < least) continue;
+        const Way x = way_of(t, Hk, D, form, qn, (int)n);
+        if (x.us < w.us) w = x;
+      }
+      s[i] = w.splits;
+      us += w.us;
+      whole = whole && w.splits == 1;
+    }
+    if (form == Form::rows && qn == 1 && !whole) continue;  // (16 rows a wave: not in parts)
+    if (us < best.us) {
+      best = {form, qn, 1, us};
+      splits[0] = s[0];
+      splits[1] = s[1];
+    }
+  }
+  for (int i = 0; i < plan.n; ++i) {
+    plan.task[i].splits = splits[i];
+    plan.parts = plan.parts || splits[i] > 1;
+  }
+  // long key ranges for many rows, 64 rows a wave: 129 600 x 4000 keys, one head, 144 -> 132 us; 400 keys 69.5 -> 74.8, 500 workgroups on the mark
+  if (best.form == Form::rows && best.qn == 2 && !plan.parts && D == 64 && chunks_of(plan.task[0], KC) >= 12 &&
+      (int64_t)plan.task[0].members * Hk * div_up(plan.task[0].rows, 256) >= 500)
+    best.qn = 4;
+  setup(best.form, best.qn);
   return plan;
 }
 
-// the kernel for (parts of the keys, scaled here, blocks of 16 rows per wave), handed to `f` with its LDS bytes
+// the kernel for (sums through the workspace, scaled here, blocks of 16 rows per wave), handed to `f` with its LDS bytes (a mask's words aside)
 template <int HD, class F>
-hipError_t with_kernel(bool split, bool scaled, int qn, const F& f) {
+hipError_t with_rows_kernel(bool parts, bool scaled, int qn, const F& f) {
   constexpr int LDS = 8 * KC * HD;
   constexpr bool SUM = HD == 32;
-  if (split) return qn == 1 ? f(cross_attention_kernel<HD, NWAVE, 1, true, true, false>, LDS) : f(cross_attention_kernel<HD, NWAVE, 2, true, true, false>, LDS);
+  if (parts) return f(cross_attention_rows_kernel<HD, NWAVE, 2, true, true, false>, LDS);
   if constexpr (HD == 64)
-    if (qn == 4) return scaled ? f(cross_attention_kernel<HD, NWAVE, 4, false, true, true>, LDS) : f(cross_attention_kernel<HD, NWAVE, 4, false, false, true>, LDS);
-  if (qn == 1) return scaled ? f(cross_attention_kernel<HD, NWAVE, 1, false, true, SUM>, LDS) : f(cross_attention_kernel<HD, NWAVE, 1, false, false, SUM>, LDS);
-  return scaled ? f(cross_attention_kernel<HD, NWAVE, 2, false, true, SUM>, LDS) : f(cross_attention_kernel<HD, NWAVE, 2, false, false, SUM>, LDS);
+    if (qn == 4) return scaled ? f(cross_attention_rows_kernel<HD, NWAVE, 4, false, true, true>, LDS) : f(cross_attention_rows_kernel<HD, NWAVE, 4, false, false, true>, LDS);
+  if (qn == 1) return scaled ? f(cross_attention_rows_kernel<HD, NWAVE, 1, false, true, SUM>, LDS) : f(cross_attention_rows_kernel<HD, NWAVE, 1, false, false, SUM>, LDS);
+  return scaled ? f(cross_attention_rows_kernel<HD, NWAVE, 2, false, true, SUM>, LDS) : f(cross_attention_rows_kernel<HD, NWAVE, 2, false, false, SUM>, LDS);
+}
+// the same for (sums through the workspace, blocks of 16 rows); with the bytes that the waves' sums take in the end
+template <int HD, int QN, bool PARTS, class F>
+hipError_t with_keys_kernel_of(const F& f) {
+  return f(cross_attention_keys_kernel<HD, NWAVE, QN, 2, PARTS>, NWAVE * 2 * 4 * 32 * HD, NWAVE * 16 * QN * (HD + 2) * 4);
+}
+template <int HD, class F>
+hipError_t with_keys_kernel(bool parts, int qn, const F& f) {
+  if (qn == 4) return parts ? with_keys_kernel_of<HD, 4, true>(f) : with_keys_kernel_of<HD, 4, false>(f);
+  if (qn == 2) return parts ? with_keys_kernel_of<HD, 2, true>(f) : with_keys_kernel_of<HD, 2, false>(f);
+  return parts ? with_keys_kernel_of<HD, 1, true>(f) : with_keys_kernel_of<HD, 1, false>(f);
 }
 template <int HD, class F>
 hipError_t with_resident_kernel(bool scaled, const F& f) {
@@ -844,7 +1121,7 @@ hipError_t launch_dim(const CrossArgs& a, Plan& plan, void* workspace, hipStream
   p.q_mul = a.q_prescaled ? 1.0f : (float)(a.scale * 1.4426950408889634);
 
   float* at = (float*)workspace;
-  for (int i = 0; i < plan.n && plan.split; ++i) {
+  for (int i = 0; i < plan.n && plan.parts; ++i) {
     Task& t = plan.task[i];
     const int64_t n = (int64_t)t.units * t.rows;
     t.o = at;
@@ -853,16 +1130,22 @@ hipError_t launch_dim(const CrossArgs& a, Plan& plan, void* workspace, hipStream
   }
   p.task[0] = plan.task[0];
   p.task[1] = plan.task[1];
-  if (plan.resident)
+  auto launch = [&](auto kernel, int64_t lds) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)plan.grid), dim3(64 * NWAVE), (uint32_t)lds, stream, p);
+    return hipGetLastError();
+  };
+  if (plan.form == Form::resident)
     return with_resident_kernel<HD>(!a.q_prescaled, [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3((unsigned)plan.grid), dim3(64 * NWAVE), (uint32_t)(plan.resident * (4 * KC * HD + 8)), stream, p, plan.resident);
       return hipGetLastError();
     });
-  const hipError_t e = with_kernel<HD>(plan.split, !a.q_prescaled, plan.qn, [&](auto kernel, int lds) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)plan.grid), dim3(64 * NWAVE), (uint32_t)(lds + plan.words * 8), stream, p);
-    return hipGetLastError();
+  const hipError_t e = plan.form == Form::rows ? with_rows_kernel<HD>(plan.parts, !a.q_prescaled, plan.qn, [&](auto kernel, int lds) {
+    return launch(kernel, lds + plan.words * 8);
+  }) : with_keys_kernel<HD>(plan.parts, plan.qn, [&](auto kernel, int64_t lds, int64_t sums) {
+    lds += plan.words * 8;
+    return launch(kernel, lds > sums ? lds : sums);
   });
-  if (e != hipSuccess || !plan.split) return e;
+  if (e != hipSuccess || !plan.parts) return e;
   JoinParams j{};
   j.task[0] = plan.task[0];
   if (plan.n > 1) j.task[1] = plan.task[1];
@@ -878,14 +1161,18 @@ hipError_t launch_dim(const CrossArgs& a, Plan& plan, void* workspace, hipStream
 template <int HD>
 hipError_t configure_dim() {
   hipError_t e = hipSuccess;
-  for (int i = 0; i < 12 && e == hipSuccess; ++i)
-    e = with_kernel<HD>(i & 1, i & 2, i >> 2 == 2 ? 4 : 1 + (i >> 2), [](auto kernel, int lds) {
-      return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds + MAX_WORDS * 8);
-    });
+  auto allow = [](auto kernel, int64_t bytes) {
+    return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  };
+  for (int i = 0; i < 6 && e == hipSuccess; ++i) {
+    const int qn = i / 2 == 2 ? 4 : 1 + i / 2;
+    for (int parts = 0; parts < 2 && e == hipSuccess; ++parts)
+      e = with_rows_kernel<HD>(parts, i & 1, qn, [&](auto kernel, int lds) { return allow(kernel, lds + MAX_WORDS * 8); });
+    if (e == hipSuccess)
+      e = with_keys_kernel<HD>(i & 1, qn, [&](auto kernel, int64_t lds, int64_t sums) { return allow(kernel, lds + MAX_WORDS * 8 > sums ? lds + MAX_WORDS * 8 : sums); });
+  }
   for (int i = 0; i < 2 && e == hipSuccess; ++i)
-    e = with_resident_kernel<HD>(i, [](auto kernel) {
-      return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)RESIDENT_LDS);
-    });
+    e = with_resident_kernel<HD>(i, [&](auto kernel) { return allow(kernel, RESIDENT_LDS); });
   return e;
 }
 
