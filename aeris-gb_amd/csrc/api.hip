@@ -397,7 +397,6 @@ int aeris_qk_norm_rope_fwd(const aeris_qk_norm_rope* a, void* stream) {
     return fail(AERIS_EINVAL, "%s: positions must be 4-byte aligned, 1 .. 2^31-1 of them", who);
   // (token numbers are formed in 32 bits, up to a block of them beyond the last)
   if (a->tokens > 0x7fffffffLL - 64) return fail(AERIS_EUNSUPPORTED, "%s: more than 2^31-65 tokens", who);
-  int64_t heads = 0;
   for (int i = 0; i < (int)a->n_parts; ++i) {
     const aeris_qk_part& p = a->parts[i];
     if (!p.x || !p.y || p.heads <= 0) return fail(AERIS_EINVAL, "%s: x/y is NULL or heads is not positive", who);
@@ -408,10 +407,9 @@ int aeris_qk_norm_rope_fwd(const aeris_qk_norm_rope* a, void* stream) {
     if (!ok || !aligned16(p.x) || !aligned16(p.y) || (p.gain && !aligned16(p.gain)) || p.gain_head_stride % eg)
       return fail(AERIS_EINVAL, "%s: x, y and gain must be 16-byte aligned, the elements of a head contiguous and the other strides multiples of 16 bytes", who);
     if (p.heads > 32767) return fail(AERIS_EUNSUPPORTED, "%s: more than 32767 heads", who);
-    heads += p.heads;
   }
-  // (workgroups of 2048 / head_dim tokens and a head at least)
-  if ((a->tokens * a->head_dim / 2048 + 1) * heads > 0x7fffffffLL) return fail(AERIS_EUNSUPPORTED, "%s: more than 2^31-1 workgroups", who);
+  if (aeris::qk_norm_rope_workgroups(*a) >= 1 << 24)  // (of 256: a grid has less than 2^32 threads)
+    return fail(AERIS_EUNSUPPORTED, "%s: tokens * heads need 2^24 workgroups or more", who);
   hipError_t e = aeris::qk_norm_rope_launch(*a, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "aeris_qk_norm_rope_fwd launch");
   return AERIS_OK;
@@ -473,6 +471,7 @@ int aeris_cross_attention_fwd(const aeris_cross_attention* a, void* workspace, i
   if (c.lengths && (reinterpret_cast<uintptr_t>(c.lengths) & 3u)) return fail(AERIS_EINVAL, "%s: lengths must be 4-byte aligned", who);
   if (c.key_mask && c.mask_batch_stride < 0) return fail(AERIS_EINVAL, "%s: mask_stride must not be negative", who);
   if (!c.q_prescaled && !(c.scale > 0.0 && c.scale < 1e30)) return fail(AERIS_EINVAL, "%s: scale must be positive", who);
+  if (!aeris::cross_attention_fits(c)) return fail(AERIS_EUNSUPPORTED, "%s: B * kv_heads or the rows need 2^24 workgroups or more", who);
   const int64_t need = aeris::cross_attention_workspace_bytes(c);
   if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
     return fail(AERIS_EINVAL, "%s: workspace must be 16-byte aligned and hold %lld bytes (got %lld)", who, (long long)need, (long long)workspace_bytes);

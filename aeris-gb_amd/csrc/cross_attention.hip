@@ -4,7 +4,8 @@
 // A unit is one member's key head (or, where all members see the same keys, the key head with the rows of all of them); its rows are
 // the queries of the heads that share the key head, 16 QN a wave.  Keys go through LDS in chunks of 64; P = exp2(logit) is formed
 // without a row maximum - softmax does not depend on the subtracted constant, the maximum only guards the range -, the range of the sums is
-// checked afterwards and the rows are done again with a running maximum where it was left.
+// checked afterwards and the rows are done again with a running maximum where it was left: 2^-20 to 2^60, so that values of v from 2^-106 to 2^67 in
+// size neither vanish nor overflow in their sums either.
 //   K, V chunk [64][HD]  global -> LDS by the load unit (buffer_load ... lds), 16-byte pieces XOR-swizzled; a key that does not take
 //                        part is not read, its row arrives as zeros (whatever it held, NaN or infinity, is multiplied by nothing)
 //   S^T = K Q^T          v_mfma_f32_16x16x32_bf16; lane = one row, registers = keys; the scale, unless the producer of q has applied it (`SCALED`),
@@ -344,7 +345,7 @@ struct Rows {
         l[n] += __shfl_xor(l[n], 32, 64);
       }
       l[n] -= (float)idle;
-      bad = bad || !(l[n] >= 0x1p-40f && l[n] >= 0x1p-10f * (float)idle && l[n] <= 0x1p100f);
+      bad = bad || !(l[n] >= 0x1p-20f && l[n] >= 0x1p-10f * (float)idle && l[n] <= 0x1p60f);
     }
     return __builtin_amdgcn_ballot_w64(bad) != 0;
   }
@@ -1188,6 +1189,15 @@ hipError_t cross_attention_configure() {
 }
 
 int64_t cross_attention_workspace_bytes(const CrossArgs& a) { return plan_of(a).bytes; }
+
+// (a grid has less than 2^32 threads; up to 1024 of them join a row)
+bool cross_attention_fits(const CrossArgs& a) {
+  const Plan plan = plan_of(a);
+  int64_t units = 0;
+  for (int i = 0; i < plan.n; ++i) units += (int64_t)plan.task[i].splits * plan.task[i].members * a.kv_heads;
+  const int parts = plan.task[0].splits + plan.task[1].splits;
+  return units < (1 << 24) && plan.grid < (1 << 24) && (!plan.parts || a.B * a.Nq * a.heads < (parts <= 16 ? 1 << 26 : parts <= 64 ? 1 << 24 : 1 << 22));
+}
 
 hipError_t cross_attention_launch(const CrossArgs& a, void* workspace, hipStream_t stream) {
   Plan plan = plan_of(a);

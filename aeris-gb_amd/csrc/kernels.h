@@ -66,6 +66,7 @@ hipError_t output_stage_launch(const void* x, int x_dtype, const void* gamma, co
 
 // norm and rotation of query and key heads (qk_norm_rope.hip)
 bool qk_norm_rope_supported(int64_t head_dim, int64_t rotated);
+int64_t qk_norm_rope_workgroups(const aeris_qk_norm_rope& a);
 hipError_t qk_norm_rope_launch(const aeris_qk_norm_rope& a, hipStream_t stream);
 
 // attention to an encoder's states (cross_attention.hip): aeris_cross_attention with the strides of dimensions with one entry 0
@@ -83,6 +84,7 @@ struct CrossArgs {
 bool cross_attention_supported(int64_t head_dim);
 hipError_t cross_attention_configure();
 int64_t cross_attention_workspace_bytes(const CrossArgs& a);
+bool cross_attention_fits(const CrossArgs& a);  // whether its grid is one that can be launched
 hipError_t cross_attention_launch(const CrossArgs& a, void* workspace, hipStream_t stream);
 
 hipError_t modulation_linear_launch(const aeris_modulation_layer* layers, int n, int B, int K, int w_dtype, int act, hipStream_t stream);

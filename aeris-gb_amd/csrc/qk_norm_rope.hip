@@ -190,6 +190,13 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkParams p) {
   }
 }
 
+// one head a thread up to 1600 workgroups of that kind: 4096 tokens, 4 + 4 heads of 64 4.2 us, with four 4.8; 8192 6.2, 5.7; 2048 tokens, 3 + 3 of
+// 128 3.8, 4.4; 4096 5.3, 5.0
+int heads_per_thread(const aeris_qk_norm_rope& a) {
+  const int64_t heads = a.parts[0].heads + (a.n_parts > 1 ? a.parts[1].heads : 0);
+  return a.tokens * a.head_dim / 2048 * heads >= 1600 ? 4 : 1;
+}
+
 template <int D, bool XF32, bool YF32, int HPT>
 hipError_t launch(const QkParams& p0, hipStream_t stream) {
   QkParams p = p0;
@@ -216,6 +223,13 @@ bool qk_norm_rope_supported(int64_t head_dim, int64_t rotated) {
   return (head_dim == 32 || head_dim == 64 || head_dim == 128) && rotated >= 0 && rotated <= head_dim && rotated % 16 == 0;
 }
 
+int64_t qk_norm_rope_workgroups(const aeris_qk_norm_rope& a) {
+  const int64_t each = heads_per_thread(a), tokens = 2048 / a.head_dim;
+  int64_t groups = 0;
+  for (int i = 0; i < (int)a.n_parts; ++i) groups += (a.parts[i].heads + each - 1) / each;
+  return (a.tokens + tokens - 1) / tokens * groups;
+}
+
 hipError_t qk_norm_rope_launch(const aeris_qk_norm_rope& a, hipStream_t stream) {
   QkParams p{};
   p.part[0] = a.parts[0];
@@ -225,10 +239,7 @@ hipError_t qk_norm_rope_launch(const aeris_qk_norm_rope& a, hipStream_t stream) 
   p.rotation = a.rotation; p.positions = a.R > 0 ? a.positions : nullptr;
   p.n_pos = p.positions ? (int)a.n_positions : a.P > 0 ? (int)a.P : 1;
   const bool xf = a.x_dtype == AERIS_F32, yf = a.y_dtype == AERIS_F32;
-  // one head a thread up to 1600 workgroups of that kind: 4096 tokens, 4 + 4 heads of 64 4.2 us, with four 4.8; 8192 6.2, 5.7; 2048 tokens, 3 + 3 of
-  // 128 3.8, 4.4; 4096 5.3, 5.0
-  const int64_t heads = a.parts[0].heads + (a.n_parts > 1 ? a.parts[1].heads : 0);
-  const bool many = a.tokens * a.head_dim / 2048 * heads >= 1600;
+  const bool many = heads_per_thread(a) == 4;
   if (a.head_dim == 32) return many ? launch_types<32, 4>(p, xf, yf, stream) : launch_types<32, 1>(p, xf, yf, stream);
   if (a.head_dim == 64) return many ? launch_types<64, 4>(p, xf, yf, stream) : launch_types<64, 1>(p, xf, yf, stream);
   return many ? launch_types<128, 4>(p, xf, yf, stream) : launch_types<128, 1>(p, xf, yf, stream);

@@ -205,6 +205,8 @@ def _made_once(key, make):
         if key[-1].type == "cuda" and torch._C._cuda_isCurrentStreamCapturing():
             return make()
         _MADE[key] = make()
+        if key[-1].type == "cuda":  # there for every stream
+            torch.cuda.current_stream(key[-1]).synchronize()
     return _MADE[key]
 
 

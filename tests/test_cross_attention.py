@@ -343,3 +343,73 @@ def test_refusals_without_a_gpu(pkg):
     t = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="GPU"):
         pkg.ops.cross_attention(t, t, t)
+
+
+# (form, head size, rows) that the sizes below lead to: rows of a wave or workgroup, the keys whole or in parts
+PLANS = [
+    (1, 2, 1, 1, 32, 73, 0), (1, 2, 2, 1, 32, 74, 4588), (1, 1374, 3, 1, 32, 102, 1153), (1, 82, 2, 1, 32, 132, 14864), (1, 4508, 2, 1, 32, 252, 3293),
+    (2, 175, 4, 4, 32, 105, 12953), (1, 1, 1, 1, 64, 74, 0), (1, 2, 1, 1, 64, 79, 4586), (1, 4130, 1, 1, 64, 119, 1308), (1, 105, 4, 4, 64, 92, 9906),
+    (1, 4428, 2, 2, 64, 244, 1954), (1, 582, 3, 3, 64, 105, 15424), (1, 1, 1, 1, 128, 74, 0), (1, 1, 2, 1, 128, 75, 9702), (1, 4151, 1, 1, 128, 212, 0),
+    (1, 296, 2, 1, 128, 159, 7899), (1, 8431, 1, 1, 128, 162, 868), (1, 604, 2, 1, 128, 75, 14617),  # the keys divided among waves: 16, 32, 64 rows
+    (40, 68, 16, 8, 32, 197, 233), (40, 238, 8, 8, 64, 147, 0), (40, 137, 8, 8, 128, 73, 0),         # keys that stay
+    (1, 5482, 3, 3, 32, 150, 0), (1, 4134, 12, 4, 32, 90, 0), (1, 628, 4, 2, 32, 129, 13739), (1, 2735, 3, 1, 64, 104, 0), (5, 1637, 2, 1, 64, 161, 464),
+    (5, 69, 9, 3, 64, 82, 12565), (5, 8613, 3, 1, 64, 108, 764), (1, 2065, 2, 1, 128, 85, 0), (2, 4129, 2, 1, 128, 82, 45), (2, 794, 1, 1, 128, 86, 15413),
+    (64, 1, 4, 4, 32, 300, 0), (66, 3, 8, 4, 32, 90, 200), (24, 100, 6, 6, 64, 130, 100), (40, 30, 4, 1, 64, 500, 300), (9, 700, 2, 2, 64, 700, 0), (1, 1, 2, 1, 32, 70, 20000),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["masked", "loud", "prescaled"])
+@pytest.mark.parametrize("B,Nq,H,Hk,D,Nk,Np", PLANS)
+def test_every_kernel(pkg, cuda, B, Nq, H, Hk, D, Nk, Np, kind):
+    """Sizes for every kernel and every way to divide a call among workgroups; the queries at the ends of blocks and some between are checked."""
+    (q, k, v), g = inputs(B, Nq, H, Hk, D, Nk, cuda, Nq + Nk + D, "rows" if Nq % 2 else "planes")
+    prefix = tuple(heads((Np, Hk, D), "fused", g, cuda) for _ in range(2)) if Np else None
+    lengths = mask = None
+    kw = {}
+    some = sorted({n for n in [0, 15, 16, 63, 64, 127, 128, 255, 256, Nq - 1] + torch.randint(0, Nq, (30,), generator=g).tolist() if n < Nq})
+    if kind == "masked":
+        lengths = torch.randint(0, Nk + 1, (B,), generator=g, dtype=torch.int32)
+        lengths[0] = Nk - 3
+        if B > 1:
+            lengths[-1] = 0
+        mask = torch.rand(B, Nk, generator=g) < 0.7
+        dead = ((torch.arange(Nk)[None] >= lengths[:, None]) | ~mask).to(cuda)
+        k[dead], v[dead] = math.nan, math.inf
+        mask, lengths = mask.to(cuda), lengths.to(cuda)
+    elif kind == "loud":  # a few queries whose logits need a maximum, among others that do not
+        q[:, some[::5]] *= 40
+    else:
+        q.copy_((q.float() * (D ** -0.5 * pkg.ops.LOG2E)).bfloat16())
+        kw = dict(q_prescaled=True)
+    got = pkg.ops.cross_attention(q, k, v, lengths=lengths, key_mask=mask, prefix=prefix, **kw)
+    assert bool(torch.isfinite(got).all())
+    check(got[:, some].contiguous(), oracle(q[:, some], k, v, lengths, mask, prefix, exp2_domain=kind == "prescaled"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,Nq,H,Hk,Nk", [(1, 1, 2, 1, 300), (1, 2, 1, 1, 4700), (1, 2735, 3, 1, 104), (40, 238, 8, 8, 147)])
+@pytest.mark.parametrize("level,power", [(6.0, 60), (-3.0, -100)])
+def test_values_of_any_size(pkg, cuda, B, Nq, H, Hk, Nk, level, power):
+    """Logits of 70 and -35 (base 2) all along with values of 2^60 and 2^-100: the result is the values' mean, weights times values do not fit fp32."""
+    (q, k, v), _ = inputs(B, Nq, H, Hk, 64, Nk, cuda, 21)
+    q.fill_(1.0)
+    k.mul_(0.1).add_(level)
+    v.mul_(2.0 ** power)
+    some = sorted({n for n in (0, 1, 130, 777, Nq - 1) if n < Nq})
+    check(pkg.ops.cross_attention(q, k, v)[:, some].contiguous(), oracle(q[:, some], k, v))
+
+
+def test_grids_that_cannot_be_launched(pkg):
+    L, at = pkg._lib, 1 << 20
+    S = pkg.ops.CROSS_ATTENTION
+
+    def call(B, Nq, heads, Nk, Np=0):
+        kb = Nk * heads * 64
+        a = S.pack(at, at, at, at, at, at, 0, 0, B, Nq, heads, 64, B, Nk, heads, Np, 0, 0, *([Nq * heads * 64, heads * 64, 64, 1] + [kb, heads * 64, 64, 1] * 2),
+                   *([heads * 64, 64, 1] * 2), 0, 0, 0.125)
+        return L.lib().aeris_cross_attention_fwd(a, at, 1 << 60, None)
+
+    for args in [(1 << 24, 1, 1, 9), (1 << 29, 1, 1, 9), (1 << 20, 1, 16, 100), (1 << 26, 1, 1, 9, 100), (1 << 28, 1, 4, 1)]:
+        # (the last has 2^28 * 4 = 2^30 rows, one more than the limit of rows lets through)
+        assert call(*args) == L.EUNSUPPORTED and ("workgroups" in L.last_error() or "rows" in L.last_error()), args

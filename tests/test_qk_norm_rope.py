@@ -224,3 +224,15 @@ def test_refusals_without_a_gpu(pkg):
     with pytest.raises(RuntimeError, match="GPU"):
         pkg.ops.qk_norm_rope(torch.zeros(4, 2, 64, dtype=torch.bfloat16))
     assert S.size == 304
+
+
+def test_grids_that_cannot_be_launched(pkg):
+    L, at = pkg._lib, 1 << 20
+
+    def call(tokens, heads, D, n):
+        part = (at, at, 0, heads, heads * D, D, 1, heads * D, D, 1, 0, 1.0)
+        a = pkg.ops.QK_NORM_ROPE.pack(*part, *part, at, 0, tokens, D, L.BF16, L.BF16, L.BF16, 1, 0, 4, 16, 0, n, 1e-6)
+        return L.lib().aeris_qk_norm_rope_fwd(a, None)
+
+    for args in [(2 ** 31 - 100, 1, 32, 1), (2 ** 30, 1, 64, 2), (2 ** 28, 8, 128, 1), (2 ** 24, 32767, 32, 2)]:
+        assert call(*args) == L.EUNSUPPORTED and "workgroups" in L.last_error(), args
