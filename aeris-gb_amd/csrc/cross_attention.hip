@@ -43,6 +43,18 @@ struct Task {
   float *o, *ml;     // PARTS: [split][member][key head][row][HD], [..][2] = maximum, sum
 };
 
+// Division of n < 2^31 by a number that a launch knows: a product's upper half and a shift
+struct Divisor {
+  uint32_t by, factor, shift;
+  __device__ __forceinline__ int of(int n) const { return by == 1 ? n : (int)(__umulhi((uint32_t)n, factor) >> shift); }
+};
+// (with 2^l >= by > 2^(l - 1), factor = floor(2^(31 + l) / by) + 1 is off by less than a part of 2^31)
+Divisor divisor(uint32_t by) {
+  uint32_t l = 1;
+  while (l < 31 && (1u << l) < by) ++l;
+  return {by, by == 1 ? 0 : (uint32_t)((1ull << (31 + l)) / by + 1), l - 1};
+}
+
 struct CrossParams {
   const uint16_t *q, *k, *v, *prefix_k, *prefix_v;
   uint16_t* out;
@@ -53,6 +65,7 @@ struct CrossParams {
   int lengths_step;  // 0: one length for all members
   int Nq, heads, kv_heads, group;
   int rows_m;        // rows of a member
+  Divisor of_group, of_rows_m;
   float q_mul;
   Task task[2];
 };
@@ -102,21 +115,34 @@ struct Rows {
     }
   }
 
-  // the rows from row0 of a unit: where their results go (in units of a head's row), and their queries into `f`
-  __device__ __forceinline__ void load_q(const CrossParams& p, int rows, int member, int hk, int row0, int lane, int64_t (&to)[QN], bf16x8 (&f)[QN][KS]) const {
+  // the lane's rows, row0 + 16 n + lane % 16 (the last one for those behind it), of a unit: member, query and head
+  __device__ __forceinline__ void row_of(const CrossParams& p, const Task& t, int hk, int row0, int n, int lane, int64_t& member, int& query, int& head) const {
+    int r = row0 + n * 16 + (lane & 15);
+    r = r < t.rows ? r : t.rows - 1;
+    const int b = p.of_rows_m.of(r), rm = r - b * p.rows_m;
+    query = p.of_group.of(rm);
+    head = hk * p.group + rm - query * p.group;
+    member += b;
+  }
+  // Whether they are neighbouring queries of one head, all there (uniform): what is then left to the lanes does not depend on the block
+  __device__ __forceinline__ bool plain(const CrossParams& p, const Task& t, int row0) const {
+    return p.group == 1 && t.rows == p.rows_m && row0 + 16 * QN <= t.rows;
+  }
+  __device__ __forceinline__ void load_q(const CrossParams& p, const Task& t, int member, int hk, int row0, int lane, bf16x8 (&f)[QN][KS]) const {
+    if (plain(p, t, row0)) {
+      const uint16_t* first = p.q + member * p.q_batch + row0 * p.q_row + hk * p.q_head;
+      const int64_t mine = (lane & 15) * p.q_row + q4 * 8;
+#pragma unroll
+      for (int n = 0; n < QN; ++n)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) f[n][s] = *reinterpret_cast<const bf16x8*>(first + n * 16 * p.q_row + mine + s * 32);
+      return;
+    }
 #pragma unroll
     for (int n = 0; n < QN; ++n) {
-      int r = row0 + n * 16 + (lane & 15);
-      if (r >= rows) r = rows - 1;
-      int query = r, head = hk;
       int64_t b = member;
-      if (p.group != 1 || rows != p.rows_m) {  // (uniform; two divisions)
-        const int bb = r / p.rows_m, rm = r - bb * p.rows_m;
-        query = rm / p.group;
-        head = hk * p.group + rm - query * p.group;
-        b += bb;
-      }
-      to[n] = (b * p.Nq + query) * p.heads + head;
+      int query, head;
+      row_of(p, t, hk, row0, n, lane, b, query, head);
       const uint16_t* qp = p.q + b * p.q_batch + query * p.q_row + head * p.q_head + q4 * 8;
 #pragma unroll
       for (int s = 0; s < KS; ++s) f[n][s] = *reinterpret_cast<const bf16x8*>(qp + s * 32);
@@ -162,6 +188,9 @@ struct Rows {
     load_v(0, 0);
     __builtin_amdgcn_sched_barrier(0);
 
+    // The wave of a SIMD that has its weights goes first: its product is the longer chain, the other's exponentials fill the gaps (1572 -> 1521 us for
+    // 1 036 800 queries, sixteen heads of 64, 256 keys; first for K Q^T as well 1531, for the exponentials alone 1595)
+    __builtin_amdgcn_s_setprio(0);
     f32x4 acc[QN][KB];
     // ---- S^T: acc[n][kb][i] = logit of key 16 kb + 4 q4 + i, row 16 n + l15; K fragments are read two ahead of their MFMAs
     {
@@ -236,6 +265,7 @@ struct Rows {
     };
 #pragma unroll
     for (int n = 0; n < QN; ++n) exp_step(0, n);
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int part = 0; part < PARTS; ++part) {
       const int step = part >> 1;
@@ -351,18 +381,31 @@ struct Rows {
   }
 
   // normalise (a row without any key is zeros), 8 consecutive elements a lane and store
-  __device__ __forceinline__ void store(uint16_t* out, const int64_t (&to)[QN], int row0, int rows, int lane) const {
-#pragma unroll
-    for (int n = 0; n < QN; ++n) {
+  __device__ __forceinline__ void store(const CrossParams& p, const Task& t, int member, int hk, int row0, int lane) const {
+    const int mine = 16 * (q4 & 1) + 8 * (q4 >> 1);
+    auto put = [&](int n, uint16_t* op, bool there) {
       const float inv = l[n] == 0.f ? 0.f : __builtin_amdgcn_rcpf(l[n]);
-      uint16_t* op = out + to[n] * HD + 16 * (q4 & 1) + 8 * (q4 >> 1);
 #pragma unroll
       for (int m2 = 0; m2 < DB / 2; ++m2) {
         const f32x4 a = o[n][2 * m2] * inv, c = o[n][2 * m2 + 1] * inv;
         const auto rx = __builtin_amdgcn_permlane16_swap(pack_bf16x2(a[0], a[1]), pack_bf16x2(c[0], c[1]), false, false);
         const auto ry = __builtin_amdgcn_permlane16_swap(pack_bf16x2(a[2], a[3]), pack_bf16x2(c[2], c[3]), false, false);
-        if (row0 + n * 16 + (lane & 15) < rows) *reinterpret_cast<u32x4*>(op + m2 * 32) = u32x4{rx[0], ry[0], rx[1], ry[1]};
+        if (there) *reinterpret_cast<u32x4*>(op + m2 * 32) = u32x4{rx[0], ry[0], rx[1], ry[1]};
       }
+    };
+    if (plain(p, t, row0)) {
+      uint16_t* first = p.out + (((int64_t)member * p.Nq + row0) * p.heads + hk) * HD;
+      const int64_t of_lane = (lane & 15) * p.heads * HD + mine;
+#pragma unroll
+      for (int n = 0; n < QN; ++n) put(n, first + (int64_t)n * 16 * p.heads * HD + of_lane, true);
+      return;
+    }
+#pragma unroll
+    for (int n = 0; n < QN; ++n) {
+      int64_t b = member;
+      int query, head;
+      row_of(p, t, hk, row0, n, lane, b, query, head);
+      put(n, p.out + ((b * p.Nq + query) * p.heads + head) * HD + mine, row0 + n * 16 + (lane & 15) < t.rows);
     }
   }
 };
@@ -531,7 +574,6 @@ cross_attention_rows_kernel(CrossParams p) {
   const bool wave_active = row0 < t.rows;  // wave-uniform: a wave without rows only loads and keeps the barriers
   Rows<HD, QN, SCALED, SUM> rows(smem, V_BASE, lane, p.q_mul);
   Load load(lane, wave);
-  int64_t to[QN];
 
   const bool masked = p.mask && t.Nk > 0;
   if (masked) {
@@ -552,7 +594,7 @@ cross_attention_rows_kernel(CrossParams p) {
     keys.seek(p, t, hk, c0);
     load.rows(lane, keys);
     if (nch > 0) issue(0, 0);
-    if (FAST) rows.load_q(p, t.rows, member, hk, row0, lane, to, rows.qf);
+    if (FAST) rows.load_q(p, t, member, hk, row0, lane, rows.qf);
     rows.reset();
     if (FAST) __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the compiler knows the queries to be there (inside the loop it would wait for the chunks too)
     for (int j0 = 0; j0 < nch; j0 += 2) {
@@ -589,7 +631,7 @@ cross_attention_rows_kernel(CrossParams p) {
     }
   }
   if (!PARTS) {
-    rows.store(p.out, to, row0, t.rows, lane);
+    rows.store(p, t, member, hk, row0, lane);
     return;
   }
 #pragma unroll
@@ -658,10 +700,7 @@ cross_attention_keys_kernel(CrossParams p) {
 #pragma unroll
     for (int u = 0; u < RB - 1; ++u)
       if (u < steps) issue(u, u);
-    if (FAST) {
-      int64_t to[QN];
-      rows.load_q(p, t.rows, member, hk, row0, lane, to, rows.qf);
-    }
+    if (FAST) rows.load_q(p, t, member, hk, row0, lane, rows.qf);
     rows.reset();
     if (FAST) __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0), see the kernel above
     for (int j0 = 0; j0 < steps; j0 += RB) {
@@ -728,7 +767,7 @@ cross_attention_keys_kernel(CrossParams p) {
       }
       __builtin_nontemporal_store(o, reinterpret_cast<f32x4*>(t.o + dst * HD + 4 * c));
     } else {
-      const int bb = r / p.rows_m, rm = r - bb * p.rows_m, query = rm / p.group, head = hk * p.group + rm - query * p.group;
+      const int bb = p.of_rows_m.of(r), rm = r - bb * p.rows_m, query = p.of_group.of(rm), head = hk * p.group + rm - query * p.group;
       const float inv = l == 0.f ? 0.f : 1.0f / l;
       *reinterpret_cast<u32x2*>(p.out + (((int64_t)(member + bb) * p.Nq + query) * p.heads + head) * HD + 4 * c) =
           u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
@@ -760,9 +799,8 @@ cross_attention_resident_kernel(CrossParams p, int max_chunks) {
   Load load(lane, wave);
   const int step = t.qblks * NWAVE * QW;
   int row0 = (part * NWAVE + wave) * QW;
-  int64_t to[QN], to_next[QN];
   bf16x8 next[QN][HD / 32];
-  if (row0 < t.rows) rows.load_q(p, t.rows, member, hk, row0, lane, to_next, next);
+  if (row0 < t.rows) rows.load_q(p, t, member, hk, row0, lane, next);
   keys.seek(p, t, hk, 0);
   load.rows(lane, keys);
   int idle = 0;
@@ -779,29 +817,45 @@ cross_attention_resident_kernel(CrossParams p, int max_chunks) {
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   __syncthreads();
-  const bool any = idle < nch * KC;
+  if (idle == nch * KC) {  // no keys
+    rows.reset();
+    for (; row0 < t.rows; row0 += step) rows.store(p, t, member, hk, row0, lane);
+    return;
+  }
 
-  for (; row0 < t.rows; row0 += step) {
+  // Rows that need a maximum come afterwards, those of all blocks together, so that the loop that nearly all take holds no registers for them: a
+  // bit for each block, or for 2, 3, .. in a row where there are more than 64
+  uint64_t again = 0;
+  const int start = row0, per_bit = ((t.rows - start + step - 1) / step + 63) / 64;
+  for (int bit = 0, j = 0; row0 < t.rows; row0 += step) {
 #pragma unroll
-    for (int n = 0; n < QN; ++n) {
-      to[n] = to_next[n];
+    for (int n = 0; n < QN; ++n)
 #pragma unroll
       for (int s = 0; s < HD / 32; ++s) rows.qf[n][s] = next[n][s];
-    }
-    if (row0 + step < t.rows) rows.load_q(p, t.rows, member, hk, row0 + step, lane, to_next, next);
+    if (row0 + step < t.rows) rows.load_q(p, t, member, hk, row0 + step, lane, next);
     rows.reset();
-    if (any) {
-      for (int c = 0; c < nch; ++c) rows.template chunk<true>(c * BYTES, ~0ull);
-      if (rows.sums(idle)) {
-        rows.reset();
-        for (int c = 0; c < nch; ++c) {
-          const uint64_t w = word_of(c);
-          if (w != 0) rows.template chunk<false>(c * BYTES, w);
-        }
-        rows.sums(0);
-      }
+    int c = 0;
+    do rows.template chunk<true>(c * BYTES, ~0ull);
+    while (++c < nch);
+    if (rows.sums(idle)) again |= 1ull << bit;
+    else rows.store(p, t, member, hk, row0, lane);
+    if (++j == per_bit) {
+      j = 0;
+      ++bit;
     }
-    rows.store(p.out, to, row0, t.rows, lane);
+  }
+  for (; again != 0; again &= again - 1) {
+    row0 = start + __builtin_ctzll(again) * per_bit * step;
+    for (int j = 0; j < per_bit && row0 < t.rows; ++j, row0 += step) {
+      rows.load_q(p, t, member, hk, row0, lane, rows.qf);
+      rows.reset();
+      for (int c = 0; c < nch; ++c) {
+        const uint64_t w = word_of(c);
+        if (w != 0) rows.template chunk<false>(c * BYTES, w);
+      }
+      rows.sums(0);
+      rows.store(p, t, member, hk, row0, lane);
+    }
   }
 }
 
@@ -911,8 +965,9 @@ __global__ void __launch_bounds__(WPR > 4 ? 64 * WPR : 256) cross_attention_join
 namespace {
 
 constexpr int NWAVE = 4;
-// Blocks of 16 rows per wave.  More of them read a K / V fragment from LDS for more rows; fewer leave registers for more waves.
-constexpr int resident_qn(int64_t head_dim) { return head_dim == 64 ? 3 : 2; }
+// Blocks of 16 rows per wave.  More of them read a K / V fragment from LDS for more rows; fewer leave registers for more waves (head size 64, 1 036 800
+// queries, sixteen heads, 256 keys: 2 1500 us, 3 1500, 4 1445; 64 800, 77 keys: 51, 55, 51; head size 32, 200 keys: 2 55, 3 56, 4 57).
+constexpr int resident_qn(int64_t head_dim) { return head_dim == 64 ? 4 : 2; }
 constexpr int64_t RESIDENT_LDS = 80 * 1024;  // two workgroups per CU
 
 // How a call is run
@@ -1018,11 +1073,12 @@ Plan plan_of(const CrossArgs& a) {
     if (plan.n < 2) plan.task[1].first = 0x7fffffff;
   };
 
-  // Few keys and many rows: a workgroup's keys stay (at least two row blocks for each of its waves)
+  // Few keys and many rows: a workgroup's keys stay (at least two row blocks for each of its waves).  As many workgroups as run at once: two per CU, four
+  // of the small ones of head size 32 (64 800 queries, sixteen heads, 77 keys: 33.5 us with 1024, 36.5 with 512; of 64: 54 and 51)
   if (!plan.parts) {
     Task& t = plan.task[0];
     const int64_t c = chunks_of(t, KC), lds = c * (4 * KC * D + 8), units = (int64_t)t.members * Hk;
-    const int64_t per = (lds <= RESIDENT_LDS / 2 ? 1024 : 512) / units, blocks = div_up(t.rows, 16 * resident_qn(D) * NWAVE);
+    const int64_t per = (D == 32 && lds <= RESIDENT_LDS / 2 ? 1024 : 512) / units, blocks = div_up(t.rows, 16 * resident_qn(D) * NWAVE);
     if (c > 0 && lds <= RESIDENT_LDS && per > 0 && blocks >= 2 * per) {
       plan.form = Form::resident;
       plan.resident = (int)c;
@@ -1118,6 +1174,7 @@ hipError_t launch_dim(const CrossArgs& a, Plan& plan, void* workspace, hipStream
   p.lengths = a.lengths; p.lengths_step = (int)a.lengths_stride; p.mask = a.key_mask;
   p.Nq = (int)a.Nq; p.heads = (int)a.heads; p.kv_heads = (int)a.kv_heads; p.group = (int)(a.heads / a.kv_heads);
   p.rows_m = p.Nq * p.group;
+  p.of_group = divisor((uint32_t)p.group); p.of_rows_m = divisor((uint32_t)p.rows_m);
   // (the kernels of divided keys multiply the logits in either case: they are bound by reading the keys)
   p.q_mul = a.q_prescaled ? 1.0f : (float)(a.scale * 1.4426950408889634);
 

@@ -351,9 +351,10 @@ PLANS = [
     (2, 175, 4, 4, 32, 105, 12953), (1, 1, 1, 1, 64, 74, 0), (1, 2, 1, 1, 64, 79, 4586), (1, 4130, 1, 1, 64, 119, 1308), (1, 105, 4, 4, 64, 92, 9906),
     (1, 4428, 2, 2, 64, 244, 1954), (1, 582, 3, 3, 64, 105, 15424), (1, 1, 1, 1, 128, 74, 0), (1, 1, 2, 1, 128, 75, 9702), (1, 4151, 1, 1, 128, 212, 0),
     (1, 296, 2, 1, 128, 159, 7899), (1, 8431, 1, 1, 128, 162, 868), (1, 604, 2, 1, 128, 75, 14617),  # the keys divided among waves: 16, 32, 64 rows
-    (40, 68, 16, 8, 32, 197, 233), (40, 238, 8, 8, 64, 147, 0), (40, 137, 8, 8, 128, 73, 0),         # keys that stay
+    (40, 68, 16, 8, 32, 197, 233), (40, 238, 8, 8, 64, 147, 0), (40, 600, 8, 8, 64, 147, 0), (40, 137, 8, 8, 128, 73, 0),         # keys that stay
     (1, 5482, 3, 3, 32, 150, 0), (1, 4134, 12, 4, 32, 90, 0), (1, 628, 4, 2, 32, 129, 13739), (1, 2735, 3, 1, 64, 104, 0), (5, 1637, 2, 1, 64, 161, 464),
     (5, 69, 9, 3, 64, 82, 12565), (5, 8613, 3, 1, 64, 108, 764), (1, 2065, 2, 1, 128, 85, 0), (2, 4129, 2, 1, 128, 82, 45), (2, 794, 1, 1, 128, 86, 15413),
+    (64, 8300, 8, 8, 32, 330, 0),  # (65 row blocks for a wave)
     (64, 1, 4, 4, 32, 300, 0), (66, 3, 8, 4, 32, 90, 200), (24, 100, 6, 6, 64, 130, 100), (40, 30, 4, 1, 64, 500, 300), (9, 700, 2, 2, 64, 700, 0), (1, 1, 2, 1, 32, 70, 20000),
 ]
 
@@ -388,7 +389,7 @@ def test_every_kernel(pkg, cuda, B, Nq, H, Hk, D, Nk, Np, kind):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("B,Nq,H,Hk,Nk", [(1, 1, 2, 1, 300), (1, 2, 1, 1, 4700), (1, 2735, 3, 1, 104), (40, 238, 8, 8, 147)])
+@pytest.mark.parametrize("B,Nq,H,Hk,Nk", [(1, 1, 2, 1, 300), (1, 2, 1, 1, 4700), (1, 2735, 3, 1, 104), (40, 238, 8, 8, 147), (40, 600, 8, 8, 147)])
 @pytest.mark.parametrize("level,power", [(6.0, 60), (-3.0, -100)])
 def test_values_of_any_size(pkg, cuda, B, Nq, H, Hk, Nk, level, power):
     """Logits of 70 and -35 (base 2) all along with values of 2^60 and 2^-100: the result is the values' mean, weights times values do not fit fp32."""
