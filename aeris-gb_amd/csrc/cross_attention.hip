@@ -18,7 +18,7 @@
 //   cross_attention_resident_kernel  few keys and many rows: a workgroup keeps the unit's keys in LDS and walks down the rows
 //   PARTS of the first two           fewer rows still: the keys divided among workgroups too, each leaves its sums in the workspace in fp32 and
 //                                    cross_attention_join_kernel adds them up, in their order
-// plan_of() chooses, by what each would cost.  1000 queries x 1000 keys, eight heads of 64: rows kernel 13.1 us, keys kernel 9.2; 4000 x 77: 6.1 and 9.4.
+// plan_of() chooses, by what each would cost (its comments: what they measured).  1000 queries x 1000 keys, eight heads of 64: rows kernel 13.1 us, keys kernel 9.2; 4000 x 77: 6.1 and 9.4.
 #include "common.h"
 #include "kernels.h"
 #include <type_traits>
@@ -989,17 +989,16 @@ struct Plan {
 
 int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// Microseconds of a launch, fitted to measurements (1 to 8000 queries, 77 to 4000 keys, 4 and 8 heads): a workgroup's step - a chunk of 64 keys, or 32
+// Microseconds of a launch, fitted to measurements (1 to 64 800 queries, 77 to 4000 keys, 4 and 8 heads): a workgroup's step - a chunk of 64 keys, or 32
 // keys for each of its waves - alone on its CU, and one of several there; what a round of workgroups costs besides; how many a CU holds.
-struct Cost { float alone, among, round; };
+struct Cost { float alone, among, round; int per_cu; };
 struct Costs {
-  Cost rows[2], keys[3];  // 16 and 32 rows per wave; 16, 32 and 64 per workgroup
-  int rows_per_cu, keys_per_cu;
+  Cost rows[3], keys[3];  // 16, 32 and 64 rows per wave; per workgroup
 };
 const Costs& costs_of(int64_t head_dim) {
-  static const Costs c32 = {{{0.48f, 0.25f, 1.6f}, {0.56f, 0.40f, 1.9f}}, {{0.32f, 0.27f, 1.2f}, {0.41f, 0.30f, 1.6f}, {0.57f, 0.45f, 2.4f}}, 4, 4};
-  static const Costs c64 = {{{0.56f, 0.40f, 1.8f}, {0.75f, 0.55f, 2.2f}}, {{0.40f, 0.30f, 1.7f}, {0.48f, 0.39f, 2.4f}, {0.70f, 0.65f, 3.6f}}, 3, 2};
-  static const Costs c128 = {{{0.86f, 0.65f, 1.9f}, {1.12f, 0.95f, 2.3f}}, {{0.60f, 0.68f, 2.0f}, {0.75f, 0.85f, 3.2f}, {1.05f, 1.20f, 5.5f}}, 2, 1};
+  static const Costs c32 = {{{0.48f, 0.25f, 1.6f, 4}, {0.56f, 0.40f, 1.9f, 4}, {}}, {{0.32f, 0.27f, 1.2f, 4}, {0.41f, 0.30f, 1.6f, 4}, {0.57f, 0.45f, 2.4f, 4}}};
+  static const Costs c64 = {{{0.56f, 0.40f, 1.8f, 3}, {0.75f, 0.55f, 2.2f, 3}, {1.32f, 0.95f, 5.5f, 2}}, {{0.40f, 0.30f, 1.7f, 2}, {0.48f, 0.39f, 2.4f, 2}, {0.70f, 0.65f, 3.6f, 2}}};
+  static const Costs c128 = {{{0.86f, 0.65f, 1.9f, 2}, {1.12f, 0.95f, 2.3f, 2}, {}}, {{0.60f, 0.68f, 2.0f, 1}, {0.75f, 0.85f, 3.2f, 1}, {1.05f, 1.20f, 5.5f, 1}}};
   return head_dim == 32 ? c32 : head_dim == 64 ? c64 : c128;
 }
 
@@ -1014,14 +1013,14 @@ int keys_of(Form form) { return form == Form::rows ? KC : 32; }
 int64_t chunks_of(const Task& t, int u) { return (int64_t)div_up(t.Np, u) + div_up(t.Nk, u); }
 Way way_of(const Task& t, int Hk, int head_dim, Form form, int qn, int splits) {
   const Costs& c = costs_of(head_dim);
-  const Cost& one = form == Form::rows ? c.rows[qn - 1] : c.keys[qn / 2];
+  const Cost& one = form == Form::rows ? c.rows[qn / 2] : c.keys[qn / 2];
   const int64_t wgs = (int64_t)t.members * Hk * div_up(t.rows, rows_of(form, qn)) * splits;
   const int64_t chunks = div_up(chunks_of(t, keys_of(form)), splits), steps = form == Form::rows ? chunks : div_up(chunks, NWAVE);
-  const int rounds = div_up(wgs, 256 * (form == Form::rows ? c.rows_per_cu : c.keys_per_cu));
+  const int rounds = div_up(wgs, 256 * one.per_cu);
   const float several = one.among * div_up(wgs, 256), step = several > one.alone ? several : one.alone;
   float us = 2.4f + rounds * one.round + steps * step;
   // reading the keys, at a rate that grows with what a CU has on its way (32 KB 5.1 TB/s, 64 KB 5.7), longer where the last round leaves part of the chip idle
-  const float slots = 256.f * (form == Form::rows ? c.rows_per_cu : c.keys_per_cu);
+  const float slots = 256.f * one.per_cu;
   const float on_way = (wgs < slots ? wgs : slots) / 256.f * (form == Form::rows ? KC : 32 * NWAVE) * head_dim * 4;
   const float read = 4e-6f * t.members * Hk * head_dim * ((float)t.Np + t.Nk) / 6.4f * (1.f + 8192.f / on_way) * (rounds > 1 ? rounds * slots / wgs : 1.f);
   us = us > read ? us : read;
@@ -1094,13 +1093,14 @@ Plan plan_of(const CrossArgs& a) {
       return plan;
     }
   }
-  // Otherwise the way that costs least.  Parts of the keys: what fills the chip once, twice, ..; no more chunks in one than a mask's words cover
+  // Otherwise the way that costs least (eight heads of 64, 1000 keys, in us: 8000 queries, 32 rows a wave 24.2, 64 27.3; 16 000 48.6 and 38.9, whose
+  // workgroups fill the chip once; 24 000 61.9 and 63; 64 800 162 and 149).  Parts of the keys: what fills the chip once, twice, ..; no more chunks in one than a mask's words cover
   Way best{Form::rows, 1, 1, 1e30f};
   int splits[2] = {1, 1};
-  for (int f = 0; f < 5; ++f) {
-    const Form form = f < 2 ? Form::rows : Form::keys;
-    const int qn = f < 2 ? f + 1 : 1 << (f - 2);
-    if (form == Form::rows && plan.parts && qn == 1) continue;
+  for (int f = 0; f < 6; ++f) {
+    const Form form = f < 3 ? Form::rows : Form::keys;
+    const int qn = 1 << (f % 3);
+    if (form == Form::rows && (plan.parts ? qn != 2 : costs_of(D).rows[qn / 2].per_cu == 0)) continue;  // (in parts 32 rows a wave)
     float us = 0.f;
     int s[2] = {1, 1};
     bool whole = true;
@@ -1109,7 +1109,7 @@ Plan plan_of(const CrossArgs& a) {
       const int64_t one = (int64_t)t.members * Hk * div_up(t.rows, rows_of(form, qn)), chunks = chunks_of(t, keys_of(form));
       const int least = masked && t.Nk > 0 ? div_up(chunks, MAX_WORDS) : 1;
       Way w = way_of(t, Hk, D, form, qn, least > 1 ? least : 1);
-      for (int slots = 256; slots <= 1024 && !(form == Form::rows && qn == 1); slots += 256) {
+      for (int slots = 256; slots <= 1024 && !(form == Form::rows && qn != 2); slots += 256) {
         const int64_t n = slots / one < div_up(chunks, NWAVE) ? slots / one : div_up(chunks, NWAVE);
         if (n <= 1 || n < least) continue;
         const Way x = way_of(t, Hk, D, form, qn, (int)n);
@@ -1119,7 +1119,7 @@ Plan plan_of(const CrossArgs& a) {
       us += w.us;
       whole = whole && w.splits == 1;
     }
-    if (form == Form::rows && qn == 1 && !whole) continue;  // (16 rows a wave: not in parts)
+    if (form == Form::rows && qn != 2 && !whole) continue;
     if (us < best.us) {
       best = {form, qn, 1, us};
       splits[0] = s[0];
@@ -1130,10 +1130,6 @@ Plan plan_of(const CrossArgs& a) {
     plan.task[i].splits = splits[i];
     plan.parts = plan.parts || splits[i] > 1;
   }
-  // long key ranges for many rows, 64 rows a wave: 129 600 x 4000 keys, one head, 144 -> 132 us; 400 keys 69.5 -> 74.8, 500 workgroups on the mark
-  if (best.form == Form::rows && best.qn == 2 && !plan.parts && D == 64 && chunks_of(plan.task[0], KC) >= 12 &&
-      (int64_t)plan.task[0].members * Hk * div_up(plan.task[0].rows, 256) >= 500)
-    best.qn = 4;
   setup(best.form, best.qn);
   return plan;
 }
