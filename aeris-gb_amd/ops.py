@@ -112,9 +112,9 @@ def workspaces(device, *requests):
 def _workspace_ptr(tag: str, nbytes: int, device) -> int:
     """``workspace`` for a call that needs its address alone: the buffer that it last used on this stream, without a tensor around it."""
     key = (tag, device, torch.uint8)
-    buf = _WORKSPACE.get(key)
-    if (buf is None or buf.numel() < nbytes or torch._C._cuda_isCurrentStreamCapturing() or
-            _WS_OWNER[key][0] != torch._C._cuda_getCurrentRawStream(device.index)):
+    buf, owner = _WORKSPACE.get(key), _WS_OWNER.get(key)  # (no owner: so far it was asked for under captures alone)
+    if (buf is None or owner is None or buf.numel() < nbytes or torch._C._cuda_isCurrentStreamCapturing() or
+            owner[0] != torch._C._cuda_getCurrentRawStream(device.index)):
         return workspace(tag, (nbytes,), torch.uint8, device).data_ptr()
     return buf.data_ptr()
 

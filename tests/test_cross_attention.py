@@ -414,3 +414,24 @@ def test_grids_that_cannot_be_launched(pkg):
     for args in [(1 << 24, 1, 1, 9), (1 << 29, 1, 1, 9), (1 << 20, 1, 16, 100), (1 << 26, 1, 1, 9, 100), (1 << 28, 1, 4, 1)]:
         # (the last has 2^28 * 4 = 2^30 rows, one more than the limit of rows lets through)
         assert call(*args) == L.EUNSUPPORTED and ("workgroups" in L.last_error() or "rows" in L.last_error()), args
+
+
+@pytest.mark.gpu
+def test_workspace_first_asked_for_under_a_capture(pkg, cuda):
+    """The sums' buffer is made by the first call that needs it, which may be one that is captured; eager calls then go on with it."""
+    ops = pkg.ops
+    (q, k, v), _ = inputs(2, 3, 4, 4, 64, 9000, cuda, 14)
+    want = oracle(q, k, v)
+    check(ops.cross_attention(q[:, :, :, :], k[:, :100], v[:, :100]), oracle(q, k[:, :100], v[:, :100]))  # (one that needs none)
+    for made in (ops._WORKSPACE, ops._WS_OWNER):
+        for key in [key for key in made if key[0] == "cross_attention"]:
+            ops._RETIRED.append(made.pop(key))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.cross_attention(q, k, v)
+    for _ in range(3):
+        check(ops.cross_attention(q, k, v), want)
+        got.fill_(5.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(got, want)
