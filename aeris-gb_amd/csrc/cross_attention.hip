@@ -1023,7 +1023,8 @@ struct Way {
 int rows_of(Form form, int qn) { return 16 * qn * (form == Form::rows ? NWAVE : 1); }
 int keys_of(Form form) { return form == Form::rows ? KC : 32; }
 int64_t chunks_of(const Task& t, int u) { return (int64_t)div_up(t.Np, u) + div_up(t.Nk, u); }
-Way way_of(const Task& t, int Hk, int head_dim, Form form, int qn, int splits) {
+// (parts: the sums go through the workspace in any case)
+Way way_of(const Task& t, int Hk, int head_dim, Form form, int qn, int splits, bool parts) {
   const Costs& c = costs_of(head_dim);
   const Cost& one = form == Form::rows ? c.rows[qn / 2] : c.keys[qn / 2];
   const int64_t wgs = (int64_t)t.members * Hk * div_up(t.rows, rows_of(form, qn)) * splits;
@@ -1034,10 +1035,12 @@ Way way_of(const Task& t, int Hk, int head_dim, Form form, int qn, int splits) {
   // reading the keys, at a rate that grows with what a CU has on its way (32 KB 5.1 TB/s, 64 KB 5.7), longer where the last round leaves part of the chip idle
   const float slots = 256.f * one.per_cu;
   const float on_way = (wgs < slots ? wgs : slots) / 256.f * (form == Form::rows ? KC : 32 * NWAVE) * head_dim * 4;
-  const float read = 4e-6f * t.members * Hk * head_dim * ((float)t.Np + t.Nk) / 6.4f * (1.f + 8192.f / on_way) * (rounds > 1 ? rounds * slots / wgs : 1.f);
+  // (members after the first find the prefix in L2, at about three times memory's rate)
+  const float read = 4e-6f * Hk * head_dim * ((1.f + 0.35f * (t.members - 1)) * t.Np + (float)t.members * t.Nk) / 6.4f * (1.f + 8192.f / on_way) * (rounds > 1 ? rounds * slots / wgs : 1.f);
   us = us > read ? us : read;
-  // the joining kernel, and what the parts' sums cost to write and read
-  if (splits > 1) us += 6.0f + 0.55f * 4e-6f * t.members * Hk * (float)t.rows * splits * head_dim;
+  // what the parts' sums cost to write and read, and the joining kernel
+  if (parts || splits > 1) us += 0.55f * 4e-6f * t.members * Hk * (float)t.rows * splits * head_dim;
+  if (splits > 1 && !parts) us += 6.0f;
   return {form, qn, splits, us};
 }
 
@@ -1048,7 +1051,7 @@ Plan plan_of(const CrossArgs& a) {
   const bool shared = !own || (a.k_batch_stride == 0 && a.v_batch_stride == 0 && (!a.lengths || a.lengths_stride == 0) &&
                                (!a.key_mask || a.mask_batch_stride == 0));
   Plan plan{};
-  auto add = [&](bool all, int64_t Nk, int64_t Np) {
+  auto add = [&](Plan& plan, bool all, int64_t Nk, int64_t Np) {
     Task& t = plan.task[plan.n++];
     t.Nk = (int)Nk;
     t.Np = (int)Np;
@@ -1057,13 +1060,9 @@ Plan plan_of(const CrossArgs& a) {
     t.splits = 1;
   };
   if (B == 1 || (shared && rows_m % 128 != 0)) {
-    add(true, a.Nk, a.Np);
-  } else if (a.Np > 0 && own && rows_m < 128) {  // the prefix once for all members
-    add(true, 0, a.Np);
-    add(false, a.Nk, 0);
-    plan.parts = true;
+    add(plan, true, a.Nk, a.Np);
   } else {
-    add(false, a.Nk, a.Np);
+    add(plan, false, a.Nk, a.Np);
   }
   auto setup = [&](Form form, int qn) {
     plan.form = form;
@@ -1106,41 +1105,60 @@ Plan plan_of(const CrossArgs& a) {
     }
   }
   // Otherwise the way that costs least (eight heads of 64, 1000 keys, in us: 8000 queries, 32 rows a wave 24.2, 64 27.3; 16 000 48.6 and 38.9, whose
-  // workgroups fill the chip once; 24 000 61.9 and 63; 64 800 162 and 149).  Parts of the keys: what fills the chip once, twice, ..; no more chunks in one than a mask's words cover
-  Way best{Form::rows, 1, 1, 1e30f};
-  int splits[2] = {1, 1};
-  for (int f = 0; f < 6; ++f) {
-    const Form form = f < 3 ? Form::rows : Form::keys;
-    const int qn = 1 << (f % 3);
-    if (form == Form::rows && (plan.parts ? qn != 2 : costs_of(D).rows[qn / 2].per_cu == 0)) continue;  // (in parts 32 rows a wave)
-    float us = 0.f;
-    int s[2] = {1, 1};
-    bool whole = true;
-    for (int i = 0; i < plan.n; ++i) {
-      const Task& t = plan.task[i];
-      const int64_t one = (int64_t)t.members * Hk * div_up(t.rows, rows_of(form, qn)), chunks = chunks_of(t, keys_of(form));
-      const int least = masked && t.Nk > 0 ? div_up(chunks, MAX_WORDS) : 1;
-      Way w = way_of(t, Hk, D, form, qn, least > 1 ? least : 1);
-      for (int slots = 256; slots <= 1024 && !(form == Form::rows && qn != 2); slots += 256) {
-        const int64_t n = slots / one < div_up(chunks, NWAVE) ? slots / one : div_up(chunks, NWAVE);
-        if (n <= 1 || n < least) continue;
-        const Way x = way_of(t, Hk, D, form, qn, (int)n);
-        if (x.us < w.us) w = x;
+  // workgroups fill the chip once; 24 000 61.9 and 63; 64 800 162 and 149).  Parts of the keys: what fills the chip once, twice, ..; no more chunks
+  // in one than a mask's words cover
+  auto choose = [&](Plan& plan) {
+    Way best{Form::rows, 1, 1, 1e30f};
+    int splits[2] = {1, 1};
+    const bool parts = plan.parts;
+    for (int f = 0; f < 6; ++f) {
+      const Form form = f < 3 ? Form::rows : Form::keys;
+      const int qn = 1 << (f % 3);
+      if (form == Form::rows && (parts ? qn != 2 : costs_of(D).rows[qn / 2].per_cu == 0)) continue;  // (in parts 32 rows a wave)
+      float us = parts ? 6.0f : 0.f;
+      int s[2] = {1, 1};
+      bool whole = true;
+      for (int i = 0; i < plan.n; ++i) {
+        const Task& t = plan.task[i];
+        const int64_t one = (int64_t)t.members * Hk * div_up(t.rows, rows_of(form, qn)), chunks = chunks_of(t, keys_of(form));
+        const int least = masked && t.Nk > 0 ? div_up(chunks, MAX_WORDS) : 1;
+        Way w = way_of(t, Hk, D, form, qn, least > 1 ? least : 1, parts);
+        for (int slots = 256; slots <= 1024 && !(form == Form::rows && qn != 2); slots += 256) {
+          const int64_t n = slots / one < div_up(chunks, NWAVE) ? slots / one : div_up(chunks, NWAVE);
+          if (n <= 1 || n < least) continue;
+          const Way x = way_of(t, Hk, D, form, qn, (int)n, parts);
+          if (x.us < w.us) w = x;
+        }
+        s[i] = w.splits;
+        us += w.us;
+        whole = whole && w.splits == 1;
       }
-      s[i] = w.splits;
-      us += w.us;
-      whole = whole && w.splits == 1;
+      if (form == Form::rows && qn != 2 && !whole) continue;
+      if (us < best.us) {
+        best = {form, qn, 1, us};
+        splits[0] = s[0];
+        splits[1] = s[1];
+      }
     }
-    if (form == Form::rows && qn != 2 && !whole) continue;
-    if (us < best.us) {
-      best = {form, qn, 1, us};
-      splits[0] = s[0];
-      splits[1] = s[1];
+    for (int i = 0; i < plan.n; ++i) {
+      plan.task[i].splits = splits[i];
+      plan.parts = plan.parts || splits[i] > 1;
     }
-  }
-  for (int i = 0; i < plan.n; ++i) {
-    plan.task[i].splits = splits[i];
-    plan.parts = plan.parts || splits[i] > 1;
+    return best;
+  };
+  Way best = choose(plan);
+  // or the prefix once for all members, behind it their own: pays from some prefix on (16 members, a query each, 12 heads of 64, 64 keys of their own:
+  // prefix of 64 4.4 us in one, 11 apart; 1000 8.8, 11.5; 4000 22, 12.4)
+  if (plan.task[0].members > 1 && a.Np > 0 && own && rows_m < 128) {
+    Plan apart{};
+    add(apart, true, 0, a.Np);
+    add(apart, false, a.Nk, 0);
+    apart.parts = true;
+    const Way way = choose(apart);
+    if (way.us < best.us) {
+      plan = apart;
+      best = way;
+    }
   }
   setup(best.form, best.qn);
   return plan;

@@ -356,6 +356,9 @@ PLANS = [
     (5, 69, 9, 3, 64, 82, 12565), (5, 8613, 3, 1, 64, 108, 764), (1, 2065, 2, 1, 128, 85, 0), (2, 4129, 2, 1, 128, 82, 45), (2, 794, 1, 1, 128, 86, 15413),
     (64, 8300, 8, 8, 32, 330, 0),  # (65 row blocks for a wave)
     (64, 1, 4, 4, 32, 300, 0), (66, 3, 8, 4, 32, 90, 200), (24, 100, 6, 6, 64, 130, 100), (40, 30, 4, 1, 64, 500, 300), (9, 700, 2, 2, 64, 700, 0), (1, 1, 2, 1, 32, 70, 20000),
+    (16, 1, 4, 4, 32, 995, 7255), (30, 65, 2, 2, 32, 124, 7057), (9, 65, 3, 3, 32, 527, 22632), (9, 2, 8, 8, 64, 1776, 3992), (30, 65, 1, 1, 64, 28, 14157),
+    (16, 65, 2, 2, 64, 2023, 25529), (5, 1, 8, 8, 128, 1807, 3165), (16, 34, 1, 1, 128, 10, 22724), (30, 35, 3, 3, 128, 1494, 5251),
+    (3, 72, 8, 8, 32, 22, 29633), (9, 65, 3, 3, 64, 30, 23859), (5, 73, 4, 4, 128, 60, 15456),  # the prefix once for all members
 ]
 
 
