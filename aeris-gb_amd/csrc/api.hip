@@ -449,7 +449,7 @@ int check_cross_sizes(const char* who, const aeris_cross_attention* a, aeris::Cr
 int64_t aeris_cross_attention_workspace_bytes(const aeris_cross_attention* a) {
   aeris::CrossArgs c;
   if (check_cross_sizes("aeris_cross_attention_workspace_bytes", a, &c)) return 0;
-  return aeris::cross_attention_workspace_bytes(c);
+  return aeris::cross_attention_plan(c).workspace_bytes;
 }
 
 int aeris_cross_attention_fwd(const aeris_cross_attention* a, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -471,12 +471,13 @@ int aeris_cross_attention_fwd(const aeris_cross_attention* a, void* workspace, i
   if (c.lengths && (reinterpret_cast<uintptr_t>(c.lengths) & 3u)) return fail(AERIS_EINVAL, "%s: lengths must be 4-byte aligned", who);
   if (c.key_mask && c.mask_batch_stride < 0) return fail(AERIS_EINVAL, "%s: mask_stride must not be negative", who);
   if (!c.q_prescaled && !(c.scale > 0.0 && c.scale < 1e30)) return fail(AERIS_EINVAL, "%s: scale must be positive", who);
-  if (!aeris::cross_attention_fits(c)) return fail(AERIS_EUNSUPPORTED, "%s: B * kv_heads or the rows need 2^24 workgroups or more", who);
-  const int64_t need = aeris::cross_attention_workspace_bytes(c);
+  const aeris::CrossPlan plan = aeris::cross_attention_plan(c);
+  if (!plan.fits) return fail(AERIS_EUNSUPPORTED, "%s: B * kv_heads or the rows need 2^24 workgroups or more", who);
+  const int64_t need = plan.workspace_bytes;
   if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
     return fail(AERIS_EINVAL, "%s: workspace must be 16-byte aligned and hold %lld bytes (got %lld)", who, (long long)need, (long long)workspace_bytes);
   if (int rc = ensure_init(stream, true)) return rc;
-  hipError_t e = aeris::cross_attention_launch(c, workspace, reinterpret_cast<hipStream_t>(stream));
+  hipError_t e = aeris::cross_attention_launch(c, plan, workspace, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "aeris_cross_attention_fwd launch");
   return AERIS_OK;
 }

@@ -21,6 +21,7 @@
 // plan_of() chooses, by what each would cost (its comments: what they measured).  1000 queries x 1000 keys, eight heads of 64: rows kernel 13.1 us, keys kernel 9.2; 4000 x 77: 6.1 and 9.4.
 #include "common.h"
 #include "kernels.h"
+#include <cstring>
 #include <type_traits>
 
 namespace aeris {
@@ -1277,19 +1278,23 @@ hipError_t cross_attention_configure() {
   return e;
 }
 
-int64_t cross_attention_workspace_bytes(const CrossArgs& a) { return plan_of(a).bytes; }
-
-// (a grid has less than 2^32 threads; up to 1024 of them join a row)
-bool cross_attention_fits(const CrossArgs& a) {
+CrossPlan cross_attention_plan(const CrossArgs& a) {
+  static_assert(std::is_trivially_copyable<Plan>::value && sizeof(Plan) <= sizeof(CrossPlan::inside), "the plan travels as bytes");
   const Plan plan = plan_of(a);
   int64_t units = 0;
   for (int i = 0; i < plan.n; ++i) units += (int64_t)plan.task[i].splits * plan.task[i].members * a.kv_heads;
   const int parts = plan.task[0].splits + plan.task[1].splits;
-  return units < (1 << 24) && plan.grid < (1 << 24) && (!plan.parts || a.B * a.Nq * a.heads < (parts <= 16 ? 1 << 26 : parts <= 64 ? 1 << 24 : 1 << 22));
+  CrossPlan c{};
+  c.workspace_bytes = plan.bytes;
+  // (a grid has less than 2^32 threads; up to 1024 of them join a row)
+  c.fits = units < (1 << 24) && plan.grid < (1 << 24) && (!plan.parts || a.B * a.Nq * a.heads < (parts <= 16 ? 1 << 26 : parts <= 64 ? 1 << 24 : 1 << 22));
+  memcpy(c.inside, &plan, sizeof(plan));
+  return c;
 }
 
-hipError_t cross_attention_launch(const CrossArgs& a, void* workspace, hipStream_t stream) {
-  Plan plan = plan_of(a);
+hipError_t cross_attention_launch(const CrossArgs& a, const CrossPlan& c, void* workspace, hipStream_t stream) {
+  Plan plan;
+  memcpy(&plan, c.inside, sizeof(plan));
   if (a.head_dim == 32) return launch_dim<32>(a, plan, workspace, stream);
   if (a.head_dim == 64) return launch_dim<64>(a, plan, workspace, stream);
   return launch_dim<128>(a, plan, workspace, stream);

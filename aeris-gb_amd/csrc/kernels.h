@@ -83,9 +83,13 @@ struct CrossArgs {
 };
 bool cross_attention_supported(int64_t head_dim);
 hipError_t cross_attention_configure();
-int64_t cross_attention_workspace_bytes(const CrossArgs& a);
-bool cross_attention_fits(const CrossArgs& a);  // whether its grid is one that can be launched
-hipError_t cross_attention_launch(const CrossArgs& a, void* workspace, hipStream_t stream);
+struct CrossPlan {           // how a call is run
+  int64_t workspace_bytes;
+  bool fits;                 // whether its grids can be launched
+  alignas(8) char inside[256];
+};
+CrossPlan cross_attention_plan(const CrossArgs& a);
+hipError_t cross_attention_launch(const CrossArgs& a, const CrossPlan& plan, void* workspace, hipStream_t stream);
 
 hipError_t modulation_linear_launch(const aeris_modulation_layer* layers, int n, int B, int K, int w_dtype, int act, hipStream_t stream);
 hipError_t heun_update_launch(const float* x, const float* f0, const float* f1, const float* t, float sigma_data, float* out, int64_t n,
