@@ -547,7 +547,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, length
     projection); heads is a multiple of the key heads, head h uses key head h // (heads // key heads); k and v of batch 1 serve every member.
     lengths int32 [B | 1]: how many of the Nk keys a member has; key_mask bool | uint8 [B | 1, Nk]: which of those take part.  What k and v
     hold elsewhere is not looked at.  prefix = (k, v), [Np, key heads, head_dim]: states that all members see ahead of their own, read once
-    for all of them where a member has few queries.  A query without any key gives zeros.
+    for all of them where that is cheaper.  A query without any key gives zeros.
     scale: head_dim^-0.5 unless given; ``q_prescaled``: q already holds q * scale * log2(e) (``qk_norm_rope(q_scale=scale * LOG2E)``).  out shares
     no memory with the inputs."""
     device, shape, kv_shape, bf16 = q.device, q.shape, k.shape, torch.bfloat16
