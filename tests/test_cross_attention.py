@@ -438,3 +438,30 @@ def test_workspace_first_asked_for_under_a_capture(pkg, cuda):
         graph.replay()
         torch.cuda.synchronize()
         check(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Nq,D", [(1, 32), (40, 64), (3000, 64), (1500, 128), (60000, 32), (60000, 64)])
+def test_masks_longer_than_a_workgroup_holds(pkg, cuda, Nq, D):
+    """More chunks of keys than a workgroup has words for their mask: the keys are divided even where the rows alone fill the chip."""
+    Nk = 70001
+    (q, k, v), g = inputs(2, Nq, 2, 1, D, Nk, cuda, 31)
+    mask = (torch.rand(2, Nk, generator=g) < 0.5).to(cuda)
+    mask[1, :40000] = False
+    lengths = torch.tensor([Nk, 65536], dtype=torch.int32, device=cuda)
+    k[~mask], v[~mask] = math.nan, math.nan
+    some = sorted({n for n in (0, 17, 63, 64, 128, 1000, Nq - 1) if n < Nq})
+    got = pkg.ops.cross_attention(q, k, v, lengths=lengths, key_mask=mask)
+    check(got[:, some].contiguous(), oracle(q[:, some], k, v, lengths, mask))
+
+
+@pytest.mark.gpu
+def test_one_set_of_states_with_a_mask_for_each_member(pkg, cuda):
+    """Keys of batch 1 and lengths or masks of every member: members share what they read, not what they see."""
+    (q, k, v), g = inputs(6, 130, 4, 2, 64, 700, cuda, 33, kv_batch=1)
+    mask = (torch.rand(6, 700, generator=g) < 0.5).to(cuda)
+    mask[2] = False
+    lengths = torch.tensor([700, 0, 300, 1, 64, 65], dtype=torch.int32, device=cuda)
+    for nq in (1, 7, 128, 130):
+        for kw in (dict(key_mask=mask), dict(lengths=lengths), dict(lengths=lengths, key_mask=mask), dict(lengths=lengths, key_mask=mask[:1])):
+            check(pkg.ops.cross_attention(q[:, :nq], k, v, **kw), oracle(q[:, :nq], k, v, kw.get("lengths"), kw.get("key_mask")))
