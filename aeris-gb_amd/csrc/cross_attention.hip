@@ -18,7 +18,8 @@
 //   cross_attention_resident_kernel  few keys and many rows: a workgroup keeps the unit's keys in LDS and walks down the rows
 //   PARTS of the first two           fewer rows still: the keys divided among workgroups too, each leaves its sums in the workspace in fp32 and
 //                                    cross_attention_join_kernel adds them up, in their order
-// plan_of() chooses, by what each would cost (its comments: what they measured).  1000 queries x 1000 keys, eight heads of 64: rows kernel 13.1 us, keys kernel 9.2; 4000 x 77: 6.1 and 9.4.
+// plan_of() chooses, by what each would cost (its comments: what they measured).  1000 queries x 1000 keys, eight heads of 64: rows kernel 13.1 us, keys
+// kernel 9.2; 4000 x 77: 6.1 and 9.4.
 #include "common.h"
 #include "kernels.h"
 #include <cstring>
@@ -908,21 +909,34 @@ __global__ void __launch_bounds__(WPR > 4 ? 64 * WPR : 256) cross_attention_join
     const int64_t bq = row / p.heads;
     const int query = (int)(bq % p.Nq), b = (int)(bq / p.Nq);
     const int hk = head / p.group, rm = query * p.group + head - hk * p.group;
+    int64_t first[2], step[2];
+    float pm2[2], pl2[2];  // of the first parts of both sets: their reads are on the way together
+    auto look = [&](int set, int s0, float& pm, float& pl) {
+      const Task& t = p.task[set];
+      pm = -3.0e38f;
+      pl = 0.f;
+      if (s0 + lane * WPR < t.splits) {
+        const float* at = t.ml + 2 * (first[set] + (s0 + lane * WPR) * step[set]);
+        pm = at[0];
+        pl = at[1];
+      }
+    };
 #pragma unroll
     for (int set = 0; set < 2; ++set) {
       const Task& t = p.task[set];
       const bool all = t.members == 1;  // a unit's rows are those of all members
-      const int64_t first = ((int64_t)(all ? 0 : b) * p.kv_heads + hk) * t.rows + (all ? b * p.rows_m : 0) + rm;
-      const int64_t step = (int64_t)t.members * p.kv_heads * t.rows;
+      first[set] = ((int64_t)(all ? 0 : b) * p.kv_heads + hk) * t.rows + (all ? b * p.rows_m : 0) + rm;
+      step[set] = (int64_t)t.members * p.kv_heads * t.rows;
+      look(set, first_part, pm2[set], pl2[set]);
+    }
+#pragma unroll
+    for (int set = 0; set < 2; ++set) {
+      const Task& t = p.task[set];
       for (int s0 = first_part; s0 < t.splits; s0 += 64 * WPR) {
         const int n = (t.splits - s0 + WPR - 1) / WPR < 64 ? (t.splits - s0 + WPR - 1) / WPR : 64;
-        float pm = -3.0e38f, pl = 0.f;
-        if (lane < n) {
-          const float* at = t.ml + 2 * (first + (s0 + lane * WPR) * step);
-          pm = at[0];
-          pl = at[1];
-          if (pl == 0.f) pm = -3.0e38f;  // no key of this part
-        }
+        float pm = pm2[set], pl = pl2[set];
+        if (s0 != first_part) look(set, s0, pm, pl);
+        if (pl == 0.f) pm = -3.0e38f;  // no key of this part
         float mx = pm;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
@@ -937,7 +951,7 @@ __global__ void __launch_bounds__(WPR > 4 ? 64 * WPR : 256) cross_attention_join
           for (int u = 0; u < AT_ONCE / SUB; ++u) {
             const int i = i0 + u * SUB + sub;
             wi[u] = __shfl(w, i, 64);
-            const int64_t at = first + (s0 + (i < n ? i : n - 1) * WPR) * step;
+            const int64_t at = first[set] + (s0 + (i < n ? i : n - 1) * WPR) * step[set];
             po[u] = *reinterpret_cast<const f32x4*>(t.o + at * HD + 4 * c);
           }
 #pragma unroll
