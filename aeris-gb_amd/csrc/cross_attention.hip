@@ -215,8 +215,18 @@ struct Rows {
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    // Keys that do not take part: their rows of K and V are zeros, so that FAST, where P is then 1, has them in the sum alone (sums() takes
-    // them out again)
+    // Keys that do not take part: their rows of K and V are zeros, so that FAST, where P is then 1, has them in the sum alone.  They are taken out of it
+    // chunk by chunk, each lane's of its own: left in until the end they would be a sum beside which small weights are rounded away (weights of 2^-12.5,
+    // a tenth of 60 000 keys masked: 2 per cent of the sum).
+    if (FAST && keys != ~0ull) {
+      const uint32_t lo = ~(uint32_t)keys >> (4 * q4) & 0x000f000fu, hi = ~(uint32_t)(keys >> 32) >> (4 * q4) & 0x000f000fu;
+      const float ones = (float)(SUM ? KC - __builtin_popcountll(keys) : __builtin_popcount(lo) + __builtin_popcount(hi));
+#pragma unroll
+      for (int n = 0; n < QN; ++n) {
+        if (SUM) lv[n][0] -= ones;
+        else l[n] -= ones;
+      }
+    }
     if (!FAST && keys != ~0ull) {
       const uint64_t mine = keys >> (4 * q4);
 #pragma unroll
@@ -321,6 +331,11 @@ struct Rows {
 #pragma unroll
           for (int n = 0; n < QN; ++n) acc[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[b][s], qf[n][s], s == 0 ? zero4 : acc[n][b], 0, 0, 0);
     }
+    if (FAST && keys != ~0u) {  // (see chunk())
+      const float ones = (float)__builtin_popcount(~keys >> (4 * q4) & 0x000f000fu);
+#pragma unroll
+      for (int n = 0; n < QN; ++n) l[n] -= ones;
+    }
     if (!FAST) {
       const uint32_t mine = keys >> (4 * q4);
 #pragma unroll
@@ -377,9 +392,10 @@ struct Rows {
     __builtin_amdgcn_sched_barrier(0);
   }
 
-  // The rows' sums, `idle` keys of the chunks that did not take part taken out of them.  Whether any row's left the range in which exp2 needs no
-  // maximum (or is not a number), or is so small beside the idle keys' ones that their difference says little.
-  __device__ __forceinline__ bool sums(int idle) {
+  // The rows' sums.  `idle` keys of the chunks did not take part; `within`: as many of their ones are still in the sums.  Whether any row's left the range
+  // in which exp2 needs no maximum (or is not a number), or is so small beside the idle keys' ones that what the two together were rounded by counts:
+  // with n additions n 2^-24 2^6 of it, 2^-15 for those of a chunk's lane, 2^-13 for those of the nine chunks that may stay in LDS.
+  __device__ __forceinline__ bool sums(int idle, int within = 0) {
     bool bad = false;
 #pragma unroll
     for (int n = 0; n < QN; ++n) {
@@ -389,8 +405,8 @@ struct Rows {
         l[n] += __shfl_xor(l[n], 16, 64);
         l[n] += __shfl_xor(l[n], 32, 64);
       }
-      l[n] -= (float)idle;
-      bad = bad || !(l[n] >= 0x1p-20f && l[n] >= 0x1p-10f * (float)idle && l[n] <= 0x1p60f);
+      l[n] -= (float)within;
+      bad = bad || !(l[n] >= 0x1p-20f && l[n] >= 0x1p-6f * (float)idle && l[n] <= 0x1p60f);
     }
     return __builtin_amdgcn_ballot_w64(bad) != 0;
   }
@@ -857,7 +873,7 @@ cross_attention_resident_kernel(CrossParams p, int max_chunks) {
       rows.template chunk<true, true>(0, ~0ull);
       while (++c < nch) rows.template chunk<true>(c * BYTES, ~0ull);
     }
-    if (rows.sums(idle)) again |= 1ull << bit;
+    if (rows.sums(idle, idle)) again |= 1ull << bit;
     else rows.store(p, t, member, hk, row0, lane);
     if (++j == per_bit) {
       j = 0;

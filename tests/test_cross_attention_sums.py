@@ -1,0 +1,80 @@
+"""ops.cross_attention where its sums are hard to form: keys that take no part beside weights that are small, values at the ends of
+bf16's range, infinities, key masks of any length; every row held to a bound of its own.
+
+Roundings.  To bf16 a value is off by half a step, 2^-8 of it at most and 0.0017 of it in the mean square (2^-8 / sqrt 3 times the mean
+of 1 / m^2 over a mantissa m, 0.54, to the half).  The kernels round the weights (sum and norm have the rounded ones alike) and the result.
+A row's error has then, per element d, the mean square 0.0017^2 (sum_i w_i^2 (v_id - o_d)^2 + o_d^2), w_i the weights of sum one.  `row_bound`
+asks for four times the root of its sum over the row's elements (32 at least; a row of one weight: 2^-8 each, 2.3 times).
+fp32 sums: an addition is off by 2^-24 of the sum at most; a lane adds Nk / 8 pairs of weights: Nk 2^-27.
+"""
+import math
+
+import pytest
+import torch
+
+from test_cross_attention import heads, inputs, oracle
+
+STEP = 0.0017
+
+
+def row_bound(q, k, v, want, keep, exp2_domain=False):
+    """[n, H] for the rows q [n, H, D] of one member whose keys are k, v [Nk, Hk, D] where keep [Nk]."""
+    bound = torch.zeros(q.shape[:2], dtype=torch.float64, device=q.device)
+    H, D = q.shape[1:]
+    for h in range(H):
+        kk, vv = k[keep, h // (H // k.shape[1])].double(), v[keep, h // (H // k.shape[1])].double()
+        w = torch.softmax(q[:, h].double() @ kk.T * (math.log(2) if exp2_domain else D ** -0.5), -1)
+        o, w2 = want[:, h], w.square()
+        spread = w2 @ vv.square() - 2 * (w2 @ vv) * o + w2.sum(-1, keepdim=True) * o.square()
+        bound[:, h] = 4 * STEP * (spread + o.square()).sum(-1).clamp_min(0).sqrt() + (k.shape[0] * 2.0 ** -27 + 2.0 ** -12) * o.norm(dim=-1)
+    return bound
+
+
+def level_inputs(Nq, D, Nk, level, cuda, seed):
+    """q (prescaled) and k whose logits, base 2, are all `level` within about 0.05."""
+    g = torch.Generator().manual_seed(seed)
+    small = (0.05 / math.sqrt(D)) ** 0.5
+    q, k = torch.randn(1, Nq, 1, D, generator=g) * small, torch.randn(1, Nk, 1, D, generator=g) * small
+    q[..., 0], k[..., 0] = -4.0, -level / 4.0
+    return q.bfloat16().to(cuda), k.bfloat16().to(cuda), g
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("Nq,Nk", [(1, 300), (1, 8000), (1, 60000), (20, 8000), (60, 60000), (600, 8000), (9000, 300), (9000, 8000), (9000, 60000), (400000, 8000), (400000, 60000),
+                                   (70000, 77), (70000, 250), (70000, 500)])
+@pytest.mark.parametrize("masked", ["tenth", "most", "lanes"])
+def test_small_weights_beside_keys_that_take_no_part(pkg, cuda, D, Nq, Nk, masked):
+    """All logits far below zero, and one value at every key that takes part: the result is that value, whatever the weights, unless the
+    sums of weights are off by half of bf16's smallest relative step, 1 / 510.  (fp32 allows for Nk 2^-27 + 2^-12 < 1 / 1400, and as much
+    again in the sums of the products.)"""
+    for level in (-7.0, -10.0, -12.5):
+        q, k, g = level_inputs(Nq, D, Nk, level, cuda, Nq + Nk)
+        if masked == "lanes":  # keys that always meet the same lanes
+            mask = (torch.arange(Nk) % 16 >= 4)[None]
+        else:
+            mask = torch.rand(1, Nk, generator=g) >= (0.1 if masked == "tenth" else 0.6)
+        v = (torch.randn(1, 1, 1, D, generator=g).bfloat16() + torch.zeros(1, Nk, 1, D, dtype=torch.bfloat16)).to(cuda)
+        want = v[:, :1].expand(1, Nq, 1, D).clone()
+        mask = mask.to(cuda)
+        v[~mask], k[~mask] = math.nan, math.inf
+        got = pkg.ops.cross_attention(q, k, v, key_mask=mask, q_prescaled=True)
+        wrong = (got != want).flatten(1).sum().item()
+        assert wrong == 0, (level, wrong, float((got.double() / want.double()).mean()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("Nq,Nk", [(1, 8000), (50, 3000), (600, 8000), (9000, 500), (70000, 77)])
+@pytest.mark.parametrize("level", [-3.0, -10.0])
+def test_rows_under_masks(pkg, cuda, D, Nq, Nk, level):
+    """Values that differ from key to key, every row by its own bound."""
+    q, k, g = level_inputs(Nq, D, Nk, level, cuda, Nk)
+    v = torch.randn(1, Nk, 1, D, generator=g).bfloat16().to(cuda)
+    mask = (torch.rand(1, Nk, generator=g) >= 0.4).to(cuda)
+    v[~mask], k[~mask] = math.nan, math.inf
+    some = sorted({n for n in [0, 15, 63, 64, 127, 128, Nq - 1] + torch.randint(0, Nq, (40,), generator=g).tolist() if n < Nq})
+    got = pkg.ops.cross_attention(q, k, v, key_mask=mask, q_prescaled=True)[:, some]
+    want = oracle(q[:, some], k, v, mask=mask, exp2_domain=True)
+    off = (got.double() - want)[0].norm(dim=-1)
+    assert bool((off <= row_bound(q[0, some], k[0], v[0], want[0], mask[0], True)).all())
