@@ -4,8 +4,9 @@
 // A unit is one member's key head (or, where all members see the same keys, the key head with the rows of all of them); its rows are
 // the queries of the heads that share the key head, 16 QN a wave.  Keys go through LDS in chunks of 64; P = exp2(logit) is formed
 // without a row maximum - softmax does not depend on the subtracted constant, the maximum only guards the range -, the range of the sums is
-// checked afterwards and the rows are done again with a running maximum where it was left: 2^-20 to 2^60, so that values of v from 2^-106 to 2^67 in
-// size neither vanish nor overflow in their sums either.
+// checked afterwards and the rows are done again with a running maximum where it was left: 2^-20 to 2^60 for the weights' (values of v from 2^-106 on do
+// not vanish in theirs), up to 2^100 for the results'.  The maximum is then taken so much higher that all weights together are below 1: finite values
+// of any size have finite sums.
 //   K, V chunk [64][HD]  global -> LDS by the load unit (buffer_load ... lds), 16-byte pieces XOR-swizzled; a key that does not take
 //                        part is not read, its row arrives as zeros (whatever it held, NaN or infinity, is multiplied by nothing)
 //   S^T = K Q^T          v_mfma_f32_16x16x32_bf16; lane = one row, registers = keys; the scale, unless the producer of q has applied it (`SCALED`),
@@ -163,9 +164,9 @@ struct Rows {
   }
 
   // The chunk `at` bytes behind the first; bit i of `keys`: key i takes part (at least one).  FAST: P = exp2(logit); otherwise with the running maximum
-  // m, accumulated output and sum rescaled whenever a maximum moves.  FIRST (and FAST): the sums start here.
+  // m, `headroom` above the logits', accumulated output and sum rescaled whenever a maximum moves.  FIRST (and FAST): the sums start here.
   template <bool FAST, bool FIRST = false>
-  __device__ __forceinline__ void chunk(uint32_t at, uint64_t keys) {
+  __device__ __forceinline__ void chunk(uint32_t at, uint64_t keys, float headroom = 0.f) {
     // PV step of 32 keys: k slots 0-3 <-> keys 32 step + 4 q4 + (0..3), slots 4-7 <-> 16 more.  The fragments of half of the row
     // blocks are read ahead of the MFMAs of the half before.
     constexpr int DH = DB / 2, PARTS = KC / 32 * 2;
@@ -250,7 +251,7 @@ struct Rows {
         cm = fmaxf(cm, __shfl_xor(cm, 16, 64));
         cm = fmaxf(cm, __shfl_xor(cm, 32, 64));
         if (SCALED) cm *= q_mul;
-        const float m_new = fmaxf(m[n], cm);
+        const float m_new = fmaxf(m[n], cm + headroom);
         if (__builtin_amdgcn_ballot_w64(m_new > m[n]) != 0) {
           const float alpha = __builtin_amdgcn_exp2f(m[n] - m_new);
           l[n] *= alpha;
@@ -306,7 +307,7 @@ struct Rows {
   // EXACT, for 16 rows, where latency or reading bounds the time: the weights as two bf16 each, what the first leaves goes into a second product (error
   // 0.0024 -> 0.0017 of the result, its own rounding; 7.1 -> 7.8 us for 250 queries, eight heads of 64, 1000 keys, nothing for one query and 64 800)
   template <bool FAST>
-  __device__ __forceinline__ void step(uint32_t at, uint32_t keys) {
+  __device__ __forceinline__ void step(uint32_t at, uint32_t keys, float headroom = 0.f) {
     constexpr bool EXACT = QN == 1;
     TrFrag vt[DB];
     f32x4 acc[QN][2];
@@ -351,7 +352,7 @@ struct Rows {
         cm = fmaxf(cm, __shfl_xor(cm, 16, 64));
         cm = fmaxf(cm, __shfl_xor(cm, 32, 64));
         if (SCALED) cm *= q_mul;
-        const float m_new = fmaxf(m[n], cm), alpha = __builtin_amdgcn_exp2f(m[n] - m_new);
+        const float m_new = fmaxf(m[n], cm + headroom), alpha = __builtin_amdgcn_exp2f(m[n] - m_new);
         l[n] *= alpha;
 #pragma unroll
         for (int db = 0; db < DB; ++db) o[n][db] *= alpha;
@@ -394,7 +395,8 @@ struct Rows {
 
   // The rows' sums.  `idle` keys of the chunks did not take part; `within`: as many of their ones are still in the sums.  Whether any row's left the range
   // in which exp2 needs no maximum (or is not a number), or is so small beside the idle keys' ones that what the two together were rounded by counts:
-  // with n additions n 2^-24 2^6 of it, 2^-15 for those of a chunk's lane, 2^-13 for those of the nine chunks that may stay in LDS.
+  // with n additions n 2^-24 2^6 of it, 2^-15 for those of a chunk's lane, 2^-13 for those of the nine chunks that may stay in LDS.  Or whether a result's
+  // sum is beyond 2^100 or not a number.
   __device__ __forceinline__ bool sums(int idle, int within = 0) {
     bool bad = false;
 #pragma unroll
@@ -407,6 +409,13 @@ struct Rows {
       }
       l[n] -= (float)within;
       bad = bad || !(l[n] >= 0x1p-20f && l[n] >= 0x1p-6f * (float)idle && l[n] <= 0x1p60f);
+      float top = 0.f;  // (maximum, not max: NaN stays)
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2)
+          top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, fabsf(o[n][db][i])), fabsf(o[n][db][i + 1]));
+      bad = bad || !(top <= 0x1p100f);
     }
     return __builtin_amdgcn_ballot_w64(bad) != 0;
   }
@@ -440,6 +449,9 @@ struct Rows {
     }
   }
 };
+
+// How far above its logits a row's maximum is taken: weights of 2^-headroom at most, half a 1 for all keys of a task together
+__device__ __forceinline__ float headroom_of(const Task& t) { return (float)(33 - __builtin_clz((uint32_t)t.Np + (uint32_t)t.Nk | 1u)); }
 
 // A unit's keys in chunks of U: the prefix, then the member's own.
 template <int U>
@@ -622,6 +634,7 @@ cross_attention_rows_kernel(CrossParams p) {
 
   auto sweep = [&](auto fast_tag) {
     constexpr bool FAST = decltype(fast_tag)::value;
+    const float headroom = FAST ? 0.f : headroom_of(t);
     keys.seek(p, t, hk, c0);
     load.rows(lane, keys);
     if (nch > 0) issue(0, 0);
@@ -640,7 +653,7 @@ cross_attention_rows_kernel(CrossParams p) {
         if (kk[u] != 0) {
           any = true;
           if (FAST) idle += KC - __builtin_popcountll(kk[u]);
-          if (wave_active) rows.template chunk<FAST>(u * BYTES, kk[u]);
+          if (wave_active) rows.template chunk<FAST>(u * BYTES, kk[u], headroom);
         }
       }
     }
@@ -728,6 +741,7 @@ cross_attention_keys_kernel(CrossParams p) {
   int idle = 0;
   auto sweep = [&](auto fast_tag) {
     constexpr bool FAST = decltype(fast_tag)::value;
+    const float headroom = FAST ? 0.f : headroom_of(t);
 #pragma unroll
     for (int u = 0; u < RB - 1; ++u)
       if (u < steps) issue(u, u);
@@ -746,7 +760,7 @@ cross_attention_keys_kernel(CrossParams p) {
         if (kk[u] != 0) {
           any = true;
           if (FAST) idle += U - __builtin_popcount(kk[u]);
-          rows.template step<FAST>(u * 2 * BYTES, kk[u]);
+          rows.template step<FAST>(u * 2 * BYTES, kk[u], headroom);
         }
       }
     }
@@ -887,7 +901,7 @@ cross_attention_resident_kernel(CrossParams p, int max_chunks) {
       rows.reset();
       for (int c = 0; c < nch; ++c) {
         const uint64_t w = word_of(c);
-        if (w != 0) rows.template chunk<false>(c * BYTES, w);
+        if (w != 0) rows.template chunk<false>(c * BYTES, w, headroom_of(t));
       }
       rows.sums(0);
       rows.store(p, t, member, hk, row0, lane);

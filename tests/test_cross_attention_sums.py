@@ -78,3 +78,41 @@ def test_rows_under_masks(pkg, cuda, D, Nq, Nk, level):
     want = oracle(q[:, some], k, v, mask=mask, exp2_domain=True)
     off = (got.double() - want)[0].norm(dim=-1)
     assert bool((off <= row_bound(q[0, some], k[0], v[0], want[0], mask[0], True)).all())
+
+
+# kernels by (B, Nq, H, Hk, D, Nk, Np): few rows, whole and in parts; many rows; keys that stay; a prefix in one and apart
+FORMS = [(1, 1, 2, 1, 64, 300, 0), (1, 2, 1, 1, 64, 4700, 0), (1, 1, 2, 1, 128, 75, 9702), (1, 105, 4, 4, 64, 92, 9906), (1, 582, 3, 3, 64, 105, 15424),
+         (1, 2735, 3, 1, 64, 104, 0), (5, 1637, 2, 1, 64, 161, 464), (1, 5482, 3, 3, 32, 150, 0), (2, 794, 1, 1, 128, 86, 15413), (1, 3000, 8, 8, 64, 1000, 0),
+         (2, 16000, 4, 4, 64, 700, 0), (40, 68, 16, 8, 32, 197, 233), (40, 238, 8, 8, 64, 147, 0), (40, 137, 8, 8, 128, 73, 0), (16, 1, 4, 4, 32, 995, 7255),
+         (16, 34, 1, 1, 128, 10, 22724)]
+
+
+def form_inputs(B, Nq, H, Hk, D, Nk, Np, cuda, seed):
+    (q, k, v), g = inputs(B, Nq, H, Hk, D, Nk, cuda, seed)
+    prefix = tuple(heads((Np, Hk, D), "rows", g, cuda) for _ in range(2)) if Np else None
+    some = sorted({n for n in [0, 16, 63, 130, Nq - 1] + torch.randint(0, Nq, (8,), generator=g).tolist() if n < Nq})
+    return q, k, v, prefix, some, g
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,Nq,H,Hk,D,Nk,Np", FORMS)
+@pytest.mark.parametrize("power", [70, 120])
+def test_large_finite_values(pkg, cuda, B, Nq, H, Hk, D, Nk, Np, power):
+    """The weighted mean of values is no larger than the largest, whatever the weights sum up to: 2^120 and the largest that bf16 holds."""
+    q, k, v, prefix, some, _ = form_inputs(B, Nq, H, Hk, D, Nk, Np, cuda, 40 + Nq)
+    for t in [v] + ([prefix[1]] if Np else []):
+        t.mul_(2.0 ** power)
+    got = pkg.ops.cross_attention(q, k, v, prefix=prefix)
+    assert bool(torch.isfinite(got).all())
+    want = oracle(q[:, some], k, v, prefix=prefix)
+    for b in range(B):
+        kk, vv = (torch.cat([prefix[i], t[b]]) if Np else t[b] for i, t in enumerate((k, v)))
+        off = (got[b, some].double() - want[b]).norm(dim=-1)
+        assert bool((off <= row_bound(q[b, some], kk, vv, want[b], torch.ones(len(kk), dtype=torch.bool, device=cuda))).all())
+    # one value at every key, the largest of either sign: it comes back
+    most = torch.finfo(torch.bfloat16).max
+    for t in [v] + ([prefix[1]] if Np else []):
+        t.fill_(most)
+        t[..., 1::2] = -most
+    got = pkg.ops.cross_attention(q, k, v, prefix=prefix)
+    assert bool((got[..., 0::2] == most).all()) and bool((got[..., 1::2] == -most).all())
