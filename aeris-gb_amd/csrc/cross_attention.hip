@@ -83,6 +83,13 @@ __device__ __forceinline__ int v_swizzle(int row) { return HD == 128 ? 2 * (row 
 // The first `n` of 64 keys, n >= 0
 __device__ __forceinline__ uint64_t first_keys(int n) { return n >= 64 ? ~0ull : (1ull << n) - 1; }
 
+// Two bf16, zeros in the place of infinities and NaN
+__device__ __forceinline__ uint32_t finite_bf16x2(uint32_t x) {
+  if ((x & 0x7f80u) == 0x7f80u) x &= 0xffff0000u;
+  if ((x & 0x7f800000u) == 0x7f800000u) x &= 0xffffu;
+  return x;
+}
+
 // A wave's 16 QN rows: queries, sums, and what a chunk in LDS does to them.
 // SUM: the row sums by the matrix cores too (a product with ones), four VALU operations fewer per 8 weights and one MFMA more per 4 to 8.
 template <int HD, int QN, bool SCALED, bool SUM>
@@ -389,6 +396,17 @@ struct Rows {
           o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(tr_frag_value(vt[d]), __builtin_bit_cast(bf16x8, u32x4{p[n][0], p[n][1], p[n][2], p[n][3]}), o[n][d], 0, 0, 0);
     };
     add(pk);
+    if (EXACT && !FAST) {
+      // An infinite value times what is left of its weight, 0 or of either sign, would undo the infinity that the first product gives.  (Where no maximum is
+      // taken the rows are done again: their sums are not finite.)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        vt[d].lo.x = finite_bf16x2(vt[d].lo.x);
+        vt[d].lo.y = finite_bf16x2(vt[d].lo.y);
+        vt[d].hi.x = finite_bf16x2(vt[d].hi.x);
+        vt[d].hi.y = finite_bf16x2(vt[d].hi.y);
+      }
+    }
     if (EXACT) add(rest);
     __builtin_amdgcn_sched_barrier(0);
   }

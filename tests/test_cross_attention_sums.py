@@ -94,6 +94,14 @@ def form_inputs(B, Nq, H, Hk, D, Nk, Np, cuda, seed):
     return q, k, v, prefix, some, g
 
 
+def whole_bound(q, k, v, prefix, want):
+    """`row_bound` for every member, all keys taking part."""
+    def of(b):
+        kk, vv = (t[b] if prefix is None else torch.cat([p, t[b]]) for p, t in zip(prefix or (None, None), (k, v)))
+        return row_bound(q[b], kk, vv, want[b], torch.ones(len(kk), dtype=torch.bool, device=q.device))
+    return torch.stack([of(b) for b in range(len(q))])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("B,Nq,H,Hk,D,Nk,Np", FORMS)
 @pytest.mark.parametrize("power", [70, 120])
@@ -105,10 +113,7 @@ def test_large_finite_values(pkg, cuda, B, Nq, H, Hk, D, Nk, Np, power):
     got = pkg.ops.cross_attention(q, k, v, prefix=prefix)
     assert bool(torch.isfinite(got).all())
     want = oracle(q[:, some], k, v, prefix=prefix)
-    for b in range(B):
-        kk, vv = (torch.cat([prefix[i], t[b]]) if Np else t[b] for i, t in enumerate((k, v)))
-        off = (got[b, some].double() - want[b]).norm(dim=-1)
-        assert bool((off <= row_bound(q[b, some], kk, vv, want[b], torch.ones(len(kk), dtype=torch.bool, device=cuda))).all())
+    assert bool(((got[:, some].double() - want).norm(dim=-1) <= whole_bound(q[:, some], k, v, prefix, want)).all())
     # one value at every key, the largest of either sign: it comes back
     most = torch.finfo(torch.bfloat16).max
     for t in [v] + ([prefix[1]] if Np else []):
@@ -116,3 +121,32 @@ def test_large_finite_values(pkg, cuda, B, Nq, H, Hk, D, Nk, Np, power):
         t[..., 1::2] = -most
     got = pkg.ops.cross_attention(q, k, v, prefix=prefix)
     assert bool((got[..., 0::2] == most).all()) and bool((got[..., 1::2] == -most).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,Nq,H,Hk,D,Nk,Np", FORMS)
+def test_infinite_values_that_take_part(pkg, cuda, B, Nq, H, Hk, D, Nk, Np):
+    """An infinity in a value is that element of every row of its heads in the result, for few rows and for many; infinities of both signs
+    leave no number; the other elements are as without them.  (Logits: standard normal, no weight is below 2^-40 of the largest.)"""
+    q, k, v, prefix, some, g = form_inputs(B, Nq, H, Hk, D, Nk, Np, cuda, 60 + Nq)
+    key, b, hk, group = Nk // 2, B - 1, Hk - 1, H // Hk
+    rows = slice(hk * group, (hk + 1) * group)
+    want = oracle(q[:, some], k, v, prefix=prefix)
+    bound = whole_bound(q[:, some], k, v, prefix, want)
+    v[b, key, hk, 3] = math.inf
+    v[b, key, hk, 9] = -math.inf
+    v[b, key, hk, 12], v[b, (key + 20) % Nk, hk, 12] = math.inf, -math.inf
+    if Np:
+        prefix[1][Np - 2, hk, 20] = -math.inf
+    got = pkg.ops.cross_attention(q, k, v, prefix=prefix)
+    assert bool((got[b, :, rows, 3] == math.inf).all()) and bool((got[b, :, rows, 9] == -math.inf).all())
+    both = got[b, :, rows, 12]  # (of ten keys the one twenty further on is the same, and holds the second alone)
+    assert bool((both.isnan() if 20 % Nk else both == -math.inf).all())
+    special = torch.zeros(got.shape, dtype=torch.bool, device=cuda)
+    special[b, :, rows, 3] = special[b, :, rows, 9] = special[b, :, rows, 12] = True
+    if Np:
+        assert bool((got[:, :, rows, 20] == -math.inf).all())
+        special[:, :, rows, 20] = True
+    assert torch.equal(special, ~torch.isfinite(got))
+    got, want = (torch.where(special[:, some], 0.0, t.double()) for t in (got[:, some], want))
+    assert bool(((got - want).norm(dim=-1) <= bound).all())
