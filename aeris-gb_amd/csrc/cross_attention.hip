@@ -30,8 +30,7 @@ namespace aeris {
 
 namespace {
 
-constexpr int KC = 64;           // keys per chunk
-constexpr int MAX_WORDS = 1024;  // chunks of a workgroup that a key mask can cover (a word of 64 bits each, in LDS)
+constexpr int KC = 64;  // keys per chunk
 
 // What a launch does: rows of units against keys
 struct Task {
@@ -569,14 +568,24 @@ struct Loader {
   }
 };
 
-// The key mask of a workgroup's chunks c0 .. c1 as words of 64 bits in LDS (of the prefix: all ones; of chunks of 32 keys the low half counts)
-template <int NWAVE, int U>
-__device__ __forceinline__ void mask_words(const uint8_t* mask, const Keys<U>& keys, int c0, int c1, uint64_t* words, int lane, int wave) {
-  for (int c = c0 + wave; c < c1; c += NWAVE) {
-    const int key = (c - keys.prefix_chunks) * U + lane;
-    const bool on = key < 0 || (key < keys.own && mask[key < keys.own ? key : 0] != 0);
-    const uint64_t word = c < keys.prefix_chunks ? ~0ull : __builtin_amdgcn_ballot_w64(on);
-    if (lane == 0) words[c - c0] = word;
+// A member's key mask, as far as it has keys
+struct Mask {
+  __amdgpu_buffer_rsrc_t rsrc;
+  __device__ __forceinline__ Mask(const CrossParams& p, int member, int own)
+      : rsrc(__builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.mask) + member * p.mask_batch, 0, own, 0x00020000)) {}
+  // The byte for the lane's key of chunk c: 0 outside the member's keys (outside the descriptor, those of the prefix too, whose numbers are negative).  A
+  // wave reads it a chunk ahead, behind that chunk's loads, and waits for both together: masks of any length cost no LDS and no pass of their own.
+  template <int U>
+  __device__ __forceinline__ uint32_t byte(const Keys<U>& keys, int c, int lane) const {
+    return __builtin_amdgcn_raw_buffer_load_b8(rsrc, (uint32_t)((c - keys.prefix_chunks) * U + lane), 0, 0);
+  }
+};
+// The mask of all of a unit's chunks of 64 as words in LDS (of the prefix: all ones), where the keys stay there and are looked at again
+template <int NWAVE>
+__device__ __forceinline__ void mask_words(const Mask& mask, const Keys<KC>& keys, uint64_t* words, int lane, int wave) {
+  for (int c = wave; c < keys.chunks; c += NWAVE) {
+    const uint64_t word = c < keys.prefix_chunks ? ~0ull : __builtin_amdgcn_ballot_w64(mask.byte(keys, c, lane) != 0);
+    if (lane == 0) words[c] = word;
   }
 }
 __device__ __forceinline__ uint64_t uniform64(uint64_t x) {
@@ -619,7 +628,6 @@ cross_attention_rows_kernel(CrossParams p) {
   constexpr int BYTES = Load::BYTES, V_BASE = 2 * BYTES;
   constexpr int QW = 16 * QN, QB = QW * NWAVE;  // rows per wave and workgroup
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  uint64_t* const words = reinterpret_cast<uint64_t*>(smem + 4 * BYTES);
   const uint32_t smem_addr = lds_byte_address(smem);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
@@ -637,15 +645,15 @@ cross_attention_rows_kernel(CrossParams p) {
   Load load(lane, wave);
 
   const bool masked = p.mask && t.Nk > 0;
-  if (masked) {
-    mask_words<NWAVE, KC>(p.mask + member * p.mask_batch, keys, c0, c1, words, lane, wave);
-    __syncthreads();
-  }
-  uint64_t kk[2];  // which keys of the chunks in the buffers take part
+  const Mask mask(p, member, keys.own);
+  uint32_t byte = 0;  // of the mask, for the chunk that is loaded next
+  uint64_t kk[2];     // which keys of the chunks in the buffers take part
   auto issue = [&](int j, int buf) {
+    const int c = c0 + j;
     kk[buf] = first_keys(keys.left);
-    if (masked) kk[buf] &= uniform64(words[j]);
-    load.issue_next(p, t, hk, lane, keys, c0 + j, kk[buf], smem_addr + buf * BYTES, smem_addr + V_BASE + buf * BYTES);
+    if (masked && c >= keys.prefix_chunks) kk[buf] &= __builtin_amdgcn_ballot_w64(byte != 0);
+    load.issue_next(p, t, hk, lane, keys, c, kk[buf], smem_addr + buf * BYTES, smem_addr + V_BASE + buf * BYTES);
+    if (masked) byte = mask.byte(keys, c + 1, lane);
   };
   bool any = false;  // whether any key took part (uniform)
   int idle = 0;      // keys that did not, of chunks with keys that did
@@ -655,6 +663,7 @@ cross_attention_rows_kernel(CrossParams p) {
     const float headroom = FAST ? 0.f : headroom_of(t);
     keys.seek(p, t, hk, c0);
     load.rows(lane, keys);
+    if (masked) byte = mask.byte(keys, c0, lane);
     if (nch > 0) issue(0, 0);
     if (FAST) rows.load_q(p, t, member, hk, row0, lane, rows.qf);
     rows.reset();
@@ -721,7 +730,6 @@ cross_attention_keys_kernel(CrossParams p) {
   constexpr int BYTES = Load::BYTES, RING = RB * 2 * BYTES;  // of K or V of a step; of a wave's buffers
   constexpr int LPS = 2 * Load::LOADS;                       // load instructions per step
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  uint64_t* const words = reinterpret_cast<uint64_t*>(smem + NWAVE * RING);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   unsigned char* const ring = smem + wave * RING;
   const uint32_t ring_addr = lds_byte_address(ring);
@@ -736,10 +744,8 @@ cross_attention_keys_kernel(CrossParams p) {
   Rows<HD, QN, true, false> rows(ring, BYTES, lane, p.q_mul);
   Load load(lane, 0);
   const bool masked = p.mask && t.Nk > 0;
-  if (masked) {
-    mask_words<NWAVE, U>(p.mask + member * p.mask_batch, keys, c0, c1, words, lane, wave);
-    __syncthreads();
-  }
+  const Mask mask(p, member, keys.own);
+  uint32_t byte = 0;  // of the mask, for the step that is loaded next
   const int steps = (c1 - c0 - wave + NWAVE - 1) / NWAVE;  // of this wave: c0 + wave, c0 + wave + NWAVE, ..
   uint32_t kk[RB];
   int part_of = -1;  // whose rows' strides the loader has: 0 the prefix's, 1 the member's own
@@ -751,15 +757,17 @@ cross_attention_keys_kernel(CrossParams p) {
       load.rows(lane, keys);
     }
     uint64_t w = first_keys(keys.left < U ? keys.left : U);
-    if (masked) w &= uniform64(words[c - c0]);
+    if (masked && c >= keys.prefix_chunks) w &= __builtin_amdgcn_ballot_w64(byte != 0);
     kk[buf] = (uint32_t)w;
     load.issue(keys, w & 0xffffffffull, ring_addr + buf * 2 * BYTES, ring_addr + buf * 2 * BYTES + BYTES);
+    if (masked) byte = mask.byte(keys, c + NWAVE, lane);
   };
   bool any = false;
   int idle = 0;
   auto sweep = [&](auto fast_tag) {
     constexpr bool FAST = decltype(fast_tag)::value;
     const float headroom = FAST ? 0.f : headroom_of(t);
+    if (masked) byte = mask.byte(keys, c0 + wave, lane);
 #pragma unroll
     for (int u = 0; u < RB - 1; ++u)
       if (u < steps) issue(u, u);
@@ -855,7 +863,7 @@ cross_attention_resident_kernel(CrossParams p, int max_chunks) {
   Keys<KC> keys(p, t, member, hk);
   const int nch = keys.chunks;
   if (p.mask && t.Nk > 0) {
-    mask_words<NWAVE, KC>(p.mask + member * p.mask_batch, keys, 0, nch, words, lane, wave);
+    mask_words<NWAVE>(Mask(p, member, keys.own), keys, words, lane, wave);
     __syncthreads();
   }
   Rows<HD, QN, SCALED, SUM> rows(smem, v_base, lane, p.q_mul);
@@ -1059,7 +1067,7 @@ struct Plan {
   int n, qn;    // tasks; blocks of 16 rows per wave
   bool parts;   // sums go through the workspace
   int resident; // chunks that a workgroup keeps in LDS
-  int64_t grid, words, bytes;  // workgroups; mask words of a workgroup; of the workspace
+  int64_t grid, bytes;  // workgroups; of the workspace
 };
 
 int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
@@ -1109,7 +1117,7 @@ Way way_of(const Task& t, int Hk, int head_dim, Form form, int qn, int splits, b
 
 Plan plan_of(const CrossArgs& a) {
   const int B = (int)a.B, Hk = (int)a.kv_heads, rows_m = (int)(a.Nq * (a.heads / a.kv_heads)), D = (int)a.head_dim;
-  const bool own = a.Nk > 0, masked = a.key_mask && own;
+  const bool own = a.Nk > 0;
   // every member sees the same keys: its rows are further rows of one unit
   const bool shared = !own || (a.k_batch_stride == 0 && a.v_batch_stride == 0 && (!a.lengths || a.lengths_stride == 0) &&
                                (!a.key_mask || a.mask_batch_stride == 0));
@@ -1130,7 +1138,7 @@ Plan plan_of(const CrossArgs& a) {
   auto setup = [&](Form form, int qn) {
     plan.form = form;
     plan.qn = qn;
-    plan.grid = plan.words = plan.bytes = 0;
+    plan.grid = plan.bytes = 0;
     for (int i = 0; i < plan.n; ++i) {
       Task& t = plan.task[i];
       t.qblks = div_up(t.rows, rows_of(form, qn));
@@ -1145,8 +1153,6 @@ Plan plan_of(const CrossArgs& a) {
       t.by_rows = by_rows < by_units;
       t.first = (int)plan.grid;
       plan.grid += 8 * (t.by_rows ? by_rows : by_units);
-      const int64_t words = div_up(chunks_of(t, keys_of(form)), t.splits);
-      if (masked && t.Nk > 0 && words > plan.words) plan.words = words;
       if (plan.parts) plan.bytes += ((int64_t)t.units * t.rows * (D + 2) * 4 + 255) / 256 * 256;
     }
     if (plan.n < 2) plan.task[1].first = 0x7fffffff;
@@ -1168,8 +1174,7 @@ Plan plan_of(const CrossArgs& a) {
     }
   }
   // Otherwise the way that costs least (eight heads of 64, 1000 keys, in us: 8000 queries, 32 rows a wave 24.2, 64 27.3; 16 000 48.6 and 38.9, whose
-  // workgroups fill the chip once; 24 000 61.9 and 63; 64 800 162 and 149).  Parts of the keys: what fills the chip once, twice, ..; no more chunks
-  // in one than a mask's words cover
+  // workgroups fill the chip once; 24 000 61.9 and 63; 64 800 162 and 149).  Parts of the keys: what fills the chip once, twice, ..
   auto choose = [&](Plan& plan) {
     Way best{Form::rows, 1, 1, 1e30f};
     int splits[2] = {1, 1};
@@ -1180,23 +1185,19 @@ Plan plan_of(const CrossArgs& a) {
       if (form == Form::rows && (parts ? qn != 2 : costs_of(D).rows[qn / 2].per_cu == 0)) continue;  // (in parts 32 rows a wave)
       float us = parts ? 6.0f : 0.f;
       int s[2] = {1, 1};
-      bool whole = true;
       for (int i = 0; i < plan.n; ++i) {
         const Task& t = plan.task[i];
         const int64_t one = (int64_t)t.members * Hk * div_up(t.rows, rows_of(form, qn)), chunks = chunks_of(t, keys_of(form));
-        const int least = masked && t.Nk > 0 ? div_up(chunks, MAX_WORDS) : 1;
-        Way w = way_of(t, Hk, D, form, qn, least > 1 ? least : 1, parts);
+        Way w = way_of(t, Hk, D, form, qn, 1, parts);
         for (int slots = 256; slots <= 1024 && !(form == Form::rows && qn != 2); slots += 256) {
           const int64_t n = slots / one < div_up(chunks, NWAVE) ? slots / one : div_up(chunks, NWAVE);
-          if (n <= 1 || n < least) continue;
+          if (n <= 1) continue;
           const Way x = way_of(t, Hk, D, form, qn, (int)n, parts);
           if (x.us < w.us) w = x;
         }
         s[i] = w.splits;
         us += w.us;
-        whole = whole && w.splits == 1;
       }
-      if (form == Form::rows && qn != 2 && !whole) continue;
       if (us < best.us) {
         best = {form, qn, 1, us};
         splits[0] = s[0];
@@ -1227,7 +1228,7 @@ Plan plan_of(const CrossArgs& a) {
   return plan;
 }
 
-// the kernel for (sums through the workspace, scaled here, blocks of 16 rows per wave), handed to `f` with its LDS bytes (a mask's words aside)
+// the kernel for (sums through the workspace, scaled here, blocks of 16 rows per wave), handed to `f` with its LDS bytes
 template <int HD, class F>
 hipError_t with_rows_kernel(bool parts, bool scaled, int qn, const F& f) {
   constexpr int LDS = 8 * KC * HD;
@@ -1293,9 +1294,8 @@ hipError_t launch_dim(const CrossArgs& a, Plan& plan, void* workspace, hipStream
       return hipGetLastError();
     });
   const hipError_t e = plan.form == Form::rows ? with_rows_kernel<HD>(plan.parts, !a.q_prescaled, plan.qn, [&](auto kernel, int lds) {
-    return launch(kernel, lds + plan.words * 8);
+    return launch(kernel, lds);
   }) : with_keys_kernel<HD>(plan.parts, plan.qn, [&](auto kernel, int64_t lds, int64_t sums) {
-    lds += plan.words * 8;
     return launch(kernel, lds > sums ? lds : sums);
   });
   if (e != hipSuccess || !plan.parts) return e;
@@ -1320,9 +1320,9 @@ hipError_t configure_dim() {
   for (int i = 0; i < 6 && e == hipSuccess; ++i) {
     const int qn = i / 2 == 2 ? 4 : 1 + i / 2;
     for (int parts = 0; parts < 2 && e == hipSuccess; ++parts)
-      e = with_rows_kernel<HD>(parts, i & 1, qn, [&](auto kernel, int lds) { return allow(kernel, lds + MAX_WORDS * 8); });
+      e = with_rows_kernel<HD>(parts, i & 1, qn, [&](auto kernel, int lds) { return allow(kernel, lds); });
     if (e == hipSuccess)
-      e = with_keys_kernel<HD>(i & 1, qn, [&](auto kernel, int64_t lds, int64_t sums) { return allow(kernel, lds + MAX_WORDS * 8 > sums ? lds + MAX_WORDS * 8 : sums); });
+      e = with_keys_kernel<HD>(i & 1, qn, [&](auto kernel, int64_t lds, int64_t sums) { return allow(kernel, lds > sums ? lds : sums); });
   }
   for (int i = 0; i < 2 && e == hipSuccess; ++i)
     e = with_resident_kernel<HD>(i, [&](auto kernel) { return allow(kernel, RESIDENT_LDS); });

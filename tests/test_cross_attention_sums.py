@@ -150,3 +150,46 @@ def test_infinite_values_that_take_part(pkg, cuda, B, Nq, H, Hk, D, Nk, Np):
     assert torch.equal(special, ~torch.isfinite(got))
     got, want = (torch.where(special[:, some], 0.0, t.double()) for t in (got[:, some], want))
     assert bool(((got - want).norm(dim=-1) <= bound).all())
+
+
+def sizes(pkg, B, Nq, H, Hk, D, Nk, Np=0, masked=False, lengths=False, prescaled=False):
+    """What the C call is told of a call's sizes, with addresses that are never read."""
+    at, row, krow = 1 << 20, H * D, Hk * D
+    return pkg.ops.CROSS_ATTENTION.pack(at, at, at, at if Np else 0, at if Np else 0, at, at if lengths else 0, at if masked else 0, B, Nq, H, D, B, Nk, Hk, Np,
+                                        B if lengths else 0, B if masked else 0, Nq * row, row, D, 1, Nk * krow, krow, D, 1, Nk * krow, krow, D, 1,
+                                        krow, D, 1, krow, D, 1, Nk if masked else 0, prescaled, D ** -0.5)
+
+
+@pytest.mark.parametrize("B,Nq,H,Hk,D,Nk,Np", [(1, 1036800, 16, 16, 64, 129600, 0), (1, 1036800, 16, 16, 64, 1036800, 0), (4, 64800, 8, 8, 128, 500, 259200),
+                                               (1, 1036800, 24, 24, 64, 1100000, 0), (2, 3, 4, 4, 64, 900000, 0), (1, 300, 8, 2, 32, 70000, 70000)])
+def test_a_mask_needs_no_workspace_of_its_own(pkg, B, Nq, H, Hk, D, Nk, Np):
+    need = pkg._lib.lib().aeris_cross_attention_workspace_bytes
+    plain, masked = (need(sizes(pkg, B, Nq, H, Hk, D, Nk, Np, masked=m)) for m in (False, True))
+    assert masked == plain
+    if Nq > 1000:
+        assert plain == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,Nq,H,Hk,D,Nk,Np", [(1, 200000, 1, 1, 32, 66000, 0), (1, 200000, 1, 1, 64, 66000, 0), (1, 200000, 1, 1, 128, 66000, 0), (2, 3, 4, 4, 64, 300000, 0),
+                                               (2, 64800, 2, 1, 64, 300, 70001), (3, 40, 2, 2, 128, 70001, 129), (8, 1, 1, 1, 32, 65, 70000)])
+def test_masks_of_any_length(pkg, cuda, B, Nq, H, Hk, D, Nk, Np):
+    """More than 65 536 keys under a mask, with rows that fill the chip and with few; masks in rows that start anywhere; whole chunks, and
+    all of a member's keys, masked; a prefix, which no mask covers, ahead of them."""
+    q, k, v, prefix, some, g = form_inputs(B, Nq, H, Hk, D, Nk, Np, cuda, 80 + Nq)
+    mask = torch.rand(B, Nk, generator=g) < 0.5
+    mask[0, Nk // 3:Nk // 3 + min(Nk // 2, 5000)] = False
+    if B > 1:
+        mask[-1] = False
+    buf = torch.ones(B * (Nk + 13) + 7, dtype=torch.bool)
+    buf[7:].view(B, Nk + 13)[:, :Nk] = mask
+    k[~mask.to(cuda)], v[~mask.to(cuda)] = math.nan, math.inf
+    mask = buf.to(cuda)[7:].view(B, Nk + 13)[:, :Nk]
+    some = some[:6]
+    got = pkg.ops.cross_attention(q, k, v, key_mask=mask, prefix=prefix)[:, some]
+    want = oracle(q[:, some], k, v, mask=mask, prefix=prefix)
+    keep = torch.cat([torch.ones(B, Np, dtype=torch.bool, device=cuda), mask], 1)
+    for b in range(B):
+        kk, vv = (t[b] if prefix is None else torch.cat([p, t[b]]) for p, t in zip(prefix or (None, None), (k, v)))
+        off = (got[b].double() - want[b]).norm(dim=-1)
+        assert bool((off <= row_bound(q[b, some], kk, vv, want[b], keep[b])).all()), b
