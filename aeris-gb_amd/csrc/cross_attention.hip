@@ -720,15 +720,14 @@ cross_attention_rows_kernel(CrossParams p) {
   }
 }
 
-// Few rows: the waves of a workgroup divide the keys among them, 32 at a time in turn, for the same 16 QN rows; each has its own buffers, RB of them, and
+// Few rows: the waves of a workgroup divide the keys among them, 32 at a time in turn, for the same 16 QN rows; each has its own two buffers and
 // keeps its own pace.  Their sums meet in LDS.  PARTS: the keys are divided among workgroups too, which leave theirs in the workspace.
-template <int HD, int NWAVE, int QN, int RB, bool PARTS>
+template <int HD, int NWAVE, int QN, bool PARTS>
 __global__ void __launch_bounds__(64 * NWAVE) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 1 : 2)))
 cross_attention_keys_kernel(CrossParams p) {
   constexpr int U = 32, QB = 16 * QN;
   using Load = Loader<HD, 1, U>;
-  constexpr int BYTES = Load::BYTES, RING = RB * 2 * BYTES;  // of K or V of a step; of a wave's buffers
-  constexpr int LPS = 2 * Load::LOADS;                       // load instructions per step
+  constexpr int BYTES = Load::BYTES, RING = 4 * BYTES;  // of K or V of a step; of a wave's buffers
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   unsigned char* const ring = smem + wave * RING;
@@ -747,7 +746,7 @@ cross_attention_keys_kernel(CrossParams p) {
   const Mask mask(p, member, keys.own);
   uint32_t byte = 0;  // of the mask, for the step that is loaded next
   const int steps = (c1 - c0 - wave + NWAVE - 1) / NWAVE;  // of this wave: c0 + wave, c0 + wave + NWAVE, ..
-  uint32_t kk[RB];
+  uint32_t kk[2];
   int part_of = -1;  // whose rows' strides the loader has: 0 the prefix's, 1 the member's own
   auto issue = [&](int j, int buf) {
     const int c = c0 + wave + j * NWAVE;
@@ -768,21 +767,18 @@ cross_attention_keys_kernel(CrossParams p) {
     constexpr bool FAST = decltype(fast_tag)::value;
     const float headroom = FAST ? 0.f : headroom_of(t);
     if (masked) byte = mask.byte(keys, c0 + wave, lane);
-#pragma unroll
-    for (int u = 0; u < RB - 1; ++u)
-      if (u < steps) issue(u, u);
+    if (steps > 0) issue(0, 0);
     if (FAST) rows.load_q(p, t, member, hk, row0, lane, rows.qf);
     rows.reset();
     if (FAST) __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0), see the kernel above
-    for (int j0 = 0; j0 < steps; j0 += RB) {
+    for (int j0 = 0; j0 < steps; j0 += 2) {
 #pragma unroll
-      for (int u = 0; u < RB; ++u) {
+      for (int u = 0; u < 2; ++u) {
         const int j = j0 + u;
         if (j >= steps) break;
-        // step j's buffers are filled (younger loads: those of the steps behind it); then the buffers that step j - 1 was done with are loaded again
-        if (RB > 2 && j + RB - 2 < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((RB - 2) * LPS) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (j + RB - 1 < steps) issue(j + RB - 1, (u + RB - 1) % RB);
+        // step j's buffer is filled; then the one that step j - 1 was done with is loaded again
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (j + 1 < steps) issue(j + 1, u ^ 1);
         if (kk[u] != 0) {
           any = true;
           if (FAST) idle += U - __builtin_popcount(kk[u]);
@@ -1160,7 +1156,7 @@ Plan plan_of(const CrossArgs& a) {
 
   // Few keys and many rows: a workgroup's keys stay (at least two row blocks for each of its waves).  As many workgroups as run at once: two per CU, four
   // of the small ones of head size 32 (64 800 queries, sixteen heads, 77 keys: 33.5 us with 1024, 36.5 with 512; of 64: 54 and 51)
-  if (!plan.parts) {
+  {
     Task& t = plan.task[0];
     const int64_t c = chunks_of(t, KC), lds = c * (4 * KC * D + 8), units = (int64_t)t.members * Hk;
     const int64_t per = (D == 32 && lds <= RESIDENT_LDS / 2 ? 1024 : 512) / units, blocks = div_up(t.rows, 16 * resident_qn(D) * NWAVE);
@@ -1242,7 +1238,7 @@ hipError_t with_rows_kernel(bool parts, bool scaled, int qn, const F& f) {
 // the same for (sums through the workspace, blocks of 16 rows); with the bytes that the waves' sums take in the end
 template <int HD, int QN, bool PARTS, class F>
 hipError_t with_keys_kernel_of(const F& f) {
-  return f(cross_attention_keys_kernel<HD, NWAVE, QN, 2, PARTS>, NWAVE * 2 * 4 * 32 * HD, NWAVE * 16 * QN * (HD + 2) * 4);
+  return f(cross_attention_keys_kernel<HD, NWAVE, QN, PARTS>, NWAVE * 2 * 4 * 32 * HD, NWAVE * 16 * QN * (HD + 2) * 4);
 }
 template <int HD, class F>
 hipError_t with_keys_kernel(bool parts, int qn, const F& f) {
