@@ -574,7 +574,7 @@ struct Mask {
   __device__ __forceinline__ Mask(const CrossParams& p, int member, int own)
       : rsrc(__builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.mask) + member * p.mask_batch, 0, own, 0x00020000)) {}
   // The byte for the lane's key of chunk c: 0 outside the member's keys (outside the descriptor, those of the prefix too, whose numbers are negative).  A
-  // wave reads it a chunk ahead, behind that chunk's loads, and waits for both together: masks of any length cost no LDS and no pass of their own.
+  // wave reads it a chunk ahead, beside that chunk's loads, and waits for both together: masks of any length cost no LDS and no pass of their own.
   template <int U>
   __device__ __forceinline__ uint32_t byte(const Keys<U>& keys, int c, int lane) const {
     return __builtin_amdgcn_raw_buffer_load_b8(rsrc, (uint32_t)((c - keys.prefix_chunks) * U + lane), 0, 0);
@@ -651,9 +651,11 @@ cross_attention_rows_kernel(CrossParams p) {
   auto issue = [&](int j, int buf) {
     const int c = c0 + j;
     kk[buf] = first_keys(keys.left);
-    if (masked && c >= keys.prefix_chunks) kk[buf] &= __builtin_amdgcn_ballot_w64(byte != 0);
+    if (masked) {
+      if (c >= keys.prefix_chunks) kk[buf] &= __builtin_amdgcn_ballot_w64(byte != 0);
+      byte = mask.byte(keys, c + 1, lane);
+    }
     load.issue_next(p, t, hk, lane, keys, c, kk[buf], smem_addr + buf * BYTES, smem_addr + V_BASE + buf * BYTES);
-    if (masked) byte = mask.byte(keys, c + 1, lane);
   };
   bool any = false;  // whether any key took part (uniform)
   int idle = 0;      // keys that did not, of chunks with keys that did
@@ -756,10 +758,12 @@ cross_attention_keys_kernel(CrossParams p) {
       load.rows(lane, keys);
     }
     uint64_t w = first_keys(keys.left < U ? keys.left : U);
-    if (masked && c >= keys.prefix_chunks) w &= __builtin_amdgcn_ballot_w64(byte != 0);
+    if (masked) {
+      if (c >= keys.prefix_chunks) w &= __builtin_amdgcn_ballot_w64(byte != 0);
+      byte = mask.byte(keys, c + NWAVE, lane);
+    }
     kk[buf] = (uint32_t)w;
     load.issue(keys, w & 0xffffffffull, ring_addr + buf * 2 * BYTES, ring_addr + buf * 2 * BYTES + BYTES);
-    if (masked) byte = mask.byte(keys, c + NWAVE, lane);
   };
   bool any = false;
   int idle = 0;
