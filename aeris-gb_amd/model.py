@@ -871,9 +871,9 @@ class LocalAERIS(nn.Module):
         """Make what the blocks' rotations read, ahead of a capture."""
         half = (self.window_size[0] // 2, self.window_size[1] // 2)
         for i, layer in enumerate(self.layers):
-            for block in getattr(layer, "modulelist", ()):
-                if isinstance(block[1], Attention):
-                    block[1].prepare(device, half if i % 2 == 1 else (0, 0))
+            for module in layer.modules():  # (wherever a layer of the caller's holds them)
+                if isinstance(module, Attention):
+                    module.prepare(device, half if i % 2 == 1 else (0, 0))
 
     def encode_context(self, states, lengths=None, key_mask=None, prefix=None):
         """What ``forward(context=...)`` takes, for all its calls with the same states (arguments: ``CrossAttention.encode``)."""

@@ -226,3 +226,16 @@ def test_options_and_state_dict(pkg):
     for Y in range(6):
         for X in range(10):
             assert int(got[Y, X]) == (Y - 1) % 6 % 3 * 5 + (X - 2) % 10 % 5
+
+
+def test_prepare_takes_layers_of_any_make(pkg):
+    """The tables are made wherever the attentions stand; blocks that are none of this package's are no error."""
+    kw = dict(heads=2, dim=128, head_dim=64, mlp_dim=256, window_size=(8, 8), image_shape=(16, 16), n_layers=5, model_in_channels=4, model_out_channels=2)
+    m = pkg.LocalAERIS(**kw, rope=True)
+    m.layers[1].modulelist = torch.nn.ModuleList([torch.nn.Linear(128, 128), torch.nn.ModuleList([torch.nn.Identity()])])
+    m.layers[2] = torch.nn.Sequential(m.layers[2].modulelist[0][1])
+    asked = []
+    for layer in (m.layers[0].modulelist[0][1], m.layers[2][0]):
+        layer.prepare = lambda device, shift, name=len(asked): asked.append((name, shift))
+    m.prepare(torch.device("cpu"))
+    assert asked == [(0, (0, 0)), (0, (0, 0))]
