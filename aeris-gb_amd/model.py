@@ -221,6 +221,7 @@ FUSE_QKV_ATTENTION = True
 class Attention(nn.Module):
     """Windowed multi-head self-attention: to_qkv GEMM -> fused window attention -> wo GEMM
     (model.py:265-309).  ``forward(x, shift=(sy, sx))`` folds a cyclic shift into the kernel."""
+    qk_norm = rotates = False  # of a module that was saved whole before it had them
 
     def __init__(self, dim, heads, head_dim, window_size, image_shape, device_mesh=None, wp_dims=(1, 1), *,
                  bias=False, rel_pos_bias=False, shift_mask=False, qk_norm=False, rope=False, **rope_kwargs):

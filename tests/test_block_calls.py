@@ -618,3 +618,15 @@ def test_a_draw_sees_parameters_that_move(pkg, calls, monkeypatch, window, what)
 def test_an_empty_model_draws(pkg, calls, monkeypatch):
     names = draw_of(pkg, calls, monkeypatch, steps=2, layers=0)
     assert names.count("aeris_output_stage_fwd") == 3 and "aeris_blocks_fwd" not in names
+
+
+def test_a_module_saved_whole_by_an_earlier_version_runs_by_single_operations(pkg, calls):
+    """The same module with a tap, which takes its blocks operation by operation, and ahead of a capture."""
+    layer = layer_of(pkg, "spec", mod_ways=0)
+    attn = layer.modulelist[0][1]
+    for name in ("qk_norm", "rotates"):
+        del attn.__dict__[name]
+    seen = []
+    layer(inputs(pkg)[0], tap=lambda name, t, block: seen.append(name))
+    assert seen[:2] == ["attn", "hidden"] and "aeris_qk_norm_rope_fwd" not in calls.names()
+    attn.prepare(torch.device("cpu"), (0, 0))
