@@ -12,7 +12,7 @@ import math
 import pytest
 import torch
 
-from test_cross_attention import heads, inputs, oracle
+from test_cross_attention import PLANS, heads, inputs, oracle
 
 STEP = 0.0017
 
@@ -80,11 +80,8 @@ def test_rows_under_masks(pkg, cuda, D, Nq, Nk, level):
     assert bool((off <= row_bound(q[0, some], k[0], v[0], want[0], mask[0], True)).all())
 
 
-# kernels by (B, Nq, H, Hk, D, Nk, Np): few rows, whole and in parts; many rows; keys that stay; a prefix in one and apart
-FORMS = [(1, 1, 2, 1, 64, 300, 0), (1, 2, 1, 1, 64, 4700, 0), (1, 1, 2, 1, 128, 75, 9702), (1, 105, 4, 4, 64, 92, 9906), (1, 582, 3, 3, 64, 105, 15424),
-         (1, 2735, 3, 1, 64, 104, 0), (5, 1637, 2, 1, 64, 161, 464), (1, 5482, 3, 3, 32, 150, 0), (2, 794, 1, 1, 128, 86, 15413), (1, 3000, 8, 8, 64, 1000, 0),
-         (2, 16000, 4, 4, 64, 700, 0), (40, 68, 16, 8, 32, 197, 233), (40, 238, 8, 8, 64, 147, 0), (40, 137, 8, 8, 128, 73, 0), (16, 1, 4, 4, 32, 995, 7255),
-         (16, 34, 1, 1, 128, 10, 22724)]
+# sizes for every kernel: few rows, whole and in parts; many rows; keys that stay; a prefix in one and apart
+FORMS = PLANS + [(1, 1, 2, 1, 64, 300, 0), (1, 1, 2, 2, 64, 20000, 0), (1, 3000, 8, 8, 64, 1000, 0), (2, 16000, 4, 4, 64, 700, 0)]
 
 
 def form_inputs(B, Nq, H, Hk, D, Nk, Np, cuda, seed):
@@ -193,3 +190,36 @@ def test_masks_of_any_length(pkg, cuda, B, Nq, H, Hk, D, Nk, Np):
         kk, vv = (t[b] if prefix is None else torch.cat([p, t[b]]) for p, t in zip(prefix or (None, None), (k, v)))
         off = (got[b].double() - want[b]).norm(dim=-1)
         assert bool((off <= row_bound(q[b, some], kk, vv, want[b], keep[b])).all()), b
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("B,Nq,H,Hk,Nk,layout", [
+    (1, 1, 1, 1, 2, "rows"), (2, 3, 4, 2, 63, "planes"), (3, 33, 2, 2, 65, "rows"), (1, 128, 3, 3, 127, "planes"), (2, 129, 2, 1, 129, "fused"),
+    (1, 300, 12, 3, 200, "rows"), (2, 5, 8, 2, 1111, "planes"), (1, 130, 1, 1, 5000, "fused"), (1, 1025, 3, 3, 257, "planes"), (1, 2500, 16, 16, 77, "rows"),
+    (2, 16001, 4, 4, 77, "planes"), (1, 4000, 8, 8, 700, "rows")])
+def test_every_row(pkg, cuda, D, B, Nq, H, Hk, Nk, layout):
+    """No row of a call hides behind the others' norm."""
+    (q, k, v), _ = inputs(B, Nq, H, Hk, D, Nk, cuda, 200 * D + Nq, layout)
+    got, want = pkg.ops.cross_attention(q, k, v), oracle(q, k, v)
+    assert bool(((got.double() - want).norm(dim=-1) <= whole_bound(q, k, v, None, want)).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("Nq", [9, 40, 150, 3000])
+def test_every_row_of_a_call_with_a_loud_one(pkg, cuda, D, Nq):
+    """A row, and ten keys, far beyond the range of exp2: that row and all others, each by its own bound.  The fp32 sum of a logit is off by D 2^-24 of the
+    sum of its products' sizes at most, the scale by 2^-23 of the logit: e_i.  Weights w_i exp(d_i) with |d_i| <= e_i give a row that is off by
+    |sum_i w_i (exp(d_i) - 1) (v_i - o)| / sum_i w_i exp(d_i) <= exp(max e) sum_i w_i (exp(e_i) - 1) |v_i - o|."""
+    (q, k, v), _ = inputs(1, Nq, 1, 1, D, 6000, cuda, 2)
+    q[0, Nq // 2] *= 200
+    k[0, 4500:4510] *= 30
+    got, want = pkg.ops.cross_attention(q, k, v), oracle(q, k, v)
+    bound = whole_bound(q, k, v, None, want)[0, :, 0]
+    qq, kk, vv, o = q[0, :, 0].double(), k[0, :, 0].double(), v[0, :, 0].double(), want[0, :, 0]
+    s = qq @ kk.T * D ** -0.5
+    e = qq.abs() @ kk.abs().T * D ** -0.5 * D * 2.0 ** -24 + s.abs() * 2.0 ** -23
+    w = torch.softmax(s, -1)
+    bound = bound + e.amax(-1).exp() * (w * e.expm1() * torch.cdist(o, vv)).sum(-1)
+    assert bool(((got[0, :, 0].double() - o).norm(dim=-1) <= bound).all())
