@@ -571,6 +571,7 @@ struct Loader {
 // A member's key mask, as far as it has keys
 struct Mask {
   __amdgpu_buffer_rsrc_t rsrc;
+  __device__ __forceinline__ Mask() : rsrc(__builtin_amdgcn_make_buffer_rsrc(nullptr, 0, 0, 0x00020000)) {}
   __device__ __forceinline__ Mask(const CrossParams& p, int member, int own)
       : rsrc(__builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.mask) + member * p.mask_batch, 0, own, 0x00020000)) {}
   // The byte for the lane's key of chunk c: 0 outside the member's keys (outside the descriptor, those of the prefix too, whose numbers are negative).  A
@@ -645,7 +646,8 @@ cross_attention_rows_kernel(CrossParams p) {
   Load load(lane, wave);
 
   const bool masked = p.mask && t.Nk > 0;
-  const Mask mask(p, member, keys.own);
+  Mask mask;
+  if (masked) mask = Mask(p, member, keys.own);
   uint32_t byte = 0;  // of the mask, for the chunk that is loaded next
   uint64_t kk[2];     // which keys of the chunks in the buffers take part
   auto issue = [&](int j, int buf) {
@@ -745,7 +747,8 @@ cross_attention_keys_kernel(CrossParams p) {
   Rows<HD, QN, true, false> rows(ring, BYTES, lane, p.q_mul);
   Load load(lane, 0);
   const bool masked = p.mask && t.Nk > 0;
-  const Mask mask(p, member, keys.own);
+  Mask mask;
+  if (masked) mask = Mask(p, member, keys.own);  // (its arguments are not waited for where there is none: 19.6 -> 19.3 us for sixteen members of one query)
   uint32_t byte = 0;  // of the mask, for the step that is loaded next
   const int steps = (c1 - c0 - wave + NWAVE - 1) / NWAVE;  // of this wave: c0 + wave, c0 + wave + NWAVE, ..
   uint32_t kk[2];
