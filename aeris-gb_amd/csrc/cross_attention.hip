@@ -12,15 +12,18 @@
 //   S^T = K Q^T          v_mfma_f32_16x16x32_bf16; lane = one row, registers = keys; the scale, unless the producer of q has applied it (`SCALED`),
 //                        multiplies the fp32 logits: q is not rounded again
 //   O^T += V^T P^T       V^T by the transposing LDS read, P^T straight from the accumulators of S^T, rounded to bf16 (v's type, the matrix cores'; for
-//                        few rows as two bf16, see step()); the row sum adds the rounded values
+//                        16 rows as two bf16, see step()); the row sum adds the rounded values.  As two bf16 the results would be off by 0.0017 in
+//                        the mean square, their own rounding, instead of 0.0023; the second product costs a quarter to a half of the time: 1 036 800
+//                        queries, sixteen heads of 64, 256 keys 1181 -> 1726 us, two members of 64 800, eight heads, 1000 keys 260 -> 369, heads of
+//                        128 252 -> 349, sixteen of 32, 200 keys 52 -> 76, eight members' nine queries behind a prefix of 64 800 54 -> 68
 // Three ways to run that, and parts:
 //   cross_attention_rows_kernel      many rows: a workgroup = a block of a unit's rows, the unit's keys streamed past its waves
 //   cross_attention_keys_kernel      few rows: the waves of a workgroup divide the keys among them for the same rows
 //   cross_attention_resident_kernel  few keys and many rows: a workgroup keeps the unit's keys in LDS and walks down the rows
 //   PARTS of the first two           fewer rows still: the keys divided among workgroups too, each leaves its sums in the workspace in fp32 and
 //                                    cross_attention_join_kernel adds them up, in their order
-// plan_of() chooses, by what each would cost (its comments: what they measured).  1000 queries x 1000 keys, eight heads of 64: rows kernel 13.1 us, keys
-// kernel 9.2; 4000 x 77: 6.1 and 9.4.
+// plan_of() chooses, by what each would cost (its comments: what they measured).  1000 queries x 1000 keys, eight heads of 64: rows kernel 16.2 us, keys
+// kernel 8.4; 4000 x 77: 5.6 and 8.0.
 #include "common.h"
 #include "kernels.h"
 #include <cstring>
@@ -197,8 +200,9 @@ struct Rows {
     load_v(0, 0);
     __builtin_amdgcn_sched_barrier(0);
 
-    // The wave of a SIMD that has its weights goes first: its product is the longer chain, the other's exponentials fill the gaps (1572 -> 1521 us for
-    // 1 036 800 queries, sixteen heads of 64, 256 keys; first for K Q^T as well 1531, for the exponentials alone 1595)
+    // The wave of a SIMD that has its weights goes first: its product is the longer chain, the other's exponentials fill the gaps (1251 -> 1191 us for
+    // 1 036 800 queries, sixteen heads of 64, 256 keys; first for K Q^T as well 1192, for the exponentials alone 1260; two members of 64 800, eight
+    // heads, 1000 keys 273 -> 265, 269 and 270)
     __builtin_amdgcn_s_setprio(0);
     f32x4 acc[QN][KB];
     // ---- S^T: acc[n][kb][i] = logit of key 16 kb + 4 q4 + i, row 16 n + l15; K fragments are read two ahead of their MFMAs
@@ -311,7 +315,8 @@ struct Rows {
 
   // 32 keys, whose 64 or fewer rows of K and V lie `at` bytes behind the first: as chunk(), for waves that divide the keys among them.
   // EXACT, for 16 rows, where latency or reading bounds the time: the weights as two bf16 each, what the first leaves goes into a second product (error
-  // 0.0024 -> 0.0017 of the result, its own rounding; 7.1 -> 7.8 us for 250 queries, eight heads of 64, 1000 keys, nothing for one query and 64 800)
+  // 0.0024 -> 0.0017 of the result, its own rounding; nothing for one query and 64 800 keys; 32 rows would be slower by 10 to 16 per cent: five members'
+  // 37 queries, 14 400 keys 25.9 -> 29.5 us, 1000 queries, eight heads of 64, 1000 keys 8.0 -> 9.3)
   template <bool FAST>
   __device__ __forceinline__ void step(uint32_t at, uint32_t keys, float headroom = 0.f) {
     constexpr bool EXACT = QN == 1;
@@ -908,11 +913,11 @@ cross_attention_resident_kernel(CrossParams p, int max_chunks) {
       for (int s = 0; s < HD / 32; ++s) rows.qf[n][s] = next[n][s];
     if (row0 + step < t.rows) rows.load_q(p, t, member, hk, row0 + step, lane, next);
     int c = 0;
-    if constexpr (HD == 32) {  // (its registers are few, its loop better one than with a first turn apart: 33.5 us, 35 for 64 800 x 77 keys)
+    if constexpr (HD == 32) {  // (its registers are few: the same time in one loop, 37.1 us and 37.5 for 64 800 x 77 keys, 52.6 and 52.2 for 200)
       rows.reset();
       do rows.template chunk<true>(c * BYTES, ~0ull);
       while (++c < nch);
-    } else {  // (80 registers that need not be cleared for each block: 51.5 -> 49.3 us, sixteen heads of 64)
+    } else {  // (80 registers that need not be cleared for each block: 1216 -> 1191 us, sixteen heads of 64, 256 keys)
       rows.template chunk<true, true>(0, ~0ull);
       while (++c < nch) rows.template chunk<true>(c * BYTES, ~0ull);
     }
@@ -1058,7 +1063,7 @@ namespace {
 
 constexpr int NWAVE = 4;
 // Blocks of 16 rows per wave.  More of them read a K / V fragment from LDS for more rows; fewer leave registers for more waves (head size 64, 1 036 800
-// queries, sixteen heads, 256 keys: 2 1500 us, 3 1500, 4 1445; 64 800, 77 keys: 51, 55, 51; head size 32, 200 keys: 2 55, 3 56, 4 57).
+// queries, sixteen heads, 256 keys: 2 1286 us, 3 1222, 4 1191; 64 800, 77 keys: 52, 52, 51-56; head size 32, 200 keys: 2 53, 3 59, 4 55).
 constexpr int resident_qn(int64_t head_dim) { return head_dim == 64 ? 4 : 2; }
 constexpr int64_t RESIDENT_LDS = 80 * 1024;  // two workgroups per CU
 
@@ -1162,7 +1167,7 @@ Plan plan_of(const CrossArgs& a) {
   };
 
   // Few keys and many rows: a workgroup's keys stay (at least two row blocks for each of its waves).  As many workgroups as run at once: two per CU, four
-  // of the small ones of head size 32 (64 800 queries, sixteen heads, 77 keys: 33.5 us with 1024, 36.5 with 512; of 64: 54 and 51)
+  // of the small ones of head size 32 (64 800 queries, sixteen heads, 77 keys: 37.1 us with 1024, 38.1 with 512; of 64: 54.5 and 50.8)
   {
     Task& t = plan.task[0];
     const int64_t c = chunks_of(t, KC), lds = c * (4 * KC * D + 8), units = (int64_t)t.members * Hk;
@@ -1176,8 +1181,8 @@ Plan plan_of(const CrossArgs& a) {
       return plan;
     }
   }
-  // Otherwise the way that costs least (eight heads of 64, 1000 keys, in us: 8000 queries, 32 rows a wave 24.2, 64 27.3; 16 000 48.6 and 38.9, whose
-  // workgroups fill the chip once; 24 000 61.9 and 63; 64 800 162 and 149).  Parts of the keys: what fills the chip once, twice, ..
+  // Otherwise the way that costs least (eight heads of 64, 1000 keys, in us: 8000 queries, 32 rows a wave 21.8, 64 24.6; 16 000 42.3 and 35.9, whose
+  // workgroups fill the chip once; 24 000 58.8 and 58.3; 64 800 150 and 140).  Parts of the keys: what fills the chip once, twice, ..
   auto choose = [&](Plan& plan) {
     Way best{Form::rows, 1, 1, 1e30f};
     int splits[2] = {1, 1};
