@@ -110,11 +110,14 @@ def workspaces(device, *requests):
 
 
 def _workspace_ptr(tag: str, nbytes: int, device) -> int:
-    """``workspace`` for a call that needs its address alone: the buffer that it last used on this stream, without a tensor around it."""
+    """``workspace`` for a call that needs its address alone: the buffer that it last used on this stream, without a tensor around it.
+    Under a capture, memory of the graph's own (which its later allocations may use again, behind the call): graphs that are replayed on
+    streams of their own, beside each other or beside eager calls, do not meet in it."""
+    if torch._C._cuda_isCurrentStreamCapturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device).data_ptr()
     key = (tag, device, torch.uint8)
-    buf, owner = _WORKSPACE.get(key), _WS_OWNER.get(key)  # (no owner: so far it was asked for under captures alone)
-    if (buf is None or owner is None or buf.numel() < nbytes or torch._C._cuda_isCurrentStreamCapturing() or
-            owner[0] != torch._C._cuda_getCurrentRawStream(device.index)):
+    buf, owner = _WORKSPACE.get(key), _WS_OWNER.get(key)
+    if buf is None or owner is None or buf.numel() < nbytes or owner[0] != torch._C._cuda_getCurrentRawStream(device.index):
         return workspace(tag, (nbytes,), torch.uint8, device).data_ptr()
     return buf.data_ptr()
 
@@ -549,7 +552,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, length
     hold elsewhere is not looked at.  prefix = (k, v), [Np, key heads, head_dim]: states that all members see ahead of their own, read once
     for all of them where that is cheaper.  A query without any key gives zeros.
     scale: head_dim^-0.5 unless given; ``q_prescaled``: q already holds q * scale * log2(e) (``qk_norm_rope(q_scale=scale * LOG2E)``).  out shares
-    no memory with the inputs."""
+    no memory with the inputs.  Eager calls whose sums go through scratch memory share it and run on one stream at a time (``workspace``); a
+    captured graph has its own."""
     device, shape, kv_shape, bf16 = q.device, q.shape, k.shape, torch.bfloat16
     if device.index != torch._C._cuda_getDevice() or k.device != device or v.device != device:
         _on_current_device(device, dict(q=q, k=k, v=v))

@@ -223,3 +223,47 @@ def test_every_row_of_a_call_with_a_loud_one(pkg, cuda, D, Nq):
     w = torch.softmax(s, -1)
     bound = bound + e.amax(-1).exp() * (w * e.expm1() * torch.cdist(o, vv)).sum(-1)
     assert bool(((got[0, :, 0].double() - o).norm(dim=-1) <= bound).all())
+
+
+@pytest.mark.gpu
+def test_graphs_on_streams_of_their_own(pkg, cuda):
+    """Two captured calls whose sums go through scratch memory, replayed beside each other and beside eager calls of a third stream."""
+    ops, calls = pkg.ops, []
+    for i, (B, Nq, H, D, Nk) in enumerate([(2, 3, 4, 64, 90000), (1, 9, 4, 128, 60000), (4, 1, 8, 64, 70000)]):
+        (q, k, v), _ = inputs(B, Nq, H, H, D, Nk, cuda, 90 + i)
+        assert pkg._lib.lib().aeris_cross_attention_workspace_bytes(sizes(pkg, B, Nq, H, H, D, Nk)) > 0
+        calls.append(((q, k, v), ops.cross_attention(q, k, v).clone()))
+    torch.cuda.synchronize()
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in range(3)]
+    for (args, _), stream in zip(calls[:2], streams):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs.append(ops.cross_attention(*args))
+        graphs.append(graph)
+    for _ in range(4):
+        for out in outs:
+            out.fill_(5.0)
+        torch.cuda.synchronize()
+        eager = []
+        for _ in range(5):
+            for graph, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+            with torch.cuda.stream(streams[2]):
+                eager.append(ops.cross_attention(*calls[2][0]))
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for out, (_, want) in zip(outs, calls)) and all(torch.equal(t, calls[2][1]) for t in eager)
+
+
+def test_a_capture_has_scratch_memory_of_its_own(pkg, monkeypatch):
+    """... and leaves the eager calls' as it is."""
+    ops, cpu = pkg.ops, torch.device("cpu")
+    shared = torch.empty(4096, dtype=torch.uint8)
+    monkeypatch.setattr(ops, "_WORKSPACE", {("cross_attention", cpu, torch.uint8): shared})
+    monkeypatch.setattr(ops, "_WS_OWNER", {("cross_attention", cpu, torch.uint8): (7, None)})
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 7, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: False, raising=False)
+    assert ops._workspace_ptr("cross_attention", 100, cpu) == shared.data_ptr()
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: True, raising=False)
+    assert ops._workspace_ptr("cross_attention", 100, cpu) != shared.data_ptr()
+    assert ops._WORKSPACE == {("cross_attention", cpu, torch.uint8): shared}
