@@ -228,7 +228,7 @@ int aeris_qk_norm_rope_fwd(const aeris_qk_norm_rope* a, void* stream);
  *   out bf16 [B, Nq, heads, head_dim], contiguous.
  *   lengths int32 [n_lengths] (B, or one for all), on the device, or NULL; key_mask uint8 [mask_batch, Nk] (mask_batch B or 1), keys contiguous,
  *   members mask_stride apart, or NULL.
- *   Finite values of v of any size give finite results; below 2^-106 in size they may vanish in the sums.
+ *   Finite values of v of any size give finite results; below 2^-100 in size they may vanish in the sums.
  *   Infinities that take part give infinities (NaN, or nothing, where their weight is below 2^-90 of the row's largest: 0 in fp32).
  *   q_prescaled != 0: q already holds q * scale * log2(e) (scale is ignored); otherwise the fp32 logits are multiplied.
  * workspace: device memory of aeris_cross_attention_workspace_bytes(a) bytes (a's addresses do not count but for being NULL; 0: none is needed),
