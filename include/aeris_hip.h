@@ -195,7 +195,7 @@ int aeris_gemm_heads_fwd(const void* A, const void* W, void* C, const void* bias
  *   n = x * rsqrt(mean(x^2) + eps) * gain  per (token, head) over the head_dim elements (normed == 0: n = x * gain)
  *   the pairs (a, b) of the first R elements become (a cos - b sin, a sin + b cos); interleaved: pairs (2j, 2j + 1), else (j, j + R/2)
  *   y = n * scale
- * in fp32, rounded once.  parts: one (n_parts 1), or two that share tokens and positions (queries, keys).  Of each: x [tokens, heads, head_dim]
+ * in fp32 (squares too: elements up to 2^60 in size), rounded once.  parts: one (n_parts 1), or two that share tokens and positions (queries, keys).  Of each: x [tokens, heads, head_dim]
  * and y of the same shape by their strides (elements, one per dimension; that of a dimension with one entry does not count; the last is 1);
  * y may be x (same strides and type) and may otherwise not overlap it; gain [head_dim] (gain_head_stride 0) or one row per head, or NULL.
  * Addresses 16-byte aligned, strides multiples of 16 bytes.
