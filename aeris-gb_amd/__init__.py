@@ -3,7 +3,7 @@
 The directory name carries a hyphen, so import it with
 ``importlib.import_module("aeris-gb_amd")``; all intra-package imports are relative.
 """
-from . import _lib, ops  # noqa: F401
+from . import _lib, grad, ops  # noqa: F401
 from ._lib import AerisError, LIB_PATH  # noqa: F401
 from .model import (  # noqa: F401
     Attention,

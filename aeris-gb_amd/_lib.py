@@ -36,6 +36,14 @@ SIGNATURES = {
     "aeris_qkv_window_attention_fwd": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp] + [_c_int] * 11 + [_c_f32, _c_vp]),
     "aeris_norm_modulate_fwd": (_c_int, [_c_vp, _c_int, _c_vp, _c_int, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_i64, _c_i64,
                                          _c_i64, _c_int, _c_int, _c_int, _c_f32, _c_vp]),
+    "aeris_norm_modulate_grad_workspace_bytes": (_c_i64, [_c_vp]),
+    "aeris_norm_modulate_bwd": (_c_int, [_c_vp, _c_vp, _c_i64, _c_vp]),
+    "aeris_linear_train_fwd": (_c_int, [_c_vp, _c_vp]),
+    "aeris_linear_grad_workspace_bytes": (_c_i64, [_c_vp]),
+    "aeris_linear_bwd": (_c_int, [_c_vp, _c_vp, _c_i64, _c_vp]),
+    "aeris_feed_forward_train_fwd": (_c_int, [_c_vp, _c_vp]),
+    "aeris_feed_forward_grad_workspace_bytes": (_c_i64, [_c_vp]),
+    "aeris_feed_forward_bwd": (_c_int, [_c_vp, _c_vp, _c_i64, _c_vp]),
     "aeris_output_stage_workspace_bytes": (_c_i64, [_c_int, _c_int, _c_int]),
     "aeris_output_stage_fwd": (_c_int, [_c_vp, _c_int, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_i64, _c_vp, _c_vp, _c_i64, _c_i64,
                                         _c_int, _c_int, _c_int, _c_f32, _c_vp, _c_i64, _c_vp]),

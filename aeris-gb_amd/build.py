@@ -19,11 +19,11 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(CSRC, "libaeris_hip.so")
 SOURCES = ["api.hip", "gemm.hip", "gemm_persistent.hip", "gemm_norm.hip", "window_attention.hip", "qkv_window_attention.hip", "window_attention_stream.hip", "norm_modulate.hip", "small_ops.hip", "output_stage.hip", "input_stage.hip",
-           "qk_norm_rope.hip", "cross_attention.hip"]
+           "qk_norm_rope.hip", "cross_attention.hip", "norm_grad.hip", "gemm_grad.hip"]
 HEADERS = ["common.h", "kernels.h", "gemm_common.h", "attention_sweep.h", os.path.join("..", "..", "include", "aeris_hip.h")]
 # sources whose transposing LDS reads are inline assembly: their device assembly is checked after every compile
 # (asm_check.py says for what); the compile keeps its temporaries for that, in a scratch directory
-ASM_CHECKED = {"window_attention.hip", "qkv_window_attention.hip", "window_attention_stream.hip", "cross_attention.hip"}
+ASM_CHECKED = {"window_attention.hip", "qkv_window_attention.hip", "window_attention_stream.hip", "cross_attention.hip", "gemm_grad.hip"}
 # packed fp32 VALU ops stay off: some of their forms have produced wrong results on this hardware
 FLAGS = ["-O3", "-std=c++17", "--offload-arch=gfx950", "-fPIC", "-Xclang", "-target-feature", "-Xclang",
          "-packed-fp32-ops", "-Wno-unused-command-line-argument"]

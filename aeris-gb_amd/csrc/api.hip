@@ -4,6 +4,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <atomic>
+#include <initializer_list>
 #include <mutex>
 
 #include "kernels.h"
@@ -255,6 +256,43 @@ int aeris_norm_modulate_fwd(const void* x, int x_dtype, void* y, int y_dtype, co
   return AERIS_OK;
 }
 
+namespace {
+// what aeris_norm_modulate_grad_workspace_bytes looks at too
+bool norm_grad_sizes_ok(const aeris_norm_modulate_grad* a) {
+  return a && a->B > 0 && a->rows_per_batch > 0 && a->d > 0 && a->d <= 0x7fffffff && aeris::norm_supported((int)a->d) && a->mod_batch_stride >= 0 &&
+         a->B <= INT64_MAX / a->rows_per_batch && a->B * a->rows_per_batch <= (INT64_MAX >> 4) / a->d;
+}
+}  // namespace
+
+int64_t aeris_norm_modulate_grad_workspace_bytes(const aeris_norm_modulate_grad* a) {
+  return norm_grad_sizes_ok(a) ? aeris::norm_grad_workspace_bytes(*a) : 0;
+}
+
+int aeris_norm_modulate_bwd(const aeris_norm_modulate_grad* a, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* who = "aeris_norm_modulate_bwd";
+  if (!a || !a->x || !a->dy || !a->gamma) return fail(AERIS_EINVAL, "%s: x/dy/gamma is NULL", who);
+  if (a->B <= 0 || a->rows_per_batch <= 0 || a->mod_batch_stride < 0) return fail(AERIS_EINVAL, "%s: B and rows_per_batch must be positive, mod_batch_stride not negative", who);
+  for (int64_t dt : {a->x_dtype, a->dy_dtype, a->param_dtype})
+    if (dt != AERIS_BF16 && dt != AERIS_F32) return fail(AERIS_EINVAL, "%s: dtype must be AERIS_BF16 or AERIS_F32", who);
+  if (a->kind != AERIS_NORM_LAYER && a->kind != AERIS_NORM_RMS) return fail(AERIS_EINVAL, "%s: unknown norm kind %lld", who, (long long)a->kind);
+  if (a->order != AERIS_NORM_THEN_MOD && a->order != AERIS_MOD_THEN_NORM) return fail(AERIS_EINVAL, "%s: unknown order %lld", who, (long long)a->order);
+  if (!(a->eps >= 0.0)) return fail(AERIS_EINVAL, "%s: eps must be non-negative", who);
+  if (!norm_grad_sizes_ok(a)) return fail(AERIS_EUNSUPPORTED, "%s: d=%lld (need d %% 8 == 0 and d <= 6144), or too many rows", who, (long long)a->d);
+  for (const void* p : {a->x, a->dy, a->gamma, a->beta, static_cast<const void*>(a->shift), static_cast<const void*>(a->scale),
+                        static_cast<const void*>(a->dx), static_cast<const void*>(a->dgamma), static_cast<const void*>(a->dbeta),
+                        static_cast<const void*>(a->dshift), static_cast<const void*>(a->dscale)})
+    if (!aligned16(p)) return fail(AERIS_EINVAL, "%s: every tensor must be 16-byte aligned", who);
+  if ((a->dbeta && !a->beta) || (a->dshift && !a->shift) || (a->dscale && !a->scale))
+    return fail(AERIS_EINVAL, "%s: dbeta, dshift and dscale need beta, shift and scale", who);
+  if (aeris::norm_grad_blocks(*a) >= 1 << 24) return fail(AERIS_EUNSUPPORTED, "%s: more than 2^24 members", who);
+  const int64_t need = aeris::norm_grad_workspace_bytes(*a);
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
+    return fail(AERIS_EINVAL, "%s: needs a 16-byte aligned workspace of %lld bytes", who, (long long)need);
+  hipError_t e = aeris::norm_grad_launch(*a, workspace, reinterpret_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, who);
+  return AERIS_OK;
+}
+
 int64_t aeris_output_stage_workspace_bytes(int N, int d, int B_mod) {
   if (B_mod <= 0 || !aeris::output_stage_supported(N, d)) return 0;
   return aeris::output_stage_workspace_bytes(N, d, B_mod);
@@ -357,6 +395,86 @@ int aeris_gemm_fwd(const void* A, const void* W, void* C, const void* bias, cons
                                     gate_batch_stride, rows_per_batch, 0, 0, 1.0f, 0, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "aeris_gemm_fwd launch");
   return AERIS_OK;
+}
+
+namespace {
+// sizes of a projection and its gradients: tiles are numbered in 32 bits, an operand's tile is addressed in 31 bits of bytes
+bool train_sizes_ok(int64_t M, int64_t N, int64_t K) {
+  return M > 0 && M < (int64_t(1) << 31) && N > 0 && K > 0 && N % 8 == 0 && K % 8 == 0 && N <= 1 << 20 && K <= 1 << 20 && N * K < 1 << 30 &&
+         ((M + 63) / 64) * ((N + 31) / 32) < 1 << 24 && ((M + 63) / 64) * ((K + 63) / 64) < 1 << 24;
+}
+int train_sizes(const char* who, int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0) return fail(AERIS_EINVAL, "%s: sizes must be positive", who);
+  if (!train_sizes_ok(M, N, K))
+    return fail(AERIS_EUNSUPPORTED, "%s: %lld rows of %lld -> %lld (widths must be multiples of 8, their product below 2^30)", who, (long long)M, (long long)K, (long long)N);
+  return AERIS_OK;
+}
+int train_aligned(const char* who, std::initializer_list<const void*> all) {
+  for (const void* p : all)
+    if (!aligned16(p)) return fail(AERIS_EINVAL, "%s: every tensor must be 16-byte aligned", who);
+  return AERIS_OK;
+}
+int train_workspace(const char* who, const void* workspace, int64_t have, int64_t need) {
+  if (need > 0 && (!workspace || !aligned16(workspace) || have < need))
+    return fail(AERIS_EINVAL, "%s: needs a 16-byte aligned workspace of %lld bytes", who, (long long)need);
+  return AERIS_OK;
+}
+}  // namespace
+
+int aeris_linear_train_fwd(const aeris_linear_train* a, void* stream) {
+  const char* who = "aeris_linear_train_fwd";
+  if (!a || !a->x || !a->w || !a->y || !a->z) return fail(AERIS_EINVAL, "%s: x/w/y/z is NULL", who);
+  if (int rc = train_sizes(who, a->M, a->N, a->K)) return rc;
+  if (a->act != AERIS_ACT_GELU && a->act != AERIS_ACT_SILU) return fail(AERIS_EINVAL, "%s: activation must be AERIS_ACT_GELU or AERIS_ACT_SILU", who);
+  if ((a->y_dtype != AERIS_BF16 && a->y_dtype != AERIS_F32) || (a->residual && a->res_dtype != AERIS_BF16 && a->res_dtype != AERIS_F32))
+    return fail(AERIS_EINVAL, "%s: dtype must be AERIS_BF16 or AERIS_F32", who);
+  if (int rc = train_aligned(who, {a->x, a->w, a->bias, a->residual, a->y, a->z})) return rc;
+  hipError_t e = aeris::linear_train_launch(*a, reinterpret_cast<hipStream_t>(stream));
+  return e == hipSuccess ? AERIS_OK : hip_fail(e, who);
+}
+
+int64_t aeris_linear_grad_workspace_bytes(const aeris_linear_grad* a) {
+  return a && train_sizes_ok(a->M, a->N, a->K) ? aeris::linear_grad_workspace_bytes(*a) : 0;
+}
+
+int aeris_linear_bwd(const aeris_linear_grad* a, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* who = "aeris_linear_bwd";
+  if (!a || !a->dy || (a->dx && !a->w) || (a->dw && !a->x)) return fail(AERIS_EINVAL, "%s: dy is NULL, dx without w or dw without x", who);
+  if (int rc = train_sizes(who, a->M, a->N, a->K)) return rc;
+  if (a->act != AERIS_ACT_NONE && a->act != AERIS_ACT_GELU && a->act != AERIS_ACT_SILU) return fail(AERIS_EINVAL, "%s: unknown activation %lld", who, (long long)a->act);
+  if (a->act != AERIS_ACT_NONE && !a->z) return fail(AERIS_EINVAL, "%s: an activation's gradient needs z", who);
+  if (a->dy_dtype != AERIS_BF16 && a->dy_dtype != AERIS_F32) return fail(AERIS_EINVAL, "%s: dtype must be AERIS_BF16 or AERIS_F32", who);
+  if (a->dz && a->act == AERIS_ACT_NONE && a->dy_dtype == AERIS_BF16) return fail(AERIS_EINVAL, "%s: dz is dy itself", who);
+  if (int rc = train_aligned(who, {a->dy, a->x, a->w, a->z, a->dx, a->dw, a->dbias, a->dz})) return rc;
+  if (int rc = train_workspace(who, workspace, workspace_bytes, aeris::linear_grad_workspace_bytes(*a))) return rc;
+  hipError_t e = aeris::linear_grad_launch(*a, workspace, reinterpret_cast<hipStream_t>(stream));
+  return e == hipSuccess ? AERIS_OK : hip_fail(e, who);
+}
+
+int aeris_feed_forward_train_fwd(const aeris_feed_forward* a, void* stream) {
+  const char* who = "aeris_feed_forward_train_fwd";
+  if (!a || !a->x || !a->w1 || !a->w2 || !a->gate_up || !a->h || !a->y) return fail(AERIS_EINVAL, "%s: a tensor is NULL", who);
+  if (int rc = train_sizes(who, a->M, a->H > 0 && a->H <= 1 << 19 ? 2 * a->H : a->H > 0 ? 1 << 30 : 0, a->d)) return rc;
+  if (int rc = train_aligned(who, {a->x, a->w1, a->w2, a->gate_up, a->h, a->y})) return rc;
+  if (a->H % 8) return fail(AERIS_EUNSUPPORTED, "%s: H=%lld must be a multiple of 8", who, (long long)a->H);
+  hipError_t e = aeris::feed_forward_train_launch(*a, reinterpret_cast<hipStream_t>(stream));
+  return e == hipSuccess ? AERIS_OK : hip_fail(e, who);
+}
+
+int64_t aeris_feed_forward_grad_workspace_bytes(const aeris_feed_forward_grad* a) {
+  return a && a->H > 0 && a->H <= 1 << 19 && a->H % 8 == 0 && train_sizes_ok(a->M, 2 * a->H, a->d) ? aeris::feed_forward_grad_workspace_bytes(*a) : 0;
+}
+
+int aeris_feed_forward_bwd(const aeris_feed_forward_grad* a, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* who = "aeris_feed_forward_bwd";
+  if (!a || !a->dy || !a->gate_up || !a->w2 || (a->dx && !a->w1) || (a->dw1 && !a->x) || (a->dw2 && !a->h))
+    return fail(AERIS_EINVAL, "%s: a tensor is NULL", who);
+  if (int rc = train_sizes(who, a->M, a->H > 0 && a->H <= 1 << 19 ? 2 * a->H : a->H > 0 ? 1 << 30 : 0, a->d)) return rc;
+  if (a->H % 8) return fail(AERIS_EUNSUPPORTED, "%s: H=%lld must be a multiple of 8", who, (long long)a->H);
+  if (int rc = train_aligned(who, {a->dy, a->x, a->w1, a->w2, a->gate_up, a->h, a->dx, a->dw1, a->dw2})) return rc;
+  if (int rc = train_workspace(who, workspace, workspace_bytes, aeris::feed_forward_grad_workspace_bytes(*a))) return rc;
+  hipError_t e = aeris::feed_forward_grad_launch(*a, workspace, reinterpret_cast<hipStream_t>(stream));
+  return e == hipSuccess ? AERIS_OK : hip_fail(e, who);
 }
 
 int aeris_gemm_heads_fwd(const void* A, const void* W, void* C, const void* bias, int64_t M, int N, int K, int head_dim,

@@ -52,6 +52,19 @@ hipError_t norm_modulate_launch(const void* x, int x_dtype, void* y, int y_dtype
                                 int param_dtype, const float* shift, const float* scale, int64_t mod_batch_stride, int64_t B,
                                 int64_t rows_per_batch, int d, int kind, int order, float eps, hipStream_t stream);
 
+// gradients of the norm and its modulation (norm_grad.hip)
+int64_t norm_grad_blocks(const aeris_norm_modulate_grad& a);
+int64_t norm_grad_workspace_bytes(const aeris_norm_modulate_grad& a);
+hipError_t norm_grad_launch(const aeris_norm_modulate_grad& a, void* workspace, hipStream_t stream);
+
+// products of a training step (gemm_grad.hip)
+hipError_t linear_train_launch(const aeris_linear_train& a, hipStream_t stream);
+int64_t linear_grad_workspace_bytes(const aeris_linear_grad& a);
+hipError_t linear_grad_launch(const aeris_linear_grad& a, void* workspace, hipStream_t stream);
+hipError_t feed_forward_train_launch(const aeris_feed_forward& a, hipStream_t stream);
+int64_t feed_forward_grad_workspace_bytes(const aeris_feed_forward_grad& a);
+hipError_t feed_forward_grad_launch(const aeris_feed_forward_grad& a, void* workspace, hipStream_t stream);
+
 // fused output stage (output_stage.hip): norm -> modulate -> head in one pass; N <= 80, d % 64 == 0
 bool output_stage_supported(int N, int d);
 int64_t output_stage_workspace_bytes(int N, int d, int B_mod);

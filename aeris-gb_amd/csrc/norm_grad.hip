@@ -1,0 +1,467 @@
+// Gradients of norm_modulate (LayerNorm / RMSNorm with the noise-level modulation) in one pass over the tokens.  With u what is
+// normed, n = (u - mean) r, r = (var + eps)^-1/2 (RMS: no mean), v = n gamma + beta and dv the gradient of v:
+//     dn = dv gamma,  du = r (dn - mean(dn) - n mean(dn n))   (RMS: without mean(dn))
+//   norm then mod (y = v (1 + s) + t):  dv = dy (1 + s), dx = du;  A = sum dy n, B = sum dy over a member's tokens give
+//     ds = gamma A + beta B,  dt = B,  dgamma = sum over members of (1 + s) A,  dbeta = sum over members of (1 + s) B
+//   mod then norm (u = x (1 + s) + t):  dv = dy, dx = du (1 + s);  dgamma = sum dy n,  dbeta = sum dy,  ds = sum du x,  dt = sum du
+// Nothing is kept from the forward pass: mean and r are recomputed from the row, which is read anyway.
+//
+// Bound by HBM: x and dy are read once, dx is written once.  A wave owns a row (rows of up to 256 or 128 elements lie beside each
+// other in it, rows beyond 2048 belong to the four waves of a workgroup), holds it in registers and asks for its next one before it
+// sums; the sums over the tokens stay in registers while a workgroup walks down its share of a member's rows.  At the end of it the
+// workgroup writes one partial sum per column, and a second kernel adds those up in a fixed order: equal calls have equal results.
+// All sums are fp32: within a lane over some hundred rows, then over lanes, waves and workgroups.
+#include "common.h"
+#include "kernels.h"
+
+namespace aeris {
+
+namespace {
+
+struct NormGradParams {
+  const void* x;
+  const void* dy;
+  void* dx;
+  const void* gamma;
+  const void* beta;
+  const float* shift;
+  const float* scale;
+  float* partial;  // [segments][blocks per segment][sums][d], or NULL: no sums
+  int64_t mod_stride;  // between the segments' modulation rows
+  int64_t rows;        // of a segment
+  int64_t rows_per_block;
+  int blocks_per_segment;
+  int d;
+  int kind;
+  int param_f32;
+  float eps;
+};
+
+__device__ __forceinline__ float param_at(const void* p, int f32, int c) {
+  return f32 ? reinterpret_cast<const float*>(p)[c] : bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(p)[c]);
+}
+
+// NV: groups of 8 columns a lane; SUB: rows beside each other in a wave; WPR: waves to a row (1 or 4)
+template <int NV, int SUB, int WPR, bool X_F32, bool DY_F32, bool PRE>
+__global__ void __launch_bounds__(256) norm_grad_kernel(NormGradParams p) {
+  static_assert(SUB == 1 || (NV == 1 && WPR == 1), "rows beside each other: one column group a lane");
+  constexpr int LPR = 64 * WPR / SUB;          // lanes of a row
+  constexpr int SLOTS = 256 / LPR;             // rows at a time
+  constexpr int GROUPS = NV * LPR;
+  constexpr int SUMS = PRE ? 4 : 2;
+  constexpr int COLS = GROUPS * 8;
+  // the parameters, first and second four of a group's columns apart (neighbouring lanes' 16-byte reads do not share banks); the
+  // sums of the row slots go over them at the end.  (Four waves to a row: a lane's columns are its own for all rows, their parameters
+  // stay in its registers.)
+  constexpr bool IN_LDS = WPR == 1;
+  __shared__ __attribute__((aligned(16))) float lds[IN_LDS ? (SLOTS > 3 ? SLOTS : 3) * COLS : 4];
+  __shared__ float cross[2][4][2];
+  f32x4* const sG = reinterpret_cast<f32x4*>(lds);
+  f32x4* const sP1 = sG + (IN_LDS ? 2 * GROUPS : 0);
+  f32x4* const sP0 = sP1 + (IN_LDS ? 2 * GROUPS : 0);
+  f32x4 rG[IN_LDS ? 1 : NV][2], rP1[IN_LDS ? 1 : NV][2], rP0[IN_LDS ? 1 : NV][2];
+  const int lane = threadIdx.x & (LPR - 1), slot = threadIdx.x / LPR;
+  const int d = p.d;
+  const float inv_d = 1.0f / (float)d;
+  const int seg = blockIdx.x / p.blocks_per_segment, blk = blockIdx.x - seg * p.blocks_per_segment;
+  const int64_t first = (int64_t)blk * p.rows_per_block;
+  int64_t end = first + p.rows_per_block;
+  if (end > p.rows) end = p.rows;
+  const int64_t row_base = (int64_t)seg * p.rows;
+  const float* const sh = p.shift ? p.shift + seg * p.mod_stride : nullptr;
+  const float* const sc = p.scale ? p.scale + seg * p.mod_stride : nullptr;
+
+  struct Raw { u32x4 xa, xb, ya, yb; };
+  auto load_row = [&](int64_t row, Raw (&raw)[NV]) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int col = (v * LPR + lane) * 8;
+      raw[v].xa = raw[v].xb = raw[v].ya = raw[v].yb = u32x4{0u, 0u, 0u, 0u};
+      if (col < d) {
+        const int64_t at = (row_base + row) * d + col;
+        if (X_F32) {
+          const u32x4* q = reinterpret_cast<const u32x4*>(reinterpret_cast<const float*>(p.x) + at);
+          raw[v].xa = __builtin_nontemporal_load(q);
+          raw[v].xb = __builtin_nontemporal_load(q + 1);
+        } else {
+          raw[v].xa = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(p.x) + at));
+        }
+        if (DY_F32) {
+          const u32x4* q = reinterpret_cast<const u32x4*>(reinterpret_cast<const float*>(p.dy) + at);
+          raw[v].ya = __builtin_nontemporal_load(q);
+          raw[v].yb = __builtin_nontemporal_load(q + 1);
+        } else {
+          raw[v].ya = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(p.dy) + at));
+        }
+      }
+    }
+  };
+  auto widen = [](const u32x4& a, const u32x4& b, bool f32, float (&o)[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (f32) {
+        o[e] = __uint_as_float(a[e]);
+        o[4 + e] = __uint_as_float(b[e]);
+      } else {
+        o[2 * e] = bf16_lo(a[e]);
+        o[2 * e + 1] = bf16_hi(a[e]);
+      }
+    }
+  };
+
+  Raw cur[NV], nxt[NV];
+  int64_t row = first + slot;
+  if (row < end) load_row(row, cur);
+
+#pragma unroll
+  for (int v = 0; v < (GROUPS + 255) / 256; ++v) {
+    const int g = v * 256 + threadIdx.x;
+    if (GROUPS % 256 && g >= GROUPS) break;
+    float G[8], P1[8], P0[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = g * 8 + e;
+      const float ga = c < d ? param_at(p.gamma, p.param_f32, c) : 0.f;
+      const float s1 = c < d && sc ? 1.f + sc[c] : 1.f;
+      G[e] = PRE ? ga : ga * s1;
+      P1[e] = s1;
+      P0[e] = c < d && sh ? sh[c] : 0.f;
+    }
+    if (!IN_LDS) {
+      rG[v][0] = f32x4{G[0], G[1], G[2], G[3]};
+      rG[v][1] = f32x4{G[4], G[5], G[6], G[7]};
+      rP1[v][0] = f32x4{P1[0], P1[1], P1[2], P1[3]};
+      rP1[v][1] = f32x4{P1[4], P1[5], P1[6], P1[7]};
+      rP0[v][0] = f32x4{P0[0], P0[1], P0[2], P0[3]};
+      rP0[v][1] = f32x4{P0[4], P0[5], P0[6], P0[7]};
+      continue;
+    }
+    sG[g] = f32x4{G[0], G[1], G[2], G[3]};
+    sG[GROUPS + g] = f32x4{G[4], G[5], G[6], G[7]};
+    if (PRE) {
+      sP1[g] = f32x4{P1[0], P1[1], P1[2], P1[3]};
+      sP1[GROUPS + g] = f32x4{P1[4], P1[5], P1[6], P1[7]};
+      sP0[g] = f32x4{P0[0], P0[1], P0[2], P0[3]};
+      sP0[GROUPS + g] = f32x4{P0[4], P0[5], P0[6], P0[7]};
+    }
+  }
+  __syncthreads();
+
+  auto gain = [&](int v, int h) { return IN_LDS ? sG[h * GROUPS + v * LPR + lane] : rG[IN_LDS ? 0 : v][h]; };
+  auto one_plus_scale = [&](int v, int h) { return IN_LDS ? sP1[h * GROUPS + v * LPR + lane] : rP1[IN_LDS ? 0 : v][h]; };
+  auto shift_of = [&](int v, int h) { return IN_LDS ? sP0[h * GROUPS + v * LPR + lane] : rP0[IN_LDS ? 0 : v][h]; };
+
+  float acc[SUMS][NV][8];
+#pragma unroll
+  for (int s = 0; s < SUMS; ++s)
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[s][v][e] = 0.f;
+
+  int turn = 0;
+  // two sums over a row, the same value in each of its lanes
+  auto row_sums = [&](float& a, float& b) {
+    if (WPR == 1) {
+      a = lanes_sum<SUB>(a);
+      b = lanes_sum<SUB>(b);
+    } else {
+      a = wave_sum(a);
+      b = wave_sum(b);
+      const int w = threadIdx.x >> 6;
+      if ((threadIdx.x & 63) == 0) {
+        cross[turn][w][0] = a;
+        cross[turn][w][1] = b;
+      }
+      __syncthreads();
+      a = (cross[turn][0][0] + cross[turn][1][0]) + (cross[turn][2][0] + cross[turn][3][0]);
+      b = (cross[turn][0][1] + cross[turn][1][1]) + (cross[turn][2][1] + cross[turn][3][1]);
+      turn ^= 1;  // the next pair goes elsewhere: a wave may be there before another has read this one
+    }
+  };
+
+  // (rows beside each other in a wave, and rows of a workgroup, take the same number of turns: the lanes of a slot without a row
+  // work on zeros, whose sums are zeros and which are not stored)
+  const int64_t turns = end > first ? (end - first + SLOTS - 1) / SLOTS : 0;
+  for (int64_t it = 0; it < turns; ++it, row += SLOTS) {
+    const bool live = row < end;
+    if (row + SLOTS < end) load_row(row + SLOTS, nxt);
+    float u[NV][8], y[NV][8], x[PRE ? NV : 1][8];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int g = v * LPR + lane;
+      const bool act = g * 8 < d;
+      if (!live) cur[v].xa = cur[v].xb = cur[v].ya = cur[v].yb = u32x4{0u, 0u, 0u, 0u};
+      widen(cur[v].xa, cur[v].xb, X_F32, u[v]);
+      widen(cur[v].ya, cur[v].yb, DY_F32, y[v]);
+      if (PRE) {
+        const f32x4 p1a = one_plus_scale(v, 0), p1b = one_plus_scale(v, 1), p0a = shift_of(v, 0), p0b = shift_of(v, 1);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[v][e] = u[v][e];
+          u[v][e] = act ? fmaf(u[v][e], e < 4 ? p1a[e] : p1b[e - 4], e < 4 ? p0a[e] : p0b[e - 4]) : 0.f;
+        }
+      }
+      const f32x4 ga = gain(v, 0), gb = gain(v, 1);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float dn = y[v][e] * (e < 4 ? ga[e] : gb[e - 4]);
+        s1 += p.kind == AERIS_NORM_RMS ? u[v][e] * u[v][e] : u[v][e];
+        s2 += p.kind == AERIS_NORM_RMS ? dn * u[v][e] : dn;
+      }
+    }
+    row_sums(s1, s2);
+    float mean = 0.f, r, c1 = 0.f, c2;  // c1 = mean(dn), c2 = r mean(dn n)
+    if (p.kind == AERIS_NORM_RMS) {
+      r = rsqrtf(s1 * inv_d + p.eps);
+      c2 = s2 * inv_d * r;
+    } else {
+      mean = s1 * inv_d;
+      c1 = s2 * inv_d;
+      float q1 = 0.f, q2 = 0.f;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int g = v * LPR + lane;
+        const bool act = g * 8 < d;
+        const f32x4 ga = gain(v, 0), gb = gain(v, 1);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          u[v][e] = act ? u[v][e] - mean : 0.f;
+          q1 = fmaf(u[v][e], u[v][e], q1);
+          q2 = fmaf(y[v][e] * (e < 4 ? ga[e] : gb[e - 4]), u[v][e], q2);
+        }
+      }
+      row_sums(q1, q2);
+      r = rsqrtf(q1 * inv_d + p.eps);
+      c2 = q2 * inv_d * r;
+    }
+    if (!live) r = c2 = 0.f;  // (eps 0: a row of zeros would have an infinite r)
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int g = v * LPR + lane, col = g * 8;
+      const f32x4 ga = gain(v, 0), gb = gain(v, 1);
+      float o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float n = u[v][e] * r;
+        float du = (y[v][e] * (e < 4 ? ga[e] : gb[e - 4]) - c1 - n * c2) * r;
+        acc[0][v][e] = fmaf(y[v][e], n, acc[0][v][e]);
+        acc[1][v][e] += y[v][e];
+        if (PRE) {
+          const f32x4 p1 = one_plus_scale(v, e >> 2);
+          acc[2][v][e] = fmaf(du, x[v][e], acc[2][v][e]);
+          acc[3][v][e] += du;
+          du *= p1[e & 3];
+        }
+        o[e] = du;
+      }
+      if (p.dx && live && col < d) {
+        const int64_t at = (row_base + row) * d + col;
+        if (X_F32) {
+          f32x4* q = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p.dx) + at);
+          __builtin_nontemporal_store(f32x4{o[0], o[1], o[2], o[3]}, q);
+          __builtin_nontemporal_store(f32x4{o[4], o[5], o[6], o[7]}, q + 1);
+        } else {
+          const u32x4 w = {pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7])};
+          __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(p.dx) + at));
+        }
+      }
+      cur[v] = nxt[v];
+    }
+  }
+  if (!p.partial) return;
+
+  // the row slots' sums, one quantity after the other through LDS
+  float* const out = p.partial + ((int64_t)seg * p.blocks_per_segment + blk) * SUMS * d;
+#pragma unroll
+  for (int s = 0; s < SUMS; ++s) {
+    if (SLOTS == 1) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int col = (v * LPR + lane) * 8;
+        if (col < d) {
+          *reinterpret_cast<f32x4*>(out + (int64_t)s * d + col) = f32x4{acc[s][v][0], acc[s][v][1], acc[s][v][2], acc[s][v][3]};
+          *reinterpret_cast<f32x4*>(out + (int64_t)s * d + col + 4) = f32x4{acc[s][v][4], acc[s][v][5], acc[s][v][6], acc[s][v][7]};
+        }
+      }
+    } else {
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        f32x4* q = reinterpret_cast<f32x4*>(lds + slot * COLS);
+        const int g = v * LPR + lane;
+        q[g] = f32x4{acc[s][v][0], acc[s][v][1], acc[s][v][2], acc[s][v][3]};
+        q[GROUPS + g] = f32x4{acc[s][v][4], acc[s][v][5], acc[s][v][6], acc[s][v][7]};
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < 2 * GROUPS; i += 256) {
+        f32x4 t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < SLOTS; ++k) t += reinterpret_cast<const f32x4*>(lds + k * COLS)[i];
+        const int col = (i % GROUPS) * 8 + (i / GROUPS) * 4;
+        if (col < d) *reinterpret_cast<f32x4*>(out + (int64_t)s * d + col) = t;
+      }
+    }
+  }
+}
+
+struct NormGradSums {
+  const float* partial;
+  const void* gamma;
+  const void* beta;
+  const float* scale;
+  void* dgamma;
+  void* dbeta;
+  float* dshift;
+  float* dscale;
+  int64_t mod_stride;
+  int segments, blocks, d, param_f32, pre;
+};
+
+// 32 columns a workgroup; 32 threads share a column's partial sums
+__global__ void __launch_bounds__(1024) norm_grad_sums_kernel(NormGradSums p) {
+  __shared__ float lds[4][32][33];
+  const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
+  const int col = blockIdx.x * 32 + c;
+  const bool ok = col < p.d;
+  const int sums = p.pre ? 4 : 2;
+  const float ga = ok ? param_at(p.gamma, p.param_f32, col) : 0.f;
+  const float be = ok && p.beta ? param_at(p.beta, p.param_f32, col) : 0.f;
+  float dgamma = 0.f, dbeta = 0.f;
+  for (int seg = 0; seg < p.segments; ++seg) {
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
+    if (ok) {
+      const float* q = p.partial + ((int64_t)seg * p.blocks + r) * sums * p.d + col;
+      for (int b = r; b < p.blocks; b += 32, q += (int64_t)32 * sums * p.d) {
+        t[0] += q[0];
+        t[1] += q[p.d];
+        if (p.pre) {
+          t[2] += q[2 * (int64_t)p.d];
+          t[3] += q[3 * (int64_t)p.d];
+        }
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) lds[s][r][c] = t[s];
+    __syncthreads();
+    // thread (c, r < 4) finishes sum r of column c
+    float v = 0.f;
+    if (r < 4) {
+#pragma unroll
+      for (int k = 0; k < 32; ++k) v += lds[r][k][c];
+    }
+    __syncthreads();
+    if (r < 4) lds[r][0][c] = v;
+    __syncthreads();
+    if (r == 0 && ok) {
+      const float A = lds[0][0][c], B = lds[1][0][c];
+      float ds, dt;
+      if (p.pre) {
+        dgamma += A;
+        dbeta += B;
+        ds = lds[2][0][c];
+        dt = lds[3][0][c];
+      } else {
+        const float one = p.scale ? 1.f + p.scale[seg * p.mod_stride + col] : 1.f;
+        dgamma = fmaf(one, A, dgamma);
+        dbeta = fmaf(one, B, dbeta);
+        ds = fmaf(ga, A, be * B);
+        dt = B;
+      }
+      if (p.dscale) p.dscale[(int64_t)seg * p.d + col] = ds;
+      if (p.dshift) p.dshift[(int64_t)seg * p.d + col] = dt;
+    }
+    __syncthreads();
+  }
+  if (r == 0 && ok) {
+    if (p.param_f32) {
+      if (p.dgamma) reinterpret_cast<float*>(p.dgamma)[col] = dgamma;
+      if (p.dbeta) reinterpret_cast<float*>(p.dbeta)[col] = dbeta;
+    } else {
+      if (p.dgamma) reinterpret_cast<uint16_t*>(p.dgamma)[col] = (uint16_t)f32_to_bf16_bits(dgamma);
+      if (p.dbeta) reinterpret_cast<uint16_t*>(p.dbeta)[col] = (uint16_t)f32_to_bf16_bits(dbeta);
+    }
+  }
+}
+
+bool wants_sums(const aeris_norm_modulate_grad& a) { return a.dgamma || a.dbeta || a.dshift || a.dscale; }
+bool is_pre(const aeris_norm_modulate_grad& a) { return a.order == AERIS_MOD_THEN_NORM && (a.shift || a.scale); }
+int64_t segments_of(const aeris_norm_modulate_grad& a) { return (a.shift || a.scale) && a.mod_batch_stride && a.B > 1 ? a.B : 1; }
+
+// Workgroups of a segment: as many as the chip holds of them at two waves a SIMD, and at least some turns each, so that the
+// parameters' and the partial sums' traffic stays small beside the rows'.
+int64_t blocks_of(const aeris_norm_modulate_grad& a) {
+  const int64_t segments = segments_of(a), rows = a.B * a.rows_per_batch / segments;
+  const int64_t slots = a.d <= 128 ? 16 : a.d <= 256 ? 8 : a.d <= 2048 ? 4 : 1;
+  int64_t n = (rows + slots * 4 - 1) / (slots * 4);
+  const int64_t cap = 1024 / segments > 0 ? 1024 / segments : 1;
+  if (n > cap) n = cap;
+  return n;
+}
+
+template <int NV, int SUB, int WPR>
+hipError_t launch(const NormGradParams& p, bool xf, bool yf, bool pre, int64_t blocks, hipStream_t stream) {
+  const dim3 grid((unsigned)blocks), block(256);
+#define GO(XF, YF, PR) hipLaunchKernelGGL((norm_grad_kernel<NV, SUB, WPR, XF, YF, PR>), grid, block, 0, stream, p)
+  if (pre) {
+    if (xf) { if (yf) GO(true, true, true); else GO(true, false, true); }
+    else { if (yf) GO(false, true, true); else GO(false, false, true); }
+  } else {
+    if (xf) { if (yf) GO(true, true, false); else GO(true, false, false); }
+    else { if (yf) GO(false, true, false); else GO(false, false, false); }
+  }
+#undef GO
+  return hipGetLastError();
+}
+
+}  // namespace
+
+int64_t norm_grad_blocks(const aeris_norm_modulate_grad& a) { return segments_of(a) * blocks_of(a); }
+
+int64_t norm_grad_workspace_bytes(const aeris_norm_modulate_grad& a) {
+  return wants_sums(a) ? norm_grad_blocks(a) * (is_pre(a) ? 4 : 2) * a.d * 4 : 0;
+}
+
+hipError_t norm_grad_launch(const aeris_norm_modulate_grad& a, void* workspace, hipStream_t stream) {
+  const bool pre = is_pre(a), xf = a.x_dtype == AERIS_F32, yf = a.dy_dtype == AERIS_F32;
+  const int64_t segments = segments_of(a);
+  NormGradParams p;
+  p.x = a.x; p.dy = a.dy; p.dx = a.dx;
+  p.gamma = a.gamma; p.beta = a.beta;
+  p.shift = a.shift; p.scale = a.scale;
+  p.partial = wants_sums(a) ? reinterpret_cast<float*>(workspace) : nullptr;
+  p.mod_stride = segments > 1 ? a.mod_batch_stride : 0;
+  p.rows = a.B * a.rows_per_batch / segments;
+  p.blocks_per_segment = (int)blocks_of(a);
+  p.rows_per_block = (p.rows + p.blocks_per_segment - 1) / p.blocks_per_segment;
+  p.d = (int)a.d;
+  p.kind = (int)a.kind;
+  p.param_f32 = a.param_dtype == AERIS_F32;
+  p.eps = (float)a.eps;
+  const int64_t blocks = segments * p.blocks_per_segment;
+  hipError_t e;
+  if (a.d <= 128) e = launch<1, 4, 1>(p, xf, yf, pre, blocks, stream);
+  else if (a.d <= 256) e = launch<1, 2, 1>(p, xf, yf, pre, blocks, stream);
+  else if (a.d <= 512) e = launch<1, 1, 1>(p, xf, yf, pre, blocks, stream);
+  else if (a.d <= 1024) e = launch<2, 1, 1>(p, xf, yf, pre, blocks, stream);
+  else if (a.d <= 1536) e = launch<3, 1, 1>(p, xf, yf, pre, blocks, stream);
+  else if (a.d <= 2048) e = launch<4, 1, 1>(p, xf, yf, pre, blocks, stream);
+  else if (a.d <= 4096) e = launch<2, 1, 4>(p, xf, yf, pre, blocks, stream);
+  else e = launch<3, 1, 4>(p, xf, yf, pre, blocks, stream);
+  if (e != hipSuccess || !p.partial) return e;
+  NormGradSums s;
+  s.partial = p.partial;
+  s.gamma = a.gamma; s.beta = a.beta; s.scale = a.scale;
+  s.dgamma = a.dgamma; s.dbeta = a.dbeta; s.dshift = a.dshift; s.dscale = a.dscale;
+  s.mod_stride = p.mod_stride;
+  s.segments = (int)segments;
+  s.blocks = p.blocks_per_segment;
+  s.d = p.d;
+  s.param_f32 = p.param_f32;
+  s.pre = pre;
+  hipLaunchKernelGGL(norm_grad_sums_kernel, dim3((unsigned)((p.d + 31) / 32)), dim3(1024), 0, stream, s);
+  return hipGetLastError();
+}
+
+}  // namespace aeris

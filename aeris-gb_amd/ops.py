@@ -61,6 +61,8 @@ def gemm_uses_big_tiles(M, N, act=None):
     return M >= 256 and (N % bn == 0 or N >= 4 * bn) and ((M + 255) // 256) * ((N + bn - 1) // bn) >= 256 and N % 4 == 0
 
 
+_KIND = {"layernorm": L.NORM_LAYER, "rmsnorm": L.NORM_RMS}
+_ORDER = {"norm_then_mod": L.NORM_THEN_MOD, "mod_then_norm": L.MOD_THEN_NORM}
 _WORKSPACE = {}
 _WS_OWNER = {}  # key -> (raw handle, stream) whose work last used the buffer
 _RETIRED = []  # outgrown buffers stay allocated: a captured HIP graph may still point into them
@@ -305,6 +307,54 @@ def norm_modulate(x: torch.Tensor, gamma: torch.Tensor, beta: Optional[torch.Ten
     return out
 
 
+NORM_GRAD = struct.Struct("=11Q9qd")  # struct aeris_norm_modulate_grad of include/aeris_hip.h
+
+
+def _scratch_ptr(nbytes: int, device):
+    """Device memory for one call, in the order of the current stream (under a capture: of the graph) like any tensor: calls on several
+    streams, and graphs replayed beside each other, do not meet in it.  -> (the tensor, to be held until the call is made, its address)"""
+    t = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    return t, _ptr(t)
+
+
+def norm_modulate_backward(dy: torch.Tensor, x: torch.Tensor, gamma: torch.Tensor, beta: Optional[torch.Tensor] = None,
+                           shift: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None, *, kind: str = "layernorm",
+                           order: str = "norm_then_mod", eps: float = 1e-5, wanted=(True, True, True, True, True)):
+    """Gradients of ``norm_modulate`` from that of its result, dy [B, S, d] (bf16 | f32) -> (dx, dgamma, dbeta, dshift, dscale), each in its
+    tensor's shape and type; None where ``wanted`` says so or the tensor is absent.  Statistics and sums in fp32, in a fixed order."""
+    _on_current_device(x.device, dict(x=x, dy=dy, gamma=gamma, beta=beta, shift=shift, scale=scale))
+    _dev(x, "x")
+    _dev(dy, "dy")
+    if x.dim() != 3 or dy.shape != x.shape:
+        raise RuntimeError(f"x and dy must be [B, S, d], got {tuple(x.shape)} and {tuple(dy.shape)}")
+    B, S, d = x.shape
+    _dev(gamma, "gamma")
+    if gamma.dtype not in _DT or gamma.shape != (d,) or x.dtype not in _DT or dy.dtype not in _DT:
+        raise RuntimeError(f"x, dy and gamma must be bf16 or f32, gamma [{d}]")
+    if beta is not None:
+        _dev(beta, "beta", gamma.dtype)
+        if beta.shape != (d,):
+            raise RuntimeError(f"beta must be [{d}], got {tuple(beta.shape)}")
+    sh_ptr, st1 = _rowvec(shift, "shift", d, B)
+    sc_ptr, st2 = _rowvec(scale, "scale", d, B)
+    if shift is not None and scale is not None and (st1 != st2 or shift.shape != scale.shape):
+        raise RuntimeError("shift and scale must share their shape and batch stride")
+    mod = shift if shift is not None else scale
+    if mod is not None and mod.shape[0] > 1 and max(st1, st2) == 0:
+        raise RuntimeError("shift and scale of several members must have memory of their own for each")
+    tensors = (x, gamma, beta, shift, scale)
+    if x.numel() == 0:
+        return tuple(torch.zeros_like(t, memory_format=torch.contiguous_format) if w and t is not None else None for t, w in zip(tensors, wanted))
+    out = tuple(torch.empty_like(t, memory_format=torch.contiguous_format) if w and t is not None else None for t, w in zip(tensors, wanted))
+    call = NORM_GRAD.pack(x.data_ptr(), dy.data_ptr(), gamma.data_ptr(), _ptr(beta) or 0, sh_ptr or 0, sc_ptr or 0, *(_ptr(t) or 0 for t in out),
+                          B, S, d, max(st1, st2), _DT[x.dtype], _DT[dy.dtype], _DT[gamma.dtype], _KIND[kind], _ORDER[order], eps)
+    need = L.lib().aeris_norm_modulate_grad_workspace_bytes(call)
+    held, ws = _scratch_ptr(need, x.device)
+    with _timed("norm_modulate_backward", float(x.numel() * (2 * x.element_size() + dy.element_size())), "byte"):
+        L.call("aeris_norm_modulate_bwd", call, ws, need, _stream())
+    return out
+
+
 def output_stage_supported(N: int, d: int, B_mod: int, rows_per_batch: int) -> bool:
     return L.lib().aeris_output_stage_workspace_bytes(N, d, max(B_mod, 1)) > 0 and (B_mod <= 1 or rows_per_batch % 64 == 0)
 
@@ -423,6 +473,141 @@ def gemm_heads(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], h
         L.call("aeris_gemm_heads_fwd", a.data_ptr(), w.data_ptr(), out.data_ptr(), _ptr(bias), M, N, K, head_dim,
                M * head_dim, float(q_scale), int(q_planes), _stream())
     return out
+
+
+LINEAR_TRAIN = struct.Struct("=6Q6q")  # struct aeris_linear_train of include/aeris_hip.h
+LINEAR_GRAD = struct.Struct("=8Q5q")  # struct aeris_linear_grad
+FEED_FORWARD = struct.Struct("=6Q3q")  # struct aeris_feed_forward
+FEED_FORWARD_GRAD = struct.Struct("=9Q3q")  # struct aeris_feed_forward_grad
+_KEPT = (L.ACT_GELU, L.ACT_SILU)  # activations whose gradient needs the value they were applied to
+
+
+def _matrix(t, name, rows, cols, dtypes=(torch.bfloat16,)):
+    """A contiguous matrix [.., cols] of so many rows on the GPU."""
+    if not t.is_cuda or not t.is_contiguous() or t.dtype not in dtypes or t.dim() < 1 or t.shape[-1] != cols or t.numel() != rows * cols:
+        _dev(t, name)
+        raise RuntimeError(f"{name} must be {' | '.join(map(str, dtypes))} [{rows}, {cols}], got {t.dtype} {tuple(t.shape)}")
+    return t
+
+
+def _train_widths(*widths):
+    for n in widths:
+        if n <= 0 or n % 8:
+            raise RuntimeError(f"widths must be positive multiples of 8 for the gradients' products, got {n}")
+
+
+def linear_train(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *, act: Optional[str] = None,
+                 residual: Optional[torch.Tensor] = None, out_dtype=torch.bfloat16):
+    """``gemm`` of a training step: (act(a[.., K] @ w[N, K]^T + bias) + residual [.., N] in out_dtype, what ``linear_backward`` needs beside a and w: the
+    bf16 value that the activation was applied to, or None without activation).  K, N multiples of 8 (without activation: K of 64)."""
+    if act not in (None, "none", "gelu", "silu"):
+        raise RuntimeError(f"act must be None, 'gelu' or 'silu', got {act!r}")
+    _on_current_device(a.device, dict(a=a, w=w, bias=bias, residual=residual))
+    if w.dim() != 2 or a.dim() < 1:
+        raise RuntimeError(f"a must be [.., K] and w [N, K], got {tuple(a.shape)} and {tuple(w.shape)}")
+    N, K = w.shape
+    _train_widths(N, K)
+    M = a.numel() // K
+    _matrix(a, "a", M, K)
+    _matrix(w, "w", N, K)
+    if out_dtype not in _DT:
+        raise RuntimeError("out_dtype must be bf16 or f32")
+    if bias is not None and bias.shape != (N,):
+        raise RuntimeError(f"bias must be [{N}], got {tuple(bias.shape)}")
+    if residual is not None:
+        _matrix(residual, "residual", M, N, tuple(_DT))
+    shape = (*a.shape[:-1], N)
+    if M == 0:
+        return torch.empty(shape, dtype=out_dtype, device=a.device), None if _ACT[act] not in _KEPT else torch.empty(shape, dtype=torch.bfloat16, device=a.device)
+    if _ACT[act] not in _KEPT:
+        return gemm(a, w, bias, residual=residual, out_dtype=out_dtype), None
+    if bias is not None:
+        _dev(bias, "bias", torch.bfloat16)
+    y, z = torch.empty(shape, dtype=out_dtype, device=a.device), torch.empty(shape, dtype=torch.bfloat16, device=a.device)
+    with _timed("linear_train", 2.0 * M * N * K, "flop"):
+        L.call("aeris_linear_train_fwd", LINEAR_TRAIN.pack(a.data_ptr(), w.data_ptr(), _ptr(bias) or 0, _ptr(residual) or 0, y.data_ptr(), z.data_ptr(), M, N, K,
+                                                           _ACT[act], 0 if residual is None else _DT[residual.dtype], _DT[out_dtype]), _stream())
+    return y, z
+
+
+def linear_backward(dy: torch.Tensor, a: torch.Tensor, w: torch.Tensor, z: Optional[torch.Tensor] = None, *, act: Optional[str] = None,
+                    wanted=(True, True, True, True)):
+    """Gradients of ``linear_train`` from that of its result, dy [.., N] (bf16 | f32) -> (da bf16, dw bf16, dbias bf16 [N], dz bf16 [.., N]), None where
+    ``wanted`` says so.  dz = dy act'(z) is rounded to bf16 for the products; dbias sums it unrounded.  (dz without activation: dy in bf16.)"""
+    _on_current_device(dy.device, dict(dy=dy, a=a, w=w, z=z))
+    N, K = w.shape
+    _train_widths(N, K)
+    M = a.numel() // K
+    _matrix(a, "a", M, K)
+    _matrix(w, "w", N, K)
+    _matrix(dy, "dy", M, N, tuple(_DT))
+    kept = _ACT[act] in _KEPT
+    if kept:
+        if z is None:
+            raise RuntimeError("an activation's gradient needs z")
+        _matrix(z, "z", M, N)
+    elif _ACT[act] != L.ACT_NONE:
+        raise RuntimeError(f"act must be None, 'gelu' or 'silu', got {act!r}")
+    bf16, device = torch.bfloat16, dy.device
+    same = not kept and dy.dtype is bf16  # dz is dy
+    if M == 0:
+        return (torch.empty_like(a) if wanted[0] else None, torch.zeros_like(w) if wanted[1] else None,
+                torch.zeros(N, dtype=bf16, device=device) if wanted[2] else None, dy.to(bf16) if wanted[3] else None)
+    da = torch.empty_like(a) if wanted[0] else None
+    dw = torch.empty_like(w) if wanted[1] else None
+    dbias = torch.empty(N, dtype=bf16, device=device) if wanted[2] else None
+    dz = torch.empty(dy.shape, dtype=bf16, device=device) if wanted[3] and not same else None
+    if not (da is None and dw is None and dbias is None and dz is None):
+        call = LINEAR_GRAD.pack(dy.data_ptr(), a.data_ptr(), w.data_ptr(), z.data_ptr() if kept else 0, _ptr(da) or 0, _ptr(dw) or 0, _ptr(dbias) or 0, _ptr(dz) or 0,
+                                M, N, K, _ACT[act], _DT[dy.dtype])
+        need = L.lib().aeris_linear_grad_workspace_bytes(call)
+        held, ws = _scratch_ptr(need, device)
+        with _timed("linear_backward", 2.0 * M * N * K * ((da is not None) + (dw is not None)), "flop"):
+            L.call("aeris_linear_bwd", call, ws, need, _stream())
+    return da, dw, dbias, dy if wanted[3] and same else dz
+
+
+def feed_forward_train(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor):
+    """The gated MLP of a training step, w2[d, H] (silu(gate) * up) with [gate | up] = x[.., d] @ w1[2H, d]^T -> (y bf16 [.., d], gate_up bf16 [.., 2H],
+    h bf16 [.., H]): the result and what ``feed_forward_backward`` needs beside x, w1 and w2.  d, H multiples of 8."""
+    _on_current_device(x.device, dict(x=x, w1=w1, w2=w2))
+    if w2.dim() != 2 or w1.dim() != 2 or x.dim() < 1:
+        raise RuntimeError(f"x must be [.., d], w1 [2H, d] and w2 [d, H], got {tuple(x.shape)}, {tuple(w1.shape)} and {tuple(w2.shape)}")
+    d, H = w2.shape
+    _train_widths(d, H)
+    M = x.numel() // d
+    _matrix(x, "x", M, d)
+    _matrix(w1, "w1", 2 * H, d)
+    _matrix(w2, "w2", d, H)
+    y = torch.empty_like(x)
+    gate_up = torch.empty(*x.shape[:-1], 2 * H, dtype=torch.bfloat16, device=x.device)
+    h = torch.empty(*x.shape[:-1], H, dtype=torch.bfloat16, device=x.device)
+    if M:
+        with _timed("feed_forward_train", 6.0 * M * H * d, "flop"):
+            L.call("aeris_feed_forward_train_fwd", FEED_FORWARD.pack(x.data_ptr(), w1.data_ptr(), w2.data_ptr(), gate_up.data_ptr(), h.data_ptr(), y.data_ptr(), M, d, H), _stream())
+    return y, gate_up, h
+
+
+def feed_forward_backward(dy: torch.Tensor, x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, gate_up: torch.Tensor, h: torch.Tensor, *,
+                          wanted=(True, True, True)):
+    """Gradients of ``feed_forward_train`` from that of its result, dy bf16 [.., d] -> (dx, dw1, dw2) bf16, None where ``wanted`` says so."""
+    _on_current_device(dy.device, dict(dy=dy, x=x, w1=w1, w2=w2, gate_up=gate_up, h=h))
+    d, H = w2.shape
+    _train_widths(d, H)
+    M = x.numel() // d
+    for t, name, rows, cols in ((x, "x", M, d), (w1, "w1", 2 * H, d), (w2, "w2", d, H), (dy, "dy", M, d), (gate_up, "gate_up", M, 2 * H), (h, "h", M, H)):
+        _matrix(t, name, rows, cols)
+    if M == 0:
+        return tuple(torch.zeros_like(t) if w else None for t, w in zip((x, w1, w2), wanted))
+    dx, dw1, dw2 = (torch.empty_like(t) if w else None for t, w in zip((x, w1, w2), wanted))
+    if any(wanted):
+        call = FEED_FORWARD_GRAD.pack(dy.data_ptr(), x.data_ptr(), w1.data_ptr(), w2.data_ptr(), gate_up.data_ptr(), h.data_ptr(), _ptr(dx) or 0, _ptr(dw1) or 0,
+                                      _ptr(dw2) or 0, M, d, H)
+        need = L.lib().aeris_feed_forward_grad_workspace_bytes(call)
+        held, ws = _scratch_ptr(need, x.device)
+        with _timed("feed_forward_backward", 2.0 * M * H * d * (bool(wanted[0] or wanted[1]) + 2 * wanted[0] + 2 * wanted[1] + wanted[2]), "flop"):
+            L.call("aeris_feed_forward_bwd", call, ws, need, _stream())
+    return dx, dw1, dw2
 
 
 def _on_current_device(device, tensors):

@@ -133,6 +133,26 @@ int aeris_norm_modulate_fwd(const void* x, int x_dtype, void* y, int y_dtype, co
                             int64_t B, int64_t rows_per_batch, int d, int kind, int order, float eps,
                             void* stream);
 
+/* Gradients of aeris_norm_modulate_fwd from that of its result.  x, gamma, beta, shift, scale, kind, order, eps, mod_batch_stride as there;
+ * dy [B*rows_per_batch, d] (dy_dtype bf16|f32).  Written, each unless NULL:
+ *   dx [B*rows_per_batch, d] (x_dtype); dgamma, dbeta [d] (param_dtype; dbeta needs beta); dshift, dscale f32 [B_mod, d], contiguous
+ *   (they need shift / scale; B_mod = B where mod_batch_stride is not 0, otherwise 1: the sum over the batch)
+ * Statistics and sums in fp32, added in an order that depends on the sizes alone.  dx may be dy or x where their types agree, and may
+ * otherwise not overlap them.  x, dy, dx, gamma, beta, shift, scale 16-byte aligned.  Supported: d % 8 == 0, d <= 6144.
+ * workspace: device memory of aeris_norm_modulate_grad_workspace_bytes(a) bytes (0 if only dx is asked for; a's addresses do not count but
+ * for being NULL), 16-byte aligned, borrowed for the call.  The reference trains this Norm and modulation by autograd (model.py:121-125,
+ * 400-401,426). */
+typedef struct aeris_norm_modulate_grad {
+  const void *x, *dy, *gamma, *beta;
+  const float *shift, *scale;
+  void *dx, *dgamma, *dbeta;
+  float *dshift, *dscale;
+  int64_t B, rows_per_batch, d, mod_batch_stride, x_dtype, dy_dtype, param_dtype, kind, order;
+  double eps;
+} aeris_norm_modulate_grad;
+int64_t aeris_norm_modulate_grad_workspace_bytes(const aeris_norm_modulate_grad* a);
+int aeris_norm_modulate_bwd(const aeris_norm_modulate_grad* a, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Output stage in one pass: out f32 [B*rows_per_batch, N] = head_w * modulate(norm(x), shift, scale)
  *   x [B*rows_per_batch, d] (x_dtype bf16|f32); gamma [d], beta [d] or NULL (param_dtype); shift, scale f32
  *   [B_mod, d] or NULL (mod_batch_stride as for aeris_norm_modulate_fwd); head_w f32 [N, d] (nn.Linear layout, no bias)
@@ -179,6 +199,51 @@ int aeris_output_stage_noalloc_fwd(const void* x, int x_dtype, const void* gamma
 int aeris_gemm_fwd(const void* A, const void* W, void* C, const void* bias, const float* gate,
                    const void* residual, int64_t M, int N, int K, int64_t ldc, int act, int res_dtype,
                    int c_dtype, int64_t gate_batch_stride, int64_t rows_per_batch, void* stream);
+
+/* A projection of a training step (nn.Linear at model.py:153-154,284-285 with what follows it), for activations whose gradient needs the value they
+ * were applied to:
+ *   z = x w^T + bias (bf16, kept for the backward pass), y = act(z in fp32) + residual
+ *   x bf16 [M, K], w bf16 [N, K], bias bf16 [N] or NULL, residual [M, N] (res_dtype) or NULL, y [M, N] (y_dtype); act AERIS_ACT_GELU (erf) | AERIS_ACT_SILU
+ * (without an activation nothing has to be kept: aeris_gemm_fwd).
+ * Gradients, from that of y (dy [M, N], dy_dtype):  dz = dy act'(z) (rounded to bf16 for the products), written unless NULL:
+ *   dx bf16 [M, K] = dz w;  dw bf16 [N, K] = dz^T x;  dbias bf16 [N] = the sums of the unrounded dz;  dz bf16 [M, N] itself (act AERIS_ACT_NONE and an
+ *   f32 dy: dy rounded, what a bf16 residual gets); w may be NULL without dx, x without dw, z with AERIS_ACT_NONE
+ * Sums in fp32, added in an order that depends on the sizes alone.  Outputs share no memory with inputs.  Every tensor contiguous and 16-byte aligned.
+ * Supported: N % 8 == 0, K % 8 == 0, N, K <= 2^20, N * K < 2^30.  workspace: aeris_linear_grad_workspace_bytes(a) bytes (addresses do not count but for being
+ * NULL), 16-byte aligned, borrowed for the call. */
+typedef struct aeris_linear_train {
+  const void *x, *w, *bias, *residual;
+  void *y, *z;
+  int64_t M, N, K, act, res_dtype, y_dtype;
+} aeris_linear_train;
+int aeris_linear_train_fwd(const aeris_linear_train* a, void* stream);
+typedef struct aeris_linear_grad {
+  const void *dy, *x, *w, *z;
+  void *dx, *dw, *dbias, *dz;
+  int64_t M, N, K, act, dy_dtype;
+} aeris_linear_grad;
+int64_t aeris_linear_grad_workspace_bytes(const aeris_linear_grad* a);
+int aeris_linear_bwd(const aeris_linear_grad* a, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The gated MLP (FeedForward, model.py:148-159) of a training step:
+ *   [gate | up] = x w1^T (bf16 [M, 2H], kept), h = silu(gate) up (bf16 [M, H], kept), y bf16 [M, d] = h w2^T
+ *   x bf16 [M, d], w1 bf16 [2H, d], w2 bf16 [d, H]; gate, up and their product are made in fp32 in one kernel
+ * Gradients, from dy bf16 [M, d], each unless NULL:  dh = dy w2 (fp32, never in memory), dgate = dh up silu'(gate), dup = dh silu(gate) (bf16);
+ *   dx bf16 [M, d] = [dgate | dup] w1;  dw1 bf16 [2H, d] = [dgate | dup]^T x;  dw2 bf16 [d, H] = dy^T h
+ * Otherwise as above.  Supported: d % 8 == 0, H % 8 == 0, d, H <= 2^19, d * H < 2^29. */
+typedef struct aeris_feed_forward {
+  const void *x, *w1, *w2;
+  void *gate_up, *h, *y;
+  int64_t M, d, H;
+} aeris_feed_forward;
+int aeris_feed_forward_train_fwd(const aeris_feed_forward* a, void* stream);
+typedef struct aeris_feed_forward_grad {
+  const void *dy, *x, *w1, *w2, *gate_up, *h;
+  void *dx, *dw1, *dw2;
+  int64_t M, d, H;
+} aeris_feed_forward_grad;
+int64_t aeris_feed_forward_grad_workspace_bytes(const aeris_feed_forward_grad* a);
+int aeris_feed_forward_bwd(const aeris_feed_forward_grad* a, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* C = A[M,K] * W[N,K]^T + bias written as N / head_dim planes of bf16 [M, head_dim], plane j = columns
  * [j*head_dim, (j+1)*head_dim), the planes plane_stride elements apart (>= M * head_dim, multiple of 8).
