@@ -41,7 +41,8 @@ SIGNATURES = {
     "aeris_linear_train_fwd": (_c_int, [_c_vp, _c_vp]),
     "aeris_linear_grad_workspace_bytes": (_c_i64, [_c_vp]),
     "aeris_linear_bwd": (_c_int, [_c_vp, _c_vp, _c_i64, _c_vp]),
-    "aeris_feed_forward_train_fwd": (_c_int, [_c_vp, _c_vp]),
+    "aeris_feed_forward_workspace_bytes": (_c_i64, [_c_vp]),
+    "aeris_feed_forward_train_fwd": (_c_int, [_c_vp, _c_vp, _c_i64, _c_vp]),
     "aeris_feed_forward_grad_workspace_bytes": (_c_i64, [_c_vp]),
     "aeris_feed_forward_bwd": (_c_int, [_c_vp, _c_vp, _c_i64, _c_vp]),
     "aeris_output_stage_workspace_bytes": (_c_i64, [_c_int, _c_int, _c_int]),

@@ -45,6 +45,7 @@ int ensure_init(void* stream = nullptr, bool from_launch = false) {
     if (g_init_status == hipSuccess) g_init_status = aeris::input_stage_configure();
     if (g_init_status == hipSuccess) g_init_status = aeris::qkv_attention_configure();
     if (g_init_status == hipSuccess) g_init_status = aeris::cross_attention_configure();
+    if (g_init_status == hipSuccess) g_init_status = aeris::gemm_grad_configure();
     g_init_done.store(true, std::memory_order_release);
   });
   if (g_init_status == hipSuccess && !from_launch) {
@@ -423,12 +424,13 @@ int train_workspace(const char* who, const void* workspace, int64_t have, int64_
 
 int aeris_linear_train_fwd(const aeris_linear_train* a, void* stream) {
   const char* who = "aeris_linear_train_fwd";
-  if (!a || !a->x || !a->w || !a->y || !a->z) return fail(AERIS_EINVAL, "%s: x/w/y/z is NULL", who);
+  if (!a || !a->x || !a->w || !a->y) return fail(AERIS_EINVAL, "%s: x/w/y is NULL", who);
   if (int rc = train_sizes(who, a->M, a->N, a->K)) return rc;
   if (a->act != AERIS_ACT_GELU && a->act != AERIS_ACT_SILU) return fail(AERIS_EINVAL, "%s: activation must be AERIS_ACT_GELU or AERIS_ACT_SILU", who);
   if ((a->y_dtype != AERIS_BF16 && a->y_dtype != AERIS_F32) || (a->residual && a->res_dtype != AERIS_BF16 && a->res_dtype != AERIS_F32))
     return fail(AERIS_EINVAL, "%s: dtype must be AERIS_BF16 or AERIS_F32", who);
   if (int rc = train_aligned(who, {a->x, a->w, a->bias, a->residual, a->y, a->z})) return rc;
+  if (int rc = ensure_init(stream, true)) return rc;
   hipError_t e = aeris::linear_train_launch(*a, reinterpret_cast<hipStream_t>(stream));
   return e == hipSuccess ? AERIS_OK : hip_fail(e, who);
 }
@@ -447,17 +449,24 @@ int aeris_linear_bwd(const aeris_linear_grad* a, void* workspace, int64_t worksp
   if (a->dz && a->act == AERIS_ACT_NONE && a->dy_dtype == AERIS_BF16) return fail(AERIS_EINVAL, "%s: dz is dy itself", who);
   if (int rc = train_aligned(who, {a->dy, a->x, a->w, a->z, a->dx, a->dw, a->dbias, a->dz})) return rc;
   if (int rc = train_workspace(who, workspace, workspace_bytes, aeris::linear_grad_workspace_bytes(*a))) return rc;
+  if (int rc = ensure_init(stream, true)) return rc;
   hipError_t e = aeris::linear_grad_launch(*a, workspace, reinterpret_cast<hipStream_t>(stream));
   return e == hipSuccess ? AERIS_OK : hip_fail(e, who);
 }
 
-int aeris_feed_forward_train_fwd(const aeris_feed_forward* a, void* stream) {
+int64_t aeris_feed_forward_workspace_bytes(const aeris_feed_forward* a) {
+  return a && a->H > 0 && a->H <= 1 << 19 && a->H % 8 == 0 && train_sizes_ok(a->M, 2 * a->H, a->d) ? aeris::feed_forward_train_workspace_bytes(*a) : 0;
+}
+
+int aeris_feed_forward_train_fwd(const aeris_feed_forward* a, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* who = "aeris_feed_forward_train_fwd";
-  if (!a || !a->x || !a->w1 || !a->w2 || !a->gate_up || !a->h || !a->y) return fail(AERIS_EINVAL, "%s: a tensor is NULL", who);
+  if (!a || !a->x || !a->w1 || !a->w2 || !a->h || !a->y) return fail(AERIS_EINVAL, "%s: a tensor is NULL", who);
   if (int rc = train_sizes(who, a->M, a->H > 0 && a->H <= 1 << 19 ? 2 * a->H : a->H > 0 ? 1 << 30 : 0, a->d)) return rc;
   if (int rc = train_aligned(who, {a->x, a->w1, a->w2, a->gate_up, a->h, a->y})) return rc;
   if (a->H % 8) return fail(AERIS_EUNSUPPORTED, "%s: H=%lld must be a multiple of 8", who, (long long)a->H);
-  hipError_t e = aeris::feed_forward_train_launch(*a, reinterpret_cast<hipStream_t>(stream));
+  if (int rc = train_workspace(who, workspace, workspace_bytes, aeris::feed_forward_train_workspace_bytes(*a))) return rc;
+  if (int rc = ensure_init(stream, true)) return rc;
+  hipError_t e = aeris::feed_forward_train_launch(*a, workspace, reinterpret_cast<hipStream_t>(stream));
   return e == hipSuccess ? AERIS_OK : hip_fail(e, who);
 }
 
@@ -473,6 +482,7 @@ int aeris_feed_forward_bwd(const aeris_feed_forward_grad* a, void* workspace, in
   if (a->H % 8) return fail(AERIS_EUNSUPPORTED, "%s: H=%lld must be a multiple of 8", who, (long long)a->H);
   if (int rc = train_aligned(who, {a->dy, a->x, a->w1, a->w2, a->gate_up, a->h, a->dx, a->dw1, a->dw2})) return rc;
   if (int rc = train_workspace(who, workspace, workspace_bytes, aeris::feed_forward_grad_workspace_bytes(*a))) return rc;
+  if (int rc = ensure_init(stream, true)) return rc;
   hipError_t e = aeris::feed_forward_grad_launch(*a, workspace, reinterpret_cast<hipStream_t>(stream));
   return e == hipSuccess ? AERIS_OK : hip_fail(e, who);
 }

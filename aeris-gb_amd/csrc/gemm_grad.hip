@@ -35,15 +35,35 @@ struct GradGemm {
   void* C;           // SWIGLU: h; SWIGLU_BWD: [dgate | dup]
   int64_t ldc;
   int c_f32;
-  int64_t k_per_split, split_stride;  // columns k of one part (a multiple of 64); elements between the parts' results
   const uint16_t* bias;
   const void* residual;
-  int res_dtype;  // -1: none
-  uint16_t* saved;  // ACT: z; SWIGLU: [gate | up], rows of 2 N
-  const uint16_t* gate_up;  // SWIGLU_BWD
+  int res_dtype;   // -1: none
+  uint16_t* kept;  // 24-bit values: ACT: z; SWIGLU, SWIGLU_BWD: [gate | up], rows of 2 N
   int act;
-  int tiles_m, tiles_n;
+  // tiles are numbered four row panels times all column tiles at a time; the first `whole` of them are made in one go, k of each of the
+  // others is cut into `parts` of k_part (a multiple of 64), summed from `partial` ([tile - whole][part][rows][columns], fp32) by another kernel
+  int tiles_m, tiles_n, whole, parts;
+  int64_t k_part;
+  float* partial;
+  float* row_sums;  // of A, over k: [tile_m][tile_n][part][rows] (each column tile has every tiles_n-th k-tile), or NULL
 };
+
+struct TileAt { int m, n; };
+__device__ __forceinline__ TileAt tile_at(int tile, int tiles_m, int tiles_n) {
+  const int grp = tile / (4 * tiles_n), within = tile - grp * 4 * tiles_n;
+  int gm = tiles_m - grp * 4;
+  if (gm > 4) gm = 4;
+  TileAt t;
+  t.n = within / gm;
+  t.m = grp * 4 + within - t.n * gm;
+  return t;
+}
+__device__ __forceinline__ int tile_number(int m, int n, int tiles_m, int tiles_n) {
+  const int grp = m / 4;
+  int gm = tiles_m - grp * 4;
+  if (gm > 4) gm = 4;
+  return grp * 4 * tiles_n + n * gm + m - grp * 4;
+}
 
 __device__ __forceinline__ float sigmoid_f(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
 // d/dx of x sigma(x)
@@ -80,6 +100,32 @@ __device__ __forceinline__ void store8(void* C, int f32, int64_t at, const float
   } else {
     *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(C) + at) = narrow8(o);
   }
+}
+
+// Values kept for the backward pass have 24 bits: sign, exponent and 15 bits of the fraction of an fp32 number, rounded to nearest, halves
+// away from zero (2^-16 relative; bf16 would be one more rounding of 2^-9 in every gradient behind it, as large as that of the operand it
+// ends in, and fp16 has not the range).  The upper 16 bits of all values lie in front, the lower 8 bits behind them.  Adding half a step to
+// the bits is all the rounding: a NaN here has come out of bf16 numbers or of the arithmetic itself, with zeros in its lower half, and stays one.
+__device__ __forceinline__ void store_kept8(uint16_t* kept, int64_t count, int64_t at, const float (&v)[8]) {
+  uint32_t b[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) b[e] = __float_as_uint(v[e]) + 0x80u;
+  u32x4 hi;
+  u32x2 lo;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) hi[e] = __builtin_amdgcn_perm(b[2 * e + 1], b[2 * e], 0x07060302u);
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    lo[e] = __builtin_amdgcn_perm(b[4 * e + 1], b[4 * e], 0x0c0c0501u) | __builtin_amdgcn_perm(b[4 * e + 3], b[4 * e + 2], 0x05010c0cu);
+  *reinterpret_cast<u32x4*>(kept + at) = hi;
+  *reinterpret_cast<u32x2*>(reinterpret_cast<uint8_t*>(kept + count) + at) = lo;
+}
+__device__ __forceinline__ void load_kept8(const uint16_t* kept, int64_t count, int64_t at, float (&v)[8]) {
+  const u32x4 hi = *reinterpret_cast<const u32x4*>(kept + at);
+  const u32x2 lo = *reinterpret_cast<const u32x2*>(reinterpret_cast<const uint8_t*>(kept + count) + at);
+#pragma unroll
+  for (int e = 0; e < 8; ++e)  // byte 0: zero, 1: of lo, 2 and 3: of hi
+    v[e] = __uint_as_float(__builtin_amdgcn_perm(hi[e >> 1], lo[e >> 2], ((e & 1) ? 0x0706000cu : 0x0504000cu) | (uint32_t)(e & 3) << 8));
 }
 
 // ---- operand panels in LDS
@@ -159,7 +205,7 @@ struct Loader {
       static_assert(RPI != 4 || P::LOADS % 4 == 0, "bit 3 of k follows from the number within the wave");
       static_assert(RPI != 8 || P::LOADS % 2 == 0, "bit 3 of k follows from the number within the wave");
     } else {
-      const bool tail = left < BK;
+      const uint32_t left32 = left < BK ? (uint32_t)left : (uint32_t)BK;
       const int64_t all = SWIGLU_ROWS ? up_rows + rows : rows < ROWS ? rows : ROWS;
       const uint32_t bytes = left > 0 ? (uint32_t)(all * ld * 2) : 0u;
       const lds_dma_rsrc rs = make_lds_dma_rsrc(base, bytes);
@@ -171,7 +217,7 @@ struct Loader {
         static_assert(P::LOADS % 2 == 0, "the parity of 8-row blocks follows from the number within the wave");
         uint32_t vo = voff[j & 1];
         // (k beyond the matrix: an offset beyond any buffer's size, which arrives as zeros)
-        if (tail && kchunk[j & 1] >= (uint32_t)left) vo = 0x80000000u;
+        if (kchunk[j & 1] >= left32) vo = 0x80000000u;
         lds_dma_load16(rs, stage + (uint32_t)i * 1024u, vo, (uint32_t)(row * ld * 2) + (uint32_t)(k0 * 2));
       }
     }
@@ -224,111 +270,157 @@ struct Fragments {
   }
 };
 
-// ---- epilogue of a wave's FM x FN fragments, rows from row0, columns from col0.  A lane has 4 consecutive columns 4 q .. of row
-// l15 of a fragment; a swap between lane rows of two neighbouring column fragments gives it 8 consecutive ones.
-template <int FM, int FN>
-__device__ __forceinline__ void eight_columns(const f32x4 (&a)[FN], int m, float (&o)[8]) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a[2 * m][e]), __float_as_uint(a[2 * m + 1][e]), false, false);
-    o[e] = __uint_as_float(r[0]);
-    o[4 + e] = __uint_as_float(r[1]);
-  }
-}
-
-template <int EPI, int FM, int FN>
-__device__ __forceinline__ void grad_epilogue(const GradGemm& p, const f32x4 (&acc)[FM][FN], int64_t row0, int col0, int split, int lane) {
+// ---- epilogue of a wave's FM x FN fragments of one item; rows from row0, columns from col0 of the result, or of the item's part of
+// `partial`.  16 rows at a time pass through 16 x FN x 16 floats of the wave's own LDS (16-byte chunks XOR-swizzled by the row), so that a
+// lane has 8 consecutive columns of a row and memory is written and read in whole row segments of the wave's width.
+template <int T, int EPI, int FM, int FN>
+__device__ __forceinline__ void grad_epilogue(const GradGemm& p, const f32x4 (&acc)[FM][FN], int64_t row0, int col0, float* part, uint32_t stage, int lane_) {
+  typedef __attribute__((address_space(3))) f32x4* lds4;
+  int lane = lane_;
+  asm volatile("" : "+v"(lane));  // what follows from the lane number is made anew here and kept out of the main loop's registers
   const int l15 = lane & 15, q = lane >> 4;
-  constexpr int NP = (EPI == EPI_SWIGLU ? FN / 2 : FN) / 2;  // column pairs of the result
+  constexpr int CH = FN * 4;                                          // chunks of a staged row
+  constexpr int CHUNKS = (EPI == EPI_SWIGLU ? FN / 2 : FN) * 2;       // of 8 columns of the result
+  constexpr int RPI = 64 / CHUNKS < 16 ? 64 / CHUNKS : 16, ITS = 16 / RPI;  // rows at a time
+  const int rrow = lane / CHUNKS, rch = lane % CHUNKS;
+  const int col = col0 + rch * 8;
+  const bool col_ok = part != nullptr || col < p.N;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
-    const int64_t row = row0 + 16 * i + l15;
 #pragma unroll
-    for (int m = 0; m < NP; ++m) {
-      const int col = col0 + 32 * m + 16 * (q & 1) + 8 * (q >> 1);
+    for (int j = 0; j < FN; ++j) *(lds4)(uintptr_t)(stage + l15 * (CH * 16) + (((j * 4 + q) ^ (l15 & (CH - 1))) << 4)) = acc[i][j];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int it = 0; it < ITS; ++it) {
+      const int r = rrow + it * RPI;
+      auto eight = [&](int c, float (&o)[8]) {
+        const f32x4 a = *(lds4)(uintptr_t)(stage + r * (CH * 16) + (((2 * c) ^ (r & (CH - 1))) << 4));
+        const f32x4 b = *(lds4)(uintptr_t)(stage + r * (CH * 16) + (((2 * c + 1) ^ (r & (CH - 1))) << 4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          o[e] = a[e];
+          o[4 + e] = b[e];
+        }
+      };
       float o[8];
-      eight_columns<FM, FN>(acc[i], m, o);
-      if constexpr (EPI == EPI_SWIGLU) {
+      eight(rch, o);
+      const int64_t row = row0 + 16 * i + r;
+      if (EPI == EPI_STORE && part != nullptr) {
+        store8(part, 1, row * T + col, o);
+        continue;
+      }
+      const bool ok = col_ok && row < p.M;
+      if constexpr (EPI == EPI_STORE) {
+        if (ok) store8(p.C, p.c_f32, row * p.ldc + col, o);
+      } else if constexpr (EPI == EPI_SWIGLU) {
         float up[8];
-        eight_columns<FM, FN>(acc[i], m + NP, up);
-        if (row >= p.M || col >= p.N) continue;
-        uint16_t* s = p.saved + row * (2 * (int64_t)p.N) + col;
-        *reinterpret_cast<u32x4*>(s) = narrow8(o);
-        *reinterpret_cast<u32x4*>(s + p.N) = narrow8(up);
+        eight(rch + CHUNKS, up);
+        if (ok) {
+          const int64_t at = row * (2 * (int64_t)p.N) + col, count = p.M * (2 * (int64_t)p.N);
+          if (p.kept) {
+            store_kept8(p.kept, count, at, o);
+            store_kept8(p.kept, count, at + p.N, up);
+          }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = silu_f(o[e]) * up[e];
-        store8(p.C, 0, row * p.ldc + col, o);
-      } else {
-        if (row >= p.M || col >= p.N) continue;
-        if constexpr (EPI == EPI_STORE) {
-          store8(p.C, p.c_f32, split * p.split_stride + row * p.ldc + col, o);
-        } else if constexpr (EPI == EPI_ACT) {
+          for (int e = 0; e < 8; ++e) o[e] = silu_f(o[e]) * up[e];
+          store8(p.C, 0, row * p.ldc + col, o);
+        }
+      } else if constexpr (EPI == EPI_ACT) {
+        if (ok) {
           if (p.bias) {
             float b[8];
             widen8(*reinterpret_cast<const u32x4*>(p.bias + col), b);
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] += b[e];
           }
-          *reinterpret_cast<u32x4*>(p.saved + row * (int64_t)p.N + col) = narrow8(o);
+          const int64_t at = row * (int64_t)p.N + col;
+          if (p.kept) store_kept8(p.kept, p.M * (int64_t)p.N, at, o);
 #pragma unroll
           for (int e = 0; e < 8; ++e) o[e] = p.act == AERIS_ACT_SILU ? silu_f(o[e]) : p.c_f32 ? gelu_erf_f(o[e]) : gelu_erf_bf16_f(o[e]);
           if (p.res_dtype >= 0) {
-            const int64_t at = row * (int64_t)p.N + col;
-            float r[8];
+            float x[8];
             if (p.res_dtype == AERIS_F32) {
               const float* src = reinterpret_cast<const float*>(p.residual) + at;
               const f32x4 a = *reinterpret_cast<const f32x4*>(src), b = *reinterpret_cast<const f32x4*>(src + 4);
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                r[e] = a[e];
-                r[4 + e] = b[e];
+                x[e] = a[e];
+                x[4 + e] = b[e];
               }
             } else {
-              widen8(*reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(p.residual) + at), r);
+              widen8(*reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(p.residual) + at), x);
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] += r[e];
+            for (int e = 0; e < 8; ++e) o[e] += x[e];
           }
-          store8(p.C, p.c_f32, row * p.ldc + col, o);
-        } else {  // EPI_SWIGLU_BWD
-          const int64_t at = row * (2 * (int64_t)p.N) + col;
-          float g[8], u[8], dg[8];
-          widen8(*reinterpret_cast<const u32x4*>(p.gate_up + at), g);
-          widen8(*reinterpret_cast<const u32x4*>(p.gate_up + at + p.N), u);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float s = sigmoid_f(g[e]);
-            dg[e] = o[e] * u[e] * dsilu_f(g[e], s);
-            o[e] *= g[e] * s;
-          }
-          store8(p.C, 0, at, dg);
-          store8(p.C, 0, at + p.N, o);
+          store8(p.C, p.c_f32, at, o);
         }
+      } else if (ok) {  // EPI_SWIGLU_BWD
+        const int64_t at = row * (2 * (int64_t)p.N) + col;
+        float g[8], u[8], dg[8];
+        load_kept8(p.kept, p.M * (2 * (int64_t)p.N), at, g);
+        load_kept8(p.kept, p.M * (2 * (int64_t)p.N), at + p.N, u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float s = sigmoid_f(g[e]);
+          dg[e] = o[e] * u[e] * dsilu_f(g[e], s);
+          o[e] *= g[e] * s;
+        }
+        store8(p.C, 0, at, dg);
+        store8(p.C, 0, at + p.N, o);
       }
     }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
+// the sums of A's rows over k that a wave has of its fragments (all four elements of a lane are the same): every fourth 16 lanes' first
+template <int T, int F>
+__device__ __forceinline__ void store_row_sums(const GradGemm& p, const f32x4 (&sums)[F], int tile_m, int tile_n, int part, int row, int lane) {
+  if (lane >= 16) return;
+  float* out = p.row_sums + (((int64_t)tile_m * p.tiles_n + tile_n) * p.parts + part) * T + row + lane;
+#pragma unroll
+  for (int f = 0; f < F; ++f) out[16 * f] = sums[f][0];
+}
+
+__device__ __forceinline__ bf16x8 all_ones() {
+  bf16x8 v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (__bf16)1.0f;
+  return v;
+}
+
 // ---- tiles of T x T (128 or 64), four waves two by two, two stages; two or more workgroups a CU fill each other's waits
+template <int T>
+constexpr int tile_lds() { return 2 * 2 * T * BK * 2; }
+
 template <int T, bool A_TR, bool B_TR, int EPI>
-__global__ void __launch_bounds__(256, 2) gemm_grad_tile_kernel(GradGemm p) {
-  constexpr bool SWIGLU = EPI == EPI_SWIGLU;
+__device__ __forceinline__ void grad_tile(const GradGemm& p, int item, unsigned char* smem) {
+  constexpr bool SWIGLU = EPI == EPI_SWIGLU, ROW_SUMS = A_TR;
   // waves over the tile: two by two; SwiGLU tiles of 64 four by one, so that a wave has a gate column's up column too
   constexpr int WN = SWIGLU && T == 64 ? 1 : 2, WM = 4 / WN;
   constexpr int FM = T / WM / 16, FN = T / WN / 16;  // fragments of a wave
+  constexpr int FS = ROW_SUMS ? FM / WN : 1;         // row fragments whose sums a wave has
   constexpr int BN_OUT = SWIGLU ? T / 2 : T;
   using PA = Panel<A_TR, T, 4>;
   using PB = Panel<B_TR, T, 4>;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * (PA::BYTES + PB::BYTES)];
+  static_assert(2 * (PA::BYTES + PB::BYTES) == tile_lds<T>(), "two stages");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
-  const int tiles = p.tiles_m * p.tiles_n;
-  const int split = blockIdx.x / tiles, tile = blockIdx.x - split * tiles;
-  const int tile_n = tile % p.tiles_n, tile_m = tile / p.tiles_n;
-  const int64_t m0 = (int64_t)tile_m * T;
-  const int n0 = tile_n * BN_OUT;
-  const int64_t k_begin = split * p.k_per_split;
-  int64_t k_end = k_begin + p.k_per_split;
+  int part = 0;
+  if (item >= p.whole) {
+    part = (item - p.whole) % p.parts;
+    item = p.whole + (item - p.whole) / p.parts;
+  }
+  const TileAt tile = tile_at(item, p.tiles_m, p.tiles_n);
+  const int64_t m0 = (int64_t)tile.m * T;
+  const int n0 = tile.n * BN_OUT;
+  const bool cut = item >= p.whole;
+  const int64_t k_begin = cut ? part * p.k_part : 0;
+  int64_t k_end = cut ? k_begin + p.k_part : p.K;
   if (k_end > p.K) k_end = p.K;
   const int turns = k_end > k_begin ? (int)((k_end - k_begin + BK - 1) / BK) : 0;
 
@@ -341,11 +433,14 @@ __global__ void __launch_bounds__(256, 2) gemm_grad_tile_kernel(GradGemm p) {
   fa.init(wm * (T / WM), lane);
   fb.init(wn * (T / WN), lane);
 
-  f32x4 acc[FM][FN];
+  f32x4 acc[FM][FN], sums[FS];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int f = 0; f < FS; ++f) sums[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const bool with_sums = ROW_SUMS && p.row_sums;
 
   const uint32_t lds0 = lds_byte_address(smem);
   auto issue = [&](int t) {
@@ -354,11 +449,13 @@ __global__ void __launch_bounds__(256, 2) gemm_grad_tile_kernel(GradGemm p) {
     lb.issue(k_begin + (int64_t)t * BK, stage + PA::BYTES);
   };
   if (turns > 0) issue(0);
+  int sum_turn = with_sums ? (int)((k_begin / BK) % p.tiles_n) : 0;
   for (int t = 0; t < turns; ++t) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();  // stage t is there; the other one has been read
     if (t + 1 < turns) issue(t + 1);
     const uint32_t sa = lds0 + (uint32_t)(t & 1) * (PA::BYTES + PB::BYTES), sb = sa + PA::BYTES;
+    const bool mine = with_sums && sum_turn == tile.n;
     auto step = [&](auto ks) {
       constexpr int KS = decltype(ks)::value;
       TrFrag ra[FM], rb[FN];
@@ -371,20 +468,256 @@ __global__ void __launch_bounds__(256, 2) gemm_grad_tile_kernel(GradGemm p) {
       for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
+      if constexpr (ROW_SUMS) {
+        if (mine) {
+#pragma unroll
+          for (int f = 0; f < FS; ++f) sums[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(all_ones(), wn == 0 ? a[f] : a[FM - FS + f], sums[f], 0, 0, 0);
+        }
+      }
     };
     step(std::integral_constant<int, 0>{});
     step(std::integral_constant<int, 1>{});
+    if (++sum_turn == p.tiles_n) sum_turn = 0;
   }
-  grad_epilogue<EPI, FM, FN>(p, acc, m0 + wm * (T / WM), n0 + wn * (BN_OUT / WN), split, lane);
+  __syncthreads();  // the stages are read: they stage the result now
+  float* const at = EPI == EPI_STORE && cut ? p.partial + ((int64_t)(item - p.whole) * p.parts + part) * (T * T) : nullptr;
+  const uint32_t stage = lds0 + wave * (16 * FN * 64);
+  if (at) grad_epilogue<T, EPI, FM, FN>(p, acc, wm * (T / WM), wn * (T / WN), at, stage, lane);
+  else grad_epilogue<T, EPI, FM, FN>(p, acc, m0 + wm * (T / WM), n0 + wn * (BN_OUT / WN), nullptr, stage, lane);
+  if constexpr (ROW_SUMS) {
+    if (with_sums) store_row_sums<T, FS>(p, sums, tile.m, tile.n, part, wm * (T / WM) + wn * FS * 16, lane);
+  }
 }
 
-// ---- sums over the parts of the tokens, in order: out[i] = sum of part[s][i]; 8 elements a thread
-__global__ void __launch_bounds__(256) split_sum_kernel(const float* part, void* out, int out_f32, int64_t n, int splits) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
-  if (i >= n) return;
+template <int T, bool A_TR, bool B_TR, int EPI>
+__global__ void __launch_bounds__(256, 2) gemm_grad_tile_kernel(GradGemm p) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[tile_lds<T>()];
+  grad_tile<T, A_TR, B_TR, EPI>(p, blockIdx.x, smem);
+}
+
+// two products that do not depend on each other in one launch: the first n workgroups make dx (or dh and what follows from it), the others dw
+template <int T, int EPI>
+__global__ void __launch_bounds__(256, 2) gemm_grad_pair_kernel(GradGemm p, GradGemm q, int n) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[tile_lds<T>()];
+  if ((int)blockIdx.x < n) grad_tile<T, false, true, EPI>(p, blockIdx.x, smem);
+  else grad_tile<T, true, true, EPI_STORE>(q, blockIdx.x - n, smem);
+}
+
+// ---- tiles of 256 x 256, eight waves (two by four, 128 x 64 each), one persistent workgroup a CU: the pipeline of the package's other
+// large product (two stages of A, three of B, the two waves of a SIMD in alternating memory and compute slots, the loads' flat sequence over
+// items and k-tiles running ahead through the epilogues), for operands of either layout.  An item is a tile of one part of k.
+// Slots of k-tile j, numbered globally: group 0 (waves 0-3) M0 C0 M1 C1 in slots 4j .. 4j+3, group 1 one slot later.  A memory slot reads half
+// a k-tile's fragments and issues 4 loads, a compute slot issues 32 MFMAs.  A: the half of a stage that a group reads is loaded by its own
+// waves, A[j+1] in M0(j) over A[j-1], last read in M1(j-1).  B: B[j+2] in M1(j) (slots 4j+2, 4j+3) over B[j-1], last read in slot 4j-1.
+// Waits, by counts of the loads issued since: the end of M1(j) leaves 8 outstanding (B[j+1] has arrived), the end of C1(j) 4 (A[j+1] has).
+constexpr int BIG_STAGE = 256 * BK * 2;
+constexpr int BIG_LDS = 5 * BIG_STAGE;
+
+template <bool A_TR, bool B_TR, int EPI>
+__global__ void __launch_bounds__(512) gemm_grad_big_kernel(GradGemm p) {
+  constexpr bool SWIGLU = EPI == EPI_SWIGLU, ROW_SUMS = A_TR;
+  constexpr int BN_OUT = SWIGLU ? 128 : 256;
+  constexpr int FM = 8, FN = 4, FS = ROW_SUMS ? 2 : 1;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int grp = wave >> 2, wn = wave & 3;
+  const uint32_t lds0 = lds_byte_address(smem), lds_b0 = lds0 + 2 * BIG_STAGE;
+
+  // Whole tiles come in full rounds of one per CU: XCD x (workgroup number mod 8) has a contiguous eighth of them, its 32 workgroups take
+  // them in turns, so that those at work together share the operands' slices in its L2.  What is left is one more round, of parts.
+  const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
+  const int rounds = p.whole >> 8, cut_items = (p.tiles_m * p.tiles_n - p.whole) * p.parts, cut_each = (cut_items + 7) >> 3;
+  const bool has_cut = slot < cut_each && xcd * cut_each + slot < cut_items;
+  const int n_my = rounds + (has_cut ? 1 : 0);
+  if (n_my == 0) return;
+  struct Item { int64_t m0, k_begin, k_end; int n0, tile_m, tile_n, part, cut; };
+  auto decode = [&](int r) {
+    Item it;
+    int tile;
+    if (r < rounds) {
+      tile = xcd * (rounds * 32) + r * 32 + slot;
+      it.cut = it.part = 0;
+      it.k_begin = 0;
+      it.k_end = p.K;
+    } else {
+      const int c = xcd * cut_each + slot;
+      it.cut = c / p.parts;
+      tile = p.whole + it.cut;
+      it.part = c - it.cut * p.parts;
+      it.cut = c + 1;
+      it.k_begin = it.part * p.k_part;
+      it.k_end = it.k_begin + p.k_part < p.K ? it.k_begin + p.k_part : p.K;
+    }
+    const TileAt t = tile_at(tile, p.tiles_m, p.tiles_n);
+    it.tile_m = t.m;
+    it.tile_n = t.n;
+    it.m0 = (int64_t)t.m * 256;
+    it.n0 = t.n * BN_OUT;
+    return it;
+  };
+  // k-tiles of an item (at least one: what lies beyond the end of k arrives as zeros)
+  const int KT_whole = (int)((p.K + BK - 1) / BK), KT_cut = (int)(p.k_part / BK);
+  auto turns_of = [&](int r) { return r < rounds ? KT_whole : KT_cut; };
+
+  Loader<A_TR, 128, 4, false> la;
+  Loader<B_TR, 256, 8, SWIGLU> lb;
+  la.init(p.A, p.lda, 0, 0, 0, lane, wn);
+  lb.init(p.B, p.ldb, 0, 0, p.N, lane, wave);
+  int la_r = 0, la_kt = 0, la_stage = 0, lb_r = 0, lb_kt = 0, lb_stage = 0;
+  int64_t la_k = 0, lb_k = 0;
+  auto la_item = [&]() {
+    if (la_r >= n_my) {  // past the end: loads from a descriptor without records, so that the counts of the waits stay the same
+      la.k_end = la_k = 0;
+      return;
+    }
+    const Item it = decode(la_r);
+    const int64_t m = it.m0 + grp * 128;
+    la.base = p.A + (A_TR ? m : m * p.lda);
+    la.rows = p.M > m ? p.M - m : 0;
+    la.k_end = it.k_end;
+    la_k = it.k_begin;
+  };
+  auto lb_item = [&]() {
+    if (lb_r >= n_my) {
+      lb.k_end = lb_k = 0;
+      return;
+    }
+    const Item it = decode(lb_r);
+    lb.base = p.B + (B_TR ? (int64_t)it.n0 : it.n0 * p.ldb);
+    lb.rows = p.N - it.n0;
+    lb.k_end = it.k_end;
+    lb_k = it.k_begin;
+  };
+  // (issue and advance apart: no branch may lie between the transposing reads of a memory slot and their wait)
+  auto issue_a = [&]() { la.issue(la_k, lds0 + la_stage * BIG_STAGE + grp * (BIG_STAGE / 2)); };
+  auto issue_b = [&]() { lb.issue(lb_k, lds_b0 + lb_stage * BIG_STAGE); };
+  auto advance_a = [&]() {
+    la_stage ^= 1;
+    la_k += BK;
+    if (++la_kt >= turns_of(la_r)) {
+      la_kt = 0;
+      ++la_r;
+      la_item();
+    }
+  };
+  auto advance_b = [&]() {
+    if (++lb_stage == 3) lb_stage = 0;
+    lb_k += BK;
+    if (++lb_kt >= turns_of(lb_r)) {
+      lb_kt = 0;
+      ++lb_r;
+      lb_item();
+    }
+  };
+
+  Fragments<A_TR, 128, 4, FM> fa;
+  Fragments<B_TR, 256, 8, FN> fb;
+  fa.init(0, lane);
+  fb.init(wn * 64, lane);
+  f32x4 acc[FM][FN];
+  auto clear = [&]() {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  };
+  clear();
+  f32x4 sums[FS];
+#pragma unroll
+  for (int f = 0; f < FS; ++f) sums[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const bool with_sums = ROW_SUMS && p.row_sums;
+
+  la_item();
+  lb_item();
+  issue_a();
+  advance_a();
+  issue_b();
+  advance_b();
+  issue_b();
+  advance_b();
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  int sa = 0, sb = 0;
+  for (int r = 0; r < n_my; ++r) {
+    if (grp == 1) __builtin_amdgcn_s_barrier();  // one slot behind group 0; group 0 waits for it ahead of its epilogue
+    const Item it = decode(r);
+    const int KT = turns_of(r);
+    int sum_turn = with_sums ? (int)((it.k_begin / BK) % p.tiles_n) : 0;
+    for (int kt = 0; kt < KT; ++kt) {
+      const bool mine = with_sums && sum_turn == it.tile_n;
+      if (++sum_turn == p.tiles_n) sum_turn = 0;
+      const uint32_t s_a = lds0 + sa * BIG_STAGE + grp * (BIG_STAGE / 2), s_b = lds_b0 + sb * BIG_STAGE;
+      sa ^= 1;
+      if (++sb == 3) sb = 0;
+      auto half = [&](auto ks) {
+        constexpr int KS = decltype(ks)::value;
+        TrFrag ra[FM], rb[FN];
+        bf16x8 a[FM], b[FN];
+        fa.template request<KS>(s_a, ra, a);
+        fb.template request<KS>(s_b, rb, b);
+        __builtin_amdgcn_sched_barrier(0);
+        if (KS == 0) issue_a();
+        else issue_b();
+        __builtin_amdgcn_sched_barrier(0);
+        fa.wait(ra, a);
+        fb.wait(rb, b);
+        __builtin_amdgcn_s_waitcnt(KS == 0 ? 0xC07F : 0x0078);  // lgkmcnt(0); vmcnt(8) lgkmcnt(0)
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (ROW_SUMS) {
+          if (mine) {
+#pragma unroll
+            for (int f = 0; f < FS; ++f) {
+              const bf16x8 x = wn < 2 ? wn == 0 ? a[f] : a[2 + f] : wn == 2 ? a[4 + f] : a[6 + f];
+              sums[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(all_ones(), x, sums[f], 0, 0, 0);
+            }
+          }
+        }
+        if (KS == 0) advance_a();
+        else advance_b();
+        if (KS == 1) __builtin_amdgcn_s_waitcnt(0x0F74);  // vmcnt(4)
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      half(std::integral_constant<int, 0>{});
+      half(std::integral_constant<int, 1>{});
+    }
+    if (grp == 0) __builtin_amdgcn_s_barrier();
+    // the A stage that is filled next is idle, and the 4 KB of it that this wave's own loads fill are written by nobody else
+    const uint32_t stage = lds0 + la_stage * BIG_STAGE + grp * (BIG_STAGE / 2) + wn * 4096;
+    if (EPI == EPI_STORE && it.cut && p.parts > 1) grad_epilogue<256, EPI, FM, FN>(p, acc, grp * 128, wn * 64, p.partial + (int64_t)(it.cut - 1) * 65536, stage, lane);
+    else grad_epilogue<256, EPI, FM, FN>(p, acc, it.m0 + grp * 128, it.n0 + wn * (BN_OUT / 4), nullptr, stage, lane);
+    clear();
+    if constexpr (ROW_SUMS) {
+      if (with_sums) {
+        store_row_sums<256, FS>(p, sums, it.tile_m, it.tile_n, it.part, grp * 128 + wn * 32, lane);
+#pragma unroll
+        for (int f = 0; f < FS; ++f) sums[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+    }
+  }
+}
+
+// ---- what is left when the products are made, each in a fixed order: the first n workgroups add up the parts of p's cut tiles, the next
+// m those of q's (8 columns a thread), the others the bias' gradient from q's sums over k
+template <int T>
+__device__ __forceinline__ void part_sum(const GradGemm& p, int block) {
+  constexpr int PER_TILE = T * T / 8 / 256;  // workgroups
+  const int tile = block / PER_TILE, at = ((block % PER_TILE) * 256 + threadIdx.x) * 8;
+  const TileAt t = tile_at(p.whole + tile, p.tiles_m, p.tiles_n);
+  const int64_t row = (int64_t)t.m * T + at / T;
+  const int col = t.n * T + at % T;
+  if (row >= p.M || col >= p.N) return;
+  const float* src = p.partial + (int64_t)tile * p.parts * (T * T) + at;
   float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < splits; ++s) {
-    const f32x4* q = reinterpret_cast<const f32x4*>(part + s * n + i);
+#pragma unroll 4
+  for (int s = 0; s < p.parts; ++s) {
+    const f32x4* q = reinterpret_cast<const f32x4*>(src + (int64_t)s * (T * T));
     const f32x4 a = q[0], b = q[1];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -392,7 +725,28 @@ __global__ void __launch_bounds__(256) split_sum_kernel(const float* part, void*
       o[4 + e] += b[e];
     }
   }
-  store8(out, out_f32, i, o);
+  store8(p.C, p.c_f32, row * p.ldc + col, o);
+}
+template <int T>
+__global__ void __launch_bounds__(256) grad_finish_kernel(GradGemm p, GradGemm q, int n, int m, uint16_t* bias) {
+  const int block = blockIdx.x;
+  if (block < n) {
+    part_sum<T>(p, block);
+  } else if (block < n + m) {
+    part_sum<T>(q, block - n);
+  } else {
+    const int64_t row = (int64_t)(block - n - m) * 256 + threadIdx.x;
+    if (row >= q.M) return;
+    const int tm = (int)(row / T);
+    float v = 0.f;
+    for (int tn = 0; tn < q.tiles_n; ++tn) {
+      const int parts = tile_number(tm, tn, q.tiles_m, q.tiles_n) < q.whole ? 1 : q.parts;
+      const float* src = q.row_sums + ((int64_t)tm * q.tiles_n + tn) * q.parts * T + row % T;
+#pragma unroll 4
+      for (int s = 0; s < parts; ++s) v += src[(int64_t)s * T];
+    }
+    bias[row] = (uint16_t)f32_to_bf16_bits(v);
+  }
 }
 
 // ---- dz = dy act'(z) (ACT_NONE: dy) rounded to bf16, and the sums of the unrounded dz over the tokens: a workgroup takes 512 columns
@@ -432,7 +786,7 @@ __global__ void __launch_bounds__(256) act_grad_kernel(ActGrad p) {
       }
       if (p.act != AERIS_ACT_NONE) {
         float z[8];
-        widen8(*reinterpret_cast<const u32x4*>(p.z + at), z);
+        load_kept8(p.z, p.M * p.N, at, z);
 #pragma unroll
         for (int e = 0; e < 8; ++e) d[e] *= p.act == AERIS_ACT_SILU ? dsilu_f(z[e], sigmoid_f(z[e])) : dgelu_f(z[e]);
       }
@@ -499,40 +853,62 @@ hipError_t act_grad_launch(const void* dy, int dy_f32, const void* z, void* dz, 
 // ---- how a product is cut
 
 struct GradPlan {
-  int tile;
-  int splits;
-  int64_t k_per_split;
+  int tile;  // 0: the result has more tiles than can be numbered
+  int tiles_m, tiles_n, whole, parts;
+  int64_t k_part;
+  double us;  // estimate
+  int64_t left() const { return (int64_t)tiles_m * tiles_n - whole; }
+  int64_t items() const { return whole + left() * parts; }
+  int64_t partial_bytes() const { return parts > 1 ? left() * parts * tile * tile * 4 : 0; }
+  int64_t row_sum_bytes() const { return ((int64_t)tiles_m * tiles_n * parts * tile * 4 + 255) / 256 * 256; }
 };
 
-GradPlan plan_of(int64_t M, int N, int64_t K, bool may_split) {
-  GradPlan g;
-  auto tiles_of = [&](int t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
-  g.tile = tiles_of(128) >= 256 || (may_split && tiles_of(128) * (K / 512) >= 256) ? 128 : 64;
-  g.splits = 1;
-  const int64_t tiles = tiles_of(g.tile);
-  if (may_split && tiles < 512) {
-    int64_t s = 512 / tiles;
-    if (s > K / 512) s = K / 512;
-    g.splits = s < 1 ? 1 : (int)s;
+// What a product of form `epi` takes in tiles of T x T, in us.  A round of 256 tiles of 256, of 512 of 128 (two a CU) or of 1280 of 64 (five) takes
+// round_k a k and tile_us beside it, a lone tile of 128 or 64 on a CU lone_k a k: fitted to products of 2048 .. 259200 rows, 128 .. 12288 columns
+// and k from 64 to 64800.  Tiles beyond the last whole round may be cut along k into as many parts as fill one: 14400 tokens' dw [12288, 1536] (288
+// tiles of 256 for 256 CUs) 710 -> 472 us; the parts go through memory once more, 16 to 256 KB each.
+GradPlan plan_tiles(int t, int64_t M, int64_t N, int64_t K, int epi) {
+  const int64_t bn = epi == EPI_SWIGLU ? t / 2 : t, tm = (M + t - 1) / t, tn = (N + bn - 1) / bn, tiles = tm * tn;
+  GradPlan best = {};
+  best.us = 1e30;
+  if (tiles >= 1 << 24) return best;
+  const int at_once = t == 256 ? 256 : t == 128 ? 512 : 1280, i = t == 256 ? 0 : t == 128 ? 1 : 2;
+  const bool kept = epi == EPI_ACT || epi == EPI_SWIGLU;  // 3 bytes a value are written beside the result
+  constexpr double K_STORE[3] = {0.0255, 0.0152, 0.0146}, K_KEPT[3] = {0.0182, 0.0122, 0.0104}, K_LONE[3] = {0.0255, 0.0085, 0.005};
+  constexpr double TILE_STORE[3] = {5.0, 3.0, 2.0}, TILE_KEPT[3] = {28.0, 16.0, 12.0};
+  const double round_k = kept ? K_KEPT[i] : K_STORE[i], lone_k = K_LONE[i] < round_k ? K_LONE[i] : round_k;
+  const double tile_us = kept || epi == EPI_SWIGLU_BWD ? TILE_KEPT[i] : TILE_STORE[i];
+  const int64_t left = tiles % at_once;
+  int64_t most = epi == EPI_STORE && left ? at_once / left : 1;
+  if (most > K / 256) most = K / 256;
+  for (int64_t parts = 1; parts == 1 || parts <= most; parts += parts < 8 ? 1 : parts / 4) {
+    const int64_t kp = (K + parts - 1) / parts + BK - 1, k_part = kp / BK * BK;
+    const double share = (double)left * parts / at_once;  // of the last round's places
+    const double last_k = lone_k + (round_k - lone_k) * share;
+    double us = (double)(tiles / at_once) * (K * round_k + tile_us) + (left ? k_part * last_k + tile_us : 0.0);
+    if (parts > 1) us += 5.0 + (double)left * parts * t * t * 4 * 2 / 5e6;
+    if (us < best.us) {
+      best.us = us;
+      best.tile = t;
+      best.tiles_m = (int)tm;
+      best.tiles_n = (int)tn;
+      best.k_part = k_part;
+      best.parts = (int)((K + k_part - 1) / k_part);
+      // (tiles of 256: the last round is addressed as parts, also where they are whole)
+      best.whole = (int)(best.parts == 1 && t != 256 ? tiles : tiles - left);
+    }
   }
-  g.k_per_split = ((K + g.splits - 1) / g.splits + BK - 1) / BK * BK;
-  if (g.k_per_split < BK) g.k_per_split = BK;
-  if (K > 0) g.splits = (int)((K + g.k_per_split - 1) / g.k_per_split);
-  return g;
+  return best;
 }
 
-template <bool A_TR, bool B_TR, int EPI>
-hipError_t launch(GradGemm p, const GradPlan& g, hipStream_t stream) {
-  const int bn = EPI == EPI_SWIGLU ? g.tile / 2 : g.tile;
-  const int64_t tm = (p.M + g.tile - 1) / g.tile, tn = (p.N + bn - 1) / bn;
-  p.tiles_m = (int)tm;
-  p.tiles_n = (int)tn;
-  p.k_per_split = g.k_per_split;
-  const int64_t blocks = tm * tn * g.splits;
-  if (blocks >= 1 << 24) return hipErrorInvalidValue;
-  if (g.tile == 128) hipLaunchKernelGGL((gemm_grad_tile_kernel<128, A_TR, B_TR, EPI>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((gemm_grad_tile_kernel<64, A_TR, B_TR, EPI>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
-  return hipGetLastError();
+GradPlan plan_of(int64_t M, int64_t N, int64_t K, int epi) {
+  GradPlan best = {};
+  best.us = 1e30;
+  for (int t : {256, 128, 64}) {
+    const GradPlan g = plan_tiles(t, M, N, K, epi);
+    if (g.us < best.us) best = g;
+  }
+  return best;
 }
 
 GradGemm product(const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int64_t ldc, int64_t M, int64_t N, int64_t K) {
@@ -550,35 +926,125 @@ GradGemm product(const void* A, int64_t lda, const void* B, int64_t ldb, void* C
   return p;
 }
 
-// dw [N, K] = dz[M, N]^T x[M, K]
-hipError_t weight_grad(const void* dz, const void* x, void* dw, int64_t M, int64_t N, int64_t K, float* partial, hipStream_t stream) {
-  const GradPlan g = plan_of(N, (int)K, M, true);
-  GradGemm p = product(dz, N, x, K, dw, K, N, K, M);
-  if (g.splits > 1) {
-    p.C = partial;
-    p.c_f32 = 1;
-    p.split_stride = N * K;
-  }
-  hipError_t e = launch<true, true, EPI_STORE>(p, g, stream);
-  if (e != hipSuccess || g.splits == 1) return e;
-  hipLaunchKernelGGL(split_sum_kernel, dim3((unsigned)((N * K / 8 + 255) / 256)), dim3(256), 0, stream, partial, dw, 0, N * K, g.splits);
-  return hipGetLastError();
-}
-int64_t weight_grad_bytes(int64_t M, int64_t N, int64_t K) {
-  const GradPlan g = plan_of(N, (int)K, M, true);
-  return g.splits > 1 ? g.splits * N * K * 4 : 0;
+void apply(GradGemm& p, const GradPlan& g, void* partial) {
+  p.tiles_m = g.tiles_m;
+  p.tiles_n = g.tiles_n;
+  p.whole = g.whole;
+  p.parts = g.parts;
+  p.k_part = g.k_part;
+  p.partial = reinterpret_cast<float*>(partial);
 }
 
-// dx [M, K] = dz[M, N] w[N, K]
-hipError_t input_grad(const void* dz, const void* w, void* dx, int64_t M, int64_t N, int64_t K, hipStream_t stream) {
-  return launch<false, true, EPI_STORE>(product(dz, N, w, K, dx, K, M, K, N), plan_of(M, (int)K, N, false), stream);
+hipError_t finish(const GradGemm& p, int64_t n, const GradGemm& q, int64_t m, int tile, uint16_t* bias, hipStream_t stream) {
+  const int64_t per_tile = tile * tile / 8 / 256;
+  n *= per_tile;
+  m *= per_tile;
+  const int64_t blocks = n + m + (bias ? (q.M + 255) / 256 : 0);
+  if (blocks == 0) return hipSuccess;
+#define GO(T) hipLaunchKernelGGL(grad_finish_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, stream, p, q, (int)n, (int)m, bias)
+  if (tile == 256) GO(256);
+  else if (tile == 128) GO(128);
+  else GO(64);
+#undef GO
+  return hipGetLastError();
+}
+
+// one product; `bias`: from the sums over k of a dw
+template <bool A_TR, bool B_TR, int EPI>
+hipError_t launch(GradGemm& p, const GradPlan& g, void* partial, uint16_t* bias, hipStream_t stream) {
+  if (g.tile == 0) return hipErrorInvalidValue;
+  apply(p, g, partial);
+  if (g.tile == 256) {
+    const unsigned grid = g.whole ? 256 : (unsigned)((g.left() * g.parts + 7) / 8 * 8);
+    hipLaunchKernelGGL((gemm_grad_big_kernel<A_TR, B_TR, EPI>), dim3(grid), dim3(512), BIG_LDS, stream, p);
+  } else if (g.tile == 128) {
+    hipLaunchKernelGGL((gemm_grad_tile_kernel<128, A_TR, B_TR, EPI>), dim3((unsigned)g.items()), dim3(256), 0, stream, p);
+  } else {
+    hipLaunchKernelGGL((gemm_grad_tile_kernel<64, A_TR, B_TR, EPI>), dim3((unsigned)g.items()), dim3(256), 0, stream, p);
+  }
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess ? e : finish(p, 0, p, g.parts > 1 ? g.left() : 0, g.tile, bias, stream);
+}
+
+// A product c [M, N] = a[M, K] w[K, N] of tokens (dx, or dh with what follows from it) and the gradient dw [K2, N2] = b[M, K2]^T x[M, N2] of a
+// weight, either of them or both: in one launch where neither is of tiles of 256, as one after the other otherwise.
+struct GradPair {
+  bool first, second, sums;
+  GradPlan g, h;
+  bool together;
+  int64_t partial_bytes, second_bytes, sum_bytes;
+};
+GradPair plan_pair(bool first, int64_t M, int64_t N, int64_t K, int epi, bool second, int64_t N2, int64_t K2, bool sums) {
+  GradPair r = {};
+  r.first = first;
+  r.second = second;
+  r.sums = sums && second;
+  if (first) r.g = plan_of(M, N, K, epi);
+  if (second) r.h = plan_of(N2, K2, M, EPI_STORE);
+  if (first && second && r.g.tile && r.h.tile && r.g.tile != 256 && r.h.tile != 256) {
+    r.together = true;
+    if (r.g.tile != r.h.tile) {  // tiles of one size
+      const GradPlan g2 = plan_tiles(r.h.tile, M, N, K, epi), h2 = plan_tiles(r.g.tile, N2, K2, M, EPI_STORE);
+      if (g2.us + r.h.us < r.g.us + h2.us) r.g = g2;
+      else r.h = h2;
+    }
+    r.together = r.g.tile == r.h.tile && r.g.items() + r.h.items() < 1 << 24;
+  }
+  r.partial_bytes = first ? r.g.partial_bytes() : 0;
+  r.second_bytes = second ? r.h.partial_bytes() : 0;
+  r.sum_bytes = r.sums ? r.h.row_sum_bytes() : 0;
+  return r;
+}
+int64_t pair_bytes(const GradPair& r) { return r.partial_bytes + r.second_bytes + r.sum_bytes; }
+
+template <int EPI>
+hipError_t launch_pair(const GradPair& r, GradGemm p, GradGemm q, void* workspace, void* bias, hipStream_t stream) {
+  unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
+  unsigned char* const ws_q = ws + r.partial_bytes;
+  if (r.sums) q.row_sums = reinterpret_cast<float*>(ws_q + r.second_bytes);
+  uint16_t* const b = r.sums ? reinterpret_cast<uint16_t*>(bias) : nullptr;
+  if (!r.together) {
+    hipError_t e = hipSuccess;
+    if (r.first) e = launch<false, true, EPI>(p, r.g, ws, nullptr, stream);
+    if (e == hipSuccess && r.second) e = launch<true, true, EPI_STORE>(q, r.h, ws_q, b, stream);
+    return e;
+  }
+  apply(p, r.g, ws);
+  apply(q, r.h, ws_q);
+  const dim3 grid((unsigned)(r.g.items() + r.h.items()));
+  if (r.g.tile == 128) hipLaunchKernelGGL((gemm_grad_pair_kernel<128, EPI>), grid, dim3(256), 0, stream, p, q, (int)r.g.items());
+  else hipLaunchKernelGGL((gemm_grad_pair_kernel<64, EPI>), grid, dim3(256), 0, stream, p, q, (int)r.g.items());
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess ? e : finish(p, r.g.parts > 1 ? r.g.left() : 0, q, r.h.parts > 1 ? r.h.left() : 0, r.g.tile, b, stream);
 }
 
 int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
 bool needs_dz(const aeris_linear_grad& a) { return (a.dy_dtype == AERIS_F32 || a.act != AERIS_ACT_NONE) && (a.dx || a.dw || a.dz); }
+// the bias' gradient: with dz where that has to be made, otherwise with dw
+bool bias_apart(const aeris_linear_grad& a) { return a.dbias && (needs_dz(a) || !a.dw || a.dy_dtype == AERIS_F32 || a.act != AERIS_ACT_NONE); }
+int64_t more(int64_t a, int64_t b) { return a > b ? a : b; }
+GradPair linear_pair(const aeris_linear_grad& a) {
+  return plan_pair(a.dx, a.M, a.K, a.N, EPI_STORE, a.dw, a.N, a.K, a.dbias && !bias_apart(a));
+}
+GradPair hidden_pair(const aeris_feed_forward_grad& a) { return plan_pair(a.dx || a.dw1, a.M, a.H, a.d, EPI_SWIGLU_BWD, a.dw2, a.d, a.H, false); }
+GradPair token_pair(const aeris_feed_forward_grad& a) { return plan_pair(a.dx, a.M, a.d, 2 * a.H, EPI_STORE, a.dw1, 2 * a.H, a.d, false); }
 
 }  // namespace
+
+hipError_t gemm_grad_configure() {
+  hipError_t e = hipSuccess;
+  auto one = [&](const void* f) {
+    if (e == hipSuccess) e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, BIG_LDS);
+  };
+  one(reinterpret_cast<const void*>(gemm_grad_big_kernel<false, false, EPI_STORE>));
+  one(reinterpret_cast<const void*>(gemm_grad_big_kernel<false, false, EPI_ACT>));
+  one(reinterpret_cast<const void*>(gemm_grad_big_kernel<false, false, EPI_SWIGLU>));
+  one(reinterpret_cast<const void*>(gemm_grad_big_kernel<false, true, EPI_STORE>));
+  one(reinterpret_cast<const void*>(gemm_grad_big_kernel<false, true, EPI_SWIGLU_BWD>));
+  one(reinterpret_cast<const void*>(gemm_grad_big_kernel<true, true, EPI_STORE>));
+  return e;
+}
 
 hipError_t linear_train_launch(const aeris_linear_train& a, hipStream_t stream) {
   GradGemm p = product(a.x, a.K, a.w, a.K, a.y, a.N, a.M, a.N, a.K);
@@ -586,17 +1052,16 @@ hipError_t linear_train_launch(const aeris_linear_train& a, hipStream_t stream) 
   p.bias = reinterpret_cast<const uint16_t*>(a.bias);
   p.residual = a.residual;
   p.res_dtype = a.residual ? (int)a.res_dtype : -1;
-  p.saved = reinterpret_cast<uint16_t*>(a.z);
+  p.kept = reinterpret_cast<uint16_t*>(a.z);
   p.act = (int)a.act;
-  return launch<false, false, EPI_ACT>(p, plan_of(a.M, (int)a.N, a.K, false), stream);
+  return launch<false, false, EPI_ACT>(p, plan_of(a.M, a.N, a.K, EPI_ACT), nullptr, nullptr, stream);
 }
 
 int64_t linear_grad_workspace_bytes(const aeris_linear_grad& a) {
   int64_t n = 0;
   if (needs_dz(a) && !a.dz) n += up256(a.M * a.N * 2);
-  if (a.dbias) n += up256((int64_t)act_grad_parts(a.M, (int)a.N) * a.N * 4);
-  if (a.dw) n += weight_grad_bytes(a.M, a.N, a.K);
-  return n;
+  if (bias_apart(a)) n += up256((int64_t)act_grad_parts(a.M, (int)a.N) * a.N * 4);
+  return n + pair_bytes(linear_pair(a));
 }
 
 hipError_t linear_grad_launch(const aeris_linear_grad& a, void* workspace, hipStream_t stream) {
@@ -608,49 +1073,40 @@ hipError_t linear_grad_launch(const aeris_linear_grad& a, void* workspace, hipSt
     if (!a.dz) ws += up256(a.M * a.N * 2);
     dz = dz_out;
   }
-  if (dz_out || a.dbias) {
+  if (dz_out || bias_apart(a)) {
     float* partial = reinterpret_cast<float*>(ws);
-    if (a.dbias) ws += up256((int64_t)act_grad_parts(a.M, (int)a.N) * a.N * 4);
-    const hipError_t e = act_grad_launch(a.dy, a.dy_dtype == AERIS_F32, a.z, dz_out, partial, a.dbias, a.M, (int)a.N, (int)a.act, stream);
+    if (bias_apart(a)) ws += up256((int64_t)act_grad_parts(a.M, (int)a.N) * a.N * 4);
+    const hipError_t e = act_grad_launch(a.dy, a.dy_dtype == AERIS_F32, a.z, dz_out, partial, bias_apart(a) ? a.dbias : nullptr, a.M, (int)a.N, (int)a.act, stream);
     if (e != hipSuccess) return e;
   }
-  if (a.dx) {
-    const hipError_t e = input_grad(dz, a.w, a.dx, a.M, a.N, a.K, stream);
-    if (e != hipSuccess) return e;
-  }
-  return a.dw ? weight_grad(dz, a.x, a.dw, a.M, a.N, a.K, reinterpret_cast<float*>(ws), stream) : hipSuccess;
+  return launch_pair<EPI_STORE>(linear_pair(a), product(dz, a.N, a.w, a.K, a.dx, a.K, a.M, a.K, a.N), product(dz, a.N, a.x, a.K, a.dw, a.K, a.N, a.K, a.M), ws, a.dbias, stream);
 }
 
-hipError_t feed_forward_train_launch(const aeris_feed_forward& a, hipStream_t stream) {
+int64_t feed_forward_train_workspace_bytes(const aeris_feed_forward& a) { return plan_of(a.M, a.d, a.H, EPI_STORE).partial_bytes(); }
+
+hipError_t feed_forward_train_launch(const aeris_feed_forward& a, void* workspace, hipStream_t stream) {
   GradGemm p = product(a.x, a.d, a.w1, a.d, a.h, a.H, a.M, a.H, a.d);
-  p.saved = reinterpret_cast<uint16_t*>(a.gate_up);
-  hipError_t e = launch<false, false, EPI_SWIGLU>(p, plan_of(a.M, (int)a.H * 2, a.d, false), stream);
+  p.kept = reinterpret_cast<uint16_t*>(a.gate_up);
+  const hipError_t e = launch<false, false, EPI_SWIGLU>(p, plan_of(a.M, a.H, a.d, EPI_SWIGLU), nullptr, nullptr, stream);
   if (e != hipSuccess) return e;
-  return launch<false, false, EPI_STORE>(product(a.h, a.H, a.w2, a.H, a.y, a.d, a.M, a.d, a.H), plan_of(a.M, (int)a.d, a.H, false), stream);
+  GradGemm q = product(a.h, a.H, a.w2, a.H, a.y, a.d, a.M, a.d, a.H);
+  return launch<false, false, EPI_STORE>(q, plan_of(a.M, a.d, a.H, EPI_STORE), workspace, nullptr, stream);
 }
 
 int64_t feed_forward_grad_workspace_bytes(const aeris_feed_forward_grad& a) {
-  int64_t n = a.dx || a.dw1 ? up256(a.M * a.H * 4) : 0;
-  int64_t part = a.dw1 ? weight_grad_bytes(a.M, 2 * a.H, a.d) : 0;
-  const int64_t part2 = a.dw2 ? weight_grad_bytes(a.M, a.d, a.H) : 0;
-  return n + (part > part2 ? part : part2);
+  return (a.dx || a.dw1 ? up256(a.M * a.H * 4) : 0) + more(pair_bytes(hidden_pair(a)), pair_bytes(token_pair(a)));
 }
 
 hipError_t feed_forward_grad_launch(const aeris_feed_forward_grad& a, void* workspace, hipStream_t stream) {
   unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
   void* dgu = ws;
   if (a.dx || a.dw1) ws += up256(a.M * a.H * 4);
-  float* partial = reinterpret_cast<float*>(ws);
-  hipError_t e = hipSuccess;
-  if (a.dx || a.dw1) {
-    GradGemm p = product(a.dy, a.d, a.w2, a.H, dgu, 2 * a.H, a.M, a.H, a.d);
-    p.gate_up = reinterpret_cast<const uint16_t*>(a.gate_up);
-    e = launch<false, true, EPI_SWIGLU_BWD>(p, plan_of(a.M, (int)a.H, a.d, false), stream);
-  }
-  if (e == hipSuccess && a.dw2) e = weight_grad(a.dy, a.h, a.dw2, a.M, a.d, a.H, partial, stream);
-  if (e == hipSuccess && a.dx) e = input_grad(dgu, a.w1, a.dx, a.M, 2 * a.H, a.d, stream);
-  if (e == hipSuccess && a.dw1) e = weight_grad(dgu, a.x, a.dw1, a.M, 2 * a.H, a.d, partial, stream);
-  return e;
+  GradGemm p = product(a.dy, a.d, a.w2, a.H, dgu, 2 * a.H, a.M, a.H, a.d);
+  p.kept = reinterpret_cast<uint16_t*>(const_cast<void*>(a.gate_up));
+  const hipError_t e = launch_pair<EPI_SWIGLU_BWD>(hidden_pair(a), p, product(a.dy, a.d, a.h, a.H, a.dw2, a.H, a.d, a.H, a.M), ws, nullptr, stream);
+  if (e != hipSuccess) return e;
+  return launch_pair<EPI_STORE>(token_pair(a), product(dgu, 2 * a.H, a.w1, a.d, a.dx, a.d, a.M, a.d, 2 * a.H), product(dgu, 2 * a.H, a.x, a.d, a.dw1, a.d, 2 * a.H, a.d, a.M),
+                                ws, nullptr, stream);
 }
 
 }  // namespace aeris

@@ -58,10 +58,12 @@ int64_t norm_grad_workspace_bytes(const aeris_norm_modulate_grad& a);
 hipError_t norm_grad_launch(const aeris_norm_modulate_grad& a, void* workspace, hipStream_t stream);
 
 // products of a training step (gemm_grad.hip)
+hipError_t gemm_grad_configure();
 hipError_t linear_train_launch(const aeris_linear_train& a, hipStream_t stream);
 int64_t linear_grad_workspace_bytes(const aeris_linear_grad& a);
 hipError_t linear_grad_launch(const aeris_linear_grad& a, void* workspace, hipStream_t stream);
-hipError_t feed_forward_train_launch(const aeris_feed_forward& a, hipStream_t stream);
+int64_t feed_forward_train_workspace_bytes(const aeris_feed_forward& a);
+hipError_t feed_forward_train_launch(const aeris_feed_forward& a, void* workspace, hipStream_t stream);
 int64_t feed_forward_grad_workspace_bytes(const aeris_feed_forward_grad& a);
 hipError_t feed_forward_grad_launch(const aeris_feed_forward_grad& a, void* workspace, hipStream_t stream);
 

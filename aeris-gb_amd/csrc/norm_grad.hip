@@ -29,7 +29,6 @@ struct NormGradParams {
   float* partial;  // [segments][blocks per segment][sums][d], or NULL: no sums
   int64_t mod_stride;  // between the segments' modulation rows
   int64_t rows;        // of a segment
-  int64_t rows_per_block;
   int blocks_per_segment;
   int d;
   int kind;
@@ -41,9 +40,13 @@ __device__ __forceinline__ float param_at(const void* p, int f32, int c) {
   return f32 ? reinterpret_cast<const float*>(p)[c] : bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(p)[c]);
 }
 
-// NV: groups of 8 columns a lane; SUB: rows beside each other in a wave; WPR: waves to a row (1 or 4)
+// NV: groups of 8 columns a lane; SUB: rows beside each other in a wave; WPR: waves to a row (1, 2 or 4)
+// Workgroups that a CU holds, which the registers are budgeted for (sums, the row and the next one)
+template <int NV, bool PRE>
+constexpr int resident() { return PRE ? (NV == 1 ? 4 : NV == 2 ? 2 : 1) : (NV == 1 ? 5 : NV == 2 ? 3 : 2); }
+
 template <int NV, int SUB, int WPR, bool X_F32, bool DY_F32, bool PRE>
-__global__ void __launch_bounds__(256) norm_grad_kernel(NormGradParams p) {
+__global__ void __launch_bounds__(256, (resident<NV, PRE>())) norm_grad_kernel(NormGradParams p) {
   static_assert(SUB == 1 || (NV == 1 && WPR == 1), "rows beside each other: one column group a lane");
   constexpr int LPR = 64 * WPR / SUB;          // lanes of a row
   constexpr int SLOTS = 256 / LPR;             // rows at a time
@@ -54,7 +57,8 @@ __global__ void __launch_bounds__(256) norm_grad_kernel(NormGradParams p) {
   // sums of the row slots go over them at the end.  (Four waves to a row: a lane's columns are its own for all rows, their parameters
   // stay in its registers.)
   constexpr bool IN_LDS = WPR == 1;
-  __shared__ __attribute__((aligned(16))) float lds[IN_LDS ? (SLOTS > 3 ? SLOTS : 3) * COLS : 4];
+  constexpr int LDS_ROWS = IN_LDS ? (SLOTS > 3 ? SLOTS : 3) : SLOTS > 1 ? SLOTS : 0;
+  __shared__ __attribute__((aligned(16))) float lds[LDS_ROWS ? LDS_ROWS * COLS : 4];
   __shared__ float cross[2][4][2];
   f32x4* const sG = reinterpret_cast<f32x4*>(lds);
   f32x4* const sP1 = sG + (IN_LDS ? 2 * GROUPS : 0);
@@ -64,49 +68,38 @@ __global__ void __launch_bounds__(256) norm_grad_kernel(NormGradParams p) {
   const int d = p.d;
   const float inv_d = 1.0f / (float)d;
   const int seg = blockIdx.x / p.blocks_per_segment, blk = blockIdx.x - seg * p.blocks_per_segment;
-  const int64_t first = (int64_t)blk * p.rows_per_block;
-  int64_t end = first + p.rows_per_block;
-  if (end > p.rows) end = p.rows;
+  // (rows in turns over the workgroups: those at work together read and write neighbouring rows)
+  const int64_t first = (int64_t)blk * SLOTS, end = p.rows, stride = (int64_t)p.blocks_per_segment * SLOTS;
   const int64_t row_base = (int64_t)seg * p.rows;
   const float* const sh = p.shift ? p.shift + seg * p.mod_stride : nullptr;
   const float* const sc = p.scale ? p.scale + seg * p.mod_stride : nullptr;
 
-  struct Raw { u32x4 xa, xb, ya, yb; };
+  // 8 columns as they lie in memory, widened where they are used
+  struct Raw { u32x4 x[X_F32 ? 2 : 1], y[DY_F32 ? 2 : 1]; };
   auto load_row = [&](int64_t row, Raw (&raw)[NV]) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int col = (v * LPR + lane) * 8;
-      raw[v].xa = raw[v].xb = raw[v].ya = raw[v].yb = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int h = 0; h < (X_F32 ? 2 : 1); ++h) raw[v].x[h] = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int h = 0; h < (DY_F32 ? 2 : 1); ++h) raw[v].y[h] = u32x4{0u, 0u, 0u, 0u};
       if (col < d) {
         const int64_t at = (row_base + row) * d + col;
-        if (X_F32) {
-          const u32x4* q = reinterpret_cast<const u32x4*>(reinterpret_cast<const float*>(p.x) + at);
-          raw[v].xa = __builtin_nontemporal_load(q);
-          raw[v].xb = __builtin_nontemporal_load(q + 1);
-        } else {
-          raw[v].xa = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(p.x) + at));
-        }
-        if (DY_F32) {
-          const u32x4* q = reinterpret_cast<const u32x4*>(reinterpret_cast<const float*>(p.dy) + at);
-          raw[v].ya = __builtin_nontemporal_load(q);
-          raw[v].yb = __builtin_nontemporal_load(q + 1);
-        } else {
-          raw[v].ya = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(p.dy) + at));
-        }
+        const u32x4* const qx = reinterpret_cast<const u32x4*>(reinterpret_cast<const unsigned char*>(p.x) + at * (X_F32 ? 4 : 2));
+        const u32x4* const qy = reinterpret_cast<const u32x4*>(reinterpret_cast<const unsigned char*>(p.dy) + at * (DY_F32 ? 4 : 2));
+#pragma unroll
+        for (int h = 0; h < (X_F32 ? 2 : 1); ++h) raw[v].x[h] = __builtin_nontemporal_load(qx + h);
+#pragma unroll
+        for (int h = 0; h < (DY_F32 ? 2 : 1); ++h) raw[v].y[h] = __builtin_nontemporal_load(qy + h);
       }
     }
   };
-  auto widen = [](const u32x4& a, const u32x4& b, bool f32, float (&o)[8]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (f32) {
-        o[e] = __uint_as_float(a[e]);
-        o[4 + e] = __uint_as_float(b[e]);
-      } else {
-        o[2 * e] = bf16_lo(a[e]);
-        o[2 * e + 1] = bf16_hi(a[e]);
-      }
-    }
+  auto x_of = [](const Raw& r, int e) {
+    return X_F32 ? __uint_as_float(r.x[X_F32 ? e >> 2 : 0][e & 3]) : (e & 1) ? bf16_hi(r.x[0][e >> 1]) : bf16_lo(r.x[0][e >> 1]);
+  };
+  auto y_of = [](const Raw& r, int e) {
+    return DY_F32 ? __uint_as_float(r.y[DY_F32 ? e >> 2 : 0][e & 3]) : (e & 1) ? bf16_hi(r.y[0][e >> 1]) : bf16_lo(r.y[0][e >> 1]);
   };
 
   Raw cur[NV], nxt[NV];
@@ -114,9 +107,9 @@ __global__ void __launch_bounds__(256) norm_grad_kernel(NormGradParams p) {
   if (row < end) load_row(row, cur);
 
 #pragma unroll
-  for (int v = 0; v < (GROUPS + 255) / 256; ++v) {
-    const int g = v * 256 + threadIdx.x;
-    if (GROUPS % 256 && g >= GROUPS) break;
+  for (int v = 0; v < (IN_LDS ? (GROUPS + 255) / 256 : NV); ++v) {
+    const int g = IN_LDS ? v * 256 + threadIdx.x : v * LPR + lane;
+    if (IN_LDS && GROUPS % 256 && g >= GROUPS) break;
     float G[8], P1[8], P0[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -147,9 +140,10 @@ __global__ void __launch_bounds__(256) norm_grad_kernel(NormGradParams p) {
   }
   __syncthreads();
 
-  auto gain = [&](int v, int h) { return IN_LDS ? sG[h * GROUPS + v * LPR + lane] : rG[IN_LDS ? 0 : v][h]; };
-  auto one_plus_scale = [&](int v, int h) { return IN_LDS ? sP1[h * GROUPS + v * LPR + lane] : rP1[IN_LDS ? 0 : v][h]; };
-  auto shift_of = [&](int v, int h) { return IN_LDS ? sP0[h * GROUPS + v * LPR + lane] : rP0[IN_LDS ? 0 : v][h]; };
+  int at_lane = lane;  // (made opaque in every turn: the parameters stay in LDS, or the compiler keeps them all in registers)
+  auto gain = [&](int v, int h) { return IN_LDS ? sG[h * GROUPS + v * LPR + at_lane] : rG[IN_LDS ? 0 : v][h]; };
+  auto one_plus_scale = [&](int v, int h) { return IN_LDS ? sP1[h * GROUPS + v * LPR + at_lane] : rP1[IN_LDS ? 0 : v][h]; };
+  auto shift_of = [&](int v, int h) { return IN_LDS ? sP0[h * GROUPS + v * LPR + at_lane] : rP0[IN_LDS ? 0 : v][h]; };
 
   float acc[SUMS][NV][8];
 #pragma unroll
@@ -174,45 +168,65 @@ __global__ void __launch_bounds__(256) norm_grad_kernel(NormGradParams p) {
         cross[turn][w][1] = b;
       }
       __syncthreads();
-      a = (cross[turn][0][0] + cross[turn][1][0]) + (cross[turn][2][0] + cross[turn][3][0]);
-      b = (cross[turn][0][1] + cross[turn][1][1]) + (cross[turn][2][1] + cross[turn][3][1]);
+      const int w0 = slot * WPR;
+      a = cross[turn][w0][0] + cross[turn][w0 + 1][0];
+      b = cross[turn][w0][1] + cross[turn][w0 + 1][1];
+      if (WPR == 4) {
+        a += cross[turn][2][0] + cross[turn][3][0];
+        b += cross[turn][2][1] + cross[turn][3][1];
+      }
       turn ^= 1;  // the next pair goes elsewhere: a wave may be there before another has read this one
     }
   };
 
   // (rows beside each other in a wave, and rows of a workgroup, take the same number of turns: the lanes of a slot without a row
   // work on zeros, whose sums are zeros and which are not stored)
-  const int64_t turns = end > first ? (end - first + SLOTS - 1) / SLOTS : 0;
-  for (int64_t it = 0; it < turns; ++it, row += SLOTS) {
+  const int64_t turns = end > first ? (end - first + stride - 1) / stride : 0;
+  for (int64_t it = 0; it < turns; ++it, row += stride) {
+    asm volatile("" : "+v"(at_lane));
     const bool live = row < end;
-    if (row + SLOTS < end) load_row(row + SLOTS, nxt);
-    float u[NV][8], y[NV][8], x[PRE ? NV : 1][8];
+    if (row + stride < end) load_row(row + stride, nxt);
+    if (!live) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+#pragma unroll
+        for (int h = 0; h < (X_F32 ? 2 : 1); ++h) cur[v].x[h] = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int h = 0; h < (DY_F32 ? 2 : 1); ++h) cur[v].y[h] = u32x4{0u, 0u, 0u, 0u};
+      }
+    }
+    // u, the value that is normed (columns beyond d: 0)
+    auto u_row = [&](int v, float (&u)[8]) {
+      if (PRE) {
+        const bool act = (v * LPR + lane) * 8 < d;
+        const f32x4 p1a = one_plus_scale(v, 0), p1b = one_plus_scale(v, 1), p0a = shift_of(v, 0), p0b = shift_of(v, 1);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = act ? fmaf(x_of(cur[v], e), e < 4 ? p1a[e] : p1b[e - 4], e < 4 ? p0a[e] : p0b[e - 4]) : 0.f;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = x_of(cur[v], e);
+      }
+    };
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int g = v * LPR + lane;
-      const bool act = g * 8 < d;
-      if (!live) cur[v].xa = cur[v].xb = cur[v].ya = cur[v].yb = u32x4{0u, 0u, 0u, 0u};
-      widen(cur[v].xa, cur[v].xb, X_F32, u[v]);
-      widen(cur[v].ya, cur[v].yb, DY_F32, y[v]);
-      if (PRE) {
-        const f32x4 p1a = one_plus_scale(v, 0), p1b = one_plus_scale(v, 1), p0a = shift_of(v, 0), p0b = shift_of(v, 1);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[v][e] = u[v][e];
-          u[v][e] = act ? fmaf(u[v][e], e < 4 ? p1a[e] : p1b[e - 4], e < 4 ? p0a[e] : p0b[e - 4]) : 0.f;
-        }
-      }
+      float u[8];
+      u_row(v, u);
       const f32x4 ga = gain(v, 0), gb = gain(v, 1);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float dn = y[v][e] * (e < 4 ? ga[e] : gb[e - 4]);
-        s1 += p.kind == AERIS_NORM_RMS ? u[v][e] * u[v][e] : u[v][e];
-        s2 += p.kind == AERIS_NORM_RMS ? dn * u[v][e] : dn;
+        const float dn = y_of(cur[v], e) * (e < 4 ? ga[e] : gb[e - 4]);
+        if (p.kind == AERIS_NORM_RMS) {
+          s1 = fmaf(u[e], u[e], s1);
+          s2 = fmaf(dn, u[e], s2);
+        } else {
+          s1 += u[e];
+          s2 += dn;
+        }
       }
     }
     row_sums(s1, s2);
-    float mean = 0.f, r, c1 = 0.f, c2;  // c1 = mean(dn), c2 = r mean(dn n)
+    float mean = 0.f, r, c1 = 0.f, c2;  // c1 = mean(dn), c2 = mean(dn n)
     if (p.kind == AERIS_NORM_RMS) {
       r = rsqrtf(s1 * inv_d + p.eps);
       c2 = s2 * inv_d * r;
@@ -222,14 +236,15 @@ __global__ void __launch_bounds__(256) norm_grad_kernel(NormGradParams p) {
       float q1 = 0.f, q2 = 0.f;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const int g = v * LPR + lane;
-        const bool act = g * 8 < d;
+        float u[8];
+        u_row(v, u);
+        const bool act = (v * LPR + lane) * 8 < d;
         const f32x4 ga = gain(v, 0), gb = gain(v, 1);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          u[v][e] = act ? u[v][e] - mean : 0.f;
-          q1 = fmaf(u[v][e], u[v][e], q1);
-          q2 = fmaf(y[v][e] * (e < 4 ? ga[e] : gb[e - 4]), u[v][e], q2);
+          const float c = act ? u[e] - mean : 0.f;
+          q1 = fmaf(c, c, q1);
+          q2 = fmaf(y_of(cur[v], e) * (e < 4 ? ga[e] : gb[e - 4]), c, q2);
         }
       }
       row_sums(q1, q2);
@@ -239,20 +254,21 @@ __global__ void __launch_bounds__(256) norm_grad_kernel(NormGradParams p) {
     if (!live) r = c2 = 0.f;  // (eps 0: a row of zeros would have an infinite r)
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int g = v * LPR + lane, col = g * 8;
+      const int col = (v * LPR + lane) * 8;
+      float u[8];
+      u_row(v, u);
       const f32x4 ga = gain(v, 0), gb = gain(v, 1);
       float o[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float n = u[v][e] * r;
-        float du = (y[v][e] * (e < 4 ? ga[e] : gb[e - 4]) - c1 - n * c2) * r;
-        acc[0][v][e] = fmaf(y[v][e], n, acc[0][v][e]);
-        acc[1][v][e] += y[v][e];
+        const float n = col < d ? (u[e] - mean) * r : 0.f, y = y_of(cur[v], e);
+        float du = (fmaf(y, e < 4 ? ga[e] : gb[e - 4], -c1) - n * c2) * r;
+        acc[0][v][e] = fmaf(y, n, acc[0][v][e]);
+        acc[1][v][e] += y;
         if (PRE) {
-          const f32x4 p1 = one_plus_scale(v, e >> 2);
-          acc[2][v][e] = fmaf(du, x[v][e], acc[2][v][e]);
+          acc[2][v][e] = fmaf(du, x_of(cur[v], e), acc[2][v][e]);
           acc[3][v][e] += du;
-          du *= p1[e & 3];
+          du *= one_plus_scale(v, e >> 2)[e & 3];
         }
         o[e] = du;
       }
@@ -319,62 +335,64 @@ struct NormGradSums {
   int segments, blocks, d, param_f32, pre;
 };
 
-// 32 columns a workgroup; 32 threads share a column's partial sums
+// 8 columns a workgroup; 128 threads share a column's partial sums
 __global__ void __launch_bounds__(1024) norm_grad_sums_kernel(NormGradSums p) {
-  __shared__ float lds[4][32][33];
-  const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
-  const int col = blockIdx.x * 32 + c;
-  const bool ok = col < p.d;
+  __shared__ float lds[16][4][8];
+  const int c = threadIdx.x & 7, r = threadIdx.x >> 3, wave = threadIdx.x >> 6;
+  const int col = blockIdx.x * 8 + c;  // (d is a multiple of 8)
   const int sums = p.pre ? 4 : 2;
-  const float ga = ok ? param_at(p.gamma, p.param_f32, col) : 0.f;
-  const float be = ok && p.beta ? param_at(p.beta, p.param_f32, col) : 0.f;
+  const float ga = param_at(p.gamma, p.param_f32, col);
+  const float be = p.beta ? param_at(p.beta, p.param_f32, col) : 0.f;
   float dgamma = 0.f, dbeta = 0.f;
   for (int seg = 0; seg < p.segments; ++seg) {
     float t[4] = {0.f, 0.f, 0.f, 0.f};
-    if (ok) {
-      const float* q = p.partial + ((int64_t)seg * p.blocks + r) * sums * p.d + col;
-      for (int b = r; b < p.blocks; b += 32, q += (int64_t)32 * sums * p.d) {
-        t[0] += q[0];
-        t[1] += q[p.d];
-        if (p.pre) {
-          t[2] += q[2 * (int64_t)p.d];
-          t[3] += q[3 * (int64_t)p.d];
-        }
+    const float* q = p.partial + ((int64_t)seg * p.blocks + r) * sums * p.d + col;
+#pragma unroll 4
+    for (int b = r; b < p.blocks; b += 128, q += (int64_t)128 * sums * p.d) {
+      t[0] += q[0];
+      t[1] += q[p.d];
+      if (p.pre) {
+        t[2] += q[2 * (int64_t)p.d];
+        t[3] += q[3 * (int64_t)p.d];
       }
     }
 #pragma unroll
-    for (int s = 0; s < 4; ++s) lds[s][r][c] = t[s];
-    __syncthreads();
-    // thread (c, r < 4) finishes sum r of column c
-    float v = 0.f;
-    if (r < 4) {
+    for (int s = 0; s < 4; ++s) {  // over the 8 rows of the wave
+      t[s] += __shfl_xor(t[s], 8);
+      t[s] += __shfl_xor(t[s], 16);
+      t[s] += __shfl_xor(t[s], 32);
+    }
+    if ((threadIdx.x & 63) < 8) {
 #pragma unroll
-      for (int k = 0; k < 32; ++k) v += lds[r][k][c];
+      for (int s = 0; s < 4; ++s) lds[wave][s][c] = t[s];
     }
     __syncthreads();
-    if (r < 4) lds[r][0][c] = v;
-    __syncthreads();
-    if (r == 0 && ok) {
-      const float A = lds[0][0][c], B = lds[1][0][c];
+    if (threadIdx.x < 8) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        t[s] = 0.f;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) t[s] += lds[w][s][c];
+      }
       float ds, dt;
       if (p.pre) {
-        dgamma += A;
-        dbeta += B;
-        ds = lds[2][0][c];
-        dt = lds[3][0][c];
+        dgamma += t[0];
+        dbeta += t[1];
+        ds = t[2];
+        dt = t[3];
       } else {
         const float one = p.scale ? 1.f + p.scale[seg * p.mod_stride + col] : 1.f;
-        dgamma = fmaf(one, A, dgamma);
-        dbeta = fmaf(one, B, dbeta);
-        ds = fmaf(ga, A, be * B);
-        dt = B;
+        dgamma = fmaf(one, t[0], dgamma);
+        dbeta = fmaf(one, t[1], dbeta);
+        ds = fmaf(ga, t[0], be * t[1]);
+        dt = t[1];
       }
       if (p.dscale) p.dscale[(int64_t)seg * p.d + col] = ds;
       if (p.dshift) p.dshift[(int64_t)seg * p.d + col] = dt;
     }
     __syncthreads();
   }
-  if (r == 0 && ok) {
+  if (threadIdx.x < 8) {
     if (p.param_f32) {
       if (p.dgamma) reinterpret_cast<float*>(p.dgamma)[col] = dgamma;
       if (p.dbeta) reinterpret_cast<float*>(p.dbeta)[col] = dbeta;
@@ -389,15 +407,28 @@ bool wants_sums(const aeris_norm_modulate_grad& a) { return a.dgamma || a.dbeta 
 bool is_pre(const aeris_norm_modulate_grad& a) { return a.order == AERIS_MOD_THEN_NORM && (a.shift || a.scale); }
 int64_t segments_of(const aeris_norm_modulate_grad& a) { return (a.shift || a.scale) && a.mod_batch_stride && a.B > 1 ? a.B : 1; }
 
-// Workgroups of a segment: as many as the chip holds of them at two waves a SIMD, and at least some turns each, so that the
-// parameters' and the partial sums' traffic stays small beside the rows'.
+// How a call is run: column groups of a lane, rows at a time, whether a row belongs to several waves.  One wave to a row of up to 2048
+// elements is the faster way (f32 x [259200, 1536] 803 against 834 us, [1036800, 1024] 2155 against 2216), but for many rows of bf16 x whose
+// modulation lies ahead of the norm: four sums a column leave one wave a SIMD, which then waits for its own arithmetic (bf16 [259200, 1536]
+// 830 -> 624 us with four waves to a row, [1036800, 1024] 1381 -> 1330 with two, [20000, 2048] 100 -> 92; [8192, 1536] 44 -> 54).
+struct Shape { int nv, slots, waves; };
+Shape shape_of(const aeris_norm_modulate_grad& a) {
+  if (a.d <= 512) return {1, a.d <= 128 ? 16 : a.d <= 256 ? 8 : 4, 1};
+  if (a.d > 2048) return {a.d <= 4096 ? 2 : 3, 1, 4};
+  if (is_pre(a) && a.x_dtype == AERIS_BF16 && a.B * a.rows_per_batch * a.d >= 30000000) return a.d <= 1024 ? Shape{1, 2, 2} : Shape{1, 1, 4};
+  return {a.d <= 1024 ? 2 : a.d <= 1536 ? 3 : 4, 4, 1};
+}
+
+// Workgroups of a segment: at most one round of what the chip holds of them, and at least 32 rows each, so that the parameters' and the
+// partial sums' traffic stays small beside the rows'.
 int64_t blocks_of(const aeris_norm_modulate_grad& a) {
   const int64_t segments = segments_of(a), rows = a.B * a.rows_per_batch / segments;
-  const int64_t slots = a.d <= 128 ? 16 : a.d <= 256 ? 8 : a.d <= 2048 ? 4 : 1;
-  int64_t n = (rows + slots * 4 - 1) / (slots * 4);
-  const int64_t cap = 1024 / segments > 0 ? 1024 / segments : 1;
-  if (n > cap) n = cap;
-  return n;
+  const Shape s = shape_of(a);
+  const bool pre = is_pre(a);
+  const int held = s.nv == 1 ? pre ? resident<1, true>() : resident<1, false>() : s.nv == 2 ? pre ? resident<2, true>() : resident<2, false>()
+                   : s.nv == 3 ? pre ? resident<3, true>() : resident<3, false>() : pre ? resident<4, true>() : resident<4, false>();
+  const int64_t least = s.slots > 8 ? 2 * s.slots : 32, n = (rows + least - 1) / least, most = 256 * held / segments;
+  return n < most ? n : most > 0 ? most : 1;
 }
 
 template <int NV, int SUB, int WPR>
@@ -412,6 +443,13 @@ hipError_t launch(const NormGradParams& p, bool xf, bool yf, bool pre, int64_t b
     else { if (yf) GO(false, true, false); else GO(false, false, false); }
   }
 #undef GO
+  return hipGetLastError();
+}
+
+template <int WPR>  // (bf16 x, the modulation ahead of the norm: see shape_of)
+hipError_t launch_wide(const NormGradParams& p, bool yf, int64_t blocks, hipStream_t stream) {
+  if (yf) hipLaunchKernelGGL((norm_grad_kernel<1, 1, WPR, false, true, true>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((norm_grad_kernel<1, 1, WPR, false, false, true>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 
@@ -434,21 +472,23 @@ hipError_t norm_grad_launch(const aeris_norm_modulate_grad& a, void* workspace, 
   p.mod_stride = segments > 1 ? a.mod_batch_stride : 0;
   p.rows = a.B * a.rows_per_batch / segments;
   p.blocks_per_segment = (int)blocks_of(a);
-  p.rows_per_block = (p.rows + p.blocks_per_segment - 1) / p.blocks_per_segment;
   p.d = (int)a.d;
   p.kind = (int)a.kind;
   p.param_f32 = a.param_dtype == AERIS_F32;
   p.eps = (float)a.eps;
   const int64_t blocks = segments * p.blocks_per_segment;
+  const Shape f = shape_of(a);
   hipError_t e;
   if (a.d <= 128) e = launch<1, 4, 1>(p, xf, yf, pre, blocks, stream);
   else if (a.d <= 256) e = launch<1, 2, 1>(p, xf, yf, pre, blocks, stream);
   else if (a.d <= 512) e = launch<1, 1, 1>(p, xf, yf, pre, blocks, stream);
-  else if (a.d <= 1024) e = launch<2, 1, 1>(p, xf, yf, pre, blocks, stream);
-  else if (a.d <= 1536) e = launch<3, 1, 1>(p, xf, yf, pre, blocks, stream);
-  else if (a.d <= 2048) e = launch<4, 1, 1>(p, xf, yf, pre, blocks, stream);
-  else if (a.d <= 4096) e = launch<2, 1, 4>(p, xf, yf, pre, blocks, stream);
-  else e = launch<3, 1, 4>(p, xf, yf, pre, blocks, stream);
+  else if (f.waves == 2) e = launch_wide<2>(p, yf, blocks, stream);
+  else if (f.waves == 4 && f.nv == 1) e = launch_wide<4>(p, yf, blocks, stream);
+  else if (f.waves == 4 && f.nv == 2) e = launch<2, 1, 4>(p, xf, yf, pre, blocks, stream);
+  else if (f.waves == 4) e = launch<3, 1, 4>(p, xf, yf, pre, blocks, stream);
+  else if (f.nv == 2) e = launch<2, 1, 1>(p, xf, yf, pre, blocks, stream);
+  else if (f.nv == 3) e = launch<3, 1, 1>(p, xf, yf, pre, blocks, stream);
+  else e = launch<4, 1, 1>(p, xf, yf, pre, blocks, stream);
   if (e != hipSuccess || !p.partial) return e;
   NormGradSums s;
   s.partial = p.partial;
@@ -460,7 +500,7 @@ hipError_t norm_grad_launch(const aeris_norm_modulate_grad& a, void* workspace, 
   s.d = p.d;
   s.param_f32 = p.param_f32;
   s.pre = pre;
-  hipLaunchKernelGGL(norm_grad_sums_kernel, dim3((unsigned)((p.d + 31) / 32)), dim3(1024), 0, stream, s);
+  hipLaunchKernelGGL(norm_grad_sums_kernel, dim3((unsigned)(p.d / 8)), dim3(1024), 0, stream, s);
   return hipGetLastError();
 }
 

@@ -3,7 +3,8 @@
 
 ``norm_modulate``, ``linear`` and ``feed_forward`` return tensors that autograd differentiates once, with the gradients of
 ``ops.norm_modulate_backward``, ``ops.linear_backward`` and ``ops.feed_forward_backward``; their results are those of the calls without
-gradients, and gradients have their tensors' types.  Only the gradients that are asked for are computed.
+gradients, and gradients have their tensors' types.  Only the gradients that are asked for are computed, and nothing is kept where
+none is.
 
 Streams and graphs: calls follow the current stream and hold no scratch memory beyond it, and a forward pass with its backward pass may
 be captured into a HIP graph.  torch's own rule for that holds here too: while the graph is captured, no eager graph of the same leaves
@@ -23,31 +24,29 @@ from . import ops
 
 __all__ = ["feed_forward", "linear", "norm_modulate"]
 
-# leaf -> the eager graphs through it that may still be alive: (weak reference to the node, raw stream)
-_EAGER = torch.utils.weak.WeakIdKeyDictionary()
+_capturing = torch._C._cuda_isCurrentStreamCapturing
+_EAGER = weakref.WeakSet()  # nodes of eager graphs that are alive, each with its stream and the identities of the leaves it was made of
 
 
-def _record(result, leaves):
-    """Notes which eager graph ``result`` made of ``leaves``."""
-    node = result.grad_fn
-    if node is None or torch._C._cuda_isCurrentStreamCapturing():
-        return result
-    entry = (weakref.ref(node), ops._stream())
-    for t in leaves:
-        if t is not None and t.requires_grad and t.is_leaf:
-            live = [e for e in _EAGER.get(t, ()) if e[0]() is not None]
-            _EAGER[t] = live + [entry]
-    return result
+def _wants_grad(leaves):
+    if torch.is_grad_enabled():
+        for t in leaves:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
-def _refuse_under_capture(leaves):
-    if not torch._C._cuda_isCurrentStreamCapturing() or not torch.is_grad_enabled():
+def _note(ctx, leaves):
+    """Notes an eager graph's node and its leaves; under a capture, refuses leaves of such a graph on another stream."""
+    of = [id(t) for t in leaves if t is not None and t.requires_grad and t.is_leaf]
+    if not _capturing():
+        ctx.stream, ctx.leaves = ops._stream(), of
+        _EAGER.add(ctx)
         return
     raw = ops._stream()
-    for t in leaves:
-        if t is not None and any(ref() is not None and stream != raw for ref, stream in _EAGER.get(t, ())):
-            raise RuntimeError("an eager graph of a tensor of this captured call is still alive on another stream: release its result before the capture "
-                               "(torch ties that stream to the capture in the backward pass, which ends the process)")
+    if any(node.stream != raw and not set(of).isdisjoint(node.leaves) for node in list(_EAGER)):
+        raise RuntimeError("an eager graph of a tensor of this captured call is still alive on another stream: release its result before the capture "
+                           "(torch ties that stream to the capture in the backward pass, which ends the process)")
 
 
 def _rows(t: Optional[torch.Tensor]):
@@ -55,24 +54,27 @@ def _rows(t: Optional[torch.Tensor]):
     return t.contiguous() if t is not None and t.dim() == 2 and t.shape[0] > 1 and t.stride(0) == 0 else t
 
 
+def _norm(x, gamma, beta, shift, scale, kind, order, eps, out_dtype):
+    if x.numel() == 0:
+        return torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    return ops.norm_modulate(x, gamma, beta, shift, scale, kind=kind, order=order, eps=eps, out_dtype=out_dtype)
+
+
 class _NormModulate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gamma, beta, shift, scale, kind, order, eps, out_dtype):
+        _note(ctx, (x, gamma, beta, shift, scale))
         shift, scale = _rows(shift), _rows(scale)
-        if x.numel() == 0:
-            y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-        else:
-            y = ops.norm_modulate(x, gamma, beta, shift, scale, kind=kind, order=order, eps=eps, out_dtype=out_dtype)
+        y = _norm(x, gamma, beta, shift, scale, kind, order, eps, out_dtype)
         ctx.save_for_backward(x, gamma, beta, shift, scale)
-        ctx.how = kind, order, eps
+        mod = shift if shift is not None else scale
+        ctx.how = mod.stride(0) if mod is not None and mod.shape[0] > 1 else 0, ops._KIND[kind], ops._ORDER[order], eps
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        kind, order, eps = ctx.how
-        return (*ops.norm_modulate_backward(dy.contiguous(), *ctx.saved_tensors, kind=kind, order=order, eps=eps, wanted=ctx.needs_input_grad[:5]),
-                None, None, None, None)
+        return (*ops._norm_grads(dy.contiguous(), *ctx.saved_tensors, *ctx.how, ctx.needs_input_grad[:5]), None, None, None, None)
 
 
 def norm_modulate(x: torch.Tensor, gamma: torch.Tensor, beta: Optional[torch.Tensor] = None, shift: Optional[torch.Tensor] = None,
@@ -83,39 +85,39 @@ def norm_modulate(x: torch.Tensor, gamma: torch.Tensor, beta: Optional[torch.Ten
     x [B, S, d] (bf16 | f32, contiguous) -> [B, S, d] in out_dtype; gamma, beta bf16 | f32 [d]; shift, scale f32 [1 | B, d], both of one shape."""
     if kind not in ops._KIND or order not in ops._ORDER:
         raise RuntimeError(f"kind must be one of {sorted(ops._KIND)} and order one of {sorted(ops._ORDER)}, got {kind!r}, {order!r}")
+    leaves = (x, gamma, beta, shift, scale)
     ops._on_current_device(x.device, dict(x=x, gamma=gamma, beta=beta, shift=shift, scale=scale))
     if x.dtype not in ops._DT or gamma.dtype not in ops._DT or out_dtype not in ops._DT:
         raise RuntimeError(f"x, gamma and the result must be bf16 or f32, got {x.dtype}, {gamma.dtype} and {out_dtype}")
     if x.dim() != 3 or gamma.shape != x.shape[2:] or (beta is not None and beta.shape != gamma.shape):
         raise RuntimeError(f"x must be [B, S, d], gamma and beta [d], got {tuple(x.shape)}, {tuple(gamma.shape)}")
-    if shift is not None and scale is not None and shift.shape != scale.shape:
-        raise RuntimeError(f"shift and scale must be of one shape, got {tuple(shift.shape)} and {tuple(scale.shape)}")
-    leaves = (x, gamma, beta, shift, scale)
-    _refuse_under_capture(leaves)
-    return _record(_NormModulate.apply(*leaves, kind, order, eps, out_dtype), leaves)
+    if shift is not None and scale is not None and (shift.shape != scale.shape or shift.stride(0) != scale.stride(0)):
+        raise RuntimeError(f"shift and scale must be of one shape and layout, got {tuple(shift.shape)} and {tuple(scale.shape)}")
+    if not _wants_grad(leaves):
+        return _norm(*leaves, kind, order, eps, out_dtype)
+    return _NormModulate.apply(*leaves, kind, order, eps, out_dtype)
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, a, w, bias, residual, act, out_dtype):
-        y, z = ops.linear_train(a, w, bias, act=act, residual=residual, out_dtype=out_dtype)
+    def forward(ctx, a, w, bias, residual, act, out_dtype, M, N, K):
+        _note(ctx, (a, w, bias, residual))
+        y, z = ops._linear_forward(a, w, bias, residual, act, out_dtype, M, N, K, ctx.needs_input_grad[0] or ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
         ctx.save_for_backward(a, w, z)
-        ctx.act, ctx.res_dtype = act, None if residual is None else residual.dtype
+        ctx.how = ops._ACT[act], M, N, K
+        ctx.res_dtype = None if residual is None else residual.dtype
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        a, w, z = ctx.saved_tensors
         need_a, need_w, need_bias, need_res = ctx.needs_input_grad[:4]
-        plain = ctx.act in (None, "none")
         dy = dy.contiguous()
-        round_res = need_res and ctx.res_dtype is not dy.dtype and plain and dy.dtype is torch.float32  # dz is what a bf16 residual gets
-        da, dw, dbias, dz = ops.linear_backward(dy, a, w, z, act=ctx.act, wanted=(need_a, need_w, need_bias, round_res))
-        dres = None
-        if need_res:
-            dres = dz if round_res else dy.to(ctx.res_dtype)
-        return da, dw, dbias, dres, None, None
+        round_res = need_res and ctx.res_dtype is not dy.dtype and dy.dtype is torch.float32 and ctx.how[0] == ops.L.ACT_NONE  # dz is what a bf16 residual gets
+        da, dw, dbias, dres = ops._linear_grads(dy, *ctx.saved_tensors, *ctx.how, (need_a, need_w, need_bias, round_res))
+        if need_res and not round_res:
+            dres = dy.to(ctx.res_dtype)
+        return da, dw, dbias, dres, None, None, None, None, None
 
 
 def linear(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *, act: Optional[str] = None,
@@ -123,32 +125,37 @@ def linear(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     """act(a[.., K] @ w[N, K]^T + bias) + residual, differentiable in all four; act None | "gelu" (erf) | "silu".
 
     a, w, bias bf16, residual [.., N] bf16 | f32, the result in out_dtype (bf16 | f32); contiguous; N a multiple of 8, K of 64 (with an
-    activation: of 8).  With an activation the bf16 value it is applied to is kept for the backward pass, otherwise a and w alone."""
+    activation: of 8).  With an activation the value it is applied to is kept for the backward pass too (24 bits), otherwise a and w alone."""
     leaves = (a, w, bias, residual)
     ops._on_current_device(a.device, dict(a=a, w=w, bias=bias, residual=residual))
-    _refuse_under_capture(leaves)
-    return _record(_Linear.apply(*leaves, act, out_dtype), leaves)
+    sizes = ops._checked_linear(a, w, bias, residual, act, out_dtype)
+    if not _wants_grad(leaves):
+        return ops._linear_forward(a, w, bias, residual, act, out_dtype, *sizes, False)[0]
+    return _Linear.apply(*leaves, act, out_dtype, *sizes)
 
 
 class _FeedForward(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w1, w2):
-        y, gate_up, h = ops.feed_forward_train(x, w1, w2)
+    def forward(ctx, x, w1, w2, M, d, H):
+        _note(ctx, (x, w1, w2))
+        y, gate_up, h = ops._feed_forward(x, w1, w2, M, d, H, True)
         ctx.save_for_backward(x, w1, w2, gate_up, h)
+        ctx.sizes = M, d, H
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        return ops.feed_forward_backward(dy.contiguous(), *ctx.saved_tensors, wanted=ctx.needs_input_grad)
+        return (*ops._feed_forward_grads(dy.contiguous(), *ctx.saved_tensors, *ctx.sizes, ctx.needs_input_grad[:3]), None, None, None)
 
 
 def feed_forward(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor) -> torch.Tensor:
     """The gated MLP ``FeedForward`` (model.py:148-159), w2 (silu(gate) * up) with [gate | up] = w1 x, differentiable in x, w1 and w2.
 
-    x bf16 [.., d], w1 bf16 [2H, d], w2 bf16 [d, H], contiguous, d and H multiples of 8 -> bf16 [.., d].  gate, up and their product (bf16,
-    3 H numbers a token) are kept for the backward pass."""
-    leaves = (x, w1, w2)
+    x bf16 [.., d], w1 bf16 [2H, d], w2 bf16 [d, H], contiguous, d and H multiples of 8 -> bf16 [.., d].  gate and up (24
+    bits) and their product (bf16) are kept for the backward pass: 8 H bytes a token."""
     ops._on_current_device(x.device, dict(x=x, w1=w1, w2=w2))
-    _refuse_under_capture(leaves)
-    return _record(_FeedForward.apply(*leaves), leaves)
+    sizes = ops._checked_feed_forward(x, w1, w2)
+    if not _wants_grad((x, w1, w2)):
+        return ops._feed_forward(x, w1, w2, *sizes, False)[0]
+    return _FeedForward.apply(x, w1, w2, *sizes)

@@ -335,23 +335,33 @@ def norm_modulate_backward(dy: torch.Tensor, x: torch.Tensor, gamma: torch.Tenso
         _dev(beta, "beta", gamma.dtype)
         if beta.shape != (d,):
             raise RuntimeError(f"beta must be [{d}], got {tuple(beta.shape)}")
-    sh_ptr, st1 = _rowvec(shift, "shift", d, B)
-    sc_ptr, st2 = _rowvec(scale, "scale", d, B)
+    _, st1 = _rowvec(shift, "shift", d, B)
+    _, st2 = _rowvec(scale, "scale", d, B)
     if shift is not None and scale is not None and (st1 != st2 or shift.shape != scale.shape):
         raise RuntimeError("shift and scale must share their shape and batch stride")
     mod = shift if shift is not None else scale
     if mod is not None and mod.shape[0] > 1 and max(st1, st2) == 0:
         raise RuntimeError("shift and scale of several members must have memory of their own for each")
+    return _norm_grads(dy, x, gamma, beta, shift, scale, max(st1, st2), _KIND[kind], _ORDER[order], eps, wanted)
+
+
+def _norm_grads(dy, x, gamma, beta, shift, scale, stride, kind, order, eps, wanted):
+    """``norm_modulate_backward`` for checked arguments."""
     tensors = (x, gamma, beta, shift, scale)
-    if x.numel() == 0:
-        return tuple(torch.zeros_like(t, memory_format=torch.contiguous_format) if w and t is not None else None for t, w in zip(tensors, wanted))
-    out = tuple(torch.empty_like(t, memory_format=torch.contiguous_format) if w and t is not None else None for t, w in zip(tensors, wanted))
-    call = NORM_GRAD.pack(x.data_ptr(), dy.data_ptr(), gamma.data_ptr(), _ptr(beta) or 0, sh_ptr or 0, sc_ptr or 0, *(_ptr(t) or 0 for t in out),
-                          B, S, d, max(st1, st2), _DT[x.dtype], _DT[dy.dtype], _DT[gamma.dtype], _KIND[kind], _ORDER[order], eps)
+    make = torch.empty_like if x.numel() else torch.zeros_like
+    out = [make(t, memory_format=torch.contiguous_format) if w and t is not None else None for t, w in zip(tensors, wanted)]
+    if not x.numel():
+        return out
+    B, S, d = x.shape
+    call = NORM_GRAD.pack(x.data_ptr(), dy.data_ptr(), gamma.data_ptr(), *(0 if t is None else t.data_ptr() for t in (beta, shift, scale, *out)),
+                          B, S, d, stride, _DT[x.dtype], _DT[dy.dtype], _DT[gamma.dtype], kind, order, eps)
     need = L.lib().aeris_norm_modulate_grad_workspace_bytes(call)
     held, ws = _scratch_ptr(need, x.device)
-    with _timed("norm_modulate_backward", float(x.numel() * (2 * x.element_size() + dy.element_size())), "byte"):
+    if _profile is None:
         L.call("aeris_norm_modulate_bwd", call, ws, need, _stream())
+    else:
+        with _timed("norm_modulate_backward", float(x.numel() * (2 * x.element_size() + dy.element_size())), "byte"):
+            L.call("aeris_norm_modulate_bwd", call, ws, need, _stream())
     return out
 
 
@@ -496,37 +506,48 @@ def _train_widths(*widths):
             raise RuntimeError(f"widths must be positive multiples of 8 for the gradients' products, got {n}")
 
 
-def linear_train(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *, act: Optional[str] = None,
-                 residual: Optional[torch.Tensor] = None, out_dtype=torch.bfloat16):
-    """``gemm`` of a training step: (act(a[.., K] @ w[N, K]^T + bias) + residual [.., N] in out_dtype, what ``linear_backward`` needs beside a and w: the
-    bf16 value that the activation was applied to, or None without activation).  K, N multiples of 8 (without activation: K of 64)."""
-    if act not in (None, "none", "gelu", "silu"):
-        raise RuntimeError(f"act must be None, 'gelu' or 'silu', got {act!r}")
-    _on_current_device(a.device, dict(a=a, w=w, bias=bias, residual=residual))
-    if w.dim() != 2 or a.dim() < 1:
-        raise RuntimeError(f"a must be [.., K] and w [N, K], got {tuple(a.shape)} and {tuple(w.shape)}")
+def _checked_linear(a, w, bias, residual, act, out_dtype):
+    """The sizes of a projection whose tensors are what ``linear_train`` takes."""
+    if a.dtype is not torch.bfloat16 or w.dtype is not torch.bfloat16 or w.dim() != 2 or a.dim() < 1 or not a.is_contiguous() or not w.is_contiguous() or a.shape[-1] != w.shape[1]:
+        raise RuntimeError(f"a must be contiguous bf16 [.., K] and w [N, K], got {a.dtype} {tuple(a.shape)} and {w.dtype} {tuple(w.shape)}")
     N, K = w.shape
     _train_widths(N, K)
     M = a.numel() // K
-    _matrix(a, "a", M, K)
-    _matrix(w, "w", N, K)
-    if out_dtype not in _DT:
-        raise RuntimeError("out_dtype must be bf16 or f32")
-    if bias is not None and bias.shape != (N,):
-        raise RuntimeError(f"bias must be [{N}], got {tuple(bias.shape)}")
-    if residual is not None:
-        _matrix(residual, "residual", M, N, tuple(_DT))
-    shape = (*a.shape[:-1], N)
+    if act not in _ACT or act == "swiglu" or out_dtype not in _DT:
+        raise RuntimeError(f"act must be None, 'gelu' or 'silu' and the result bf16 or f32, got {act!r}, {out_dtype}")
+    if bias is not None and (bias.shape != (N,) or bias.dtype is not torch.bfloat16 or not bias.is_contiguous()):
+        raise RuntimeError(f"bias must be contiguous bf16 [{N}], got {bias.dtype} {tuple(bias.shape)}")
+    if residual is not None and (residual.dtype not in _DT or residual.numel() != M * N or residual.shape[-1] != N or not residual.is_contiguous()):
+        raise RuntimeError(f"residual must be contiguous bf16 or f32 [{M}, {N}], got {residual.dtype} {tuple(residual.shape)}")
+    return M, N, K
+
+
+def linear_train(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, *, act: Optional[str] = None,
+                 residual: Optional[torch.Tensor] = None, out_dtype=torch.bfloat16, keep: bool = True):
+    """``gemm`` of a training step: (act(a[.., K] @ w[N, K]^T + bias) + residual [.., N] in out_dtype, what ``linear_backward`` needs beside a and w: the
+    value that the activation was applied to, in 24 bits (uint8 [M * N * 3]), or None without activation or ``keep``).  K, N multiples of 8 (without
+    activation: K of 64)."""
+    _on_current_device(a.device, dict(a=a, w=w, bias=bias, residual=residual))
+    M, N, K = _checked_linear(a, w, bias, residual, act, out_dtype)
+    return _linear_forward(a, w, bias, residual, act, out_dtype, M, N, K, keep)
+
+
+def _linear_forward(a, w, bias, residual, act, out_dtype, M, N, K, keep):
+    """``linear_train`` for checked arguments."""
+    code, device = _ACT[act], a.device
+    y = torch.empty(*a.shape[:-1], N, dtype=out_dtype, device=device)
+    z = torch.empty(3 * M * N, dtype=torch.uint8, device=device) if keep and code in _KEPT else None
     if M == 0:
-        return torch.empty(shape, dtype=out_dtype, device=a.device), None if _ACT[act] not in _KEPT else torch.empty(shape, dtype=torch.bfloat16, device=a.device)
-    if _ACT[act] not in _KEPT:
-        return gemm(a, w, bias, residual=residual, out_dtype=out_dtype), None
-    if bias is not None:
-        _dev(bias, "bias", torch.bfloat16)
-    y, z = torch.empty(shape, dtype=out_dtype, device=a.device), torch.empty(shape, dtype=torch.bfloat16, device=a.device)
-    with _timed("linear_train", 2.0 * M * N * K, "flop"):
-        L.call("aeris_linear_train_fwd", LINEAR_TRAIN.pack(a.data_ptr(), w.data_ptr(), _ptr(bias) or 0, _ptr(residual) or 0, y.data_ptr(), z.data_ptr(), M, N, K,
-                                                           _ACT[act], 0 if residual is None else _DT[residual.dtype], _DT[out_dtype]), _stream())
+        return y, z
+    if code not in _KEPT:
+        return gemm(a, w, bias, residual=residual, out=y), None
+    call = LINEAR_TRAIN.pack(a.data_ptr(), w.data_ptr(), _ptr(bias) or 0, _ptr(residual) or 0, y.data_ptr(), _ptr(z) or 0, M, N, K, code,
+                             0 if residual is None else _DT[residual.dtype], _DT[out_dtype])
+    if _profile is None:
+        L.call("aeris_linear_train_fwd", call, _stream())
+    else:
+        with _timed("linear_train", 2.0 * M * N * K, "flop"):
+            L.call("aeris_linear_train_fwd", call, _stream())
     return y, z
 
 
@@ -535,56 +556,71 @@ def linear_backward(dy: torch.Tensor, a: torch.Tensor, w: torch.Tensor, z: Optio
     """Gradients of ``linear_train`` from that of its result, dy [.., N] (bf16 | f32) -> (da bf16, dw bf16, dbias bf16 [N], dz bf16 [.., N]), None where
     ``wanted`` says so.  dz = dy act'(z) is rounded to bf16 for the products; dbias sums it unrounded.  (dz without activation: dy in bf16.)"""
     _on_current_device(dy.device, dict(dy=dy, a=a, w=w, z=z))
-    N, K = w.shape
-    _train_widths(N, K)
-    M = a.numel() // K
-    _matrix(a, "a", M, K)
-    _matrix(w, "w", N, K)
+    M, N, K = _checked_linear(a, w, None, None, act, dy.dtype)
     _matrix(dy, "dy", M, N, tuple(_DT))
-    kept = _ACT[act] in _KEPT
-    if kept:
+    if _ACT[act] in _KEPT:
         if z is None:
             raise RuntimeError("an activation's gradient needs z")
-        _matrix(z, "z", M, N)
-    elif _ACT[act] != L.ACT_NONE:
-        raise RuntimeError(f"act must be None, 'gelu' or 'silu', got {act!r}")
+        _matrix(z, "z", 1, 3 * M * N, (torch.uint8,))
+    return _linear_grads(dy, a, w, z, _ACT[act], M, N, K, wanted)
+
+
+def _linear_grads(dy, a, w, z, code, M, N, K, wanted):
+    """``linear_backward`` for checked arguments."""
+    want_a, want_w, want_bias, want_dz = wanted
     bf16, device = torch.bfloat16, dy.device
-    same = not kept and dy.dtype is bf16  # dz is dy
+    same = code == L.ACT_NONE and dy.dtype is bf16  # dz is dy
+    da = torch.empty_like(a) if want_a else None
     if M == 0:
-        return (torch.empty_like(a) if wanted[0] else None, torch.zeros_like(w) if wanted[1] else None,
-                torch.zeros(N, dtype=bf16, device=device) if wanted[2] else None, dy.to(bf16) if wanted[3] else None)
-    da = torch.empty_like(a) if wanted[0] else None
-    dw = torch.empty_like(w) if wanted[1] else None
-    dbias = torch.empty(N, dtype=bf16, device=device) if wanted[2] else None
-    dz = torch.empty(dy.shape, dtype=bf16, device=device) if wanted[3] and not same else None
-    if not (da is None and dw is None and dbias is None and dz is None):
-        call = LINEAR_GRAD.pack(dy.data_ptr(), a.data_ptr(), w.data_ptr(), z.data_ptr() if kept else 0, _ptr(da) or 0, _ptr(dw) or 0, _ptr(dbias) or 0, _ptr(dz) or 0,
-                                M, N, K, _ACT[act], _DT[dy.dtype])
+        return da, torch.zeros_like(w) if want_w else None, torch.zeros(N, dtype=bf16, device=device) if want_bias else None, dy.to(bf16) if want_dz else None
+    dw = torch.empty_like(w) if want_w else None
+    dbias = torch.empty(N, dtype=bf16, device=device) if want_bias else None
+    dz = torch.empty(dy.shape, dtype=bf16, device=device) if want_dz and not same else None
+    if want_a or want_w or want_bias or dz is not None:
+        call = LINEAR_GRAD.pack(dy.data_ptr(), a.data_ptr(), w.data_ptr(), 0 if z is None else z.data_ptr(), da.data_ptr() if want_a else 0, dw.data_ptr() if want_w else 0,
+                                dbias.data_ptr() if want_bias else 0, 0 if dz is None else dz.data_ptr(), M, N, K, code, _DT[dy.dtype])
         need = L.lib().aeris_linear_grad_workspace_bytes(call)
         held, ws = _scratch_ptr(need, device)
-        with _timed("linear_backward", 2.0 * M * N * K * ((da is not None) + (dw is not None)), "flop"):
+        if _profile is None:
             L.call("aeris_linear_bwd", call, ws, need, _stream())
-    return da, dw, dbias, dy if wanted[3] and same else dz
+        else:
+            with _timed("linear_backward", 2.0 * M * N * K * (want_a + want_w), "flop"):
+                L.call("aeris_linear_bwd", call, ws, need, _stream())
+    return da, dw, dbias, dy if want_dz and same else dz
 
 
-def feed_forward_train(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor):
-    """The gated MLP of a training step, w2[d, H] (silu(gate) * up) with [gate | up] = x[.., d] @ w1[2H, d]^T -> (y bf16 [.., d], gate_up bf16 [.., 2H],
-    h bf16 [.., H]): the result and what ``feed_forward_backward`` needs beside x, w1 and w2.  d, H multiples of 8."""
-    _on_current_device(x.device, dict(x=x, w1=w1, w2=w2))
-    if w2.dim() != 2 or w1.dim() != 2 or x.dim() < 1:
-        raise RuntimeError(f"x must be [.., d], w1 [2H, d] and w2 [d, H], got {tuple(x.shape)}, {tuple(w1.shape)} and {tuple(w2.shape)}")
+def _checked_feed_forward(x, w1, w2):
+    bf16 = torch.bfloat16
+    if (w2.dim() != 2 or x.dim() < 1 or x.shape[-1] != w2.shape[0] or w1.shape != (2 * w2.shape[1], w2.shape[0]) or x.dtype is not bf16 or w1.dtype is not bf16 or
+            w2.dtype is not bf16 or not x.is_contiguous() or not w1.is_contiguous() or not w2.is_contiguous()):
+        raise RuntimeError(f"x must be [.., d], w1 [2H, d] and w2 [d, H], bf16 and contiguous, got {x.dtype} {tuple(x.shape)}, {w1.dtype} {tuple(w1.shape)} and {w2.dtype} {tuple(w2.shape)}")
     d, H = w2.shape
     _train_widths(d, H)
-    M = x.numel() // d
-    _matrix(x, "x", M, d)
-    _matrix(w1, "w1", 2 * H, d)
-    _matrix(w2, "w2", d, H)
+    return x.numel() // d, d, H
+
+
+def feed_forward_train(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, keep: bool = True):
+    """The gated MLP of a training step, w2[d, H] (silu(gate) * up) with [gate | up] = x[.., d] @ w1[2H, d]^T -> (y bf16 [.., d], gate_up: gate and up in 24 bits
+    (uint8 [M * 2H * 3], None without ``keep``), h bf16 [.., H]): the result and what ``feed_forward_backward`` needs beside x, w1 and w2.  d, H multiples of 8."""
+    _on_current_device(x.device, dict(x=x, w1=w1, w2=w2))
+    return _feed_forward(x, w1, w2, *_checked_feed_forward(x, w1, w2), keep)
+
+
+def _feed_forward(x, w1, w2, M, d, H, keep):
+    """``feed_forward_train`` for checked arguments."""
+    device = x.device
     y = torch.empty_like(x)
-    gate_up = torch.empty(*x.shape[:-1], 2 * H, dtype=torch.bfloat16, device=x.device)
-    h = torch.empty(*x.shape[:-1], H, dtype=torch.bfloat16, device=x.device)
+    gate_up = torch.empty(6 * M * H, dtype=torch.uint8, device=device) if keep else None
+    h = torch.empty(*x.shape[:-1], H, dtype=torch.bfloat16, device=device)
     if M:
-        with _timed("feed_forward_train", 6.0 * M * H * d, "flop"):
-            L.call("aeris_feed_forward_train_fwd", FEED_FORWARD.pack(x.data_ptr(), w1.data_ptr(), w2.data_ptr(), gate_up.data_ptr(), h.data_ptr(), y.data_ptr(), M, d, H), _stream())
+        call = FEED_FORWARD.pack(x.data_ptr(), w1.data_ptr(), w2.data_ptr(), gate_up.data_ptr() if keep else 0, h.data_ptr(), y.data_ptr(), M, d, H)
+        need = L.lib().aeris_feed_forward_workspace_bytes(call)
+        held, ws = _scratch_ptr(need, device)
+        if _profile is None:
+            L.call("aeris_feed_forward_train_fwd", call, ws, need, _stream())
+        else:
+            with _timed("feed_forward_train", 6.0 * M * H * d, "flop"):
+                L.call("aeris_feed_forward_train_fwd", call, ws, need, _stream())
     return y, gate_up, h
 
 
@@ -592,22 +628,29 @@ def feed_forward_backward(dy: torch.Tensor, x: torch.Tensor, w1: torch.Tensor, w
                           wanted=(True, True, True)):
     """Gradients of ``feed_forward_train`` from that of its result, dy bf16 [.., d] -> (dx, dw1, dw2) bf16, None where ``wanted`` says so."""
     _on_current_device(dy.device, dict(dy=dy, x=x, w1=w1, w2=w2, gate_up=gate_up, h=h))
-    d, H = w2.shape
-    _train_widths(d, H)
-    M = x.numel() // d
-    for t, name, rows, cols in ((x, "x", M, d), (w1, "w1", 2 * H, d), (w2, "w2", d, H), (dy, "dy", M, d), (gate_up, "gate_up", M, 2 * H), (h, "h", M, H)):
-        _matrix(t, name, rows, cols)
+    M, d, H = _checked_feed_forward(x, w1, w2)
+    _matrix(dy, "dy", M, d)
+    _matrix(h, "h", M, H)
+    _matrix(gate_up, "gate_up", 1, 6 * M * H, (torch.uint8,))
+    return _feed_forward_grads(dy, x, w1, w2, gate_up, h, M, d, H, wanted)
+
+
+def _feed_forward_grads(dy, x, w1, w2, gate_up, h, M, d, H, wanted):
+    """``feed_forward_backward`` for checked arguments."""
     if M == 0:
-        return tuple(torch.zeros_like(t) if w else None for t, w in zip((x, w1, w2), wanted))
-    dx, dw1, dw2 = (torch.empty_like(t) if w else None for t, w in zip((x, w1, w2), wanted))
+        return [torch.zeros_like(t) if w else None for t, w in zip((x, w1, w2), wanted)]
+    out = [torch.empty_like(t) if w else None for t, w in zip((x, w1, w2), wanted)]
     if any(wanted):
-        call = FEED_FORWARD_GRAD.pack(dy.data_ptr(), x.data_ptr(), w1.data_ptr(), w2.data_ptr(), gate_up.data_ptr(), h.data_ptr(), _ptr(dx) or 0, _ptr(dw1) or 0,
-                                      _ptr(dw2) or 0, M, d, H)
+        call = FEED_FORWARD_GRAD.pack(dy.data_ptr(), x.data_ptr(), w1.data_ptr(), w2.data_ptr(), gate_up.data_ptr(), h.data_ptr(),
+                                      *(0 if t is None else t.data_ptr() for t in out), M, d, H)
         need = L.lib().aeris_feed_forward_grad_workspace_bytes(call)
         held, ws = _scratch_ptr(need, x.device)
-        with _timed("feed_forward_backward", 2.0 * M * H * d * (bool(wanted[0] or wanted[1]) + 2 * wanted[0] + 2 * wanted[1] + wanted[2]), "flop"):
+        if _profile is None:
             L.call("aeris_feed_forward_bwd", call, ws, need, _stream())
-    return dx, dw1, dw2
+        else:
+            with _timed("feed_forward_backward", 2.0 * M * H * d * (bool(wanted[0] or wanted[1]) + 2 * wanted[0] + 2 * wanted[1] + wanted[2]), "flop"):
+                L.call("aeris_feed_forward_bwd", call, ws, need, _stream())
+    return out
 
 
 def _on_current_device(device, tensors):

@@ -202,7 +202,7 @@ int aeris_gemm_fwd(const void* A, const void* W, void* C, const void* bias, cons
 
 /* A projection of a training step (nn.Linear at model.py:153-154,284-285 with what follows it), for activations whose gradient needs the value they
  * were applied to:
- *   z = x w^T + bias (bf16, kept for the backward pass), y = act(z in fp32) + residual
+ *   z = x w^T + bias, y = act(z) + residual; z is kept for the backward pass, in 24 bits (3 M N bytes; z NULL: not kept)
  *   x bf16 [M, K], w bf16 [N, K], bias bf16 [N] or NULL, residual [M, N] (res_dtype) or NULL, y [M, N] (y_dtype); act AERIS_ACT_GELU (erf) | AERIS_ACT_SILU
  * (without an activation nothing has to be kept: aeris_gemm_fwd).
  * Gradients, from that of y (dy [M, N], dy_dtype):  dz = dy act'(z) (rounded to bf16 for the products), written unless NULL:
@@ -226,7 +226,7 @@ int64_t aeris_linear_grad_workspace_bytes(const aeris_linear_grad* a);
 int aeris_linear_bwd(const aeris_linear_grad* a, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* The gated MLP (FeedForward, model.py:148-159) of a training step:
- *   [gate | up] = x w1^T (bf16 [M, 2H], kept), h = silu(gate) up (bf16 [M, H], kept), y bf16 [M, d] = h w2^T
+ *   [gate | up] = x w1^T (kept in 24 bits: gate_up, 6 M H bytes; gate_up NULL: not kept), h = silu(gate) up (bf16 [M, H], kept), y bf16 [M, d] = h w2^T
  *   x bf16 [M, d], w1 bf16 [2H, d], w2 bf16 [d, H]; gate, up and their product are made in fp32 in one kernel
  * Gradients, from dy bf16 [M, d], each unless NULL:  dh = dy w2 (fp32, never in memory), dgate = dh up silu'(gate), dup = dh silu(gate) (bf16);
  *   dx bf16 [M, d] = [dgate | dup] w1;  dw1 bf16 [2H, d] = [dgate | dup]^T x;  dw2 bf16 [d, H] = dy^T h
@@ -236,7 +236,8 @@ typedef struct aeris_feed_forward {
   void *gate_up, *h, *y;
   int64_t M, d, H;
 } aeris_feed_forward;
-int aeris_feed_forward_train_fwd(const aeris_feed_forward* a, void* stream);
+int64_t aeris_feed_forward_workspace_bytes(const aeris_feed_forward* a);
+int aeris_feed_forward_train_fwd(const aeris_feed_forward* a, void* workspace, int64_t workspace_bytes, void* stream);
 typedef struct aeris_feed_forward_grad {
   const void *dy, *x, *w1, *w2, *gate_up, *h;
   void *dx, *dw1, *dw2;

@@ -12,6 +12,7 @@ import pytest
 import torch
 
 U, E, SLACK = 2.0 ** -8, 2.0 ** -24, 1.02
+KEPT = 2.0 ** -16  # half a step of the 24-bit values (15 bits of fraction) that a forward pass keeps
 LIP, LIP2, FN = 1.13, 0.8, 1e-6
 BF16, F32 = torch.bfloat16, torch.float32
 
@@ -218,6 +219,12 @@ def test_norm_nan_and_infinity_stay_in_their_row(pkg, cuda):
 # ----------------------------------------------------------------------------------------------
 # projections
 
+def kept(z):
+    """Values as they are kept for the backward pass: the upper 16 bits of all of them, then bits 8 to 15."""
+    bits = z.float().contiguous().flatten().view(torch.int32)
+    return torch.cat([(bits >> 16).to(torch.int16).view(torch.uint8), ((bits >> 8) & 255).to(torch.uint8)])
+
+
 def act_of(z, act):
     if act == "gelu":
         return z * torch.special.ndtr(z)
@@ -250,15 +257,15 @@ def check_linear(pkg, cuda, g, M, N, K, act, bias, residual, y_dtype, lead=None)
     A, W, D = a.double().abs(), w.double().abs(), dy.double().abs()
     ez = (K + 3) * E * (A @ W.T + (b.double().abs() if bias else 0))
     z = z.detach()
-    kept = act in ("gelu", "silu")
-    ey = (LIP * ez + FN * z.abs().clamp_min(1)) if kept else ez
+    bent = act in ("gelu", "silu")
+    ey = (LIP * ez + FN * z.abs().clamp_min(1)) if bent else ez
     ey = ey + (half_step(y_dtype) + 2 * E) * (want_y.detach().abs() + ey) + 2 * E * (act_of(z, act).abs())
     close(y.view(M, N), want_y.detach(), ey, "y")
-    ez = ez + U * z.abs()  # as kept
+    ez = ez + KEPT * z.abs()  # as kept
     zz = z.clone().requires_grad_()
     dz = torch.autograd.grad(act_of(zz, act), zz, dy.double())[0]
-    edz = D * (LIP2 * ez + FN * z.abs().clamp_min(1)) if kept else torch.zeros_like(dz)
-    edzr = edz + (U * (dz.abs() + edz) if kept or y_dtype is F32 else 0)  # rounded for the products
+    edz = D * (LIP2 * ez + FN * z.abs().clamp_min(1)) if bent else torch.zeros_like(dz)
+    edzr = edz + (U * (dz.abs() + edz) if bent or y_dtype is F32 else 0)  # rounded for the products
     Z = dz.abs()
     close(got["a"].view(M, K), want["a"], edzr @ W + (N + 2) * E * (Z @ W) + U * want["a"].abs(), "da")
     close(got["w"], want["w"], edzr.T @ A + (M + 70) * E * (Z.T @ A) + U * want["w"].abs(), "dw")
@@ -327,7 +334,7 @@ def test_activation_gradients_of_any_value(pkg, cuda, act):
     n = z.numel() // 8 * 8
     z = z[:n].view(-1, 8)
     dy, a, w = torch.ones_like(z), torch.zeros(z.shape[0], 8, dtype=BF16), torch.zeros(8, 8, dtype=BF16)
-    dz = pkg.ops.linear_backward(dy.to(cuda), a.to(cuda), w.to(cuda), z.to(cuda), act=act, wanted=(False, False, False, True))[3].double().cpu()
+    dz = pkg.ops.linear_backward(dy.to(cuda), a.to(cuda), w.to(cuda), kept(z).to(cuda), act=act, wanted=(False, False, False, True))[3].double().cpu()
     x = z.double()
     if act == "gelu":
         want = torch.special.ndtr(x) + torch.where(x.abs() < 1e3, x * (-0.5 * x * x).exp(), 0.0) / math.sqrt(2 * math.pi)
@@ -336,7 +343,7 @@ def test_activation_gradients_of_any_value(pkg, cuda, act):
         want = s + torch.where(x.abs() < 1e3, x * s * (1 - s), 0.0)
     close(dz, want, U * want.abs() + FN, act)
     bad = torch.tensor([[math.nan] * 8], dtype=BF16)
-    dz = pkg.ops.linear_backward(dy[:1].to(cuda), a[:1].to(cuda), w.to(cuda), bad.to(cuda), act=act, wanted=(False, False, False, True))[3]
+    dz = pkg.ops.linear_backward(dy[:1].to(cuda), a[:1].to(cuda), w.to(cuda), kept(bad).to(cuda), act=act, wanted=(False, False, False, True))[3]
     assert torch.isnan(dz).all()
 
 
@@ -365,7 +372,7 @@ def check_feed_forward(pkg, cuda, g, M, d, H, lead=None, loud=1.0):
     eh = (LIP * eg + fn) * up.abs() + silu.abs() * eu + 4 * E * h
     eh = eh + U * (h + eh)
     close(y.view(M, d), want_y.detach(), eh @ W2.T + (H + 2) * E * (h @ W2.T) + U * want_y.detach().abs(), "y")
-    eg, eu = eg + U * gate.abs(), eu + U * up.abs()  # as kept
+    eg, eu = eg + KEPT * gate.abs(), eu + KEPT * up.abs()  # as kept
     dh = (dy.double() @ w2.double()).abs()
     edh = (d + 2) * E * (D @ W2)
     dup, dgate = dh * silu.abs(), dh * up.abs() * ds
@@ -636,7 +643,7 @@ def test_native_argument_checks_need_no_gpu(pkg):
     assert norm_call(ws=p + 8, size=1 << 20) == L.EINVAL
 
     train = dict(x=p, w=p, bias=0, res=0, y=p, z=p, M=4, N=16, K=64, act=1, rt=0, yt=0)
-    for change, rc in ((dict(x=0), -1), (dict(z=0), -1), (dict(M=0), -1), (dict(act=0), -1), (dict(act=2), -1), (dict(yt=3), -1), (dict(res=p, rt=7), -1), (dict(bias=p + 2), -1),
+    for change, rc in ((dict(x=0), -1), (dict(y=0), -1), (dict(M=0), -1), (dict(act=0), -1), (dict(act=2), -1), (dict(yt=3), -1), (dict(res=p, rt=7), -1), (dict(bias=p + 2), -1),
                        (dict(N=12), -2), (dict(K=63), -2), (dict(N=1 << 21), -2), (dict(N=1 << 20, K=1 << 16), -2), (dict(M=1 << 31), -2), (dict(M=1 << 30, N=1 << 16), -2)):
         assert lib.aeris_linear_train_fwd(ops.LINEAR_TRAIN.pack(*{**train, **change}.values()), None) == rc, change
     lin = dict(dy=p, x=p, w=p, z=0, dx=p, dw=p, db=p, dz=0, M=4, N=16, K=64, act=0, yt=0)
@@ -649,10 +656,10 @@ def test_native_argument_checks_need_no_gpu(pkg):
     assert linear_call() == L.EINVAL and "workspace" in L.last_error()
     ff = dict(x=p, w1=p, w2=p, gu=p, h=p, y=p, M=4, d=64, H=128)
     for change, rc in ((dict(x=0), -1), (dict(h=0), -1), (dict(M=0), -1), (dict(H=0), -1), (dict(H=12), -2), (dict(d=4), -2), (dict(H=1 << 62), -2), (dict(d=1 << 19, H=1 << 19), -2), (dict(y=p + 1), -1)):
-        assert lib.aeris_feed_forward_train_fwd(ops.FEED_FORWARD.pack(*{**ff, **change}.values()), None) == rc, change
+        assert lib.aeris_feed_forward_train_fwd(ops.FEED_FORWARD.pack(*{**ff, **change}.values()), p, 1 << 40, None) == rc, change
     ffg = dict(dy=p, x=p, w1=p, w2=p, gu=p, h=p, dx=p, dw1=p, dw2=p, M=4, d=64, H=128)
     for change, rc in ((dict(dy=0), -1), (dict(x=0), -1), (dict(w1=0), -1), (dict(h=0), -1), (dict(H=-8), -1), (dict(H=4), -2), (dict(dx=p + 2), -1)):
         assert lib.aeris_feed_forward_bwd(ops.FEED_FORWARD_GRAD.pack(*{**ffg, **change}.values()), p, 1 << 40, None) == rc, change
     assert lib.aeris_feed_forward_bwd(ops.FEED_FORWARD_GRAD.pack(*ffg.values()), None, 0, None) == L.EINVAL
-    for f in (lib.aeris_norm_modulate_grad_workspace_bytes, lib.aeris_linear_grad_workspace_bytes, lib.aeris_feed_forward_grad_workspace_bytes):
+    for f in (lib.aeris_norm_modulate_grad_workspace_bytes, lib.aeris_linear_grad_workspace_bytes, lib.aeris_feed_forward_workspace_bytes, lib.aeris_feed_forward_grad_workspace_bytes):
         assert f(None) == 0
