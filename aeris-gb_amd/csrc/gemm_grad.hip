@@ -120,12 +120,14 @@ __device__ __forceinline__ void store_kept8(uint16_t* kept, int64_t count, int64
   *reinterpret_cast<u32x4*>(kept + at) = hi;
   *reinterpret_cast<u32x2*>(reinterpret_cast<uint8_t*>(kept + count) + at) = lo;
 }
-__device__ __forceinline__ void load_kept8(const uint16_t* kept, int64_t count, int64_t at, float (&v)[8]) {
-  const u32x4 hi = *reinterpret_cast<const u32x4*>(kept + at);
-  const u32x2 lo = *reinterpret_cast<const u32x2*>(reinterpret_cast<const uint8_t*>(kept + count) + at);
+struct Kept8 { u32x4 hi; u32x2 lo; };
+__device__ __forceinline__ Kept8 load_kept8(const uint16_t* kept, int64_t count, int64_t at) {
+  return Kept8{*reinterpret_cast<const u32x4*>(kept + at), *reinterpret_cast<const u32x2*>(reinterpret_cast<const uint8_t*>(kept + count) + at)};
+}
+__device__ __forceinline__ void widen_kept8(const Kept8& k, float (&v)[8]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e)  // byte 0: zero, 1: of lo, 2 and 3: of hi
-    v[e] = __uint_as_float(__builtin_amdgcn_perm(hi[e >> 1], lo[e >> 2], ((e & 1) ? 0x0706000cu : 0x0504000cu) | (uint32_t)(e & 3) << 8));
+    v[e] = __uint_as_float(__builtin_amdgcn_perm(k.hi[e >> 1], k.lo[e >> 2], ((e & 1) ? 0x0706000cu : 0x0504000cu) | (uint32_t)(e & 3) << 8));
 }
 
 // ---- operand panels in LDS
@@ -146,80 +148,95 @@ struct Panel {
   static_assert(LOADS * WAVES * 1024 == BYTES, "whole load instructions");
 };
 
-// One wave's loads of a panel.  `base`: the tile's first row (column, TR) at k = 0; rows: how many of them the matrix has from there.
+// One wave's loads of a panel, k-tile after k-tile.  What a load instruction needs is made ahead of the slot that issues it: `next` leaves a
+// descriptor and offsets behind, `issue` only uses them (made at the loads, some seventy scalar instructions a k-tile stood between a memory
+// slot's LDS reads and its end).
 // SWIGLU weights: row 64 c + s of the tile is gate row 32 c + s, from s = 32 on up row 32 c + s - 32 (`up_rows` further on).
 template <bool TR, int ROWS, int WAVES, bool SWIGLU_ROWS>
 struct Loader {
   using P = Panel<TR, ROWS, WAVES>;
-  const uint16_t* base;
-  int64_t ld, rows, k_end;
-  int64_t up_rows;
-  uint32_t voff[2];
-  uint32_t kchunk[2];
-  int wave;
+  static constexpr int RPI = 512 / P::COLS;  // TR: k rows of a load instruction
+  static_assert(!TR || (RPI == 4 && P::LOADS % 4 == 0) || (RPI == 8 && P::LOADS % 2 == 0), "bit 3 of an instruction's k follows from its number within the wave");
+  static_assert(TR || P::LOADS % 2 == 0, "the parity of 8-row blocks follows from their number within the wave");
+  static_assert(!TR || ((P::COLS * BK * 2 / 1024) % P::LOADS == 0), "a wave's load instructions lie in one panel");
+  lds_dma_rsrc rsrc;
+  uint64_t at;             // TR: address of the k-tile's first row
+  uint32_t soff[P::LOADS]; // between the load instructions
+  uint32_t koff;           // otherwise: of the k-tile within a row
+  uint32_t voff[2], vtail[2];
+  uint32_t step, whole_bytes, tail_bytes;
+  int valid;               // k-tiles from here on that hold anything
+  int panel;               // TR: of this wave
 
-  __device__ __forceinline__ void init(const uint16_t* b, int64_t ld_, int64_t rows_, int64_t k_end_, int64_t up, int lane, int wave_) {
-    base = b;
-    ld = ld_;
-    rows = rows_;
-    k_end = k_end_;
-    up_rows = up;
-    wave = wave_;
+  __device__ __forceinline__ void init(int64_t ld, int64_t up_rows, int lane, int wave) {
+    step = TR ? (uint32_t)(BK * ld * 2) : BK * 2;
+    constexpr int IPP = P::COLS * BK * 2 / 1024;  // TR: instructions of a panel
+    panel = wave * P::LOADS / IPP;
+#pragma unroll
+    for (int j = 0; j < P::LOADS; ++j) {
+      const int i = wave * P::LOADS + j;  // instruction of the tile: rows 8 i .., or of panel i / IPP
+      int64_t row = TR ? (i % IPP) * RPI : 8 * i;
+      if (SWIGLU_ROWS) row = (i >> 3) * 32 + (i & 3) * 8 + ((i & 4) ? up_rows : 0);
+      soff[j] = (uint32_t)(row * ld * 2);
+    }
 #pragma unroll
     for (int par = 0; par < 2; ++par) {
       if (TR) {
-        constexpr int RPI = 512 / P::COLS, CPR = P::COLS / 8;  // k rows of a load instruction, chunks of a row
+        constexpr int CPR = P::COLS / 8;  // chunks of a row
         const int kr = lane / CPR, pos = lane % CPR;
         // pair_key of the instruction's k rows: with the instruction's number (par: whether k has bit 3) and the lane's
         const int key = P::COLS == 128 ? kr | (par << 2) : ((kr >> 1) & 1) | (par << 1);
-        static_assert(RPI == 4 || RPI == 8, "panels of 128 or 64 columns");
         voff[par] = (uint32_t)(kr * ld * 2) + (uint32_t)((pos ^ (2 * key)) * 16);
-        kchunk[par] = 0;
       } else {
         const int dr = lane >> 4, pos = lane & 15;
         const int logical = pos ^ (par * 4 + dr);
         voff[par] = (uint32_t)((dr * 2 + (logical >> 3)) * ld * 2 + (logical & 7) * 16);
-        kchunk[par] = (uint32_t)(logical & 7) * 8;
       }
     }
   }
 
-  // k-tile that begins at k0, into the stage at LDS address `stage`
-  __device__ __forceinline__ void issue(int64_t k0, uint32_t stage) const {
-    int64_t left = k_end - k0;  // of k
-    if (left < 0) left = 0;
+  // from k = k_begin to k_end (at or before k_begin: nothing but zeros).  `base`: the tile's first row (column, TR) at k = 0; rows: how many of
+  // them the matrix has from there
+  __device__ __forceinline__ void start(const uint16_t* base, int64_t ld, int64_t rows, int64_t up_rows, int64_t k_begin, int64_t k_end, int lane) {
+    const int64_t left = k_end > k_begin ? k_end - k_begin : 0;
+    valid = (int)((left + BK - 1) / BK);
+    const int64_t tail = left - (int64_t)(valid - 1) * BK;  // k of the last of them
     if (TR) {
-      const int64_t kr = left < BK ? left : BK;
-      constexpr int PANELS = ROWS / P::COLS, IPP = P::COLS * BK * 2 / 1024;  // instructions of a panel
-      constexpr int RPI = 512 / P::COLS;
-#pragma unroll
-      for (int j = 0; j < P::LOADS; ++j) {
-        const int i = wave * P::LOADS + j;  // instruction of the tile: panel i / IPP
-        const int panel = i / IPP, ip = i % IPP;
-        const int64_t cols = rows - panel * P::COLS;
-        const uint32_t bytes = kr > 0 && cols > 0 ? (uint32_t)(((kr - 1) * ld + cols) * 2) : 0u;
-        const lds_dma_rsrc rs = make_lds_dma_rsrc(base + k0 * ld + panel * P::COLS, bytes);
-        lds_dma_load16(rs, stage + (uint32_t)i * 1024u, voff[RPI == 4 ? (j >> 1) & 1 : j & 1], (uint32_t)(ip * RPI) * (uint32_t)(ld * 2));
-      }
-      static_assert(PANELS == 1 || PANELS == 2, "one or two panels");
-      static_assert(RPI != 4 || P::LOADS % 4 == 0, "bit 3 of k follows from the number within the wave");
-      static_assert(RPI != 8 || P::LOADS % 2 == 0, "bit 3 of k follows from the number within the wave");
+      int64_t cols = rows - panel * P::COLS;
+      if (cols < 0) cols = 0;
+      at = reinterpret_cast<uint64_t>(base + k_begin * ld + panel * P::COLS);
+      whole_bytes = cols ? (uint32_t)(((BK - 1) * ld + cols) * 2) : 0u;
+      tail_bytes = cols ? (uint32_t)(((tail - 1) * ld + cols) * 2) : 0u;
     } else {
-      const uint32_t left32 = left < BK ? (uint32_t)left : (uint32_t)BK;
-      const int64_t all = SWIGLU_ROWS ? up_rows + rows : rows < ROWS ? rows : ROWS;
-      const uint32_t bytes = left > 0 ? (uint32_t)(all * ld * 2) : 0u;
-      const lds_dma_rsrc rs = make_lds_dma_rsrc(base, bytes);
+      at = reinterpret_cast<uint64_t>(base);
+      koff = (uint32_t)(k_begin * 2);
+      const int64_t all = rows <= 0 ? 0 : SWIGLU_ROWS ? up_rows + rows : rows < ROWS ? rows : ROWS;
+      whole_bytes = tail_bytes = (uint32_t)(all * ld * 2);
 #pragma unroll
-      for (int j = 0; j < P::LOADS; ++j) {
-        const int i = wave * P::LOADS + j;  // rows 8 i ..
-        int64_t row = 8 * i;
-        if (SWIGLU_ROWS) row = (i >> 3) * 32 + (i & 3) * 8 + ((i & 4) ? up_rows : 0);
-        static_assert(P::LOADS % 2 == 0, "the parity of 8-row blocks follows from the number within the wave");
-        uint32_t vo = voff[j & 1];
+      for (int par = 0; par < 2; ++par) {
         // (k beyond the matrix: an offset beyond any buffer's size, which arrives as zeros)
-        if (kchunk[j & 1] >= left32) vo = 0x80000000u;
-        lds_dma_load16(rs, stage + (uint32_t)i * 1024u, vo, (uint32_t)(row * ld * 2) + (uint32_t)(k0 * 2));
+        const int chunk = ((lane & 15) ^ (par * 4 + (lane >> 4))) & 7;
+        vtail[par] = chunk * 8 < tail ? voff[par] : 0x80000000u;
       }
+    }
+    describe();
+  }
+  __device__ __forceinline__ void describe() {
+    rsrc = make_lds_dma_rsrc(reinterpret_cast<const void*>(at), valid > 1 ? whole_bytes : valid == 1 ? tail_bytes : 0u);
+  }
+  __device__ __forceinline__ void next() {
+    --valid;
+    if (TR) at += step;
+    else koff += step;
+    describe();
+  }
+  // into the stage at LDS address `stage` + this wave's instructions'
+  __device__ __forceinline__ void issue(uint32_t stage) const {
+#pragma unroll
+    for (int j = 0; j < P::LOADS; ++j) {
+      const int par = TR && RPI == 4 ? (j >> 1) & 1 : j & 1;
+      if (TR) lds_dma_load16(rsrc, stage + (uint32_t)j * 1024u, voff[par], soff[j]);
+      else lds_dma_load16(rsrc, stage + (uint32_t)j * 1024u, valid > 1 ? voff[par] : vtail[par], soff[j] + koff);
     }
   }
 };
@@ -285,8 +302,44 @@ __device__ __forceinline__ void grad_epilogue(const GradGemm& p, const f32x4 (&a
   const int rrow = lane / CHUNKS, rch = lane % CHUNKS;
   const int col = col0 + rch * 8;
   const bool col_ok = part != nullptr || col < p.N;
+  // What the epilogue reads is asked for ahead of its stores (vector memory operations complete in order: a load behind a store would
+  // be waited for together with it): the bias once, the other rows one row fragment ahead.  Rows and columns beyond the result: its last.
+  constexpr bool LOADS = EPI == EPI_ACT || EPI == EPI_SWIGLU_BWD;
+  u32x4 bias = {0u, 0u, 0u, 0u};
+  u32x4 ahead[LOADS ? 2 : 1][LOADS ? ITS : 1][EPI == EPI_SWIGLU_BWD ? 3 : 2];  // residual, or upper halves of gate and up and both lower bytes
+  const int64_t last_row = p.M - 1;
+  const int load_col = col < p.N ? col : p.N - 8;
+  auto ask = [&](int i) {
+    if constexpr (LOADS) {
+#pragma unroll
+      for (int it = 0; it < ITS; ++it) {
+        int64_t row = row0 + 16 * i + rrow + it * RPI;
+        if (row > last_row) row = last_row;
+        u32x4(&to)[EPI == EPI_SWIGLU_BWD ? 3 : 2] = ahead[i & 1][it];
+        if constexpr (EPI == EPI_SWIGLU_BWD) {
+          const int64_t at = row * (2 * (int64_t)p.N) + load_col, count = p.M * (2 * (int64_t)p.N);
+          const Kept8 g = load_kept8(p.kept, count, at), u = load_kept8(p.kept, count, at + p.N);
+          to[0] = g.hi;
+          to[1] = u.hi;
+          to[2] = u32x4{g.lo.x, g.lo.y, u.lo.x, u.lo.y};
+        } else {
+          const int64_t at = row * (int64_t)p.N + load_col;
+          if (p.res_dtype == AERIS_F32) {
+            const u32x4* src = reinterpret_cast<const u32x4*>(reinterpret_cast<const float*>(p.residual) + at);
+            to[0] = src[0];
+            to[1] = src[1];
+          } else if (p.res_dtype == AERIS_BF16) {
+            to[0] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(p.residual) + at);
+          }
+        }
+      }
+    }
+  };
+  if (EPI == EPI_ACT && p.bias) bias = *reinterpret_cast<const u32x4*>(p.bias + load_col);
+  ask(0);
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
+    if (i + 1 < FM) ask(i + 1);
 #pragma unroll
     for (int j = 0; j < FN; ++j) *(lds4)(uintptr_t)(stage + l15 * (CH * 16) + (((j * 4 + q) ^ (l15 & (CH - 1))) << 4)) = acc[i][j];
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -329,28 +382,25 @@ __device__ __forceinline__ void grad_epilogue(const GradGemm& p, const f32x4 (&a
         }
       } else if constexpr (EPI == EPI_ACT) {
         if (ok) {
-          if (p.bias) {
-            float b[8];
-            widen8(*reinterpret_cast<const u32x4*>(p.bias + col), b);
+          float b[8];
+          widen8(bias, b);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] += b[e];
-          }
+          for (int e = 0; e < 8; ++e) o[e] += b[e];
           const int64_t at = row * (int64_t)p.N + col;
           if (p.kept) store_kept8(p.kept, p.M * (int64_t)p.N, at, o);
 #pragma unroll
           for (int e = 0; e < 8; ++e) o[e] = p.act == AERIS_ACT_SILU ? silu_f(o[e]) : p.c_f32 ? gelu_erf_f(o[e]) : gelu_erf_bf16_f(o[e]);
           if (p.res_dtype >= 0) {
             float x[8];
+            const u32x4(&r)[2] = ahead[i & 1][it];
             if (p.res_dtype == AERIS_F32) {
-              const float* src = reinterpret_cast<const float*>(p.residual) + at;
-              const f32x4 a = *reinterpret_cast<const f32x4*>(src), b = *reinterpret_cast<const f32x4*>(src + 4);
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                x[e] = a[e];
-                x[4 + e] = b[e];
+                x[e] = __uint_as_float(r[0][e]);
+                x[4 + e] = __uint_as_float(r[1][e]);
               }
             } else {
-              widen8(*reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(p.residual) + at), x);
+              widen8(r[0], x);
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] += x[e];
@@ -360,8 +410,9 @@ __device__ __forceinline__ void grad_epilogue(const GradGemm& p, const f32x4 (&a
       } else if (ok) {  // EPI_SWIGLU_BWD
         const int64_t at = row * (2 * (int64_t)p.N) + col;
         float g[8], u[8], dg[8];
-        load_kept8(p.kept, p.M * (2 * (int64_t)p.N), at, g);
-        load_kept8(p.kept, p.M * (2 * (int64_t)p.N), at + p.N, u);
+        const u32x4(&r)[3] = ahead[i & 1][it];
+        widen_kept8(Kept8{r[0], u32x2{r[2].x, r[2].y}}, g);
+        widen_kept8(Kept8{r[1], u32x2{r[2].z, r[2].w}}, u);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float s = sigmoid_f(g[e]);
@@ -412,8 +463,9 @@ __device__ __forceinline__ void grad_tile(const GradGemm& p, int item, unsigned 
   const int wm = wave / WN, wn = wave % WN;
   int part = 0;
   if (item >= p.whole) {
-    part = (item - p.whole) % p.parts;
-    item = p.whole + (item - p.whole) / p.parts;
+    const int c = item - p.whole, cut_tiles = p.tiles_m * p.tiles_n - p.whole;
+    part = c / cut_tiles;
+    item = p.whole + c - part * cut_tiles;
   }
   const TileAt tile = tile_at(item, p.tiles_m, p.tiles_n);
   const int64_t m0 = (int64_t)tile.m * T;
@@ -426,8 +478,10 @@ __device__ __forceinline__ void grad_tile(const GradGemm& p, int item, unsigned 
 
   Loader<A_TR, T, 4, false> la;
   Loader<B_TR, T, 4, SWIGLU> lb;
-  la.init(p.A + (A_TR ? m0 : m0 * p.lda), p.lda, p.M - m0, k_end, 0, lane, wave);
-  lb.init(p.B + (B_TR ? (int64_t)n0 : n0 * p.ldb), p.ldb, p.N - n0, k_end, p.N, lane, wave);
+  la.init(p.lda, 0, lane, wave);
+  lb.init(p.ldb, p.N, lane, wave);
+  la.start(p.A + (A_TR ? m0 : m0 * p.lda), p.lda, p.M - m0, 0, k_begin, k_end, lane);
+  lb.start(p.B + (B_TR ? (int64_t)n0 : n0 * p.ldb), p.ldb, p.N - n0, p.N, k_begin, k_end, lane);
   Fragments<A_TR, T, 4, FM> fa;
   Fragments<B_TR, T, 4, FN> fb;
   fa.init(wm * (T / WM), lane);
@@ -445,8 +499,10 @@ __device__ __forceinline__ void grad_tile(const GradGemm& p, int item, unsigned 
   const uint32_t lds0 = lds_byte_address(smem);
   auto issue = [&](int t) {
     const uint32_t stage = lds0 + (uint32_t)(t & 1) * (PA::BYTES + PB::BYTES);
-    la.issue(k_begin + (int64_t)t * BK, stage);
-    lb.issue(k_begin + (int64_t)t * BK, stage + PA::BYTES);
+    la.issue(stage + wave * (PA::LOADS * 1024));
+    lb.issue(stage + PA::BYTES + wave * (PB::LOADS * 1024));
+    la.next();
+    lb.next();
   };
   if (turns > 0) issue(0);
   int sum_turn = with_sums ? (int)((k_begin / BK) % p.tiles_n) : 0;
@@ -489,18 +545,29 @@ __device__ __forceinline__ void grad_tile(const GradGemm& p, int item, unsigned 
   }
 }
 
+// Workgroup b runs on XCD b mod 8: neighbouring items, which share rows and columns of their operands, go to one XCD (a permutation of 0 .. n - 1),
+// the whole tiles and the parts of the others each among themselves
+__device__ __forceinline__ int xcd_order(int b, int n) {
+  const int xcd = b & 7, each = n >> 3, more = n & 7;
+  return xcd * each + (xcd < more ? xcd : more) + (b >> 3);
+}
+__device__ __forceinline__ int xcd_item(const GradGemm& p, int b, int n) {
+  return b < p.whole ? xcd_order(b, p.whole) : p.whole + xcd_order(b - p.whole, n - p.whole);
+}
+
 template <int T, bool A_TR, bool B_TR, int EPI>
 __global__ void __launch_bounds__(256, 2) gemm_grad_tile_kernel(GradGemm p) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[tile_lds<T>()];
-  grad_tile<T, A_TR, B_TR, EPI>(p, blockIdx.x, smem);
+  const int item = xcd_item(p, blockIdx.x, gridDim.x);
+  grad_tile<T, A_TR, B_TR, EPI>(p, item, smem);
 }
 
 // two products that do not depend on each other in one launch: the first n workgroups make dx (or dh and what follows from it), the others dw
 template <int T, int EPI>
 __global__ void __launch_bounds__(256, 2) gemm_grad_pair_kernel(GradGemm p, GradGemm q, int n) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[tile_lds<T>()];
-  if ((int)blockIdx.x < n) grad_tile<T, false, true, EPI>(p, blockIdx.x, smem);
-  else grad_tile<T, true, true, EPI_STORE>(q, blockIdx.x - n, smem);
+  if ((int)blockIdx.x < n) grad_tile<T, false, true, EPI>(p, xcd_item(p, blockIdx.x, n), smem);
+  else grad_tile<T, true, true, EPI_STORE>(q, xcd_item(q, blockIdx.x - n, gridDim.x - n), smem);
 }
 
 // ---- tiles of 256 x 256, eight waves (two by four, 128 x 64 each), one persistent workgroup a CU: the pipeline of the package's other
@@ -526,7 +593,7 @@ __global__ void __launch_bounds__(512) gemm_grad_big_kernel(GradGemm p) {
   // Whole tiles come in full rounds of one per CU: XCD x (workgroup number mod 8) has a contiguous eighth of them, its 32 workgroups take
   // them in turns, so that those at work together share the operands' slices in its L2.  What is left is one more round, of parts.
   const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
-  const int rounds = p.whole >> 8, cut_items = (p.tiles_m * p.tiles_n - p.whole) * p.parts, cut_each = (cut_items + 7) >> 3;
+  const int rounds = p.whole >> 8, cut_tiles = p.tiles_m * p.tiles_n - p.whole, cut_items = cut_tiles * p.parts, cut_each = (cut_items + 7) >> 3;
   const bool has_cut = slot < cut_each && xcd * cut_each + slot < cut_items;
   const int n_my = rounds + (has_cut ? 1 : 0);
   if (n_my == 0) return;
@@ -540,11 +607,11 @@ __global__ void __launch_bounds__(512) gemm_grad_big_kernel(GradGemm p) {
       it.k_begin = 0;
       it.k_end = p.K;
     } else {
-      const int c = xcd * cut_each + slot;
-      it.cut = c / p.parts;
-      tile = p.whole + it.cut;
-      it.part = c - it.cut * p.parts;
-      it.cut = c + 1;
+      const int c = xcd * cut_each + slot;  // (the tiles of one part beside each other: they read the same rows)
+      it.part = c / cut_tiles;
+      const int n = c - it.part * cut_tiles;
+      tile = p.whole + n;
+      it.cut = n * p.parts + it.part + 1;
       it.k_begin = it.part * p.k_part;
       it.k_end = it.k_begin + p.k_part < p.K ? it.k_begin + p.k_part : p.K;
     }
@@ -561,50 +628,47 @@ __global__ void __launch_bounds__(512) gemm_grad_big_kernel(GradGemm p) {
 
   Loader<A_TR, 128, 4, false> la;
   Loader<B_TR, 256, 8, SWIGLU> lb;
-  la.init(p.A, p.lda, 0, 0, 0, lane, wn);
-  lb.init(p.B, p.ldb, 0, 0, p.N, lane, wave);
-  int la_r = 0, la_kt = 0, la_stage = 0, lb_r = 0, lb_kt = 0, lb_stage = 0;
-  int64_t la_k = 0, lb_k = 0;
+  la.init(p.lda, 0, lane, wn);
+  lb.init(p.ldb, p.N, lane, wave);
+  int la_r = 0, la_left = 0, la_stage = 0, lb_r = 0, lb_left = 0, lb_stage = 0;  // item, its k-tiles that are left, stage
   auto la_item = [&]() {
+    la_left = turns_of(la_r);
     if (la_r >= n_my) {  // past the end: loads from a descriptor without records, so that the counts of the waits stay the same
-      la.k_end = la_k = 0;
+      la.start(p.A, p.lda, 0, 0, 0, 0, lane);
       return;
     }
     const Item it = decode(la_r);
     const int64_t m = it.m0 + grp * 128;
-    la.base = p.A + (A_TR ? m : m * p.lda);
-    la.rows = p.M > m ? p.M - m : 0;
-    la.k_end = it.k_end;
-    la_k = it.k_begin;
+    la.start(p.A + (A_TR ? m : m * p.lda), p.lda, p.M - m, 0, it.k_begin, it.k_end, lane);
   };
   auto lb_item = [&]() {
+    lb_left = turns_of(lb_r);
     if (lb_r >= n_my) {
-      lb.k_end = lb_k = 0;
+      lb.start(p.B, p.ldb, 0, 0, 0, 0, lane);
       return;
     }
     const Item it = decode(lb_r);
-    lb.base = p.B + (B_TR ? (int64_t)it.n0 : it.n0 * p.ldb);
-    lb.rows = p.N - it.n0;
-    lb.k_end = it.k_end;
-    lb_k = it.k_begin;
+    lb.start(p.B + (B_TR ? (int64_t)it.n0 : it.n0 * p.ldb), p.ldb, p.N - it.n0, p.N, it.k_begin, it.k_end, lane);
   };
   // (issue and advance apart: no branch may lie between the transposing reads of a memory slot and their wait)
-  auto issue_a = [&]() { la.issue(la_k, lds0 + la_stage * BIG_STAGE + grp * (BIG_STAGE / 2)); };
-  auto issue_b = [&]() { lb.issue(lb_k, lds_b0 + lb_stage * BIG_STAGE); };
-  auto advance_a = [&]() {
+  auto issue_a = [&]() { la.issue(lds0 + la_stage * BIG_STAGE + grp * (BIG_STAGE / 2) + wn * 4096); };
+  auto issue_b = [&]() { lb.issue(lds_b0 + lb_stage * BIG_STAGE + wave * 4096); };
+  auto step_a = [&]() {
     la_stage ^= 1;
-    la_k += BK;
-    if (++la_kt >= turns_of(la_r)) {
-      la_kt = 0;
+    la.next();
+  };
+  auto step_b = [&]() {
+    lb_stage = lb_stage == 2 ? 0 : lb_stage + 1;
+    lb.next();
+  };
+  auto turn_a = [&]() {
+    if (--la_left == 0) {
       ++la_r;
       la_item();
     }
   };
-  auto advance_b = [&]() {
-    if (++lb_stage == 3) lb_stage = 0;
-    lb_k += BK;
-    if (++lb_kt >= turns_of(lb_r)) {
-      lb_kt = 0;
+  auto turn_b = [&]() {
+    if (--lb_left == 0) {
       ++lb_r;
       lb_item();
     }
@@ -630,11 +694,14 @@ __global__ void __launch_bounds__(512) gemm_grad_big_kernel(GradGemm p) {
   la_item();
   lb_item();
   issue_a();
-  advance_a();
-  issue_b();
-  advance_b();
-  issue_b();
-  advance_b();
+  step_a();
+  turn_a();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    issue_b();
+    step_b();
+    turn_b();
+  }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   int sa = 0, sb = 0;
@@ -664,11 +731,12 @@ __global__ void __launch_bounds__(512) gemm_grad_big_kernel(GradGemm p) {
         __builtin_amdgcn_s_waitcnt(KS == 0 ? 0xC07F : 0x0078);  // lgkmcnt(0); vmcnt(8) lgkmcnt(0)
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
+        if (KS == 0) step_a();
+        else step_b();
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
           for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
         if constexpr (ROW_SUMS) {
           if (mine) {
 #pragma unroll
@@ -678,8 +746,8 @@ __global__ void __launch_bounds__(512) gemm_grad_big_kernel(GradGemm p) {
             }
           }
         }
-        if (KS == 0) advance_a();
-        else advance_b();
+        if (KS == 0) turn_a();
+        else turn_b();
         if (KS == 1) __builtin_amdgcn_s_waitcnt(0x0F74);  // vmcnt(4)
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
@@ -749,50 +817,70 @@ __global__ void __launch_bounds__(256) grad_finish_kernel(GradGemm p, GradGemm q
   }
 }
 
-// ---- dz = dy act'(z) (ACT_NONE: dy) rounded to bf16, and the sums of the unrounded dz over the tokens: a workgroup takes 512 columns
-// and a share of the rows, its four waves every fourth of them; 8 columns a lane
+// ---- dz = dy act'(z) (ACT_NONE: dy) rounded to bf16, and the sums of the unrounded dz over the tokens.  Bound by HBM: a workgroup takes 512
+// columns of 16 rows at a time, in turns with the others; a wave asks for its four rows (8 columns a lane) before it uses the first.
+// f32 dy [1036800, 1024] without activation: 1257 us, 5.1 TB/s (sums alone 750, 5.7; a cast to bf16 alone 1086); rows one by one and a contiguous
+// share of them a workgroup: 1276 and 57 more for the sums.
 struct ActGrad {
   const void* dy;
   const uint16_t* z;
   uint16_t* dz;    // NULL: not wanted (dy is bf16 and there is no activation)
-  float* partial;  // [row shares][N], or NULL
-  int64_t M, rows_per_block;
-  int N, dy_f32, act;
+  float* partial;  // [workgroups of a column block][N], or NULL
+  int64_t M;
+  int N, act;
 };
 
+template <bool DY_F32, bool ACT, bool STREAM>
 __global__ void __launch_bounds__(256) act_grad_kernel(ActGrad p) {
+  constexpr int ROWS = 4;
   __shared__ f32x4 lds[4][128];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int col = (blockIdx.y * 64 + lane) * 8;
   const bool ok = col < p.N;
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  const int64_t first = (int64_t)blockIdx.x * p.rows_per_block;
-  int64_t end = first + p.rows_per_block;
-  if (end > p.M) end = p.M;
   if (ok) {
-    for (int64_t row = first + w; row < end; row += 4) {
-      const int64_t at = row * p.N + col;
-      float d[8];
-      if (p.dy_f32) {
-        const f32x4* q = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(p.dy) + at);
-        const f32x4 a = q[0], b = q[1];
+    for (int64_t row = ((int64_t)blockIdx.x * 4 + w) * ROWS; row < p.M; row += (int64_t)gridDim.x * 4 * ROWS) {
+      u32x4 a[ROWS], b[ROWS];
+      Kept8 z[ROWS];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          d[e] = a[e];
-          d[4 + e] = b[e];
+      for (int r = 0; r < ROWS; ++r) {
+        const int64_t at = (row + r < p.M ? row + r : p.M - 1) * p.N + col;
+        if (DY_F32) {
+          const u32x4* q = reinterpret_cast<const u32x4*>(reinterpret_cast<const float*>(p.dy) + at);
+          a[r] = __builtin_nontemporal_load(q);
+          b[r] = __builtin_nontemporal_load(q + 1);
+        } else {
+          a[r] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(p.dy) + at);
         }
-      } else {
-        widen8(*reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(p.dy) + at), d);
-      }
-      if (p.act != AERIS_ACT_NONE) {
-        float z[8];
-        load_kept8(p.z, p.M * p.N, at, z);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] *= p.act == AERIS_ACT_SILU ? dsilu_f(z[e], sigmoid_f(z[e])) : dgelu_f(z[e]);
+        if (ACT) z[r] = load_kept8(p.z, p.M * p.N, at);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] += d[e];
-      if (p.dz) *reinterpret_cast<u32x4*>(p.dz + at) = narrow8(d);
+      for (int r = 0; r < ROWS; ++r) {
+        if (row + r >= p.M) break;
+        float d[8];
+        if (DY_F32) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            d[e] = __uint_as_float(a[r][e]);
+            d[4 + e] = __uint_as_float(b[r][e]);
+          }
+        } else {
+          widen8(a[r], d);
+        }
+        if (ACT) {
+          float v[8];
+          widen_kept8(z[r], v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d[e] *= p.act == AERIS_ACT_SILU ? dsilu_f(v[e], sigmoid_f(v[e])) : dgelu_f(v[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += d[e];
+        if (p.dz) {
+          u32x4* const out = reinterpret_cast<u32x4*>(p.dz + (row + r) * p.N + col);
+          if (STREAM) __builtin_nontemporal_store(narrow8(d), out);
+          else *out = narrow8(d);
+        }
+      }
     }
   }
   if (!p.partial) return;
@@ -806,28 +894,29 @@ __global__ void __launch_bounds__(256) act_grad_kernel(ActGrad p) {
   }
 }
 
-// 32 columns a workgroup, 8 threads share a column's partial sums
-__global__ void __launch_bounds__(256) bias_sum_kernel(const float* partial, uint16_t* out, int parts, int N) {
-  __shared__ float lds[8][33];
-  const int c = threadIdx.x & 31, r = threadIdx.x >> 5, col = blockIdx.x * 32 + c;
+// 8 columns a workgroup, 128 threads share a column's partial sums
+__global__ void __launch_bounds__(1024) bias_sum_kernel(const float* partial, uint16_t* out, int parts, int N) {
+  __shared__ float lds[16][8];
+  const int c = threadIdx.x & 7, r = threadIdx.x >> 3, col = blockIdx.x * 8 + c;  // (N is a multiple of 8)
   float t = 0.f;
-  if (col < N)
-    for (int b = r; b < parts; b += 8) t += partial[(int64_t)b * N + col];
-  lds[r][c] = t;
+#pragma unroll 4
+  for (int b = r; b < parts; b += 128) t += partial[(int64_t)b * N + col];
+  t += __shfl_xor(t, 8);
+  t += __shfl_xor(t, 16);
+  t += __shfl_xor(t, 32);
+  if ((threadIdx.x & 63) < 8) lds[threadIdx.x >> 6][c] = t;
   __syncthreads();
-  if (r == 0 && col < N) {
-    float v = 0.f;
+  if (threadIdx.x < 8) {
+    t = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v += lds[k][c];
-    out[col] = (uint16_t)f32_to_bf16_bits(v);
+    for (int w = 0; w < 16; ++w) t += lds[w][c];
+    out[col] = (uint16_t)f32_to_bf16_bits(t);
   }
 }
 
 int act_grad_parts(int64_t M, int N) {
-  const int64_t col_blocks = (N + 511) / 512;
-  int64_t n = 2048 / col_blocks;
-  if (n > (M + 15) / 16) n = (M + 15) / 16;
-  return n < 1 ? 1 : (int)n;
+  const int64_t n = 1280 / ((N + 511) / 512), most = (M + 15) / 16;
+  return n < 1 ? 1 : n < most ? (int)n : (int)most;
 }
 
 hipError_t act_grad_launch(const void* dy, int dy_f32, const void* z, void* dz, float* partial, void* dbias, int64_t M, int N, int act,
@@ -839,14 +928,24 @@ hipError_t act_grad_launch(const void* dy, int dy_f32, const void* z, void* dz, 
   p.partial = dbias ? partial : nullptr;
   p.M = M;
   p.N = N;
-  p.dy_f32 = dy_f32;
   p.act = act;
   const int parts = act_grad_parts(M, N);
-  p.rows_per_block = (M + parts - 1) / parts;
-  hipLaunchKernelGGL(act_grad_kernel, dim3((unsigned)parts, (unsigned)((N + 511) / 512)), dim3(256), 0, stream, p);
-  hipError_t e = hipGetLastError();
+  const dim3 grid((unsigned)parts, (unsigned)((N + 511) / 512));
+  const bool stream_out = M * N * 2 > (int64_t)256 << 20;  // more than the last-level cache holds until the products read it
+#define GO(DY, ACT, ST) hipLaunchKernelGGL((act_grad_kernel<DY, ACT, ST>), grid, dim3(256), 0, stream, p)
+  if (act != AERIS_ACT_NONE) {
+    if (dy_f32) { if (stream_out) GO(true, true, true); else GO(true, true, false); }
+    else { if (stream_out) GO(false, true, true); else GO(false, true, false); }
+  } else if (dy_f32) {
+    if (stream_out) GO(true, false, true);
+    else GO(true, false, false);
+  } else {
+    GO(false, false, false);  // (no dz)
+  }
+#undef GO
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !dbias) return e;
-  hipLaunchKernelGGL(bias_sum_kernel, dim3((unsigned)((N + 31) / 32)), dim3(256), 0, stream, partial, reinterpret_cast<uint16_t*>(dbias), parts, N);
+  hipLaunchKernelGGL(bias_sum_kernel, dim3((unsigned)(N / 8)), dim3(1024), 0, stream, partial, reinterpret_cast<uint16_t*>(dbias), parts, N);
   return hipGetLastError();
 }
 
@@ -874,7 +973,7 @@ GradPlan plan_tiles(int t, int64_t M, int64_t N, int64_t K, int epi) {
   if (tiles >= 1 << 24) return best;
   const int at_once = t == 256 ? 256 : t == 128 ? 512 : 1280, i = t == 256 ? 0 : t == 128 ? 1 : 2;
   const bool kept = epi == EPI_ACT || epi == EPI_SWIGLU;  // 3 bytes a value are written beside the result
-  constexpr double K_STORE[3] = {0.0255, 0.0152, 0.0146}, K_KEPT[3] = {0.0182, 0.0122, 0.0104}, K_LONE[3] = {0.0255, 0.0085, 0.005};
+  constexpr double K_STORE[3] = {0.0245, 0.0165, 0.018}, K_KEPT[3] = {0.0182, 0.0135, 0.0115}, K_LONE[3] = {0.0245, 0.0085, 0.005};
   constexpr double TILE_STORE[3] = {5.0, 3.0, 2.0}, TILE_KEPT[3] = {28.0, 16.0, 12.0};
   const double round_k = kept ? K_KEPT[i] : K_STORE[i], lone_k = K_LONE[i] < round_k ? K_LONE[i] : round_k;
   const double tile_us = kept || epi == EPI_SWIGLU_BWD ? TILE_KEPT[i] : TILE_STORE[i];
@@ -1082,13 +1181,20 @@ hipError_t linear_grad_launch(const aeris_linear_grad& a, void* workspace, hipSt
   return launch_pair<EPI_STORE>(linear_pair(a), product(dz, a.N, a.w, a.K, a.dx, a.K, a.M, a.K, a.N), product(dz, a.N, a.x, a.K, a.dw, a.K, a.N, a.K, a.M), ws, a.dbias, stream);
 }
 
-int64_t feed_forward_train_workspace_bytes(const aeris_feed_forward& a) { return plan_of(a.M, a.d, a.H, EPI_STORE).partial_bytes(); }
+// The second projection has nothing to keep: it is the inference kernels' product (14400 tokens, H 6144 -> 1536: 204 us, here 240), but for few
+// tokens of many hidden channels, whose k only the kernels here cut into parts (9 tokens: 22 us there, 12 here; both passes of 384 tokens 59 and 54, of
+// 512 the same; H 4096: 29 and 28; H 2048 and less: 1 to 3 us shorter there), and for k that is no multiple of 64.
+static bool second_is_cut(const aeris_feed_forward& a) { return a.H % 64 != 0 || (a.M <= 384 && a.H >= 4096); }
+
+int64_t feed_forward_train_workspace_bytes(const aeris_feed_forward& a) { return !second_is_cut(a) ? 0 : plan_of(a.M, a.d, a.H, EPI_STORE).partial_bytes(); }
 
 hipError_t feed_forward_train_launch(const aeris_feed_forward& a, void* workspace, hipStream_t stream) {
   GradGemm p = product(a.x, a.d, a.w1, a.d, a.h, a.H, a.M, a.H, a.d);
   p.kept = reinterpret_cast<uint16_t*>(a.gate_up);
   const hipError_t e = launch<false, false, EPI_SWIGLU>(p, plan_of(a.M, a.H, a.d, EPI_SWIGLU), nullptr, nullptr, stream);
   if (e != hipSuccess) return e;
+  if (!second_is_cut(a))
+    return gemm_launch(a.h, a.w2, a.y, nullptr, nullptr, nullptr, a.M, (int)a.d, (int)a.H, a.d, AERIS_ACT_NONE, 0, AERIS_BF16, 0, a.M, 0, 0, 1.0f, 0, stream);
   GradGemm q = product(a.h, a.H, a.w2, a.H, a.y, a.d, a.M, a.d, a.H);
   return launch<false, false, EPI_STORE>(q, plan_of(a.M, a.d, a.H, EPI_STORE), workspace, nullptr, stream);
 }
