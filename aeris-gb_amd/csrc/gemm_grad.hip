@@ -29,10 +29,12 @@ enum GradEpi { EPI_STORE, EPI_ACT, EPI_SWIGLU, EPI_SWIGLU_BWD };
 struct GradGemm {
   const uint16_t* A;
   const uint16_t* B;
+  const uint16_t *A_low, *B_low;  // the remainders of an operand that has two bf16 a value (few tokens; tiles of up to 128), or NULL
   int64_t M, K;
   int64_t lda, ldb;  // elements between rows
   int N;             // columns of the result
   void* C;           // SWIGLU: h; SWIGLU_BWD: [dgate | dup]
+  uint16_t* C_low;   // of these, what the rounding left over, or NULL
   int64_t ldc;
   int c_f32;
   const uint16_t* bias;
@@ -91,6 +93,15 @@ __device__ __forceinline__ void widen8(const u32x4& w, float (&o)[8]) {
 }
 __device__ __forceinline__ u32x4 narrow8(const float (&o)[8]) {
   return u32x4{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7])};
+}
+// what rounding to bf16 leaves over, rounded to bf16
+__device__ __forceinline__ u32x4 remainder8(const float (&o)[8]) {
+  const u32x4 hi = narrow8(o);
+  float h[8], r[8];
+  widen8(hi, h);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = fabsf(h[e]) <= 3.3895314e38f ? o[e] - h[e] : 0.0f;  // (nothing is left over of an infinity or a NaN)
+  return narrow8(r);
 }
 __device__ __forceinline__ void store8(void* C, int f32, int64_t at, const float (&o)[8]) {
   if (f32) {
@@ -379,6 +390,7 @@ __device__ __forceinline__ void grad_epilogue(const GradGemm& p, const f32x4 (&a
 #pragma unroll
           for (int e = 0; e < 8; ++e) o[e] = silu_f(o[e]) * up[e];
           store8(p.C, 0, row * p.ldc + col, o);
+          if (T <= 128 && p.C_low) *reinterpret_cast<u32x4*>(p.C_low + row * p.ldc + col) = remainder8(o);
         }
       } else if constexpr (EPI == EPI_ACT) {
         if (ok) {
@@ -421,6 +433,10 @@ __device__ __forceinline__ void grad_epilogue(const GradGemm& p, const f32x4 (&a
         }
         store8(p.C, 0, at, dg);
         store8(p.C, 0, at + p.N, o);
+        if (T <= 128 && p.C_low) {
+          *reinterpret_cast<u32x4*>(p.C_low + at) = remainder8(dg);
+          *reinterpret_cast<u32x4*>(p.C_low + at + p.N) = remainder8(o);
+        }
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -480,8 +496,12 @@ __device__ __forceinline__ void grad_tile(const GradGemm& p, int item, unsigned 
   Loader<B_TR, T, 4, SWIGLU> lb;
   la.init(p.lda, 0, lane, wave);
   lb.init(p.ldb, p.N, lane, wave);
-  la.start(p.A + (A_TR ? m0 : m0 * p.lda), p.lda, p.M - m0, 0, k_begin, k_end, lane);
-  lb.start(p.B + (B_TR ? (int64_t)n0 : n0 * p.ldb), p.ldb, p.N - n0, p.N, k_begin, k_end, lane);
+  auto start = [&](const uint16_t* A, const uint16_t* B) {
+    la.start(A + (A_TR ? m0 : m0 * p.lda), p.lda, p.M - m0, 0, k_begin, k_end, lane);
+    lb.start(B + (B_TR ? (int64_t)n0 : n0 * p.ldb), p.ldb, p.N - n0, p.N, k_begin, k_end, lane);
+  };
+  start(p.A, p.B);
+  const bool low = p.A_low || p.B_low;  // once more over k, with the remainders of the operand that has them
   Fragments<A_TR, T, 4, FM> fa;
   Fragments<B_TR, T, 4, FN> fb;
   fa.init(wm * (T / WM), lane);
@@ -498,6 +518,7 @@ __device__ __forceinline__ void grad_tile(const GradGemm& p, int item, unsigned 
 
   const uint32_t lds0 = lds_byte_address(smem);
   auto issue = [&](int t) {
+    if (low && t == turns) start(p.A_low ? p.A_low : p.A, p.B_low ? p.B_low : p.B);
     const uint32_t stage = lds0 + (uint32_t)(t & 1) * (PA::BYTES + PB::BYTES);
     la.issue(stage + wave * (PA::LOADS * 1024));
     lb.issue(stage + PA::BYTES + wave * (PB::LOADS * 1024));
@@ -506,10 +527,11 @@ __device__ __forceinline__ void grad_tile(const GradGemm& p, int item, unsigned 
   };
   if (turns > 0) issue(0);
   int sum_turn = with_sums ? (int)((k_begin / BK) % p.tiles_n) : 0;
-  for (int t = 0; t < turns; ++t) {
+  const int all_turns = low ? 2 * turns : turns;
+  for (int t = 0; t < all_turns; ++t) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();  // stage t is there; the other one has been read
-    if (t + 1 < turns) issue(t + 1);
+    if (t + 1 < all_turns) issue(t + 1);
     const uint32_t sa = lds0 + (uint32_t)(t & 1) * (PA::BYTES + PB::BYTES), sb = sa + PA::BYTES;
     const bool mine = with_sums && sum_turn == tile.n;
     auto step = [&](auto ks) {
@@ -825,6 +847,7 @@ struct ActGrad {
   const void* dy;
   const uint16_t* z;
   uint16_t* dz;    // NULL: not wanted (dy is bf16 and there is no activation)
+  uint16_t* dz_low;  // what the rounding of dz left over, or NULL
   float* partial;  // [workgroups of a column block][N], or NULL
   int64_t M;
   int N, act;
@@ -879,6 +902,7 @@ __global__ void __launch_bounds__(256) act_grad_kernel(ActGrad p) {
           u32x4* const out = reinterpret_cast<u32x4*>(p.dz + (row + r) * p.N + col);
           if (STREAM) __builtin_nontemporal_store(narrow8(d), out);
           else *out = narrow8(d);
+          if (!STREAM && p.dz_low) *reinterpret_cast<u32x4*>(p.dz_low + (row + r) * p.N + col) = remainder8(d);
         }
       }
     }
@@ -919,19 +943,20 @@ int act_grad_parts(int64_t M, int N) {
   return n < 1 ? 1 : n < most ? (int)n : (int)most;
 }
 
-hipError_t act_grad_launch(const void* dy, int dy_f32, const void* z, void* dz, float* partial, void* dbias, int64_t M, int N, int act,
+hipError_t act_grad_launch(const void* dy, int dy_f32, const void* z, void* dz, void* dz_low, float* partial, void* dbias, int64_t M, int N, int act,
                            hipStream_t stream) {
   ActGrad p;
   p.dy = dy;
   p.z = reinterpret_cast<const uint16_t*>(z);
   p.dz = reinterpret_cast<uint16_t*>(dz);
+  p.dz_low = reinterpret_cast<uint16_t*>(dz_low);
   p.partial = dbias ? partial : nullptr;
   p.M = M;
   p.N = N;
   p.act = act;
   const int parts = act_grad_parts(M, N);
   const dim3 grid((unsigned)parts, (unsigned)((N + 511) / 512));
-  const bool stream_out = M * N * 2 > (int64_t)256 << 20;  // more than the last-level cache holds until the products read it
+  const bool stream_out = !dz_low && M * N * 2 > (int64_t)256 << 20;  // more than the last-level cache holds until the products read it
 #define GO(DY, ACT, ST) hipLaunchKernelGGL((act_grad_kernel<DY, ACT, ST>), grid, dim3(256), 0, stream, p)
   if (act != AERIS_ACT_NONE) {
     if (dy_f32) { if (stream_out) GO(true, true, true); else GO(true, true, false); }
@@ -966,16 +991,16 @@ struct GradPlan {
 // round_k a k and tile_us beside it, a lone tile of 128 or 64 on a CU lone_k a k: fitted to products of 2048 .. 259200 rows, 128 .. 12288 columns
 // and k from 64 to 64800.  Tiles beyond the last whole round may be cut along k into as many parts as fill one: 14400 tokens' dw [12288, 1536] (288
 // tiles of 256 for 256 CUs) 710 -> 472 us; the parts go through memory once more, 16 to 256 KB each.
-GradPlan plan_tiles(int t, int64_t M, int64_t N, int64_t K, int epi) {
+GradPlan plan_tiles(int t, int64_t M, int64_t N, int64_t K, int epi, bool low) {
   const int64_t bn = epi == EPI_SWIGLU ? t / 2 : t, tm = (M + t - 1) / t, tn = (N + bn - 1) / bn, tiles = tm * tn;
   GradPlan best = {};
   best.us = 1e30;
-  if (tiles >= 1 << 24) return best;
+  if (tiles >= 1 << 24 || (low && t == 256)) return best;
   const int at_once = t == 256 ? 256 : t == 128 ? 512 : 1280, i = t == 256 ? 0 : t == 128 ? 1 : 2;
   const bool kept = epi == EPI_ACT || epi == EPI_SWIGLU;  // 3 bytes a value are written beside the result
   constexpr double K_STORE[3] = {0.0245, 0.0165, 0.018}, K_KEPT[3] = {0.0182, 0.0135, 0.0115}, K_LONE[3] = {0.0245, 0.0085, 0.005};
   constexpr double TILE_STORE[3] = {5.0, 3.0, 2.0}, TILE_KEPT[3] = {28.0, 16.0, 12.0};
-  const double round_k = kept ? K_KEPT[i] : K_STORE[i], lone_k = K_LONE[i] < round_k ? K_LONE[i] : round_k;
+  const double twice = low ? 2.0 : 1.0, round_k = twice * (kept ? K_KEPT[i] : K_STORE[i]), lone_k = twice * K_LONE[i] < round_k ? twice * K_LONE[i] : round_k;
   const double tile_us = kept || epi == EPI_SWIGLU_BWD ? TILE_KEPT[i] : TILE_STORE[i];
   const int64_t left = tiles % at_once;
   int64_t most = epi == EPI_STORE && left ? at_once / left : 1;
@@ -1000,11 +1025,11 @@ GradPlan plan_tiles(int t, int64_t M, int64_t N, int64_t K, int epi) {
   return best;
 }
 
-GradPlan plan_of(int64_t M, int64_t N, int64_t K, int epi) {
+GradPlan plan_of(int64_t M, int64_t N, int64_t K, int epi, bool low) {
   GradPlan best = {};
   best.us = 1e30;
   for (int t : {256, 128, 64}) {
-    const GradPlan g = plan_tiles(t, M, N, K, epi);
+    const GradPlan g = plan_tiles(t, M, N, K, epi, low);
     if (g.us < best.us) best = g;
   }
   return best;
@@ -1073,17 +1098,17 @@ struct GradPair {
   bool together;
   int64_t partial_bytes, second_bytes, sum_bytes;
 };
-GradPair plan_pair(bool first, int64_t M, int64_t N, int64_t K, int epi, bool second, int64_t N2, int64_t K2, bool sums) {
+GradPair plan_pair(bool first, int64_t M, int64_t N, int64_t K, int epi, bool low, bool second, int64_t N2, int64_t K2, bool low2, bool sums) {
   GradPair r = {};
   r.first = first;
   r.second = second;
   r.sums = sums && second;
-  if (first) r.g = plan_of(M, N, K, epi);
-  if (second) r.h = plan_of(N2, K2, M, EPI_STORE);
+  if (first) r.g = plan_of(M, N, K, epi, low);
+  if (second) r.h = plan_of(N2, K2, M, EPI_STORE, low2);
   if (first && second && r.g.tile && r.h.tile && r.g.tile != 256 && r.h.tile != 256) {
     r.together = true;
     if (r.g.tile != r.h.tile) {  // tiles of one size
-      const GradPlan g2 = plan_tiles(r.h.tile, M, N, K, epi), h2 = plan_tiles(r.g.tile, N2, K2, M, EPI_STORE);
+      const GradPlan g2 = plan_tiles(r.h.tile, M, N, K, epi, low), h2 = plan_tiles(r.g.tile, N2, K2, M, EPI_STORE, low2);
       if (g2.us + r.h.us < r.g.us + h2.us) r.g = g2;
       else r.h = h2;
     }
@@ -1118,16 +1143,26 @@ hipError_t launch_pair(const GradPair& r, GradGemm p, GradGemm q, void* workspac
 }
 
 int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+int64_t more(int64_t a, int64_t b) { return a > b ? a : b; }
+
+// Few tokens: what one product rounds for the next (h; dgate and dup; dz) is kept as two bf16 a value, and the products behind it go over k
+// twice.  Their errors do not average out over many tokens, and the products are bound by the weights' way through memory (9 tokens, 1536 ->
+// 6144: both passes 70 us with and without).
+bool few(int64_t M) { return M <= AERIS_FEW_TOKENS; }
 
 bool needs_dz(const aeris_linear_grad& a) { return (a.dy_dtype == AERIS_F32 || a.act != AERIS_ACT_NONE) && (a.dx || a.dw || a.dz); }
 // the bias' gradient: with dz where that has to be made, otherwise with dw
 bool bias_apart(const aeris_linear_grad& a) { return a.dbias && (needs_dz(a) || !a.dw || a.dy_dtype == AERIS_F32 || a.act != AERIS_ACT_NONE); }
-int64_t more(int64_t a, int64_t b) { return a > b ? a : b; }
+bool low_dz(const aeris_linear_grad& a) { return needs_dz(a) && few(a.M) && (a.dx || a.dw); }
 GradPair linear_pair(const aeris_linear_grad& a) {
-  return plan_pair(a.dx, a.M, a.K, a.N, EPI_STORE, a.dw, a.N, a.K, a.dbias && !bias_apart(a));
+  return plan_pair(a.dx, a.M, a.K, a.N, EPI_STORE, low_dz(a), a.dw, a.N, a.K, low_dz(a), a.dbias && !bias_apart(a));
 }
-GradPair hidden_pair(const aeris_feed_forward_grad& a) { return plan_pair(a.dx || a.dw1, a.M, a.H, a.d, EPI_SWIGLU_BWD, a.dw2, a.d, a.H, false); }
-GradPair token_pair(const aeris_feed_forward_grad& a) { return plan_pair(a.dx, a.M, a.d, 2 * a.H, EPI_STORE, a.dw1, 2 * a.H, a.d, false); }
+GradPair hidden_pair(const aeris_feed_forward_grad& a) {  // (few tokens: no tiles of 256, whose epilogue has no remainders)
+  return plan_pair(a.dx || a.dw1, a.M, a.H, a.d, EPI_SWIGLU_BWD, few(a.M), a.dw2, a.d, a.H, few(a.M), false);
+}
+GradPair token_pair(const aeris_feed_forward_grad& a) {
+  return plan_pair(a.dx, a.M, a.d, 2 * a.H, EPI_STORE, few(a.M), a.dw1, 2 * a.H, a.d, few(a.M), false);
+}
 
 }  // namespace
 
@@ -1153,66 +1188,78 @@ hipError_t linear_train_launch(const aeris_linear_train& a, hipStream_t stream) 
   p.res_dtype = a.residual ? (int)a.res_dtype : -1;
   p.kept = reinterpret_cast<uint16_t*>(a.z);
   p.act = (int)a.act;
-  return launch<false, false, EPI_ACT>(p, plan_of(a.M, a.N, a.K, EPI_ACT), nullptr, nullptr, stream);
+  return launch<false, false, EPI_ACT>(p, plan_of(a.M, a.N, a.K, EPI_ACT, false), nullptr, nullptr, stream);
 }
 
 int64_t linear_grad_workspace_bytes(const aeris_linear_grad& a) {
   int64_t n = 0;
   if (needs_dz(a) && !a.dz) n += up256(a.M * a.N * 2);
+  if (low_dz(a)) n += up256(a.M * a.N * 2);
   if (bias_apart(a)) n += up256((int64_t)act_grad_parts(a.M, (int)a.N) * a.N * 4);
   return n + pair_bytes(linear_pair(a));
 }
 
 hipError_t linear_grad_launch(const aeris_linear_grad& a, void* workspace, hipStream_t stream) {
   unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
-  const void* dz = a.dy;
-  void* dz_out = nullptr;
-  if (needs_dz(a)) {
-    dz_out = a.dz ? a.dz : ws;
-    if (!a.dz) ws += up256(a.M * a.N * 2);
-    dz = dz_out;
-  }
-  if (dz_out || bias_apart(a)) {
-    float* partial = reinterpret_cast<float*>(ws);
-    if (bias_apart(a)) ws += up256((int64_t)act_grad_parts(a.M, (int)a.N) * a.N * 4);
-    const hipError_t e = act_grad_launch(a.dy, a.dy_dtype == AERIS_F32, a.z, dz_out, partial, bias_apart(a) ? a.dbias : nullptr, a.M, (int)a.N, (int)a.act, stream);
+  auto take = [&](int64_t bytes) {
+    unsigned char* const at = ws;
+    ws += up256(bytes);
+    return at;
+  };
+  void* const dz = !needs_dz(a) ? nullptr : a.dz ? a.dz : take(a.M * a.N * 2);
+  void* const dz_low = low_dz(a) ? take(a.M * a.N * 2) : nullptr;
+  if (dz || bias_apart(a)) {
+    float* const partial = bias_apart(a) ? reinterpret_cast<float*>(take((int64_t)act_grad_parts(a.M, (int)a.N) * a.N * 4)) : nullptr;
+    const hipError_t e = act_grad_launch(a.dy, a.dy_dtype == AERIS_F32, a.z, dz, dz_low, partial, bias_apart(a) ? a.dbias : nullptr, a.M, (int)a.N, (int)a.act, stream);
     if (e != hipSuccess) return e;
   }
-  return launch_pair<EPI_STORE>(linear_pair(a), product(dz, a.N, a.w, a.K, a.dx, a.K, a.M, a.K, a.N), product(dz, a.N, a.x, a.K, a.dw, a.K, a.N, a.K, a.M), ws, a.dbias, stream);
+  const void* const g = dz ? dz : a.dy;
+  GradGemm p = product(g, a.N, a.w, a.K, a.dx, a.K, a.M, a.K, a.N), q = product(g, a.N, a.x, a.K, a.dw, a.K, a.N, a.K, a.M);
+  p.A_low = q.A_low = reinterpret_cast<const uint16_t*>(dz_low);
+  return launch_pair<EPI_STORE>(linear_pair(a), p, q, ws, a.dbias, stream);
 }
 
 // The second projection has nothing to keep: it is the inference kernels' product (14400 tokens, H 6144 -> 1536: 204 us, here 240), but for few
 // tokens of many hidden channels, whose k only the kernels here cut into parts (9 tokens: 22 us there, 12 here; both passes of 384 tokens 59 and 54, of
-// 512 the same; H 4096: 29 and 28; H 2048 and less: 1 to 3 us shorter there), and for k that is no multiple of 64.
-static bool second_is_cut(const aeris_feed_forward& a) { return a.H % 64 != 0 || (a.M <= 384 && a.H >= 4096); }
+// 512 the same; H 4096: 29 and 28; H 2048 and less: 1 to 3 us shorter there), where h has remainders, and for k that is no multiple of 64.
+static bool second_is_own(const aeris_feed_forward& a) { return a.H % 64 != 0 || (a.M <= 384 && a.H >= 4096) || few(a.M); }
 
-int64_t feed_forward_train_workspace_bytes(const aeris_feed_forward& a) { return !second_is_cut(a) ? 0 : plan_of(a.M, a.d, a.H, EPI_STORE).partial_bytes(); }
+int64_t feed_forward_train_workspace_bytes(const aeris_feed_forward& a) {
+  return second_is_own(a) ? plan_of(a.M, a.d, a.H, EPI_STORE, few(a.M)).partial_bytes() : 0;
+}
 
 hipError_t feed_forward_train_launch(const aeris_feed_forward& a, void* workspace, hipStream_t stream) {
   GradGemm p = product(a.x, a.d, a.w1, a.d, a.h, a.H, a.M, a.H, a.d);
   p.kept = reinterpret_cast<uint16_t*>(a.gate_up);
-  const hipError_t e = launch<false, false, EPI_SWIGLU>(p, plan_of(a.M, a.H, a.d, EPI_SWIGLU), nullptr, nullptr, stream);
+  if (few(a.M)) p.C_low = reinterpret_cast<uint16_t*>(a.h) + a.M * a.H;
+  const hipError_t e = launch<false, false, EPI_SWIGLU>(p, plan_of(a.M, a.H, a.d, EPI_SWIGLU, few(a.M)), nullptr, nullptr, stream);
   if (e != hipSuccess) return e;
-  if (!second_is_cut(a))
+  if (!second_is_own(a))
     return gemm_launch(a.h, a.w2, a.y, nullptr, nullptr, nullptr, a.M, (int)a.d, (int)a.H, a.d, AERIS_ACT_NONE, 0, AERIS_BF16, 0, a.M, 0, 0, 1.0f, 0, stream);
   GradGemm q = product(a.h, a.H, a.w2, a.H, a.y, a.d, a.M, a.d, a.H);
-  return launch<false, false, EPI_STORE>(q, plan_of(a.M, a.d, a.H, EPI_STORE), workspace, nullptr, stream);
+  q.A_low = p.C_low;
+  return launch<false, false, EPI_STORE>(q, plan_of(a.M, a.d, a.H, EPI_STORE, few(a.M)), workspace, nullptr, stream);
 }
 
 int64_t feed_forward_grad_workspace_bytes(const aeris_feed_forward_grad& a) {
-  return (a.dx || a.dw1 ? up256(a.M * a.H * 4) : 0) + more(pair_bytes(hidden_pair(a)), pair_bytes(token_pair(a)));
+  return (a.dx || a.dw1 ? up256(a.M * a.H * (few(a.M) ? 8 : 4)) : 0) + more(pair_bytes(hidden_pair(a)), pair_bytes(token_pair(a)));
 }
 
 hipError_t feed_forward_grad_launch(const aeris_feed_forward_grad& a, void* workspace, hipStream_t stream) {
   unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
-  void* dgu = ws;
-  if (a.dx || a.dw1) ws += up256(a.M * a.H * 4);
-  GradGemm p = product(a.dy, a.d, a.w2, a.H, dgu, 2 * a.H, a.M, a.H, a.d);
+  uint16_t* const dgu = reinterpret_cast<uint16_t*>(ws);
+  uint16_t* const dgu_low = few(a.M) ? dgu + a.M * 2 * a.H : nullptr;
+  if (a.dx || a.dw1) ws += up256(a.M * a.H * (few(a.M) ? 8 : 4));
+  GradGemm p = product(a.dy, a.d, a.w2, a.H, dgu, 2 * a.H, a.M, a.H, a.d), q = product(a.dy, a.d, a.h, a.H, a.dw2, a.H, a.d, a.H, a.M);
   p.kept = reinterpret_cast<uint16_t*>(const_cast<void*>(a.gate_up));
-  const hipError_t e = launch_pair<EPI_SWIGLU_BWD>(hidden_pair(a), p, product(a.dy, a.d, a.h, a.H, a.dw2, a.H, a.d, a.H, a.M), ws, nullptr, stream);
+  p.C_low = dgu_low;
+  if (few(a.M)) q.B_low = q.B + a.M * a.H;
+  const hipError_t e = launch_pair<EPI_SWIGLU_BWD>(hidden_pair(a), p, q, ws, nullptr, stream);
   if (e != hipSuccess) return e;
-  return launch_pair<EPI_STORE>(token_pair(a), product(dgu, 2 * a.H, a.w1, a.d, a.dx, a.d, a.M, a.d, 2 * a.H), product(dgu, 2 * a.H, a.x, a.d, a.dw1, a.d, 2 * a.H, a.d, a.M),
-                                ws, nullptr, stream);
+  p = product(dgu, 2 * a.H, a.w1, a.d, a.dx, a.d, a.M, a.d, 2 * a.H);
+  q = product(dgu, 2 * a.H, a.x, a.d, a.dw1, a.d, 2 * a.H, a.d, a.M);
+  p.A_low = q.A_low = dgu_low;
+  return launch_pair<EPI_STORE>(token_pair(a), p, q, ws, nullptr, stream);
 }
 
 }  // namespace aeris

@@ -489,6 +489,7 @@ LINEAR_TRAIN = struct.Struct("=6Q6q")  # struct aeris_linear_train of include/ae
 LINEAR_GRAD = struct.Struct("=8Q5q")  # struct aeris_linear_grad
 FEED_FORWARD = struct.Struct("=6Q3q")  # struct aeris_feed_forward
 FEED_FORWARD_GRAD = struct.Struct("=9Q3q")  # struct aeris_feed_forward_grad
+_FEW_TOKENS = 64  # AERIS_FEW_TOKENS: up to so many, h has remainders behind it
 _KEPT = (L.ACT_GELU, L.ACT_SILU)  # activations whose gradient needs the value they were applied to
 
 
@@ -601,7 +602,7 @@ def _checked_feed_forward(x, w1, w2):
 
 def feed_forward_train(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, keep: bool = True):
     """The gated MLP of a training step, w2[d, H] (silu(gate) * up) with [gate | up] = x[.., d] @ w1[2H, d]^T -> (y bf16 [.., d], gate_up: gate and up in 24 bits
-    (uint8 [M * 2H * 3], None without ``keep``), h bf16 [.., H]): the result and what ``feed_forward_backward`` needs beside x, w1 and w2.  d, H multiples of 8."""
+    (uint8 [M * 2H * 3], None without ``keep``), h: their product (bf16 [M * H], of up to 64 tokens two numbers a value)): the result and what ``feed_forward_backward`` needs beside x, w1 and w2.  d, H multiples of 8."""
     _on_current_device(x.device, dict(x=x, w1=w1, w2=w2))
     return _feed_forward(x, w1, w2, *_checked_feed_forward(x, w1, w2), keep)
 
@@ -611,7 +612,7 @@ def _feed_forward(x, w1, w2, M, d, H, keep):
     device = x.device
     y = torch.empty_like(x)
     gate_up = torch.empty(6 * M * H, dtype=torch.uint8, device=device) if keep else None
-    h = torch.empty(*x.shape[:-1], H, dtype=torch.bfloat16, device=device)
+    h = torch.empty((M if M > _FEW_TOKENS else 2 * M) * H, dtype=torch.bfloat16, device=device)
     if M:
         call = FEED_FORWARD.pack(x.data_ptr(), w1.data_ptr(), w2.data_ptr(), gate_up.data_ptr() if keep else 0, h.data_ptr(), y.data_ptr(), M, d, H)
         need = L.lib().aeris_feed_forward_workspace_bytes(call)
@@ -630,7 +631,7 @@ def feed_forward_backward(dy: torch.Tensor, x: torch.Tensor, w1: torch.Tensor, w
     _on_current_device(dy.device, dict(dy=dy, x=x, w1=w1, w2=w2, gate_up=gate_up, h=h))
     M, d, H = _checked_feed_forward(x, w1, w2)
     _matrix(dy, "dy", M, d)
-    _matrix(h, "h", M, H)
+    _matrix(h, "h", 1, (M if M > _FEW_TOKENS else 2 * M) * H)
     _matrix(gate_up, "gate_up", 1, 6 * M * H, (torch.uint8,))
     return _feed_forward_grads(dy, x, w1, w2, gate_up, h, M, d, H, wanted)
 

@@ -208,9 +208,11 @@ int aeris_gemm_fwd(const void* A, const void* W, void* C, const void* bias, cons
  * Gradients, from that of y (dy [M, N], dy_dtype):  dz = dy act'(z) (rounded to bf16 for the products), written unless NULL:
  *   dx bf16 [M, K] = dz w;  dw bf16 [N, K] = dz^T x;  dbias bf16 [N] = the sums of the unrounded dz;  dz bf16 [M, N] itself (act AERIS_ACT_NONE and an
  *   f32 dy: dy rounded, what a bf16 residual gets); w may be NULL without dx, x without dw, z with AERIS_ACT_NONE
+ * Up to AERIS_FEW_TOKENS tokens the products take dz as two bf16 a value.
  * Sums in fp32, added in an order that depends on the sizes alone.  Outputs share no memory with inputs.  Every tensor contiguous and 16-byte aligned.
  * Supported: N % 8 == 0, K % 8 == 0, N, K <= 2^20, N * K < 2^30.  workspace: aeris_linear_grad_workspace_bytes(a) bytes (addresses do not count but for being
  * NULL), 16-byte aligned, borrowed for the call. */
+#define AERIS_FEW_TOKENS 64
 typedef struct aeris_linear_train {
   const void *x, *w, *bias, *residual;
   void *y, *z;
@@ -226,9 +228,11 @@ int64_t aeris_linear_grad_workspace_bytes(const aeris_linear_grad* a);
 int aeris_linear_bwd(const aeris_linear_grad* a, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* The gated MLP (FeedForward, model.py:148-159) of a training step:
- *   [gate | up] = x w1^T (kept in 24 bits: gate_up, 6 M H bytes; gate_up NULL: not kept), h = silu(gate) up (bf16 [M, H], kept), y bf16 [M, d] = h w2^T
+ *   [gate | up] = x w1^T (kept in 24 bits: gate_up, 6 M H bytes; gate_up NULL: not kept), h = silu(gate) up (bf16 [M, H], kept; with up to
+ *   AERIS_FEW_TOKENS tokens [2, M, H]: behind it what its rounding left over, which y and the gradients take into account), y bf16 [M, d] = h w2^T
  *   x bf16 [M, d], w1 bf16 [2H, d], w2 bf16 [d, H]; gate, up and their product are made in fp32 in one kernel
- * Gradients, from dy bf16 [M, d], each unless NULL:  dh = dy w2 (fp32, never in memory), dgate = dh up silu'(gate), dup = dh silu(gate) (bf16);
+ * Gradients, from dy bf16 [M, d], each unless NULL:  dh = dy w2 (fp32, never in memory), dgate = dh up silu'(gate), dup = dh silu(gate) (bf16, of few tokens two a
+ * value);
  *   dx bf16 [M, d] = [dgate | dup] w1;  dw1 bf16 [2H, d] = [dgate | dup]^T x;  dw2 bf16 [d, H] = dy^T h
  * Otherwise as above.  Supported: d % 8 == 0, H % 8 == 0, d, H <= 2^19, d * H < 2^29. */
 typedef struct aeris_feed_forward {
