@@ -261,7 +261,7 @@ namespace {
 // what aeris_norm_modulate_grad_workspace_bytes looks at too
 bool norm_grad_sizes_ok(const aeris_norm_modulate_grad* a) {
   return a && a->B > 0 && a->rows_per_batch > 0 && a->d > 0 && a->d <= 0x7fffffff && aeris::norm_supported((int)a->d) && a->mod_batch_stride >= 0 &&
-         a->B <= INT64_MAX / a->rows_per_batch && a->B * a->rows_per_batch <= (INT64_MAX >> 4) / a->d;
+         a->B <= INT64_MAX / a->rows_per_batch && a->B * a->rows_per_batch <= (INT64_MAX >> 6) / a->d;
 }
 }  // namespace
 
@@ -285,7 +285,9 @@ int aeris_norm_modulate_bwd(const aeris_norm_modulate_grad* a, void* workspace, 
     if (!aligned16(p)) return fail(AERIS_EINVAL, "%s: every tensor must be 16-byte aligned", who);
   if ((a->dbeta && !a->beta) || (a->dshift && !a->shift) || (a->dscale && !a->scale))
     return fail(AERIS_EINVAL, "%s: dbeta, dshift and dscale need beta, shift and scale", who);
-  if (aeris::norm_grad_blocks(*a) >= 1 << 24) return fail(AERIS_EUNSUPPORTED, "%s: more than 2^24 members", who);
+  // (a workgroup of 256 for every member's rows, one of 1024 for every member and 8 columns; a grid has less than 2^32 threads, 65536 of them in y)
+  if ((a->shift || a->scale) && a->mod_batch_stride && (a->B > 65535 || a->B * (a->d / 8) >= 1 << 22))
+    return fail(AERIS_EUNSUPPORTED, "%s: %lld members of %lld channels with modulation rows of their own", who, (long long)a->B, (long long)a->d);
   const int64_t need = aeris::norm_grad_workspace_bytes(*a);
   if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
     return fail(AERIS_EINVAL, "%s: needs a 16-byte aligned workspace of %lld bytes", who, (long long)need);

@@ -460,11 +460,13 @@ __device__ __forceinline__ bf16x8 all_ones() {
   return v;
 }
 
-// ---- tiles of T x T (128 or 64), four waves two by two, two stages; two or more workgroups a CU fill each other's waits
-template <int T>
-constexpr int tile_lds() { return 2 * 2 * T * BK * 2; }
+// ---- tiles of T x T (128 or 64), four waves two by two.  Two stages, and two to five workgroups a CU that fill each other's waits; tiles of 64
+// whose workgroups are few have four stages instead, or each k-tile would take the time of a load (300 tokens, 4096 -> 1024 with GELU 35 -> 25 us; the
+// gated MLP of 9 tokens, 1536 -> 6144 and back: 33 -> 27 us).
+template <int T, int STAGES>
+constexpr int tile_lds() { return STAGES * 2 * T * BK * 2; }
 
-template <int T, bool A_TR, bool B_TR, int EPI>
+template <int T, int STAGES, bool A_TR, bool B_TR, int EPI>
 __device__ __forceinline__ void grad_tile(const GradGemm& p, int item, unsigned char* smem) {
   constexpr bool SWIGLU = EPI == EPI_SWIGLU, ROW_SUMS = A_TR;
   // waves over the tile: two by two; SwiGLU tiles of 64 four by one, so that a wave has a gate column's up column too
@@ -474,7 +476,7 @@ __device__ __forceinline__ void grad_tile(const GradGemm& p, int item, unsigned 
   constexpr int BN_OUT = SWIGLU ? T / 2 : T;
   using PA = Panel<A_TR, T, 4>;
   using PB = Panel<B_TR, T, 4>;
-  static_assert(2 * (PA::BYTES + PB::BYTES) == tile_lds<T>(), "two stages");
+  static_assert(STAGES * (PA::BYTES + PB::BYTES) == tile_lds<T, STAGES>(), "the stages");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   int part = 0;
@@ -517,22 +519,23 @@ __device__ __forceinline__ void grad_tile(const GradGemm& p, int item, unsigned 
   const bool with_sums = ROW_SUMS && p.row_sums;
 
   const uint32_t lds0 = lds_byte_address(smem);
-  auto issue = [&](int t) {
+  const int all_turns = low ? 2 * turns : turns;
+  auto issue = [&](int t) {  // (past the last k-tile: loads of nothing, which keep the count of the waits the same)
     if (low && t == turns) start(p.A_low ? p.A_low : p.A, p.B_low ? p.B_low : p.B);
-    const uint32_t stage = lds0 + (uint32_t)(t & 1) * (PA::BYTES + PB::BYTES);
+    const uint32_t stage = lds0 + (uint32_t)(t % STAGES) * (PA::BYTES + PB::BYTES);
     la.issue(stage + wave * (PA::LOADS * 1024));
     lb.issue(stage + PA::BYTES + wave * (PB::LOADS * 1024));
     la.next();
     lb.next();
   };
-  if (turns > 0) issue(0);
+#pragma unroll
+  for (int t = 0; t < STAGES - 1; ++t) issue(t);
   int sum_turn = with_sums ? (int)((k_begin / BK) % p.tiles_n) : 0;
-  const int all_turns = low ? 2 * turns : turns;
   for (int t = 0; t < all_turns; ++t) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();  // stage t is there; the other one has been read
-    if (t + 1 < all_turns) issue(t + 1);
-    const uint32_t sa = lds0 + (uint32_t)(t & 1) * (PA::BYTES + PB::BYTES), sb = sa + PA::BYTES;
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * (PA::LOADS + PB::LOADS)) : "memory");
+    __syncthreads();  // stage t is there; the one that is filled next has been read
+    issue(t + STAGES - 1);
+    const uint32_t sa = lds0 + (uint32_t)(t % STAGES) * (PA::BYTES + PB::BYTES), sb = sa + PA::BYTES;
     const bool mine = with_sums && sum_turn == tile.n;
     auto step = [&](auto ks) {
       constexpr int KS = decltype(ks)::value;
@@ -557,7 +560,8 @@ __device__ __forceinline__ void grad_tile(const GradGemm& p, int item, unsigned 
     step(std::integral_constant<int, 1>{});
     if (++sum_turn == p.tiles_n) sum_turn = 0;
   }
-  __syncthreads();  // the stages are read: they stage the result now
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();  // the stages are read and nothing more arrives in them: they stage the result now
   float* const at = EPI == EPI_STORE && cut ? p.partial + ((int64_t)(item - p.whole) * p.parts + part) * (T * T) : nullptr;
   const uint32_t stage = lds0 + wave * (16 * FN * 64);
   if (at) grad_epilogue<T, EPI, FM, FN>(p, acc, wm * (T / WM), wn * (T / WN), at, stage, lane);
@@ -577,19 +581,19 @@ __device__ __forceinline__ int xcd_item(const GradGemm& p, int b, int n) {
   return b < p.whole ? xcd_order(b, p.whole) : p.whole + xcd_order(b - p.whole, n - p.whole);
 }
 
-template <int T, bool A_TR, bool B_TR, int EPI>
+template <int T, int STAGES, bool A_TR, bool B_TR, int EPI>
 __global__ void __launch_bounds__(256, 2) gemm_grad_tile_kernel(GradGemm p) {
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[tile_lds<T>()];
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[tile_lds<T, STAGES>()];
   const int item = xcd_item(p, blockIdx.x, gridDim.x);
-  grad_tile<T, A_TR, B_TR, EPI>(p, item, smem);
+  grad_tile<T, STAGES, A_TR, B_TR, EPI>(p, item, smem);
 }
 
 // two products that do not depend on each other in one launch: the first n workgroups make dx (or dh and what follows from it), the others dw
-template <int T, int EPI>
+template <int T, int STAGES, int EPI>
 __global__ void __launch_bounds__(256, 2) gemm_grad_pair_kernel(GradGemm p, GradGemm q, int n) {
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[tile_lds<T>()];
-  if ((int)blockIdx.x < n) grad_tile<T, false, true, EPI>(p, xcd_item(p, blockIdx.x, n), smem);
-  else grad_tile<T, true, true, EPI_STORE>(q, xcd_item(q, blockIdx.x - n, gridDim.x - n), smem);
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[tile_lds<T, STAGES>()];
+  if ((int)blockIdx.x < n) grad_tile<T, STAGES, false, true, EPI>(p, xcd_item(p, blockIdx.x, n), smem);
+  else grad_tile<T, STAGES, true, true, EPI_STORE>(q, xcd_item(q, blockIdx.x - n, gridDim.x - n), smem);
 }
 
 // ---- tiles of 256 x 256, eight waves (two by four, 128 x 64 each), one persistent workgroup a CU: the pipeline of the package's other
@@ -1073,6 +1077,9 @@ hipError_t finish(const GradGemm& p, int64_t n, const GradGemm& q, int64_t m, in
   return hipGetLastError();
 }
 
+// up to two workgroups a CU, which tiles of 64 in four stages have room for (beyond: 1536 of them, [2048, 2048] of k = 256, 12.3 -> 15.3 us)
+bool few_items(int64_t n) { return n <= 512; }
+
 // one product; `bias`: from the sums over k of a dw
 template <bool A_TR, bool B_TR, int EPI>
 hipError_t launch(GradGemm& p, const GradPlan& g, void* partial, uint16_t* bias, hipStream_t stream) {
@@ -1081,10 +1088,11 @@ hipError_t launch(GradGemm& p, const GradPlan& g, void* partial, uint16_t* bias,
   if (g.tile == 256) {
     const unsigned grid = g.whole ? 256 : (unsigned)((g.left() * g.parts + 7) / 8 * 8);
     hipLaunchKernelGGL((gemm_grad_big_kernel<A_TR, B_TR, EPI>), dim3(grid), dim3(512), BIG_LDS, stream, p);
-  } else if (g.tile == 128) {
-    hipLaunchKernelGGL((gemm_grad_tile_kernel<128, A_TR, B_TR, EPI>), dim3((unsigned)g.items()), dim3(256), 0, stream, p);
   } else {
-    hipLaunchKernelGGL((gemm_grad_tile_kernel<64, A_TR, B_TR, EPI>), dim3((unsigned)g.items()), dim3(256), 0, stream, p);
+    const dim3 grid((unsigned)g.items()), block(256);
+    if (g.tile == 128) hipLaunchKernelGGL((gemm_grad_tile_kernel<128, 2, A_TR, B_TR, EPI>), grid, block, 0, stream, p);
+    else if (few_items(g.items())) hipLaunchKernelGGL((gemm_grad_tile_kernel<64, 4, A_TR, B_TR, EPI>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((gemm_grad_tile_kernel<64, 2, A_TR, B_TR, EPI>), grid, block, 0, stream, p);
   }
   const hipError_t e = hipGetLastError();
   return e != hipSuccess ? e : finish(p, 0, p, g.parts > 1 ? g.left() : 0, g.tile, bias, stream);
@@ -1135,9 +1143,11 @@ hipError_t launch_pair(const GradPair& r, GradGemm p, GradGemm q, void* workspac
   }
   apply(p, r.g, ws);
   apply(q, r.h, ws_q);
-  const dim3 grid((unsigned)(r.g.items() + r.h.items()));
-  if (r.g.tile == 128) hipLaunchKernelGGL((gemm_grad_pair_kernel<128, EPI>), grid, dim3(256), 0, stream, p, q, (int)r.g.items());
-  else hipLaunchKernelGGL((gemm_grad_pair_kernel<64, EPI>), grid, dim3(256), 0, stream, p, q, (int)r.g.items());
+  const dim3 grid((unsigned)(r.g.items() + r.h.items())), block(256);
+  const int n = (int)r.g.items();
+  if (r.g.tile == 128) hipLaunchKernelGGL((gemm_grad_pair_kernel<128, 2, EPI>), grid, block, 0, stream, p, q, n);
+  else if (few_items(r.g.items() + r.h.items())) hipLaunchKernelGGL((gemm_grad_pair_kernel<64, 4, EPI>), grid, block, 0, stream, p, q, n);
+  else hipLaunchKernelGGL((gemm_grad_pair_kernel<64, 2, EPI>), grid, block, 0, stream, p, q, n);
   const hipError_t e = hipGetLastError();
   return e != hipSuccess ? e : finish(p, r.g.parts > 1 ? r.g.left() : 0, q, r.h.parts > 1 ? r.h.left() : 0, r.g.tile, b, stream);
 }
@@ -1147,7 +1157,7 @@ int64_t more(int64_t a, int64_t b) { return a > b ? a : b; }
 
 // Few tokens: what one product rounds for the next (h; dgate and dup; dz) is kept as two bf16 a value, and the products behind it go over k
 // twice.  Their errors do not average out over many tokens, and the products are bound by the weights' way through memory (9 tokens, 1536 ->
-// 6144: both passes 70 us with and without).
+// 6144: forward 27 us either way, backward 43 -> 55).
 bool few(int64_t M) { return M <= AERIS_FEW_TOKENS; }
 
 bool needs_dz(const aeris_linear_grad& a) { return (a.dy_dtype == AERIS_F32 || a.act != AERIS_ACT_NONE) && (a.dx || a.dw || a.dz); }

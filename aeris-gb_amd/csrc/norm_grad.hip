@@ -323,7 +323,8 @@ __global__ void __launch_bounds__(256, (resident<NV, PRE>())) norm_grad_kernel(N
 }
 
 struct NormGradSums {
-  const float* partial;
+  const float* partial;  // [segments][blocks][sums][d]
+  float* members;        // [segments][2][d]: every segment's share of dgamma and dbeta, added up by another kernel; or NULL: by this one
   const void* gamma;
   const void* beta;
   const float* scale;
@@ -335,72 +336,96 @@ struct NormGradSums {
   int segments, blocks, d, param_f32, pre;
 };
 
-// 8 columns a workgroup; 128 threads share a column's partial sums
+__device__ __forceinline__ void store_param_grads(const NormGradSums& p, int col, float dgamma, float dbeta) {
+  if (p.param_f32) {
+    if (p.dgamma) reinterpret_cast<float*>(p.dgamma)[col] = dgamma;
+    if (p.dbeta) reinterpret_cast<float*>(p.dbeta)[col] = dbeta;
+  } else {
+    if (p.dgamma) reinterpret_cast<uint16_t*>(p.dgamma)[col] = (uint16_t)f32_to_bf16_bits(dgamma);
+    if (p.dbeta) reinterpret_cast<uint16_t*>(p.dbeta)[col] = (uint16_t)f32_to_bf16_bits(dbeta);
+  }
+}
+
+// 8 columns a workgroup (d is a multiple of 8); 128 threads share a column's sums over `rows` rows, q(row, sum) the address of one.
+// The results are thread 0 .. 7's, whose columns they are.
+template <int SUMS, class At>
+__device__ __forceinline__ void column_sums(int rows, const At& q, float (*lds)[4][8], float (&t)[SUMS]) {
+  const int c = threadIdx.x & 7, r = threadIdx.x >> 3;
+#pragma unroll
+  for (int s = 0; s < SUMS; ++s) t[s] = 0.f;
+#pragma unroll 4
+  for (int b = r; b < rows; b += 128)
+#pragma unroll
+    for (int s = 0; s < SUMS; ++s) t[s] += *q(b, s);
+#pragma unroll
+  for (int s = 0; s < SUMS; ++s) {  // over the 8 rows of the wave
+    t[s] += __shfl_xor(t[s], 8);
+    t[s] += __shfl_xor(t[s], 16);
+    t[s] += __shfl_xor(t[s], 32);
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) < 8) {
+#pragma unroll
+    for (int s = 0; s < SUMS; ++s) lds[threadIdx.x >> 6][s][c] = t[s];
+  }
+  __syncthreads();
+  if (threadIdx.x < 8) {
+#pragma unroll
+    for (int s = 0; s < SUMS; ++s) {
+      t[s] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 16; ++w) t[s] += lds[w][s][c];
+    }
+  }
+}
+
+template <bool PRE>
 __global__ void __launch_bounds__(1024) norm_grad_sums_kernel(NormGradSums p) {
+  constexpr int SUMS = PRE ? 4 : 2;
   __shared__ float lds[16][4][8];
-  const int c = threadIdx.x & 7, r = threadIdx.x >> 3, wave = threadIdx.x >> 6;
-  const int col = blockIdx.x * 8 + c;  // (d is a multiple of 8)
-  const int sums = p.pre ? 4 : 2;
+  const int col = blockIdx.x * 8 + (threadIdx.x & 7);
   const float ga = param_at(p.gamma, p.param_f32, col);
   const float be = p.beta ? param_at(p.beta, p.param_f32, col) : 0.f;
   float dgamma = 0.f, dbeta = 0.f;
-  for (int seg = 0; seg < p.segments; ++seg) {
-    float t[4] = {0.f, 0.f, 0.f, 0.f};
-    const float* q = p.partial + ((int64_t)seg * p.blocks + r) * sums * p.d + col;
-#pragma unroll 4
-    for (int b = r; b < p.blocks; b += 128, q += (int64_t)128 * sums * p.d) {
-      t[0] += q[0];
-      t[1] += q[p.d];
-      if (p.pre) {
-        t[2] += q[2 * (int64_t)p.d];
-        t[3] += q[3 * (int64_t)p.d];
-      }
-    }
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {  // over the 8 rows of the wave
-      t[s] += __shfl_xor(t[s], 8);
-      t[s] += __shfl_xor(t[s], 16);
-      t[s] += __shfl_xor(t[s], 32);
-    }
-    if ((threadIdx.x & 63) < 8) {
-#pragma unroll
-      for (int s = 0; s < 4; ++s) lds[wave][s][c] = t[s];
-    }
-    __syncthreads();
+  const int first = p.members ? blockIdx.y : 0, last = p.members ? blockIdx.y + 1 : p.segments;
+  for (int seg = first; seg < last; ++seg) {
+    float t[SUMS];
+    const float* const base = p.partial + (int64_t)seg * p.blocks * SUMS * p.d + col;
+    column_sums<SUMS>(p.blocks, [&](int b, int s) { return base + ((int64_t)b * SUMS + s) * p.d; }, lds, t);
     if (threadIdx.x < 8) {
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        t[s] = 0.f;
-#pragma unroll
-        for (int w = 0; w < 16; ++w) t[s] += lds[w][s][c];
-      }
-      float ds, dt;
-      if (p.pre) {
-        dgamma += t[0];
-        dbeta += t[1];
-        ds = t[2];
-        dt = t[3];
+      float A = t[0], B = t[1], ds, dt;
+      if (PRE) {
+        ds = t[SUMS - 2];
+        dt = t[SUMS - 1];
       } else {
         const float one = p.scale ? 1.f + p.scale[seg * p.mod_stride + col] : 1.f;
-        dgamma = fmaf(one, t[0], dgamma);
-        dbeta = fmaf(one, t[1], dbeta);
-        ds = fmaf(ga, t[0], be * t[1]);
-        dt = t[1];
+        ds = fmaf(ga, A, be * B);
+        dt = B;
+        A *= one;
+        B *= one;
       }
       if (p.dscale) p.dscale[(int64_t)seg * p.d + col] = ds;
       if (p.dshift) p.dshift[(int64_t)seg * p.d + col] = dt;
+      dgamma += A;
+      dbeta += B;
     }
-    __syncthreads();
   }
   if (threadIdx.x < 8) {
-    if (p.param_f32) {
-      if (p.dgamma) reinterpret_cast<float*>(p.dgamma)[col] = dgamma;
-      if (p.dbeta) reinterpret_cast<float*>(p.dbeta)[col] = dbeta;
+    if (p.members) {
+      p.members[((int64_t)blockIdx.y * 2) * p.d + col] = dgamma;
+      p.members[((int64_t)blockIdx.y * 2 + 1) * p.d + col] = dbeta;
     } else {
-      if (p.dgamma) reinterpret_cast<uint16_t*>(p.dgamma)[col] = (uint16_t)f32_to_bf16_bits(dgamma);
-      if (p.dbeta) reinterpret_cast<uint16_t*>(p.dbeta)[col] = (uint16_t)f32_to_bf16_bits(dbeta);
+      store_param_grads(p, col, dgamma, dbeta);
     }
   }
+}
+
+__global__ void __launch_bounds__(1024) norm_grad_members_kernel(NormGradSums p) {
+  __shared__ float lds[16][4][8];
+  const int col = blockIdx.x * 8 + (threadIdx.x & 7);
+  float t[2];
+  column_sums<2>(p.segments, [&](int b, int s) { return p.members + ((int64_t)b * 2 + s) * p.d + col; }, lds, t);
+  if (threadIdx.x < 8) store_param_grads(p, col, t[0], t[1]);
 }
 
 bool wants_sums(const aeris_norm_modulate_grad& a) { return a.dgamma || a.dbeta || a.dshift || a.dscale; }
@@ -457,8 +482,11 @@ hipError_t launch_wide(const NormGradParams& p, bool yf, int64_t blocks, hipStre
 
 int64_t norm_grad_blocks(const aeris_norm_modulate_grad& a) { return segments_of(a) * blocks_of(a); }
 
+// many members: their sums side by side, and another kernel for what adds up over them
+static bool members_apart(const aeris_norm_modulate_grad& a) { return segments_of(a) > 8; }
+
 int64_t norm_grad_workspace_bytes(const aeris_norm_modulate_grad& a) {
-  return wants_sums(a) ? norm_grad_blocks(a) * (is_pre(a) ? 4 : 2) * a.d * 4 : 0;
+  return wants_sums(a) ? (norm_grad_blocks(a) * (is_pre(a) ? 4 : 2) + (members_apart(a) ? 2 * segments_of(a) : 0)) * a.d * 4 : 0;
 }
 
 hipError_t norm_grad_launch(const aeris_norm_modulate_grad& a, void* workspace, hipStream_t stream) {
@@ -500,7 +528,13 @@ hipError_t norm_grad_launch(const aeris_norm_modulate_grad& a, void* workspace, 
   s.d = p.d;
   s.param_f32 = p.param_f32;
   s.pre = pre;
-  hipLaunchKernelGGL(norm_grad_sums_kernel, dim3((unsigned)(p.d / 8)), dim3(1024), 0, stream, s);
+  s.members = members_apart(a) ? p.partial + blocks * (pre ? 4 : 2) * p.d : nullptr;
+  const dim3 grid((unsigned)(p.d / 8), s.members ? (unsigned)segments : 1u);
+  if (pre) hipLaunchKernelGGL(norm_grad_sums_kernel<true>, grid, dim3(1024), 0, stream, s);
+  else hipLaunchKernelGGL(norm_grad_sums_kernel<false>, grid, dim3(1024), 0, stream, s);
+  e = hipGetLastError();
+  if (e != hipSuccess || !s.members || !(a.dgamma || a.dbeta)) return e;
+  hipLaunchKernelGGL(norm_grad_members_kernel, dim3((unsigned)(p.d / 8)), dim3(1024), 0, stream, s);
   return hipGetLastError();
 }
 

@@ -8,9 +8,9 @@ none is.
 
 Streams and graphs: calls follow the current stream and hold no scratch memory beyond it, and a forward pass with its backward pass may
 be captured into a HIP graph.  torch's own rule for that holds here too: while the graph is captured, no eager graph of the same leaves
-may be alive on another stream (torch would tie that stream to the capture and the process would end).  A captured call on a
-leaf for which an eager result of this module still lives is refused with a RuntimeError; release the result, or do the eager passes on
-the stream that captures.
+may be alive on another stream (torch would tie that stream to the capture and the process would end).  A captured call on
+tensors whose leaves an eager result of this module still has behind it is refused with a RuntimeError; release the result, or do the eager
+passes on the stream that captures.
 """
 from __future__ import annotations
 
@@ -25,7 +25,7 @@ from . import ops
 __all__ = ["feed_forward", "linear", "norm_modulate"]
 
 _capturing = torch._C._cuda_isCurrentStreamCapturing
-_EAGER = weakref.WeakSet()  # nodes of eager graphs that are alive, each with its stream and the identities of the leaves it was made of
+_EAGER = weakref.WeakSet()  # nodes of eager graphs that are alive, each with its stream
 
 
 def _wants_grad(leaves):
@@ -36,17 +36,39 @@ def _wants_grad(leaves):
     return False
 
 
-def _note(ctx, leaves):
-    """Notes an eager graph's node and its leaves; under a capture, refuses leaves of such a graph on another stream."""
-    of = [id(t) for t in leaves if t is not None and t.requires_grad and t.is_leaf]
+def _leaves(nodes):
+    """Identities of the tensors whose gradients the graphs behind these nodes accumulate."""
+    seen, found, todo = set(), set(), [n for n in nodes if n is not None]
+    while todo:
+        node = todo.pop()
+        if id(node) in seen:
+            continue
+        seen.add(id(node))
+        found.add(id(getattr(node, "variable", None)))
+        todo += [n for n, _ in node.next_functions if n is not None]
+    return found - {id(None)}
+
+
+def _note(ctx, inputs):
+    """Notes an eager graph's node; under a capture, refuses inputs whose leaves an eager graph of another stream has too."""
+    raw = ops._stream()
     if not _capturing():
-        ctx.stream, ctx.leaves = ops._stream(), of
+        ctx.stream = raw
         _EAGER.add(ctx)
         return
-    raw = ops._stream()
-    if any(node.stream != raw and not set(of).isdisjoint(node.leaves) for node in list(_EAGER)):
-        raise RuntimeError("an eager graph of a tensor of this captured call is still alive on another stream: release its result before the capture "
-                           "(torch ties that stream to the capture in the backward pass, which ends the process)")
+    others = [node for node in list(_EAGER) if node.stream != raw]
+    if others:
+        inputs = [t for t in inputs if t is not None and t.requires_grad]
+        mine = {id(t) for t in inputs if t.is_leaf} | _leaves([t.grad_fn for t in inputs])
+        if not mine.isdisjoint(_leaves(others)):
+            raise RuntimeError("an eager graph of a tensor of this captured call is still alive on another stream: release its result before the capture "
+                               "(torch ties that stream to the capture in the backward pass, which ends the process)")
+
+
+def _incoming(dy):
+    """A result's gradient as the kernels read it: contiguous, its address a multiple of 16."""
+    dy = dy.contiguous()
+    return dy.clone() if dy.data_ptr() & 15 else dy
 
 
 def _rows(t: Optional[torch.Tensor]):
@@ -74,7 +96,7 @@ class _NormModulate(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        return (*ops._norm_grads(dy.contiguous(), *ctx.saved_tensors, *ctx.how, ctx.needs_input_grad[:5]), None, None, None, None)
+        return (*ops._norm_grads(_incoming(dy), *ctx.saved_tensors, *ctx.how, ctx.needs_input_grad[:5]), None, None, None, None)
 
 
 def norm_modulate(x: torch.Tensor, gamma: torch.Tensor, beta: Optional[torch.Tensor] = None, shift: Optional[torch.Tensor] = None,
@@ -105,18 +127,19 @@ class _Linear(torch.autograd.Function):
         y, z = ops._linear_forward(a, w, bias, residual, act, out_dtype, M, N, K, ctx.needs_input_grad[0] or ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
         ctx.save_for_backward(a, w, z)
         ctx.how = ops._ACT[act], M, N, K
-        ctx.res_dtype = None if residual is None else residual.dtype
+        ctx.residual = None if residual is None else (residual.dtype, residual.shape)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         need_a, need_w, need_bias, need_res = ctx.needs_input_grad[:4]
-        dy = dy.contiguous()
-        round_res = need_res and ctx.res_dtype is not dy.dtype and dy.dtype is torch.float32 and ctx.how[0] == ops.L.ACT_NONE  # dz is what a bf16 residual gets
+        dy = _incoming(dy)
+        res_dtype, res_shape = ctx.residual if need_res else (None, None)
+        round_res = need_res and res_dtype is not dy.dtype and dy.dtype is torch.float32 and ctx.how[0] == ops.L.ACT_NONE  # dz is what a bf16 residual gets
         da, dw, dbias, dres = ops._linear_grads(dy, *ctx.saved_tensors, *ctx.how, (need_a, need_w, need_bias, round_res))
-        if need_res and not round_res:
-            dres = dy.to(ctx.res_dtype)
+        if need_res:
+            dres = (dres if round_res else dy.to(res_dtype)).view(res_shape)
         return da, dw, dbias, dres, None, None, None, None, None
 
 
@@ -146,7 +169,7 @@ class _FeedForward(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        return (*ops._feed_forward_grads(dy.contiguous(), *ctx.saved_tensors, *ctx.sizes, ctx.needs_input_grad[:3]), None, None, None)
+        return (*ops._feed_forward_grads(_incoming(dy), *ctx.saved_tensors, *ctx.sizes, ctx.needs_input_grad[:3]), None, None, None)
 
 
 def feed_forward(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor) -> torch.Tensor:

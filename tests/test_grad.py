@@ -18,10 +18,10 @@ BF16, F32 = torch.bfloat16, torch.float32
 
 
 def close(got, want, bound, name):
-    got = got.detach().double().cpu()
+    got = got.detach().double().to(want.device)
     assert got.shape == want.shape, (name, got.shape, want.shape)
     over = (got - want).abs() - SLACK * bound - 1e-30
-    worst = over.max() if over.numel() else torch.tensor(-1.0)
+    worst = over.max().cpu() if over.numel() else torch.tensor(-1.0)
     assert worst <= 0, f"{name}: {int((over > 0).sum())} of {over.numel()} beyond their bound, by up to {float(worst):.3g} (bound there {float(bound.flatten()[over.argmax()]):.3g})"
     assert not torch.isnan(got).any(), name
 
@@ -231,7 +231,8 @@ def act_of(z, act):
     return z * torch.sigmoid(z) if act == "silu" else z
 
 
-def check_linear(pkg, cuda, g, M, N, K, act, bias, residual, y_dtype, lead=None):
+def check_linear(pkg, cuda, g, M, N, K, act, bias, residual, y_dtype, lead=None, at="cpu"):
+    """``at``: where the 64-bit products are made."""
     shape = lead or (M,)
     a = tokens(g, M, K).to(BF16)
     w = (torch.randn(N, K, generator=g) * K ** -0.5).to(BF16)
@@ -249,7 +250,8 @@ def check_linear(pkg, cuda, g, M, N, K, act, bias, residual, y_dtype, lead=None)
     assert y.shape == (*shape, N) and y.dtype is y_dtype
     got = dict(zip(on, torch.autograd.grad(y, list(on.values()), dy.to(cuda).view(y.shape))))
     # the definition
-    p64 = {n: t.double().requires_grad_() for n, t in p.items() if t is not None}
+    a, w, b, dy = a.to(at), w.to(at), None if b is None else b.to(at), dy.to(at)
+    p64 = {n: t.to(at).double().requires_grad_() for n, t in p.items() if t is not None}
     z = p64["a"] @ p64["w"].T + (p64["bias"] if bias else 0)
     want_y = act_of(z, act) + (p64["residual"] if residual else 0)
     want = dict(zip(p64, torch.autograd.grad(want_y, list(p64.values()), dy.double())))
@@ -312,6 +314,21 @@ def test_linear_many_tokens_few_weights(pkg, cuda, M):
     check_linear(pkg, cuda, torch.Generator().manual_seed(M), M, 128, 64, None, True, None, BF16)
 
 
+# Products large enough for tiles of 256: whole rounds of them, a last round cut along k, rows, columns and k that end inside a tile, in all three
+# layouts and with every epilogue.
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K,act,y_dtype,residual", [(8200, 2056, 1088, None, BF16, None), (4113, 4104, 1024, "gelu", BF16, BF16), (16500, 1032, 512, "silu", F32, F32),
+                                                        (33000, 520, 1536, None, F32, F32), (2304, 6152, 2048, "gelu", F32, None)])
+def test_linear_large_products(pkg, cuda, M, N, K, act, y_dtype, residual):
+    check_linear(pkg, cuda, torch.Generator().manual_seed(M), M, N, K, act, True, residual, y_dtype, at=cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,d,H", [(8200, 512, 2056), (16400, 264, 1088), (4100, 1544, 3080)])
+def test_feed_forward_large_products(pkg, cuda, M, d, H):
+    check_feed_forward(pkg, cuda, torch.Generator().manual_seed(M), M, d, H, at=cuda)
+
+
 @pytest.mark.gpu
 def test_what_lies_behind_the_rows_of_a_k_tile_does_not_matter(pkg, cuda):
     """N = 72 ends inside a k-tile of da = dz w: the next row's elements, NaN here, take no part in a row's sums."""
@@ -350,7 +367,7 @@ def test_activation_gradients_of_any_value(pkg, cuda, act):
 # ----------------------------------------------------------------------------------------------
 # the gated MLP
 
-def check_feed_forward(pkg, cuda, g, M, d, H, lead=None, loud=1.0):
+def check_feed_forward(pkg, cuda, g, M, d, H, lead=None, loud=1.0, at="cpu"):
     x = (loud * tokens(g, M, d)).to(BF16)
     w1, w2 = (torch.randn(2 * H, d, generator=g) * d ** -0.5).to(BF16), (torch.randn(d, H, generator=g) * H ** -0.5).to(BF16)
     dy = torch.randn(M, d, generator=g).to(BF16)
@@ -358,6 +375,7 @@ def check_feed_forward(pkg, cuda, g, M, d, H, lead=None, loud=1.0):
     y = pkg.grad.feed_forward(*on)
     assert y.shape == on[0].shape and y.dtype is BF16
     got = torch.autograd.grad(y, on, dy.to(cuda).view(y.shape))
+    x, w1, w2, dy = (t.to(at) for t in (x, w1, w2, dy))
     p = [t.double().requires_grad_() for t in (x, w1, w2)]
     gate, up = (p[0] @ p[1].T).chunk(2, dim=-1)
     want_y = (gate * torch.sigmoid(gate) * up) @ p[2].T
@@ -584,6 +602,131 @@ def test_capture_beside_a_living_eager_graph_is_refused(pkg, cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("through", ["view", "cast"])
+def test_capture_beside_a_living_eager_graph_of_what_an_input_was_made_of(pkg, cuda, through):
+    """The leaf is not an input of the call itself: a modulation matrix that is cut into vectors, an f32 weight that is cast."""
+    G = pkg.grad
+    x = torch.randn(1, 20, 64, device=cuda).to(BF16)
+    gamma = torch.ones(64, dtype=BF16, device=cuda)
+    leaf = torch.zeros(1, 128, device=cuda, requires_grad=True) if through == "view" else torch.zeros(64, 64, device=cuda, requires_grad=True)
+
+    def call():
+        return G.norm_modulate(x, gamma, None, leaf[:, :64], leaf[:, 64:]) if through == "view" else G.linear(x, leaf.to(BF16))
+    alive = call()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+            call()
+    torch.cuda.synchronize()
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        y = call()
+        got, = torch.autograd.grad(y, [leaf], torch.ones_like(y))
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        y = call()
+        want, = torch.autograd.grad(y, [leaf], torch.ones_like(y))
+        assert torch.equal(got, want)
+        del y
+
+
+@pytest.mark.gpu
+def test_captured_call_without_gradients_beside_an_eager_graph(pkg, cuda):
+    leaf, _ = make(pkg, cuda, 10)
+    y = branches(pkg.grad, leaf)
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        out = branches(pkg.grad, leaf)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, y)
+
+
+@pytest.mark.gpu
+def test_many_members_with_modulation_rows_of_their_own(pkg, cuda):
+    g = torch.Generator().manual_seed(12)
+    for B, S, d, order in ((9, 5, 64, "norm_then_mod"), (40, 3, 136, "mod_then_norm"), (300, 1, 8, "norm_then_mod"), (1500, 2, 128, "mod_then_norm")):
+        p, dy = norm_case(g, B, S, d, "layernorm", "members", F32, BF16, F32)
+        check_norm(pkg, cuda, p, dy, "layernorm", order, 1e-5, {"x": F32, "gamma": F32})
+
+
+@pytest.mark.gpu
+def test_bf16_rows_that_belong_to_several_waves(pkg, cuda):
+    """bf16 tokens, the modulation ahead of the norm, enough of them for two and four waves to a row; 64-bit reference on the GPU."""
+    g = torch.Generator().manual_seed(13)
+    for B, S, d in ((1, 40001, 776), (2, 10007, 1536), (1, 15001, 2048)):
+        for y_dtype in (BF16, F32):
+            p, dy = norm_case(g, B, S, d, "rmsnorm", "members", BF16, y_dtype, BF16, beta=False)
+            y, got, on = run_norm(pkg, cuda, p, dy, "rmsnorm", "mod_then_norm", 1e-6)
+            p64 = [None if t is None else t.to(cuda).double().requires_grad_() for t in p]
+            names = [n for n, t in zip(NAMES, p64) if t is not None]
+            want = torch.autograd.grad(norm_definition(*p64, "rmsnorm", "mod_then_norm", 1e-6), [t for t in p64 if t is not None], dy.to(cuda).double())
+            bounds = norm_bounds(p64, dy.to(cuda).double(), "rmsnorm", "mod_then_norm", 1e-6, {"x": BF16, "gamma": BF16})
+            for n, w in zip(names, want):
+                close(got[n], w, bounds[n], n)
+
+
+@pytest.mark.gpu
+def test_gradients_that_arrive_at_odd_addresses(pkg, cuda):
+    leaf, dy = make(pkg, cuda, 14)
+    y = branches(pkg.grad, leaf)
+    want = torch.autograd.grad(y, list(leaf.values()), dy, retain_graph=True)
+    odd = torch.empty(dy.numel() + 3, dtype=BF16, device=cuda)[3:].view(dy.shape).copy_(dy)
+    assert odd.data_ptr() % 16 and odd.is_contiguous()
+    got = torch.autograd.grad(y, list(leaf.values()), odd)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_a_residual_of_another_shape(pkg, cuda):
+    g = torch.Generator().manual_seed(15)
+    x, w = torch.randn(2, 30, 64, generator=g).to(BF16).to(cuda), torch.randn(16, 64, generator=g).to(BF16).to(cuda)
+    for dtype, y_dtype in ((BF16, F32), (F32, F32), (F32, BF16)):
+        res = torch.randn(60, 16, generator=g).to(dtype).to(cuda).requires_grad_()
+        dy = torch.randn(2, 30, 16, generator=g).to(y_dtype).to(cuda)
+        got, = torch.autograd.grad(pkg.grad.linear(x, w, residual=res, out_dtype=y_dtype), [res], dy)
+        assert got.dtype is dtype and torch.equal(got, dy.to(dtype).view(60, 16))
+
+
+@pytest.mark.gpu
+def test_gradients_of_gradients_are_refused(pkg, cuda):
+    leaf, dy = make(pkg, cuda, 16)
+    y = branches(pkg.grad, leaf)
+    got, = torch.autograd.grad(y, [leaf["x"]], dy, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(got.sum(), [leaf["x"]])
+
+
+@pytest.mark.gpu
+def test_a_parameter_changed_in_place_is_noticed(pkg, cuda):
+    leaf, dy = make(pkg, cuda, 17)
+    y = branches(pkg.grad, leaf)
+    with torch.no_grad():
+        leaf["w1"].mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(y, [leaf["w1"]], dy)
+
+
+@pytest.mark.gpu
+def test_a_step_of_training(pkg, cuda):
+    """Two eager steps with an optimizer on the leaves, through ``backward``: the gradients that accumulate are those of each step."""
+    leaf, dy = make(pkg, cuda, 18)
+    opt = torch.optim.SGD(list(leaf.values()), lr=1e-3)
+    for _ in range(2):
+        opt.zero_grad()
+        want = torch.autograd.grad(branches(pkg.grad, leaf), list(leaf.values()), dy)
+        branches(pkg.grad, leaf).backward(dy)
+        assert all(torch.equal(t.grad, w) for t, w in zip(leaf.values(), want))
+        branches(pkg.grad, leaf).backward(dy)
+        assert all(torch.equal(t.grad, w + w) for t, w in zip(leaf.values(), want))
+        opt.step()
+
+
+@pytest.mark.gpu
 def test_refusals(pkg, cuda):
     G = pkg.grad
     x = torch.zeros(1, 4, 64, dtype=BF16, device=cuda)
@@ -637,7 +780,8 @@ def test_native_argument_checks_need_no_gpu(pkg):
     for change in (dict(x=0), dict(dy=0), dict(gamma=0), dict(B=0), dict(rows=-1), dict(xt=2), dict(yt=9), dict(pt=-1), dict(kind=2), dict(order=5), dict(eps=-1.0),
                    dict(eps=float("nan")), dict(stride=-4), dict(x=p + 4), dict(dgamma=p + 2), dict(dbeta=p), dict(dshift=p), dict(dscale=p)):
         assert norm_call(**change) == L.EINVAL, change
-    for change in (dict(d=60), dict(d=6152), dict(d=0), dict(rows=1 << 60), dict(B=1 << 40, rows=1 << 40)):
+    for change in (dict(d=60), dict(d=6152), dict(d=0), dict(rows=1 << 60), dict(B=1 << 40, rows=1 << 40), dict(B=70000, rows=1, shift=p, stride=64),
+                   dict(B=60000, rows=1, d=1024, shift=p, stride=1024)):
         assert norm_call(**change) == L.EUNSUPPORTED, change
     assert norm_call() == L.EINVAL and "workspace" in L.last_error()  # too small
     assert norm_call(ws=p + 8, size=1 << 20) == L.EINVAL
