@@ -1,9 +1,9 @@
-"""Build libaeris_hip.so (gfx950) in-tree with hipcc.
+"""Build libaeris_hip.so (gfx950) in-tree with hipcc, and aeris_grad.so, the autograd nodes that call it, with g++ against torch.
 
     python aeris-gb_amd/build.py [--force]
 
-Cross-compiles without a GPU.  The shared library lands next to the sources
-(``csrc/libaeris_hip.so``) so that it travels with the tree.
+Cross-compiles without a GPU.  The shared libraries land next to the sources
+(``csrc/libaeris_hip.so``, ``csrc/aeris_grad.so``) so that they travel with the tree.
 """
 from __future__ import annotations
 
@@ -18,6 +18,7 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(CSRC, "libaeris_hip.so")
+GRAD_SOURCE, GRAD_LIB = os.path.join(CSRC, "grad_functions.cpp"), os.path.join(CSRC, "aeris_grad.so")
 SOURCES = ["api.hip", "gemm.hip", "gemm_persistent.hip", "gemm_norm.hip", "window_attention.hip", "qkv_window_attention.hip", "window_attention_stream.hip", "norm_modulate.hip", "small_ops.hip", "output_stage.hip", "input_stage.hip",
            "qk_norm_rope.hip", "cross_attention.hip", "norm_grad.hip", "gemm_grad.hip"]
 HEADERS = ["common.h", "kernels.h", "gemm_common.h", "attention_sweep.h", os.path.join("..", "..", "include", "aeris_hip.h")]
@@ -34,6 +35,19 @@ def _hipcc():
         if c and (os.path.isabs(c) and os.path.exists(c) or not os.path.isabs(c)):
             return c
     raise RuntimeError("hipcc not found")
+
+
+def _grad_command():
+    """g++ of the autograd extension: host code alone, linked to torch and to the library beside it."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), os.path.join(rocm, "include"), sysconfig.get_paths()["include"]]
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *[a for i in includes for a in ("-isystem", i)], GRAD_SOURCE, "-o", GRAD_LIB, "-L" + os.path.join(root, "lib"), "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",
+            "-ltorch_python", "-L" + CSRC, "-l:libaeris_hip.so", "-Wl,-rpath,$ORIGIN"]
 
 
 def _stale(target, deps):
@@ -99,6 +113,8 @@ def build(force: bool = False, verbose: bool = True) -> str:
         list(ex.map(compile_one, jobs))
     if force or jobs or _stale(LIB, objs):
         run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs])
+    if force or _stale(GRAD_LIB, [GRAD_SOURCE, hdrs[-1]]):
+        run(_grad_command())
     return LIB
 
 

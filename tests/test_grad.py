@@ -318,13 +318,13 @@ def test_linear_many_tokens_few_weights(pkg, cuda, M):
 # layouts and with every epilogue.
 @pytest.mark.gpu
 @pytest.mark.parametrize("M,N,K,act,y_dtype,residual", [(8200, 2056, 1088, None, BF16, None), (4113, 4104, 1024, "gelu", BF16, BF16), (16500, 1032, 512, "silu", F32, F32),
-                                                        (33000, 520, 1536, None, F32, F32), (2304, 6152, 2048, "gelu", F32, None)])
+                                                        (33000, 520, 1536, None, F32, F32), (2304, 6152, 2048, "gelu", F32, None), (9000, 6152, 3136, None, BF16, None)])
 def test_linear_large_products(pkg, cuda, M, N, K, act, y_dtype, residual):
     check_linear(pkg, cuda, torch.Generator().manual_seed(M), M, N, K, act, True, residual, y_dtype, at=cuda)
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("M,d,H", [(8200, 512, 2056), (16400, 264, 1088), (4100, 1544, 3080)])
+@pytest.mark.parametrize("M,d,H", [(8200, 512, 2056), (16400, 264, 1088), (4100, 1544, 3080), (20000, 1024, 2056)])
 def test_feed_forward_large_products(pkg, cuda, M, d, H):
     check_feed_forward(pkg, cuda, torch.Generator().manual_seed(M), M, d, H, at=cuda)
 
@@ -751,6 +751,13 @@ def test_cpu_tensors_are_refused(pkg):
     for bad in (lambda: G.norm_modulate(x, torch.ones(64, dtype=BF16)), lambda: G.linear(x, w), lambda: G.feed_forward(x, w, w)):
         with pytest.raises(RuntimeError, match="GPU"):
             bad()
+
+
+def test_a_missing_extension_is_an_error(pkg, monkeypatch, tmp_path):
+    monkeypatch.setattr(pkg.grad, "_loaded", None)
+    monkeypatch.setattr(pkg.grad, "EXTENSION_PATH", str(tmp_path / "aeris_grad.so"))
+    with pytest.raises(RuntimeError, match="missing"):
+        pkg.grad.feed_forward(*[torch.zeros(8, 8, dtype=BF16)] * 3)
 
 
 def test_packed_records_match_the_header(pkg):
