@@ -1009,7 +1009,10 @@ GradPlan plan_tiles(int t, int64_t M, int64_t N, int64_t K, int epi, bool low) {
   const int64_t left = tiles % at_once;
   int64_t most = epi == EPI_STORE && left ? at_once / left : 1;
   if (most > K / 256) most = K / 256;
-  for (int64_t parts = 1; parts == 1 || parts <= most; parts += parts < 8 ? 1 : parts / 4) {
+  if (most < 1) most = 1;
+  for (int64_t next = 1, parts = 1; parts <= most; parts = next) {  // 1 .. 8, steps of a quarter, the most
+    next = parts + (parts < 8 ? 1 : parts / 4);
+    if (parts < most && next > most) next = most;
     const int64_t kp = (K + parts - 1) / parts + BK - 1, k_part = kp / BK * BK;
     const double share = (double)left * parts / at_once;  // of the last round's places
     const double last_k = lone_k + (round_k - lone_k) * share;

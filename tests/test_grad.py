@@ -727,6 +727,40 @@ def test_a_step_of_training(pkg, cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M", [5, 700])
+def test_explicit_passes_have_the_same_bits(pkg, cuda, M):
+    """``ops``' forward and backward calls, for callers without autograd, against the nodes of ``grad``."""
+    ops, G, g = pkg.ops, pkg.grad, torch.Generator().manual_seed(M)
+    x, dy = (torch.randn(1, M, 128, generator=g).to(BF16).to(cuda) for _ in range(2))
+    gamma, beta = (torch.randn(128, generator=g).to(cuda) for _ in range(2))
+    mod = torch.randn(1, 256, generator=g).to(cuda)
+    w, b = torch.randn(128, 128, generator=g).to(BF16).to(cuda), torch.randn(128, generator=g).to(BF16).to(cuda)
+    w1, w2 = torch.randn(512, 128, generator=g).to(BF16).to(cuda), torch.randn(128, 256, generator=g).to(BF16).to(cuda)
+    res = torch.randn(1, M, 128, generator=g).to(cuda)
+
+    def through(f, inputs, dy):
+        leaves = [t.detach().clone().requires_grad_() for t in inputs]
+        y = f(*leaves)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    def same(got, want):
+        assert len(got) == len(want) and all(torch.equal(s, t) for s, t in zip(got, want))
+    norm = (x, gamma, beta, mod[:, :128].contiguous(), mod[:, 128:].contiguous())
+    for kw in (dict(), dict(kind="rmsnorm", order="mod_then_norm", eps=1e-6)):
+        same([ops.norm_modulate(*norm, **kw), *ops.norm_modulate_backward(dy, *norm, **kw)], through(lambda *a: G.norm_modulate(*a, **kw), norm, dy))
+    y, z = ops.linear_train(x, w, b, act="silu")
+    same([y, *ops.linear_backward(dy, x, w, z, act="silu", wanted=(True, True, True, False))[:3]], through(lambda *a: G.linear(*a, act="silu"), (x, w, b), dy))
+    y, z = ops.linear_train(x, w, b, residual=res, out_dtype=F32)
+    assert z is None
+    same([y, *ops.linear_backward(dy.float(), x, w, wanted=(True, True, True, False))[:3], dy.float()],
+         through(lambda x, w, b, r: G.linear(x, w, b, residual=r, out_dtype=F32), (x, w, b, res), dy.float()))
+    assert torch.equal(ops.linear_backward(dy.float(), x, w)[3], dy) and ops.linear_backward(dy, x, w)[3] is dy
+    assert ops.linear_train(x, w, act="gelu", keep=False)[1] is None and ops.feed_forward_train(x, w1, w2, keep=False)[1] is None
+    y, gate_up, h = ops.feed_forward_train(x, w1, w2)
+    same([y, *ops.feed_forward_backward(dy, x, w1, w2, gate_up, h)], through(G.feed_forward, (x, w1, w2), dy))
+
+
+@pytest.mark.gpu
 def test_refusals(pkg, cuda):
     G = pkg.grad
     x = torch.zeros(1, 4, 64, dtype=BF16, device=cuda)
@@ -739,6 +773,9 @@ def test_refusals(pkg, cuda):
                 lambda: G.linear(x.transpose(1, 2), torch.zeros(16, 4, dtype=BF16, device=cuda)), lambda: G.linear(x, w, act="gelu", residual=torch.zeros(1, 4, 16, dtype=torch.float16, device=cuda)),
                 lambda: G.feed_forward(x, w, w), lambda: G.feed_forward(x, torch.zeros(24, 64, dtype=BF16, device=cuda), torch.zeros(64, 12, dtype=BF16, device=cuda)),
                 lambda: G.feed_forward(x.float(), torch.zeros(32, 64, dtype=BF16, device=cuda), torch.zeros(64, 16, dtype=BF16, device=cuda)),
+                lambda: pkg.ops.linear_train(x, w, act="swiglu"), lambda: pkg.ops.linear_train(x, w.float()), lambda: pkg.ops.linear_train(x, w, residual=x),
+                lambda: pkg.ops.feed_forward_train(x, w, w), lambda: pkg.ops.norm_modulate_backward(x[:, :2], x, gamma), lambda: pkg.ops.norm_modulate_backward(x, x, gamma[:32]),
+                lambda: pkg.ops.norm_modulate_backward(x.expand(2, 4, 64).contiguous(), x.expand(2, 4, 64).contiguous(), gamma, None, torch.zeros(1, 64, device=cuda).expand(2, 64)),
                 lambda: pkg.ops.norm_modulate_backward(x, x, gamma, None, torch.zeros(1, 64, device=cuda).expand(4, 64)[:1].expand(1, 64), torch.zeros(2, 64, device=cuda)),
                 lambda: pkg.ops.linear_backward(torch.zeros(1, 4, 16, dtype=BF16, device=cuda), x, w, act="gelu")):
         with pytest.raises(RuntimeError):
