@@ -53,7 +53,6 @@ hipError_t norm_modulate_launch(const void* x, int x_dtype, void* y, int y_dtype
                                 int64_t rows_per_batch, int d, int kind, int order, float eps, hipStream_t stream);
 
 // gradients of the norm and its modulation (norm_grad.hip)
-int64_t norm_grad_blocks(const aeris_norm_modulate_grad& a);
 int64_t norm_grad_workspace_bytes(const aeris_norm_modulate_grad& a);
 hipError_t norm_grad_launch(const aeris_norm_modulate_grad& a, void* workspace, hipStream_t stream);
 

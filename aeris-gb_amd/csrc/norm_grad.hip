@@ -7,10 +7,11 @@
 // Nothing is kept from the forward pass: mean and r are recomputed from the row, which is read anyway.
 //
 // Bound by HBM: x and dy are read once, dx is written once.  A wave owns a row (rows of up to 256 or 128 elements lie beside each
-// other in it, rows beyond 2048 belong to the four waves of a workgroup), holds it in registers and asks for its next one before it
+// other in it, rows beyond 2048 and some of bf16 belong to two or four waves of a workgroup), holds it in registers and asks for its next one before it
 // sums; the sums over the tokens stay in registers while a workgroup walks down its share of a member's rows.  At the end of it the
 // workgroup writes one partial sum per column, and a second kernel adds those up in a fixed order: equal calls have equal results.
 // All sums are fp32: within a lane over some hundred rows, then over lanes, waves and workgroups.
+// f32 x [1036800, 1024], bf16 dy: 2155 us, 4.9 TB/s; an element-wise sum of the same streams takes 2035 us here.
 #include "common.h"
 #include "kernels.h"
 
@@ -40,7 +41,7 @@ __device__ __forceinline__ float param_at(const void* p, int f32, int c) {
   return f32 ? reinterpret_cast<const float*>(p)[c] : bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(p)[c]);
 }
 
-// NV: groups of 8 columns a lane; SUB: rows beside each other in a wave; WPR: waves to a row (1, 2 or 4)
+// NV: groups of 8 columns a lane; SUB: rows beside each other in a wave; WPR: waves to a row (1, 2 or 4).
 // Workgroups that a CU holds, which the registers are budgeted for (sums, the row and the next one)
 template <int NV, bool PRE>
 constexpr int resident() { return PRE ? (NV == 1 ? 4 : NV == 2 ? 2 : 1) : (NV == 1 ? 5 : NV == 2 ? 3 : 2); }
@@ -480,7 +481,7 @@ hipError_t launch_wide(const NormGradParams& p, bool yf, int64_t blocks, hipStre
 
 }  // namespace
 
-int64_t norm_grad_blocks(const aeris_norm_modulate_grad& a) { return segments_of(a) * blocks_of(a); }
+static int64_t norm_grad_blocks(const aeris_norm_modulate_grad& a) { return segments_of(a) * blocks_of(a); }
 
 // many members: their sums side by side, and another kernel for what adds up over them
 static bool members_apart(const aeris_norm_modulate_grad& a) { return segments_of(a) > 8; }
