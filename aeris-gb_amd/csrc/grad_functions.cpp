@@ -189,6 +189,8 @@ Tensor norm_modulate(const Tensor& x, const Tensor& gamma, const Optional& beta_
     TORCH_CHECK(shift.sizes() == scale.sizes() && (shift.size(0) == 1 || shift.stride(0) == scale.stride(0)), "shift and scale must be of one shape and layout, got ", shift.sizes(),
                 " and ", scale.sizes());
   if (!wants_grad({&x, &gamma, &beta, &shift, &scale})) return norm_forward(x, gamma, beta, shift, scale, {kind, order, eps}, out_f32 ? F32 : BF16);
+  const Tensor& mod = shift.defined() ? shift : scale;
+  TORCH_CHECK(!mod.defined() || mod.size(0) == 1 || (B <= 65535 && B * (d / 8) < 1 << 22), "no gradients of ", B, " members of ", d, " channels with modulation rows of their own");
   refuse_other_streams({&x, &gamma, &beta, &shift, &scale});
   return NormModulate::apply(x, gamma, beta_, shift_, scale_, kind, order, eps, (int64_t)out_f32);
 }
@@ -196,6 +198,13 @@ Tensor norm_modulate(const Tensor& x, const Tensor& gamma, const Optional& beta_
 // ---- projection
 
 struct Sizes { int64_t M, N, K; };
+
+// what aeris_linear_bwd and aeris_feed_forward_bwd take, so that a call whose gradients would be refused is refused itself
+void check_gradients_sizes(const Sizes& s) {
+  constexpr int64_t WIDE = 1 << 20, PRODUCT = 1 << 30, TILES = 1 << 24;
+  TORCH_CHECK(s.M < int64_t(1) << 31 && s.N <= WIDE && s.K <= WIDE && s.N * s.K < PRODUCT && (s.M + 63) / 64 * ((s.N + 31) / 32) < TILES && (s.M + 63) / 64 * ((s.K + 63) / 64) < TILES,
+              "no gradients of ", s.M, " rows of ", s.K, " -> ", s.N, " (widths up to 2^20, their product below 2^30, fewer than 2^24 tiles of 64 x 32)");
+}
 
 Tensor linear_forward(const Tensor& a, const Tensor& w, const Tensor& bias, const Tensor& residual, int64_t act, at::ScalarType out, const Sizes& s, Tensor* z) {
   Tensor y = at::empty(rows_of(a, s.N), a.options().dtype(out));
@@ -293,6 +302,7 @@ Tensor linear(const Tensor& a, const Tensor& w, const Optional& bias_, int64_t a
     TORCH_CHECK(known(residual) && residual.numel() == M * N && residual.dim() >= 1 && residual.size(-1) == N && residual.is_contiguous(),
                 "residual must be contiguous bf16 or f32 [", M, ", ", N, "], got ", residual.scalar_type(), " ", residual.sizes());
   if (!wants_grad({&a, &w, &bias, &residual})) return linear_forward(a, w, bias, residual, act, out_f32 ? F32 : BF16, {M, N, K}, nullptr);
+  check_gradients_sizes({M, N, K});
   refuse_other_streams({&a, &w, &bias, &residual});
   return Linear::apply(a, w, bias_, residual_, act, (int64_t)out_f32, M);
 }

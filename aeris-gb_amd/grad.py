@@ -1,7 +1,7 @@
 """The block's operators outside its attention, differentiable: what a training step calls in place of ``ops.norm_modulate``,
 ``ops.gemm`` and the gated MLP.  (The reference trains these modules by autograd over ATen operations, model.py:121-159,311-325,395-403.)
 
-``norm_modulate``, ``linear`` and ``feed_forward`` return tensors that autograd differentiates once, with the gradients of
+``norm_modulate``, ``linear`` and ``feed_forward`` return tensors that autograd differentiates once, in reverse mode, with the gradients of
 ``ops.norm_modulate_backward``, ``ops.linear_backward`` and ``ops.feed_forward_backward``; their results are those of the calls without
 gradients, and gradients have their tensors' types.  Only the gradients that are asked for are computed, and nothing is kept where
 none is.  The nodes of the autograd graph are C++ (csrc/grad_functions.cpp, built to csrc/aeris_grad.so): a small block's pass is bound by the host.

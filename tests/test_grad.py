@@ -782,6 +782,129 @@ def test_refusals(pkg, cuda):
             bad()
 
 
+@pytest.mark.gpu
+def test_calls_whose_gradients_would_be_refused_are_refused_themselves(pkg, cuda):
+    G, ops = pkg.grad, pkg.ops
+    a, w = torch.zeros(1, 32768, dtype=BF16, device=cuda), torch.zeros(32768, 32768, dtype=BF16, device=cuda)
+    assert G.linear(a, w).shape == (1, 32768)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        G.linear(a.requires_grad_(), w)
+    x, gamma, m = torch.zeros(65536, 1, 8, dtype=BF16, device=cuda), torch.ones(8, device=cuda), torch.zeros(65536, 16, device=cuda)
+    assert G.norm_modulate(x, gamma, None, m[:, :8], m[:, 8:]).shape == x.shape
+    with pytest.raises(RuntimeError, match="no gradients"):
+        G.norm_modulate(x, gamma, None, m[:, :8].requires_grad_(), m[:, 8:])
+    y = G.norm_modulate(x.requires_grad_(), gamma, None, m[:1, :8], m[:1, 8:])  # one row for all of them
+    assert torch.autograd.grad(y, x, torch.ones_like(y))[0].shape == x.shape
+
+
+# More than 2^32 bytes of every operand in turn, a few rows of gradients at the start, in the middle and at the end: the weights' gradients are those
+# rows' alone, and the rest of the tokens' gradients is 0.
+FAR = 1_060_003
+
+
+def far_rows(M):
+    return torch.cat([torch.arange(0, 70), torch.arange(M // 2 - 9, M // 2 + 60), torch.arange(M - 300, M)])
+
+
+def noise(cuda, seed, M, N, dtype=BF16):
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    t = torch.empty(M, N, dtype=dtype, device=cuda)
+    for r in range(0, M, 1 << 17):
+        part = t[r:r + (1 << 17)]
+        part.copy_(torch.randn(part.shape, generator=g, device=cuda))
+    return t
+
+
+def only(rows, values, M):
+    dy = torch.zeros(M, values.shape[1], dtype=values.dtype, device=values.device)
+    dy[rows] = values
+    return dy
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K,act,y_dtype", [(2048, 64, "gelu", BF16), (64, 2048, None, BF16), (2048, 64, None, F32), (64, 2048, "silu", F32)])
+def test_linear_offsets_past_32_bits(pkg, cuda, N, K, act, y_dtype):
+    M = FAR
+    rows = far_rows(M).to(cuda)
+    a, w = noise(cuda, 1, M, K), (noise(cuda, 2, N, K) * K ** -0.5).to(BF16)
+    res = noise(cuda, 3, M, N, y_dtype)
+    dy = only(rows, noise(cuda, 4, len(rows), N, y_dtype), M)
+    on = [a.requires_grad_(), w.requires_grad_(), res.requires_grad_()]
+    y = pkg.grad.linear(a, w, act=act, residual=res, out_dtype=y_dtype)
+    da, dw, dres = torch.autograd.grad(y, on, dy)
+    near = [t.detach()[rows].requires_grad_() if t is not w else t for t in on]
+    y_near = pkg.grad.linear(near[0], w, act=act, residual=near[2], out_dtype=y_dtype)
+    da_near, dw_near, dres_near = torch.autograd.grad(y_near, near, dy[rows])
+    # (the same numbers summed in another order, then rounded: steps of fp32 sums of K or N numbers of size 1, and one of the result's type)
+    a_, w_, d_ = a.detach()[rows].double().abs(), w.detach().double().abs(), dy[rows].double().abs()
+    ez = 2 * (K + 3) * E * (a_ @ w_.T)
+    z = a_ @ w_.T if act is None else (a.detach()[rows].double() @ w.detach().double().T).abs()
+    edz = d_ * (LIP2 * (ez + 2 * KEPT * z) + 2 * FN * z.clamp_min(1)) if act else 0 * d_
+    Z = d_ * 1.2  # |act'| <= 1.13
+    edz = edz + (2 * U * (Z + edz) if act or y_dtype is F32 else 0)
+    top = y_near.detach().double().abs()
+    close(y.detach()[rows], y_near.detach().double(), (LIP if act else 1) * ez + 2 * FN * z.clamp_min(1) * (act is not None) + 2 * half_step(y_dtype) * (top + ez) + 4 * E * (z + top), "y")
+    close(da[rows], da_near.double(), edz @ w_ + 2 * (N + 2) * E * (Z @ w_) + 2 * U * da_near.double().abs(), "da")
+    close(dw, dw_near.double(), edz.T @ a_ + 2 * (len(rows) + 70) * E * (Z.T @ a_) + 2 * U * dw_near.double().abs(), "dw")
+    assert torch.equal(dres, dy)
+    da[rows] = 0
+    assert not da.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,H", [(2048, 64), (64, 2048)])
+def test_feed_forward_offsets_past_32_bits(pkg, cuda, d, H):
+    M = FAR
+    rows = far_rows(M).to(cuda)
+    x, w1, w2 = noise(cuda, 1, M, d), (noise(cuda, 2, 2 * H, d) * d ** -0.5).to(BF16), (noise(cuda, 3, d, H) * H ** -0.5).to(BF16)
+    dy = only(rows, noise(cuda, 4, len(rows), d), M)
+    y = pkg.grad.feed_forward(x.requires_grad_(), w1.requires_grad_(), w2.requires_grad_())
+    dx, dw1, dw2 = torch.autograd.grad(y, [x, w1, w2], dy)
+    near = x.detach()[rows].requires_grad_()
+    y_near = pkg.grad.feed_forward(near, w1, w2)
+    want = torch.autograd.grad(y_near, [near, w1, w2], dy[rows])
+    # (two roundings of h and of dgate and dup that may differ by a step each: 2^-8 of the sums of the sizes)
+    x_, a1, a2, d_ = near.detach().double().abs(), w1.detach().double().abs(), w2.detach().double().abs(), dy[rows].double().abs()
+    gate, up = (near.detach().double() @ w1.detach().double().T).chunk(2, dim=-1)
+    s = torch.sigmoid(gate)
+    h, silu, ds = (gate * s * up).abs(), (gate * s).abs(), (s * (1 + gate * (1 - s))).abs()
+    dh = (dy[rows].double() @ w2.detach().double()).abs()
+    D1 = torch.cat([dh * up.abs() * ds, dh * silu], 1)
+    small = 2 * (d + 2) * E * (x_ @ a1.T)
+    eg, eu = small[:, :H] + 2 * KEPT * gate.abs(), small[:, H:] + 2 * KEPT * up.abs()
+    fn = 2 * FN * gate.abs().clamp_min(1)
+    eh = (LIP * eg + fn) * up.abs() + silu * eu + 2 * U * h * (1 + U)
+    edh = 2 * (d + 2) * E * (d_ @ a2)
+    E1 = torch.cat([edh * up.abs() * ds + dh * eu * (ds + fn) + dh * up.abs() * (LIP2 * eg + fn), edh * silu + dh * (LIP * eg + fn)], 1) + 2 * U * D1 * (1 + U)
+    close(y.detach()[rows], y_near.detach().double(), eh @ a2.T + 2 * (H + 2) * E * (h @ a2.T) + 2 * U * y_near.detach().double().abs(), "y")
+    close(dx[rows], want[0].double(), E1 @ a1 + 2 * (2 * H + 2) * E * (D1 @ a1) + 2 * U * want[0].double().abs(), "dx")
+    close(dw1, want[1].double(), E1.T @ x_ + 2 * (len(rows) + 70) * E * (D1.T @ x_) + 2 * U * want[1].double().abs(), "dw1")
+    close(dw2, want[2].double(), d_.T @ eh + 2 * (len(rows) + 70) * E * (d_.T @ h) + 2 * U * want[2].double().abs(), "dw2")
+    dx[rows] = 0
+    assert not dx.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["norm_then_mod", "mod_then_norm"])
+@pytest.mark.parametrize("x_dtype", [BF16, F32])
+def test_norm_offsets_past_32_bits(pkg, cuda, x_dtype, order):
+    M, d = FAR, 2048
+    rows = far_rows(M).to(cuda)
+    x, gamma, m = noise(cuda, 1, M, d, x_dtype)[None], (1 + 0.2 * torch.randn(d)).to(cuda), (0.3 * torch.randn(1, 2 * d)).to(cuda)
+    dy = only(rows, noise(cuda, 4, len(rows), d), M)[None]
+    on = [x.requires_grad_(), gamma.requires_grad_(), m[:, :d].detach().requires_grad_(), m[:, d:].detach().requires_grad_()]
+    y = pkg.grad.norm_modulate(on[0], gamma, None, on[2], on[3], order=order)
+    got = torch.autograd.grad(y, on, dy)
+    near = [x.detach()[:, rows].requires_grad_(), *on[1:]]
+    p64 = [t.detach().double().cpu().requires_grad_() for t in near]
+    want = torch.autograd.grad(norm_definition(p64[0], p64[1], None, p64[2], p64[3], "layernorm", order, 1e-5), p64, dy[:, rows].double().cpu())
+    bounds = norm_bounds([p64[0], p64[1], None, p64[2], p64[3]], dy[:, rows].double().cpu(), "layernorm", order, 1e-5, dict(x=x_dtype, gamma=F32))
+    for name, g, v in zip(("x", "gamma", "shift", "scale"), (got[0][:, rows], *got[1:]), want):
+        close(g, v.to(cuda), bounds[name].to(cuda), name)
+    got[0][:, rows] = 0
+    assert not got[0].any()
+
+
 def test_cpu_tensors_are_refused(pkg):
     G = pkg.grad
     x, w = torch.zeros(1, 4, 64, dtype=BF16), torch.zeros(16, 64, dtype=BF16)
