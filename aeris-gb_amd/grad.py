@@ -10,7 +10,8 @@ Streams and graphs: calls follow the current stream and hold no scratch memory b
 be captured into a HIP graph.  torch's own rule for that holds here too: what the captured graph differentiates must have no autograd nodes of
 another stream - an eager graph of the same leaves that is still alive, or an input computed outside the capture - or torch would tie that stream to
 the capture and the process would end.  Such a call is refused with a RuntimeError; release the eager result, or do the eager passes on the stream
-that captures.
+that captures.  (A backward pass alone, of a forward pass outside the capture, is torch's to start and cannot be refused here: capture both.)
+``ops.profile_begin`` records the calls of ``ops``, not these.
 """
 from __future__ import annotations
 
