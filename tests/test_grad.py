@@ -761,6 +761,27 @@ def test_explicit_passes_have_the_same_bits(pkg, cuda, M):
 
 
 @pytest.mark.gpu
+def test_one_tensor_as_several_inputs(pkg, cuda):
+    """Its gradient is the sum of theirs, and the result's gradient stays what it was."""
+    G, g = pkg.grad, torch.Generator().manual_seed(3)
+    x, dy = (torch.randn(1, 90, 64, generator=g).to(BF16).to(cuda) for _ in range(2))
+    w, gamma, m = torch.randn(64, 64, generator=g).to(BF16).to(cuda), torch.randn(64, generator=g).to(cuda), torch.randn(1, 64, generator=g).to(cuda)
+
+    def both(f, *inputs):
+        """f of the tensor for both inputs, against f of two copies of it."""
+        t, *rest = inputs
+        one, kept = t.clone().requires_grad_(), dy.clone()
+        got = torch.autograd.grad(f(one, one, *rest), one, kept)[0]
+        two = [t.clone().requires_grad_() for _ in range(2)]
+        a, b = torch.autograd.grad(f(*two, *rest), two, kept)
+        assert torch.equal(got, a + b) and torch.equal(kept, dy)
+    both(lambda a, r: G.linear(a, w, residual=r), x)
+    both(lambda a, r: G.linear(a, w, act="gelu", residual=r), x)
+    both(lambda p, q: G.norm_modulate(x, p, q), gamma)
+    both(lambda p, q: G.norm_modulate(x, gamma, None, p, q, order="mod_then_norm"), m)
+
+
+@pytest.mark.gpu
 def test_refusals(pkg, cuda):
     G = pkg.grad
     x = torch.zeros(1, 4, 64, dtype=BF16, device=cuda)
