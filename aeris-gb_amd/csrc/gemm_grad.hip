@@ -848,10 +848,10 @@ __global__ void __launch_bounds__(256) grad_finish_kernel(GradGemm p, GradGemm q
   }
 }
 
-// ---- dz = dy act'(z) (ACT_NONE: dy) rounded to bf16, and the sums of the unrounded dz over the tokens.  Bound by HBM: a workgroup takes 512
-// columns of 16 rows at a time, in turns with the others; a wave asks for its four rows (8 columns a lane) before it uses the first.
-// f32 dy [1036800, 1024] without activation: 1257 us, 5.1 TB/s (sums alone 750, 5.7; a cast to bf16 alone 1086); rows one by one and a contiguous
-// share of them a workgroup: 1276 and 57 more for the sums.
+// ---- dz = dy act'(z) (ACT_NONE: dy) rounded to bf16, and the sums of the unrounded dz over the tokens.  Bound by HBM: a wave takes 512 columns of
+// one row at a time (two without activation, which it asks for before it uses the first), workgroups in turns, three a CU.  More of either in flight
+// is slower: f32 dy [1036800, 1024] without activation 1145 us, 5.6 TB/s (four rows, five workgroups 1253; a cast to bf16 alone 1086), bf16 [8192, 6144]
+// with GELU 65, 5.4 TB/s (76), [100000, 2048] with SiLU 260 (297).
 struct ActGrad {
   const void* dy;
   const uint16_t* z;
@@ -864,7 +864,7 @@ struct ActGrad {
 
 template <bool DY_F32, bool ACT, bool STREAM>
 __global__ void __launch_bounds__(256) act_grad_kernel(ActGrad p) {
-  constexpr int ROWS = 4;
+  constexpr int ROWS = ACT ? 1 : 2;
   __shared__ f32x4 lds[4][128];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int col = (blockIdx.y * 64 + lane) * 8;
@@ -947,8 +947,9 @@ __global__ void __launch_bounds__(1024) bias_sum_kernel(const float* partial, ui
   }
 }
 
+// (at least two turns of a workgroup's four waves, one without activation: 300 rows of 1024 with GELU 5.6 us, with four of them 6.8)
 int act_grad_parts(int64_t M, int N) {
-  const int64_t n = 1280 / ((N + 511) / 512), most = (M + 15) / 16;
+  const int64_t n = 768 / ((N + 511) / 512), most = (M + 7) / 8;
   return n < 1 ? 1 : n < most ? (int)n : (int)most;
 }
 
