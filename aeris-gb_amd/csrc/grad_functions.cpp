@@ -47,6 +47,8 @@ bool capturing() {
   return hipStreamIsCapturing(c10::hip::getCurrentHIPStream().stream(), &status) == hipSuccess && status != hipStreamCaptureStatusNone;
 }
 bool wants_grad(std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), "these operators are differentiable in reverse mode only");
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : inputs)
     if (t->defined() && t->requires_grad()) return true;

@@ -702,6 +702,19 @@ def test_gradients_of_gradients_are_refused(pkg, cuda):
 
 
 @pytest.mark.gpu
+def test_forward_mode_is_refused(pkg, cuda):
+    from torch.autograd import forward_ad
+    G, x, w, gamma = pkg.grad, torch.ones(1, 3, 64, dtype=BF16, device=cuda), torch.ones(64, 64, dtype=BF16, device=cuda), torch.ones(64, device=cuda)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: G.norm_modulate(dual, gamma), lambda: G.linear(dual, w), lambda: G.linear(x, w, residual=dual), lambda: G.feed_forward(dual, torch.cat([w, w]), w)):
+            with pytest.raises(RuntimeError, match="reverse mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="reverse mode"):
+                call()
+
+
+@pytest.mark.gpu
 def test_a_parameter_changed_in_place_is_noticed(pkg, cuda):
     leaf, dy = make(pkg, cuda, 17)
     y = branches(pkg.grad, leaf)
