@@ -8,6 +8,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -85,17 +86,16 @@ Tensor incoming(const Tensor& dy) {
   Tensor g = dy.contiguous();
   return reinterpret_cast<uintptr_t>(g.data_ptr()) & 15 ? g.clone() : g;
 }
-// Gradients that themselves have none: asked for a graph of the backward pass, they refuse to be differentiated
-variable_list outgoing(variable_list grads) {
+// Gradients that themselves have none: where a graph of the backward pass is asked for, they refuse to be differentiated.  Behind the node that
+// refuses lie the operator's inputs and the result's gradient dy: autograd, asked for the gradients of a few tensors, runs only what leads to
+// those, and would leave the term out without a word.
+variable_list outgoing(variable_list grads, const Tensor& dy) {
   if (!at::GradMode::is_enabled()) return grads;
-  variable_list some;
+  torch::autograd::edge_list behind = torch::autograd::get_current_node()->next_edges();
+  behind.push_back(torch::autograd::impl::gradient_edge(dy));
+  const auto refusal = std::make_shared<torch::autograd::Error>("these operators are differentiable once", std::move(behind));
   for (const Tensor& t : grads)
-    if (t.defined()) some.push_back(t);
-  auto refusal = std::make_shared<torch::autograd::DelayedError>("these operators are differentiable once", (int64_t)some.size());
-  variable_list marked = (*refusal)(std::move(some));
-  size_t n = 0;
-  for (Tensor& t : grads)
-    if (t.defined()) t = marked[n++];
+    if (t.defined()) torch::autograd::set_history(t, refusal);
   return grads;
 }
 Tensor scratch(int64_t bytes, const Tensor& like) { return bytes ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor(); }
@@ -168,7 +168,7 @@ struct NormModulate : torch::autograd::Function<NormModulate> {
       const Tensor ws = scratch(need, x);
       check(aeris_norm_modulate_bwd(&a, ptr(ws), need, stream()));
     }
-    return outgoing({grads[0], grads[1], grads[2], grads[3], grads[4], Tensor(), Tensor(), Tensor(), Tensor()});
+    return outgoing({grads[0], grads[1], grads[2], grads[3], grads[4], Tensor(), Tensor(), Tensor(), Tensor()}, given[0]);
   }
 };
 
@@ -260,7 +260,8 @@ struct Linear : torch::autograd::Function<Linear> {
                need_res = has_res && ctx->needs_input_grad(has_bias ? 3 : 2);
     const auto res_dtype = need_res && ctx->saved_data["residual_f32"].toBool() ? F32 : BF16;
     // dy rounded to bf16 is what the products read of an f32 dy, and what a bf16 residual gets
-    const bool round_res = need_res && res_dtype == BF16 && dy.scalar_type() == F32 && act == AERIS_ACT_NONE && M;
+    // (not where a graph of the backward pass is asked for: torch's own cast has one)
+    const bool round_res = need_res && res_dtype == BF16 && dy.scalar_type() == F32 && act == AERIS_ACT_NONE && M && !at::GradMode::is_enabled();
     Tensor da, dw, dbias, dz, dres;
     if (need_a) da = at::empty_like(a, at::MemoryFormat::Contiguous);
     if (need_w) dw = M ? at::empty_like(w) : at::zeros_like(w);
@@ -286,7 +287,9 @@ struct Linear : torch::autograd::Function<Linear> {
       check(aeris_linear_bwd(&c, ptr(ws), need, stream()));
     }
     if (need_res) dres = (round_res ? dz : dy.to(res_dtype)).view(ctx->saved_data["residual_shape"].toIntVector());
-    return outgoing({da, dw, dbias, dres, Tensor(), Tensor(), Tensor()});
+    variable_list grads = outgoing({da, dw, dbias}, given[0]);
+    grads.insert(grads.end(), {dres, Tensor(), Tensor(), Tensor()});
+    return grads;
   }
 };
 
@@ -366,7 +369,7 @@ struct FeedForward : torch::autograd::Function<FeedForward> {
       const Tensor ws = scratch(need, x);
       check(aeris_feed_forward_bwd(&c, ptr(ws), need, stream()));
     }
-    return outgoing({grads[0], grads[1], grads[2]});
+    return outgoing({grads[0], grads[1], grads[2]}, given[0]);
   }
 };
 

@@ -1,0 +1,71 @@
+"""Calls of ``grad`` beyond a single pass: gradients of gradients."""
+import pytest
+import torch
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def normal(g, *shape, dtype=F32, std=1.0):
+    return (std * torch.randn(*shape, generator=g)).to(dtype)
+
+
+def operators(pkg, cuda, seed=0):
+    """name -> (the call, its inputs by name), each on leaves of its own."""
+    G, g = pkg.grad, torch.Generator().manual_seed(seed)
+
+    def leaves(**tensors):
+        return {n: t.to(cuda).requires_grad_() for n, t in tensors.items()}
+    M, d, H = 70, 64, 96
+    norm = leaves(x=normal(g, 2, 35, d), gamma=normal(g, d), beta=normal(g, d), shift=normal(g, 2, d, std=0.3), scale=normal(g, 2, d, std=0.3))
+    linear = leaves(a=normal(g, M, d, dtype=BF16), w=normal(g, H, d, dtype=BF16, std=d ** -0.5), bias=normal(g, H, dtype=BF16))
+    mlp = leaves(x=normal(g, M, d, dtype=BF16), w1=normal(g, 2 * H, d, dtype=BF16, std=d ** -0.5), w2=normal(g, d, H, dtype=BF16, std=H ** -0.5))
+    return {
+        "norm": (lambda: G.norm_modulate(*norm.values()), norm),
+        "mod_norm": (lambda: G.norm_modulate(*norm.values(), order="mod_then_norm", out_dtype=F32), norm),
+        "linear": (lambda: G.linear(*linear.values()), linear),
+        "gelu": (lambda: G.linear(*linear.values(), act="gelu", out_dtype=F32), linear),
+        "mlp": (lambda: G.feed_forward(*mlp.values()), mlp),
+    }
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["norm", "mod_norm", "linear", "gelu", "mlp"])
+def test_a_penalty_on_a_gradient_is_refused_beside_other_terms(pkg, cuda, name):
+    """A loss of the result and of a gradient: what the gradient's term adds cannot be left out without a word, whichever inputs are asked for."""
+    call, inputs = operators(pkg, cuda)[name]
+    once = {n: torch.autograd.grad(call().float().sum(), t)[0] for n, t in inputs.items()}
+    for n, t in inputs.items():
+        y = call()
+        g, = torch.autograd.grad(y.float().sum(), t, create_graph=True)
+        assert g.requires_grad and torch.equal(g.detach(), once[n])
+        loss = y.float().square().sum() + g.float().square().sum()
+        for other in inputs.values():
+            with pytest.raises(RuntimeError, match="differentiable once"):
+                torch.autograd.grad(loss, other, retain_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            loss.backward()
+    # through the result's gradient alone
+    y = call()
+    dy = torch.ones_like(y).requires_grad_()
+    for g in torch.autograd.grad(y, list(inputs.values()), dy, create_graph=True):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(g.float().square().sum() + dy.float().sum(), dy, retain_graph=True)
+    for t in inputs.values():
+        t.grad = None
+    call().float().sum().backward(create_graph=True)
+    assert all(torch.equal(t.grad.detach(), once[n]) for n, t in inputs.items())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,y_dtype", [(BF16, BF16), (F32, F32), (BF16, F32), (F32, BF16)])
+def test_a_residual_is_differentiable_more_than_once(pkg, cuda, dtype, y_dtype):
+    """Its gradient is the result's, in its type: torch's own operations, whose derivative is 1."""
+    g = torch.Generator().manual_seed(1)
+    a, w = normal(g, 70, 64, dtype=BF16).to(cuda), normal(g, 32, 64, dtype=BF16).to(cuda)
+    for shape in ((70, 32), (7, 10, 32)):
+        res = normal(g, *shape, dtype=dtype).to(cuda).requires_grad_()
+        dy = normal(g, 70, 32, dtype=y_dtype).to(cuda).requires_grad_()
+        got, = torch.autograd.grad(pkg.grad.linear(a, w, residual=res, out_dtype=y_dtype), res, dy, create_graph=True)
+        assert got.shape == shape and torch.equal(got.detach().view(70, 32), dy.detach().to(dtype))
+        again, = torch.autograd.grad(got.sum(), dy)
+        assert (again == 1).all()
