@@ -286,7 +286,13 @@ struct Linear : torch::autograd::Function<Linear> {
       const Tensor ws = scratch(need, a);
       check(aeris_linear_bwd(&c, ptr(ws), need, stream()));
     }
-    if (need_res) dres = (round_res ? dz : dy.to(res_dtype)).view(ctx->saved_data["residual_shape"].toIntVector());
+    if (need_res) {
+      // dy itself where it has the residual's type and shape, as torch's own addition returns it; otherwise memory of its own.  Never a view of dy: the
+      // accumulation takes a tensor that nobody else holds for its own and adds the next pass's gradient into it
+      const auto shape = ctx->saved_data["residual_shape"].toIntVector();
+      dres = round_res ? dz : dy.to(res_dtype);
+      if (dres.sizes() != at::IntArrayRef(shape)) dres = (dres.is_same(dy) ? dres.clone() : dres).view(shape);
+    }
     variable_list grads = outgoing({da, dw, dbias}, given[0]);
     grads.insert(grads.end(), {dres, Tensor(), Tensor(), Tensor()});
     return grads;

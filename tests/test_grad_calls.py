@@ -1,4 +1,4 @@
-"""Calls of ``grad`` beyond a single pass: gradients of gradients."""
+"""Calls of ``grad`` beyond a single pass: gradients of gradients, gradients that accumulate."""
 import pytest
 import torch
 
@@ -69,3 +69,27 @@ def test_a_residual_is_differentiable_more_than_once(pkg, cuda, dtype, y_dtype):
         assert got.shape == shape and torch.equal(got.detach().view(70, 32), dy.detach().to(dtype))
         again, = torch.autograd.grad(got.sum(), dy)
         assert (again == 1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", [None, "gelu"])
+@pytest.mark.parametrize("dtype,y_dtype", [(BF16, BF16), (F32, F32), (BF16, F32), (F32, BF16)])
+@pytest.mark.parametrize("shape", [(2, 30, 16), (60, 16)])
+def test_residual_gradients_that_accumulate(pkg, cuda, shape, dtype, y_dtype, act):
+    """Several passes into ``.grad`` with one gradient of the result (whole numbers, whose sums are exact in bf16): three times that gradient, which
+    itself stays what it was; so does the gradient of what else the result is added to."""
+    g = torch.Generator().manual_seed(2)
+    a, w = normal(g, 2, 30, 64, dtype=BF16).to(cuda), normal(g, 16, 64, dtype=BF16).to(cuda).requires_grad_()
+    dy = torch.randint(-8, 9, (2, 30, 16), generator=g).to(y_dtype).to(cuda)
+    kept = dy.clone()
+    res = torch.zeros(shape, dtype=dtype, device=cuda, requires_grad=True)
+    for n in range(1, 4):
+        pkg.grad.linear(a, w, act=act, residual=res, out_dtype=y_dtype).backward(dy)
+        assert torch.equal(dy, kept) and torch.equal(res.grad, (n * kept).to(dtype).view(shape)), n
+    # two leaves whose gradients are the same numbers, and whose gradients arrive from a graph that nobody holds
+    res = torch.zeros(shape, dtype=dtype, device=cuda, requires_grad=True)
+    other = torch.zeros(2, 30, 16, dtype=y_dtype, device=cuda, requires_grad=True)
+    for n in range(1, 4):
+        y = pkg.grad.linear(a, w, act=act, residual=res, out_dtype=y_dtype) + other
+        (y * kept).sum().backward()
+        assert torch.equal(res.grad, (n * kept).to(dtype).view(shape)) and torch.equal(other.grad, n * kept), n
