@@ -47,9 +47,10 @@ bool capturing() {
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   return hipStreamIsCapturing(c10::hip::getCurrentHIPStream().stream(), &status) == hipSuccess && status != hipStreamCaptureStatusNone;
 }
+constexpr const char* REVERSE_ONLY = "these operators are differentiable in reverse mode only";
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
 bool wants_grad(std::initializer_list<const Tensor*> inputs) {
-  for (const Tensor* t : inputs)
-    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), "these operators are differentiable in reverse mode only");
+  for (const Tensor* t : inputs) TORCH_CHECK(!has_tangent(*t), REVERSE_ONLY);
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : inputs)
     if (t->defined() && t->requires_grad()) return true;
@@ -81,8 +82,9 @@ void refuse_other_streams(std::initializer_list<const Tensor*> inputs) {
   }
 }
 
-// a result's gradient as the kernels read it: contiguous, its address a multiple of 16
+// a result's gradient as the kernels read it: contiguous, its address a multiple of 16, without a tangent, which they would drop
 Tensor incoming(const Tensor& dy) {
+  TORCH_CHECK(!has_tangent(dy), REVERSE_ONLY);
   Tensor g = dy.contiguous();
   return reinterpret_cast<uintptr_t>(g.data_ptr()) & 15 ? g.clone() : g;
 }
@@ -253,21 +255,21 @@ struct Linear : torch::autograd::Function<Linear> {
   static variable_list backward(AutogradContext* ctx, variable_list given) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &a = saved[0], &w = saved[1], &z = saved[2];
-    const Tensor dy = incoming(given[0]);
     const int64_t act = ctx->saved_data["act"].toInt(), N = w.size(0), K = w.size(1), M = a.numel() / K;
     const bool has_bias = ctx->saved_data["bias"].toBool(), has_res = ctx->saved_data.count("residual_f32") != 0;  // (only inputs that are there have an edge)
     const bool need_a = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_bias = has_bias && ctx->needs_input_grad(2),
                need_res = has_res && ctx->needs_input_grad(has_bias ? 3 : 2);
+    const Tensor dy = need_a || need_w || need_bias ? incoming(given[0]) : given[0].contiguous();
     const auto res_dtype = need_res && ctx->saved_data["residual_f32"].toBool() ? F32 : BF16;
     // dy rounded to bf16 is what the products read of an f32 dy, and what a bf16 residual gets
-    // (not where a graph of the backward pass is asked for: torch's own cast has one)
-    const bool round_res = need_res && res_dtype == BF16 && dy.scalar_type() == F32 && act == AERIS_ACT_NONE && M && !at::GradMode::is_enabled();
+    // (made beside the products; alone, or where a graph of the backward pass is asked for, by torch's own cast, which is differentiable)
+    const bool round_res = need_res && res_dtype == BF16 && dy.scalar_type() == F32 && act == AERIS_ACT_NONE && M && (need_a || need_w || need_bias) && !at::GradMode::is_enabled();
     Tensor da, dw, dbias, dz, dres;
     if (need_a) da = at::empty_like(a, at::MemoryFormat::Contiguous);
     if (need_w) dw = M ? at::empty_like(w) : at::zeros_like(w);
     if (need_bias) dbias = M ? at::empty({N}, w.options()) : at::zeros({N}, w.options());
     if (round_res) dz = at::empty_like(dy, dy.options().dtype(BF16));
-    if (M && (need_a || need_w || need_bias || round_res)) {
+    if (M && (need_a || need_w || need_bias)) {
       aeris_linear_grad c;
       c.dy = dy.data_ptr();
       c.x = a.data_ptr();

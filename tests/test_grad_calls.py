@@ -93,3 +93,39 @@ def test_residual_gradients_that_accumulate(pkg, cuda, shape, dtype, y_dtype, ac
         y = pkg.grad.linear(a, w, act=act, residual=res, out_dtype=y_dtype) + other
         (y * kept).sum().backward()
         assert torch.equal(res.grad, (n * kept).to(dtype).view(shape)) and torch.equal(other.grad, n * kept), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["norm", "mod_norm", "linear", "gelu", "mlp"])
+def test_a_tangent_of_the_result_s_gradient_is_refused(pkg, cuda, name):
+    """Forward mode over reverse mode: nothing of the call's inputs has a tangent, but what its result is multiplied with has."""
+    from torch.autograd import forward_ad
+    call, inputs = operators(pkg, cuda)[name]
+    with forward_ad.dual_level():
+        y = call()
+        factor = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
+        for t in inputs.values():
+            with pytest.raises(RuntimeError, match="reverse mode"):
+                torch.autograd.grad((y * factor).sum(), t, retain_graph=True)
+        assert all(torch.isfinite(t).all() for t in torch.autograd.grad(y.sum(), list(inputs.values())))
+
+
+@pytest.mark.gpu
+def test_a_tangent_of_the_result_s_gradient_reaches_the_residual_s(pkg, cuda):
+    from torch.autograd import forward_ad
+    a, w, res = torch.zeros(70, 64, dtype=BF16, device=cuda), torch.zeros(32, 64, dtype=BF16, device=cuda), torch.zeros(70, 32, device=cuda, requires_grad=True)
+    with forward_ad.dual_level():
+        y = pkg.grad.linear(a, w, residual=res, out_dtype=F32)
+        g, = torch.autograd.grad((y * forward_ad.make_dual(torch.ones_like(y), torch.full_like(y, 3.0))).sum(), res)
+        primal, tangent = forward_ad.unpack_dual(g)
+        assert (primal == 1).all() and (tangent == 3).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["norm", "mod_norm", "linear", "gelu", "mlp"])
+def test_batches_of_gradients_are_refused(pkg, cuda, name):
+    """Vectorised Jacobians (vmap over the backward pass)."""
+    call, inputs = operators(pkg, cuda)[name]
+    y = call()
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, list(inputs.values()), torch.ones_like(y).expand(3, *y.shape), is_grads_batched=True)
