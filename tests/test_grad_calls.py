@@ -1,4 +1,6 @@
-"""Calls of ``grad`` beyond a single pass: gradients of gradients, gradients that accumulate."""
+"""Calls of ``grad`` beyond a single pass: gradients of gradients, gradients that accumulate, operands that hold infinities."""
+import math
+
 import pytest
 import torch
 
@@ -129,3 +131,72 @@ def test_batches_of_gradients_are_refused(pkg, cuda, name):
     y = call()
     with pytest.raises(RuntimeError):
         torch.autograd.grad(y, list(inputs.values()), torch.ones_like(y).expand(3, *y.shape), is_grads_batched=True)
+
+
+def same_kind(got, want):
+    """Infinities where the formula has them, with their signs, NaN where it has NaN; -> where the formula is finite."""
+    got, want = got.detach().double().cpu(), want.double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    far = torch.isinf(want)
+    assert torch.equal(torch.isinf(got), far) and torch.equal(got[far], want[far])
+    return torch.isfinite(want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 9, 64, 65, 300])
+@pytest.mark.parametrize("act", [None, "gelu"])
+def test_infinite_operands_of_a_projection_s_gradients(pkg, cuda, M, act):
+    """An infinity in w or a makes infinities of the sign of the numbers that it is multiplied with, in its column of the gradient alone."""
+    g = torch.Generator().manual_seed(M)
+    N, K = 136, 192
+    dy, a, w = normal(g, M, N), normal(g, M, K, dtype=BF16), normal(g, N, K, dtype=BF16, std=K ** -0.5)
+    _, z = pkg.ops.linear_train(a.to(cuda), w.to(cuda), act=act)
+
+    def grads(a, w):
+        return pkg.ops.linear_backward(dy.to(cuda), a.to(cuda), w.to(cuda), z, act=act, wanted=(True, True, False, True))[:4]
+    clean_a, clean_w, _, dz = grads(a, w)
+    w_far, a_far = w.clone(), a.clone()
+    w_far[3, 5], w_far[100, 7], a_far[M // 2, 11], a_far[0, 150] = math.inf, -math.inf, -math.inf, math.inf
+    da, dw = grads(a_far, w_far)[:2]
+    dz = dz.double().cpu()
+    finite = same_kind(da, dz @ w_far.double())
+    assert torch.equal(da.cpu()[finite], clean_a.cpu()[finite]) and not finite[:, [5, 7]].any() and finite.sum() == M * (K - 2)
+    finite = same_kind(dw, dz.T @ a_far.double())
+    assert torch.equal(dw.cpu()[finite], clean_w.cpu()[finite]) and finite.sum() == N * (K - 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 9, 64, 65, 300])
+def test_infinite_operands_of_the_gated_mlp(pkg, cuda, M):
+    """In w2 for the result, in the result's gradient for that of w2, in w1 and x for those of x and w1 (whose gates are kept finite here)."""
+    g = torch.Generator().manual_seed(M)
+    ops, d, H = pkg.ops, 64, 136
+    x, dy = normal(g, M, d, dtype=BF16), normal(g, M, d, dtype=BF16)
+    w1, w2 = normal(g, 2 * H, d, dtype=BF16, std=d ** -0.5), normal(g, d, H, dtype=BF16, std=H ** -0.5)
+    on = [t.to(cuda) for t in (x, w1, w2)]
+    clean_y, gate_up, h = ops.feed_forward_train(*on)
+    clean = ops.feed_forward_backward(dy.to(cuda), *on, gate_up, h)
+    gate, up = (x.double() @ w1.double().T).chunk(2, dim=-1)
+    s = torch.sigmoid(gate)
+    h64, dh = gate * s * up, dy.double() @ w2.double()
+    both = torch.cat([dh * up * s * (1 + gate * (1 - s)), dh * gate * s], 1)
+
+    far = w2.clone()
+    far[3, 5], far[40, 100] = math.inf, -math.inf
+    y = ops.feed_forward_train(on[0], on[1], far.to(cuda))[0]
+    finite = same_kind(y, h64 @ far.double().T)
+    assert torch.equal(y.cpu()[finite], clean_y.cpu()[finite]) and finite.sum() == M * (d - 2)
+
+    far = dy.clone()
+    far[M // 2, 9], far[0, 50] = math.inf, -math.inf
+    dw2 = ops.feed_forward_backward(far.to(cuda), *on, gate_up, h, wanted=(False, False, True))[2]
+    finite = same_kind(dw2, far.double().T @ h64)
+    assert torch.equal(dw2.cpu()[finite], clean[2].cpu()[finite]) and finite.sum() == (d - 2) * H
+
+    far_w1, far_x = w1.clone(), x.clone()
+    far_w1[3, 5], far_w1[2 * H - 1, 60], far_x[M // 2, 1], far_x[0, 33] = math.inf, -math.inf, math.inf, -math.inf
+    dx, dw1, _ = ops.feed_forward_backward(dy.to(cuda), far_x.to(cuda), far_w1.to(cuda), on[2], gate_up, h, wanted=(True, True, False))
+    finite = same_kind(dx, both @ far_w1.double())
+    assert torch.equal(dx.cpu()[finite], clean[0].cpu()[finite]) and finite.sum() == M * (d - 2)
+    finite = same_kind(dw1, both.T @ far_x.double())
+    assert torch.equal(dw1.cpu()[finite], clean[1].cpu()[finite]) and finite.sum() == 2 * H * (d - 2)
