@@ -37,6 +37,17 @@ def _hipcc():
     raise RuntimeError("hipcc not found")
 
 
+def grad_marker():
+    """What aeris_grad.so carries of the torch that it was built against: it uses torch's C++ classes, which another build of torch may lay out otherwise."""
+    import torch
+    return f"aeris_grad for torch {torch.__version__} {torch.version.git_version}"
+
+
+def grad_built_for_this_torch(path=GRAD_LIB):
+    with open(path, "rb") as f:
+        return grad_marker().encode() + b"\0" in f.read()
+
+
 def _grad_command():
     """g++ of the autograd extension: host code alone, linked to torch and to the library beside it."""
     import sysconfig
@@ -46,6 +57,7 @@ def _grad_command():
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
     includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), os.path.join(rocm, "include"), sysconfig.get_paths()["include"]]
     return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            f'-DAERIS_GRAD_MARKER="{grad_marker()}"',
             *[a for i in includes for a in ("-isystem", i)], GRAD_SOURCE, "-o", GRAD_LIB, "-L" + os.path.join(root, "lib"), "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",
             "-ltorch_python", "-L" + CSRC, "-l:libaeris_hip.so", "-Wl,-rpath,$ORIGIN"]
 
@@ -113,7 +125,7 @@ def build(force: bool = False, verbose: bool = True) -> str:
         list(ex.map(compile_one, jobs))
     if force or jobs or _stale(LIB, objs):
         run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs])
-    if force or _stale(GRAD_LIB, [GRAD_SOURCE, hdrs[-1]]):
+    if force or _stale(GRAD_LIB, [GRAD_SOURCE, hdrs[-1]]) or not grad_built_for_this_torch():
         run(_grad_command())
     return LIB
 

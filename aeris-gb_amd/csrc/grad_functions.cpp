@@ -401,6 +401,7 @@ Tensor feed_forward(const Tensor& x, const Tensor& w1, const Tensor& w2) {
 
 PYBIND11_MODULE(aeris_grad, m) {
   const auto free = pybind11::call_guard<pybind11::gil_scoped_release>();
+  m.attr("marker") = AERIS_GRAD_MARKER;  // the torch that this was built against, which build.py and grad.py look for in the file
   m.def("norm_modulate", &norm_modulate, free);
   m.def("linear", &linear, free);
   m.def("feed_forward", &feed_forward, free);

@@ -23,7 +23,7 @@ from typing import Optional
 import torch
 
 from . import _lib as L
-from . import ops
+from . import build, ops
 
 __all__ = ["feed_forward", "linear", "norm_modulate"]
 
@@ -39,6 +39,8 @@ def _functions():
     if _loaded is None:
         if not os.path.exists(EXTENSION_PATH):
             raise RuntimeError(f"{EXTENSION_PATH} is missing: build it with `python aeris-gb_amd/build.py` (there is no fallback path)")
+        if not build.grad_built_for_this_torch(EXTENSION_PATH):
+            raise RuntimeError(f"{EXTENSION_PATH} was built against another torch than {torch.__version__}: build it again with `python aeris-gb_amd/build.py`")
         L.lib()
         loader = importlib.machinery.ExtensionFileLoader("aeris_grad", EXTENSION_PATH)
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("aeris_grad", loader))

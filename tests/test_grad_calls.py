@@ -200,3 +200,26 @@ def test_infinite_operands_of_the_gated_mlp(pkg, cuda, M):
     assert torch.equal(dx.cpu()[finite], clean[0].cpu()[finite]) and finite.sum() == M * (d - 2)
     finite = same_kind(dw1, both.T @ far_x.double())
     assert torch.equal(dw1.cpu()[finite], clean[1].cpu()[finite]) and finite.sum() == 2 * H * (d - 2)
+
+
+def test_an_extension_built_against_another_torch_is_an_error(pkg, monkeypatch, tmp_path):
+    """It is neither loaded nor taken for up to date by the build."""
+    build = pkg.grad.build
+    assert build.grad_built_for_this_torch() and pkg.grad._functions().marker == build.grad_marker()
+    other = tmp_path / "aeris_grad.so"
+    with open(build.GRAD_LIB, "rb") as f:
+        other.write_bytes(f.read().replace(build.grad_marker().encode(), build.grad_marker().encode()[::-1]))
+    assert not build.grad_built_for_this_torch(str(other))
+    monkeypatch.setattr(pkg.grad, "_loaded", None)
+    monkeypatch.setattr(pkg.grad, "EXTENSION_PATH", str(other))
+    with pytest.raises(RuntimeError, match="another torch"):
+        pkg.grad.feed_forward(*[torch.zeros(8, 8, dtype=BF16)] * 3)
+    # a build with everything else up to date compiles the extension, and nothing else, again
+    monkeypatch.setattr(build, "_stale", lambda target, deps: False)
+    made = []
+    monkeypatch.setattr(build.subprocess, "run", lambda cmd, **kw: made.append(cmd) or build.subprocess.CompletedProcess(cmd, 0, "", ""))
+    build.build(verbose=False)
+    assert not made
+    monkeypatch.setattr(build, "grad_marker", lambda: "aeris_grad for torch 0.0")
+    build.build(verbose=False)
+    assert len(made) == 1 and made[0][0] == "g++" and build.GRAD_SOURCE in made[0]
