@@ -406,10 +406,19 @@ bool train_sizes_ok(int64_t M, int64_t N, int64_t K) {
   return M > 0 && M < (int64_t(1) << 31) && N > 0 && K > 0 && N % 8 == 0 && K % 8 == 0 && N <= 1 << 20 && K <= 1 << 20 && N * K < 1 << 30 &&
          ((M + 63) / 64) * ((N + 31) / 32) < 1 << 24 && ((M + 63) / 64) * ((K + 63) / 64) < 1 << 24;
 }
+constexpr const char* TRAIN_LIMITS =
+    "widths: multiples of 8, at most 2^20, their product below 2^30; rows: fewer than 2^31, and fewer than 2^24 tiles of 64 x 32 of the result and of 64 x 64 of what is projected";
 int train_sizes(const char* who, int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0) return fail(AERIS_EINVAL, "%s: sizes must be positive", who);
-  if (!train_sizes_ok(M, N, K))
-    return fail(AERIS_EUNSUPPORTED, "%s: %lld rows of %lld -> %lld (widths must be multiples of 8, their product below 2^30)", who, (long long)M, (long long)K, (long long)N);
+  if (!train_sizes_ok(M, N, K)) return fail(AERIS_EUNSUPPORTED, "%s: %lld rows of %lld -> %lld (%s)", who, (long long)M, (long long)K, (long long)N, TRAIN_LIMITS);
+  return AERIS_OK;
+}
+// the gated MLP: its first projection has 2 H columns
+bool mlp_sizes_ok(int64_t M, int64_t d, int64_t H) { return H > 0 && H <= 1 << 19 && H % 8 == 0 && train_sizes_ok(M, 2 * H, d); }
+int mlp_sizes(const char* who, int64_t M, int64_t d, int64_t H) {
+  if (M <= 0 || d <= 0 || H <= 0) return fail(AERIS_EINVAL, "%s: sizes must be positive", who);
+  if (!mlp_sizes_ok(M, d, H))
+    return fail(AERIS_EUNSUPPORTED, "%s: %lld rows of d=%lld, H=%lld (H a multiple of 8, and as a projection d -> 2 H, %s)", who, (long long)M, (long long)d, (long long)H, TRAIN_LIMITS);
   return AERIS_OK;
 }
 int train_aligned(const char* who, std::initializer_list<const void*> all) {
@@ -457,15 +466,14 @@ int aeris_linear_bwd(const aeris_linear_grad* a, void* workspace, int64_t worksp
 }
 
 int64_t aeris_feed_forward_workspace_bytes(const aeris_feed_forward* a) {
-  return a && a->H > 0 && a->H <= 1 << 19 && a->H % 8 == 0 && train_sizes_ok(a->M, 2 * a->H, a->d) ? aeris::feed_forward_train_workspace_bytes(*a) : 0;
+  return a && mlp_sizes_ok(a->M, a->d, a->H) ? aeris::feed_forward_train_workspace_bytes(*a) : 0;
 }
 
 int aeris_feed_forward_train_fwd(const aeris_feed_forward* a, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* who = "aeris_feed_forward_train_fwd";
   if (!a || !a->x || !a->w1 || !a->w2 || !a->h || !a->y) return fail(AERIS_EINVAL, "%s: a tensor is NULL", who);
-  if (int rc = train_sizes(who, a->M, a->H > 0 && a->H <= 1 << 19 ? 2 * a->H : a->H > 0 ? 1 << 30 : 0, a->d)) return rc;
+  if (int rc = mlp_sizes(who, a->M, a->d, a->H)) return rc;
   if (int rc = train_aligned(who, {a->x, a->w1, a->w2, a->gate_up, a->h, a->y})) return rc;
-  if (a->H % 8) return fail(AERIS_EUNSUPPORTED, "%s: H=%lld must be a multiple of 8", who, (long long)a->H);
   if (int rc = train_workspace(who, workspace, workspace_bytes, aeris::feed_forward_train_workspace_bytes(*a))) return rc;
   if (int rc = ensure_init(stream, true)) return rc;
   hipError_t e = aeris::feed_forward_train_launch(*a, workspace, reinterpret_cast<hipStream_t>(stream));
@@ -473,15 +481,14 @@ int aeris_feed_forward_train_fwd(const aeris_feed_forward* a, void* workspace, i
 }
 
 int64_t aeris_feed_forward_grad_workspace_bytes(const aeris_feed_forward_grad* a) {
-  return a && a->H > 0 && a->H <= 1 << 19 && a->H % 8 == 0 && train_sizes_ok(a->M, 2 * a->H, a->d) ? aeris::feed_forward_grad_workspace_bytes(*a) : 0;
+  return a && mlp_sizes_ok(a->M, a->d, a->H) ? aeris::feed_forward_grad_workspace_bytes(*a) : 0;
 }
 
 int aeris_feed_forward_bwd(const aeris_feed_forward_grad* a, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* who = "aeris_feed_forward_bwd";
   if (!a || !a->dy || !a->gate_up || !a->w2 || (a->dx && !a->w1) || (a->dw1 && !a->x) || (a->dw2 && !a->h))
     return fail(AERIS_EINVAL, "%s: a tensor is NULL", who);
-  if (int rc = train_sizes(who, a->M, a->H > 0 && a->H <= 1 << 19 ? 2 * a->H : a->H > 0 ? 1 << 30 : 0, a->d)) return rc;
-  if (a->H % 8) return fail(AERIS_EUNSUPPORTED, "%s: H=%lld must be a multiple of 8", who, (long long)a->H);
+  if (int rc = mlp_sizes(who, a->M, a->d, a->H)) return rc;
   if (int rc = train_aligned(who, {a->dy, a->x, a->w1, a->w2, a->gate_up, a->h, a->dx, a->dw1, a->dw2})) return rc;
   if (int rc = train_workspace(who, workspace, workspace_bytes, aeris::feed_forward_grad_workspace_bytes(*a))) return rc;
   if (int rc = ensure_init(stream, true)) return rc;

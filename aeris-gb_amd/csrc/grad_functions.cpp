@@ -207,7 +207,7 @@ struct Sizes { int64_t M, N, K; };
 void check_gradients_sizes(const Sizes& s) {
   constexpr int64_t WIDE = 1 << 20, PRODUCT = 1 << 30, TILES = 1 << 24;
   TORCH_CHECK(s.M < int64_t(1) << 31 && s.N <= WIDE && s.K <= WIDE && s.N * s.K < PRODUCT && (s.M + 63) / 64 * ((s.N + 31) / 32) < TILES && (s.M + 63) / 64 * ((s.K + 63) / 64) < TILES,
-              "no gradients of ", s.M, " rows of ", s.K, " -> ", s.N, " (widths up to 2^20, their product below 2^30, fewer than 2^24 tiles of 64 x 32)");
+              "no gradients of ", s.M, " rows of ", s.K, " -> ", s.N, " (widths up to 2^20, their product below 2^30, fewer than 2^31 rows, and fewer than 2^24 tiles of 64 x 32 of the result and of 64 x 64 of what is projected)");
 }
 
 Tensor linear_forward(const Tensor& a, const Tensor& w, const Tensor& bias, const Tensor& residual, int64_t act, at::ScalarType out, const Sizes& s, Tensor* z) {

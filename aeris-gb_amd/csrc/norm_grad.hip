@@ -334,7 +334,7 @@ struct NormGradSums {
   float* dshift;
   float* dscale;
   int64_t mod_stride;
-  int segments, blocks, d, param_f32, pre;
+  int segments, blocks, d, param_f32;
 };
 
 __device__ __forceinline__ void store_param_grads(const NormGradSums& p, int col, float dgamma, float dbeta) {
@@ -528,7 +528,6 @@ hipError_t norm_grad_launch(const aeris_norm_modulate_grad& a, void* workspace, 
   s.blocks = p.blocks_per_segment;
   s.d = p.d;
   s.param_f32 = p.param_f32;
-  s.pre = pre;
   s.members = members_apart(a) ? p.partial + blocks * (pre ? 4 : 2) * p.d : nullptr;
   const dim3 grid((unsigned)(p.d / 8), s.members ? (unsigned)segments : 1u);
   if (pre) hipLaunchKernelGGL(norm_grad_sums_kernel<true>, grid, dim3(1024), 0, stream, s);

@@ -210,7 +210,8 @@ int aeris_gemm_fwd(const void* A, const void* W, void* C, const void* bias, cons
  *   f32 dy: dy rounded, what a bf16 residual gets); w may be NULL without dx, x without dw, z with AERIS_ACT_NONE
  * Up to AERIS_FEW_TOKENS tokens the products take dz as two bf16 a value.
  * Sums in fp32, added in an order that depends on the sizes alone.  Outputs share no memory with inputs.  Every tensor contiguous and 16-byte aligned.
- * Supported: N % 8 == 0, K % 8 == 0, N, K <= 2^20, N * K < 2^30.  workspace: aeris_linear_grad_workspace_bytes(a) bytes (addresses do not count but for being
+ * Supported: N % 8 == 0, K % 8 == 0, N, K <= 2^20, N * K < 2^30; M < 2^31, ceil(M / 64) * ceil(N / 32) < 2^24 and ceil(M / 64) * ceil(K / 64) < 2^24 (4.1 million
+ * tokens for N = 8192).  workspace: aeris_linear_grad_workspace_bytes(a) bytes (addresses do not count but for being
  * NULL), 16-byte aligned, borrowed for the call. */
 #define AERIS_FEW_TOKENS 64
 typedef struct aeris_linear_train {
@@ -234,7 +235,8 @@ int aeris_linear_bwd(const aeris_linear_grad* a, void* workspace, int64_t worksp
  * Gradients, from dy bf16 [M, d], each unless NULL:  dh = dy w2 (fp32, never in memory), dgate = dh up silu'(gate), dup = dh silu(gate) (bf16, of few tokens two a
  * value);
  *   dx bf16 [M, d] = [dgate | dup] w1;  dw1 bf16 [2H, d] = [dgate | dup]^T x;  dw2 bf16 [d, H] = dy^T h
- * Otherwise as above.  Supported: d % 8 == 0, H % 8 == 0, d, H <= 2^19, d * H < 2^29. */
+ * Otherwise as above.  Supported: d % 8 == 0, H % 8 == 0, and what a projection d -> 2 H is: d <= 2^20, H <= 2^19, d * H < 2^29; M < 2^31, ceil(M / 64) * ceil(H / 16) < 2^24
+ * and ceil(M / 64) * ceil(d / 64) < 2^24. */
 typedef struct aeris_feed_forward {
   const void *x, *w1, *w2;
   void *gate_up, *h, *y;

@@ -223,3 +223,24 @@ def test_an_extension_built_against_another_torch_is_an_error(pkg, monkeypatch, 
     monkeypatch.setattr(build, "grad_marker", lambda: "aeris_grad for torch 0.0")
     build.build(verbose=False)
     assert len(made) == 1 and made[0][0] == "g++" and build.GRAD_SOURCE in made[0]
+
+
+def test_refusals_of_sizes_name_the_limit(pkg):
+    """As many tokens as the documented limit of tiles allows are taken (up to the workspace, which is missing here), one tile more is refused with
+    a message that speaks of rows; the gated MLP's names H as it was given."""
+    L, ops = pkg._lib, pkg.ops
+    lib, p = L.lib(), 0x1000
+    most = ((1 << 24) - 1) // 256 * 64  # rows of a projection to 8192 columns
+
+    def linear(M, N=8192, K=64):
+        return lib.aeris_linear_bwd(ops.LINEAR_GRAD.pack(p, p, p, 0, p, p, p, 0, M, N, K, 0, L.F32), None, 0, None)
+    assert linear(most) == L.EINVAL and "workspace" in L.last_error()
+    assert linear(most + 1) == L.EUNSUPPORTED and "rows: fewer than 2^31" in L.last_error() and "2^24 tiles" in L.last_error()
+
+    def mlp(M, d=64, H=4096):
+        return lib.aeris_feed_forward_bwd(ops.FEED_FORWARD_GRAD.pack(p, p, p, p, p, p, p, p, p, M, d, H), None, 0, None)
+    assert mlp(most) == L.EINVAL and "workspace" in L.last_error()
+    assert mlp(most + 1) == L.EUNSUPPORTED and "H=4096" in L.last_error() and "2^24 tiles" in L.last_error()
+    assert mlp(1, H=1 << 20) == L.EUNSUPPORTED and f"H={1 << 20} " in L.last_error()
+    assert mlp(1, H=12) == L.EUNSUPPORTED and "H=12 (H a multiple of 8" in L.last_error()
+    assert mlp(1, d=0) == L.EINVAL and mlp(0) == L.EINVAL and mlp(1, H=-8) == L.EINVAL
