@@ -2,9 +2,11 @@
 ``ops.gemm`` and the gated MLP.  (The reference trains these modules by autograd over ATen operations, model.py:121-159,311-325,395-403.)
 
 ``norm_modulate``, ``linear`` and ``feed_forward`` return tensors that autograd differentiates once, in reverse mode, with the gradients of
-``ops.norm_modulate_backward``, ``ops.linear_backward`` and ``ops.feed_forward_backward``; their results are those of the calls without
-gradients, and gradients have their tensors' types.  Only the gradients that are asked for are computed, and nothing is kept where
-none is.  The nodes of the autograd graph are C++ (csrc/grad_functions.cpp, built to csrc/aeris_grad.so): a small block's pass is bound by the host.
+``ops.norm_modulate_backward``, ``ops.linear_backward`` and ``ops.feed_forward_backward``, in their tensors' types.  A result has the same bits
+whether or not it is to be differentiated; those of ``ops.norm_modulate`` and of ``ops.gemm`` without activation are the same too, ``ops.gemm`` with
+GELU or SiLU and the module ``FeedForward`` differ in the last roundings (up to 64 tokens ``feed_forward`` keeps h in two bf16).  Only the gradients
+that are asked for are computed, and nothing is kept where none is; how their products are cut and in what order their sums are added depends on
+the sizes, the types and which of them are asked for.  The nodes of the autograd graph are C++ (csrc/grad_functions.cpp, built to csrc/aeris_grad.so): a small block's pass is bound by the host.
 
 Streams and graphs: calls follow the current stream and hold no scratch memory beyond it, and a forward pass with its backward pass may
 be captured into a HIP graph.  torch's own rule for that holds here too: what the captured graph differentiates must have no autograd nodes of

@@ -137,7 +137,7 @@ int aeris_norm_modulate_fwd(const void* x, int x_dtype, void* y, int y_dtype, co
  * dy [B*rows_per_batch, d] (dy_dtype bf16|f32).  Written, each unless NULL:
  *   dx [B*rows_per_batch, d] (x_dtype); dgamma, dbeta [d] (param_dtype; dbeta needs beta); dshift, dscale f32 [B_mod, d], contiguous
  *   (they need shift / scale; B_mod = B where mod_batch_stride is not 0, otherwise 1: the sum over the batch)
- * Statistics and sums in fp32, added in an order that depends on the sizes alone.  dx may be dy or x where their types agree, and may
+ * Statistics and sums in fp32, added in an order that depends on the sizes, types and kinds alone.  dx may be dy or x where their types agree, and may
  * otherwise not overlap them.  x, dy, dx, gamma, beta, shift, scale 16-byte aligned.  Supported: d % 8 == 0, d <= 6144.
  * workspace: device memory of aeris_norm_modulate_grad_workspace_bytes(a) bytes (0 if only dx is asked for; a's addresses do not count but
  * for being NULL), 16-byte aligned, borrowed for the call.  The reference trains this Norm and modulation by autograd (model.py:121-125,
@@ -209,7 +209,7 @@ int aeris_gemm_fwd(const void* A, const void* W, void* C, const void* bias, cons
  *   dx bf16 [M, K] = dz w;  dw bf16 [N, K] = dz^T x;  dbias bf16 [N] = the sums of the unrounded dz;  dz bf16 [M, N] itself (act AERIS_ACT_NONE and an
  *   f32 dy: dy rounded, what a bf16 residual gets); w may be NULL without dx, x without dw, z with AERIS_ACT_NONE
  * Up to AERIS_FEW_TOKENS tokens the products take dz as two bf16 a value.
- * Sums in fp32, added in an order that depends on the sizes alone.  Outputs share no memory with inputs.  Every tensor contiguous and 16-byte aligned.
+ * Sums in fp32, added in an order that depends on the sizes and types, and on which of the gradients are asked for.  Outputs share no memory with inputs.  Every tensor contiguous and 16-byte aligned.
  * Supported: N % 8 == 0, K % 8 == 0, N, K <= 2^20, N * K < 2^30; M < 2^31, ceil(M / 64) * ceil(N / 32) < 2^24 and ceil(M / 64) * ceil(K / 64) < 2^24 (4.1 million
  * tokens for N = 8192).  workspace: aeris_linear_grad_workspace_bytes(a) bytes (addresses do not count but for being
  * NULL), 16-byte aligned, borrowed for the call. */

@@ -244,3 +244,19 @@ def test_refusals_of_sizes_name_the_limit(pkg):
     assert mlp(1, H=1 << 20) == L.EUNSUPPORTED and f"H={1 << 20} " in L.last_error()
     assert mlp(1, H=12) == L.EUNSUPPORTED and "H=12 (H a multiple of 8" in L.last_error()
     assert mlp(1, d=0) == L.EINVAL and mlp(0) == L.EINVAL and mlp(1, H=-8) == L.EINVAL
+
+
+@pytest.mark.gpu
+def test_infinite_operands_of_a_wide_projection_s_gradients(pkg, cuda):
+    """64 tokens, dw in tiles of 128, da cut along k: an infinity in one part, in two of the same sign, and in two of different signs."""
+    g = torch.Generator().manual_seed(64)
+    M, N, K = 64, 6144, 4096
+    dy, a, w = normal(g, M, N).to(cuda), normal(g, M, K, dtype=BF16).to(cuda), normal(g, N, K, dtype=BF16, std=K ** -0.5).to(cuda)
+    clean_a, clean_w, _, dz = pkg.ops.linear_backward(dy, a, w)
+    a[40, 4000], w[5, 7], w[6000, 7], w[3, 9], w[4, 2048] = math.inf, math.inf, math.inf, -math.inf, math.inf
+    da, dw = pkg.ops.linear_backward(dy, a, w, wanted=(True, True, False, False))[:2]
+    dz = dz.double()
+    finite = same_kind(da, (dz @ w.double()).cpu())
+    assert torch.equal(da.cpu()[finite], clean_a.cpu()[finite]) and finite.sum() == M * (K - 3)
+    finite = same_kind(dw, (dz.T @ a.double()).cpu())
+    assert torch.equal(dw.cpu()[finite], clean_w.cpu()[finite]) and finite.sum() == N * (K - 1)
