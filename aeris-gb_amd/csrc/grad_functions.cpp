@@ -88,6 +88,20 @@ Tensor incoming(const Tensor& dy) {
   Tensor g = dy.contiguous();
   return reinterpret_cast<uintptr_t>(g.data_ptr()) & 15 ? g.clone() : g;
 }
+std::vector<int64_t> rows_of(const Tensor& t, int64_t columns) {
+  std::vector<int64_t> shape = t.sizes().vec();
+  shape.back() = columns;
+  return shape;
+}
+
+// What is kept for the backward pass may come back from hooks of the caller's (torch.autograd.graph.saved_tensors_hooks).  The kernels read it by its
+// address and by sizes that follow from those of dy, so it is held to them.
+void check_kept(const Tensor& t, const Tensor& dy, at::IntArrayRef sizes, bool right_type) {
+  TORCH_CHECK(right_type && t.device() == dy.device() && t.sizes() == sizes && t.is_contiguous(), "a tensor kept for the backward pass came back as ", t.scalar_type(), " ", t.sizes(),
+              " with strides ", t.strides(), " on ", t.device(), ", not as contiguous ", sizes, " on ", dy.device(), " in the type that it was kept in");
+}
+void check_kept(const Tensor& t, const Tensor& dy, at::IntArrayRef sizes, at::ScalarType type = BF16) { check_kept(t, dy, sizes, t.scalar_type() == type); }
+
 // Gradients that themselves have none: where a graph of the backward pass is asked for, they refuse to be differentiated.  Behind the node that
 // refuses lie the operator's inputs and the result's gradient dy: autograd, asked for the gradients of a few tensors, runs only what leads to
 // those, and would leave the term out without a word.
@@ -101,11 +115,6 @@ variable_list outgoing(variable_list grads, const Tensor& dy) {
   return grads;
 }
 Tensor scratch(int64_t bytes, const Tensor& like) { return bytes ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor(); }
-std::vector<int64_t> rows_of(const Tensor& t, int64_t columns) {
-  std::vector<int64_t> shape = t.sizes().vec();
-  shape.back() = columns;
-  return shape;
-}
 
 // ---- norm and modulation
 
@@ -138,19 +147,33 @@ struct NormModulate : torch::autograd::Function<NormModulate> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &gamma = saved[1];
     const Tensor dy = incoming(given[0]);
+    const int64_t d = dy.size(2);
+    check_kept(x, dy, dy.sizes(), known(x));
+    check_kept(gamma, dy, {d}, known(gamma));
+    if (saved[2].defined()) check_kept(saved[2], dy, {d}, gamma.scalar_type());
+    // (modulation rows are columns of one matrix, unless a hook gave them memory of their own)
+    Tensor shift = saved[3], scale = saved[4];
+    for (Tensor* t : {&shift, &scale})
+      if (t->defined()) {
+        const bool member_rows = t->dim() == 2 && t->size(0) > 1, both = shift.defined() && scale.defined();
+        if (member_rows && (t->stride(1) != 1 || t->stride(0) < d || (both && shift.strides() != scale.strides()))) *t = t->contiguous();
+        TORCH_CHECK(t->device() == dy.device() && t->scalar_type() == F32 && t->dim() == 2 && t->size(1) == d && (d == 1 || t->stride(1) == 1) &&
+                        (t->size(0) == 1 || t->size(0) == dy.size(0)) && (!both || shift.size(0) == scale.size(0)),
+                    "modulation rows kept for the backward pass came back as ", t->scalar_type(), " ", t->sizes(), " with strides ", t->strides(), " on ", t->device());
+      }
     Tensor grads[5];
     for (size_t i = 0, edge = 0; i < 5; ++i)  // (only inputs that are there have an edge)
       if (saved[i].defined() && ctx->needs_input_grad(edge++))
         grads[i] = x.numel() ? at::empty_like(saved[i], at::MemoryFormat::Contiguous) : at::zeros_like(saved[i], at::MemoryFormat::Contiguous);
     if (x.numel()) {
-      const Tensor& mod = saved[3].defined() ? saved[3] : saved[4];
+      const Tensor& mod = shift.defined() ? shift : scale;
       aeris_norm_modulate_grad a;
       a.x = x.data_ptr();
       a.dy = dy.data_ptr();
       a.gamma = gamma.data_ptr();
       a.beta = ptr(saved[2]);
-      a.shift = static_cast<const float*>(ptr(saved[3]));
-      a.scale = static_cast<const float*>(ptr(saved[4]));
+      a.shift = static_cast<const float*>(ptr(shift));
+      a.scale = static_cast<const float*>(ptr(scale));
       a.dx = ptr(grads[0]);
       a.dgamma = ptr(grads[1]);
       a.dbeta = ptr(grads[2]);
@@ -255,11 +278,14 @@ struct Linear : torch::autograd::Function<Linear> {
   static variable_list backward(AutogradContext* ctx, variable_list given) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &a = saved[0], &w = saved[1], &z = saved[2];
-    const int64_t act = ctx->saved_data["act"].toInt(), N = w.size(0), K = w.size(1), M = a.numel() / K;
+    const int64_t act = ctx->saved_data["act"].toInt(), N = given[0].size(-1), K = w.size(-1), M = given[0].numel() / N;
     const bool has_bias = ctx->saved_data["bias"].toBool(), has_res = ctx->saved_data.count("residual_f32") != 0;  // (only inputs that are there have an edge)
     const bool need_a = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_bias = has_bias && ctx->needs_input_grad(2),
                need_res = has_res && ctx->needs_input_grad(has_bias ? 3 : 2);
     const Tensor dy = need_a || need_w || need_bias ? incoming(given[0]) : given[0].contiguous();
+    check_kept(w, dy, {N, K});
+    check_kept(a, dy, rows_of(dy, K));
+    if (z.defined()) check_kept(z, dy, {3 * M * N}, at::kByte);
     const auto res_dtype = need_res && ctx->saved_data["residual_f32"].toBool() ? F32 : BF16;
     // dy rounded to bf16 is what the products read of an f32 dy, and what a bf16 residual gets
     // (made beside the products; alone, or where a graph of the backward pass is asked for, by torch's own cast, which is differentiable)
@@ -355,7 +381,12 @@ struct FeedForward : torch::autograd::Function<FeedForward> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w2 = saved[2];
     const Tensor dy = incoming(given[0]);
-    const int64_t d = w2.size(0), H = w2.size(1), M = x.numel() / d;
+    const int64_t d = dy.size(-1), H = w2.size(-1), M = dy.numel() / d;
+    check_kept(x, dy, dy.sizes());
+    check_kept(saved[1], dy, {2 * H, d});
+    check_kept(w2, dy, {d, H});
+    check_kept(saved[3], dy, {6 * M * H}, at::kByte);
+    check_kept(saved[4], dy, {(M > AERIS_FEW_TOKENS ? 1 : 2) * M * H});
     Tensor grads[3];
     for (int i = 0; i < 3; ++i)
       if (ctx->needs_input_grad(i)) grads[i] = M ? at::empty_like(saved[i], at::MemoryFormat::Contiguous) : at::zeros_like(saved[i], at::MemoryFormat::Contiguous);

@@ -260,3 +260,74 @@ def test_infinite_operands_of_a_wide_projection_s_gradients(pkg, cuda):
     assert torch.equal(da.cpu()[finite], clean_a.cpu()[finite]) and finite.sum() == M * (K - 3)
     finite = same_kind(dw, (dz.T @ a.double()).cpu())
     assert torch.equal(dw.cpu()[finite], clean_w.cpu()[finite]) and finite.sum() == N * (K - 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["norm", "mod_norm", "linear", "gelu", "mlp"])
+def test_what_is_kept_may_pass_through_hooks(pkg, cuda, name):
+    """Kept on the host, or made again by a checkpoint, as torch's own operations allow it."""
+    call, inputs = operators(pkg, cuda)[name]
+    y = call()
+    dy = torch.randn(y.shape, generator=torch.Generator().manual_seed(3)).to(y.dtype).to(cuda)
+    want = (y, *torch.autograd.grad(y, list(inputs.values()), dy))
+    with torch.autograd.graph.save_on_cpu():
+        y = call()
+    got = (y, *torch.autograd.grad(y, list(inputs.values()), dy))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    y = torch.utils.checkpoint.checkpoint(lambda *_: call(), *inputs.values(), use_reentrant=False)
+    got = (y, *torch.autograd.grad(y, list(inputs.values()), dy))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["norm", "mod_norm"])
+@pytest.mark.parametrize("which", [0, 1])
+def test_modulation_rows_of_which_a_hook_moves_one(pkg, cuda, name, which):
+    """Two columns' views of one matrix when they went in, rows of two strides when they come back."""
+    call, inputs = operators(pkg, cuda)[name]
+    g = torch.Generator().manual_seed(4)
+    mod = normal(g, 2, 128, std=0.3).to(cuda).requires_grad_()
+    x, gamma, beta, *_ = inputs.values()
+    order = "mod_then_norm" if name == "mod_norm" else "norm_then_mod"
+
+    def once(pack):
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+            y = pkg.grad.norm_modulate(x, gamma, beta, mod[:, :64], mod[:, 64:], order=order)
+        return torch.autograd.grad(y.float().square().sum(), [x, gamma, beta, mod])
+    rows = []
+
+    def move_one(t):
+        if t.shape == (2, 64):
+            rows.append(t)
+            return t.clone() if len(rows) == which + 1 else t
+        return t
+    want = once(lambda t: t)
+    got = once(move_one)
+    assert len(rows) == 2 and rows[0].stride(0) == 128
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["norm", "mod_norm", "linear", "gelu", "mlp"])
+@pytest.mark.parametrize("change", ["host", "half", "strides", "fewer", "flat"])
+def test_what_hooks_bring_back_changed_is_refused(pkg, cuda, name, change):
+    """A tensor that is not what was kept, one after the other: each is an error, none is read."""
+    how = {"host": lambda t: t.cpu(), "half": lambda t: t.to(torch.float64), "strides": lambda t: t.as_strided(t.shape, [0] * t.dim()),
+           "fewer": lambda t: t[:-1] if t.dim() == 1 else t[..., :-8].contiguous(), "flat": lambda t: t.reshape(1, -1) if t.dim() == 1 else t.flatten()}[change]
+    call, inputs = operators(pkg, cuda)[name]
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+        call()
+    assert kept
+    for i in range(len(kept)):
+        if change == "strides" and kept[i].shape == (2, 64):
+            continue  # (rows of modulation may have any distance)
+        n = []
+
+        def unpack(t):
+            n.append(t)
+            return how(t) if len(n) == i + 1 else t
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            y = call()
+        with pytest.raises(RuntimeError, match="came back as"):
+            torch.autograd.grad(y.float().sum(), list(inputs.values()))
