@@ -322,6 +322,8 @@ def norm_modulate_backward(dy: torch.Tensor, x: torch.Tensor, gamma: torch.Tenso
                            order: str = "norm_then_mod", eps: float = 1e-5, wanted=(True, True, True, True, True)):
     """Gradients of ``norm_modulate`` from that of its result, dy [B, S, d] (bf16 | f32) -> (dx, dgamma, dbeta, dshift, dscale), each in its
     tensor's shape and type; None where ``wanted`` says so or the tensor is absent.  Statistics and sums in fp32, in a fixed order."""
+    if kind not in _KIND or order not in _ORDER:
+        raise RuntimeError(f"kind must be one of {sorted(_KIND)} and order one of {sorted(_ORDER)}, got {kind!r} and {order!r}")
     _on_current_device(x.device, dict(x=x, dy=dy, gamma=gamma, beta=beta, shift=shift, scale=scale))
     _dev(x, "x")
     _dev(dy, "dy")

@@ -331,3 +331,12 @@ def test_what_hooks_bring_back_changed_is_refused(pkg, cuda, name, change):
             y = call()
         with pytest.raises(RuntimeError, match="came back as"):
             torch.autograd.grad(y.float().sum(), list(inputs.values()))
+
+
+def test_an_unknown_norm_is_the_operators_own_error(pkg):
+    x = torch.zeros(1, 4, 64)
+    for kw in (dict(kind="batchnorm"), dict(order="both"), dict(kind=None)):
+        with pytest.raises(RuntimeError, match="kind must be one of"):
+            pkg.ops.norm_modulate_backward(x, x, x[0, 0], **kw)
+    with pytest.raises(RuntimeError, match="GPU"):
+        pkg.ops.norm_modulate_backward(x, x, x[0, 0])
