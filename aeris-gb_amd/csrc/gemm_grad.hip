@@ -467,7 +467,7 @@ __device__ __forceinline__ bf16x8 all_ones() {
 
 // ---- tiles of T x T (128 or 64), four waves two by two.  Two stages, and two to five workgroups a CU that fill each other's waits; tiles of 64
 // whose workgroups are few have four stages instead, or each k-tile would take the time of a load (300 tokens, 4096 -> 1024 with GELU 35 -> 25 us; the
-// gated MLP of 9 tokens, 1536 -> 6144 and back: 33 -> 27 us).
+// gated MLP's forward pass of 9 tokens, 1536 -> 6144: 33 -> 27 us, now 24).
 template <int T, int STAGES>
 constexpr int tile_lds() { return STAGES * 2 * T * BK * 2; }
 
@@ -874,7 +874,8 @@ __global__ void __launch_bounds__(256) grad_finish_kernel(GradGemm p, GradGemm q
 // ---- dz = dy act'(z) (ACT_NONE: dy) rounded to bf16, and the sums of the unrounded dz over the tokens.  Bound by HBM: a wave takes 512 columns of
 // one row at a time (two without activation, which it asks for before it uses the first), workgroups in turns, three a CU.  More of either in flight
 // is slower: f32 dy [1036800, 1024] without activation 1145 us, 5.6 TB/s (four rows, five workgroups 1253; a cast to bf16 alone 1086), bf16 [8192, 6144]
-// with GELU 65, 5.4 TB/s (76), [100000, 2048] with SiLU 260 (297).
+// with GELU 65, 5.4 TB/s (76), [100000, 2048] with SiLU 260 (297).  That is for widths near a multiple of 512: narrower rows, and the last columns of others,
+// leave lanes without work and a wave with few loads in flight (300000 rows with GELU: 512 columns 195 us, 5.5 TB/s, 520 271, 4.0, 136 125, 2.3, 64 128, 1.1).
 struct ActGrad {
   const void* dy;
   const uint16_t* z;
@@ -1208,8 +1209,8 @@ int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 int64_t more(int64_t a, int64_t b) { return a > b ? a : b; }
 
 // Few tokens: what one product rounds for the next (h; dgate and dup; dz) is kept as two bf16 a value, and the products behind it go over k
-// twice.  Their errors do not average out over many tokens, and the products are bound by the weights' way through memory (9 tokens, 1536 ->
-// 6144: forward 27 us either way, backward 43 -> 55).
+// twice.  Their errors do not average out over many tokens, and the products are bound by the weights' way through memory more than by the second sweep
+// (9 tokens, 1536 -> 6144: forward 20 us with one bf16 a value, 24 with two, backward 40 and 51; 33 tokens, 384 -> 1088: 10 and 13, 13 and 16).
 bool few(int64_t M) { return M <= AERIS_FEW_TOKENS; }
 
 bool needs_dz(const aeris_linear_grad& a) { return (a.dy_dtype == AERIS_F32 || a.act != AERIS_ACT_NONE) && (a.dx || a.dw || a.dz); }

@@ -11,7 +11,10 @@
 // sums; the sums over the tokens stay in registers while a workgroup walks down its share of a member's rows.  At the end of it the
 // workgroup writes one partial sum per column, and a second kernel adds those up in a fixed order: equal calls have equal results.
 // All sums are fp32: within a lane over some hundred rows, then over lanes, waves and workgroups.
-// f32 x [1036800, 1024], bf16 dy: 2155 us, 4.9 TB/s; an element-wise sum of the same streams takes 2035 us here.
+// f32 x [1036800, 1024], bf16 dy: 2155 us, 4.9 TB/s; an element-wise sum of the same streams takes 2035 us here.  Rows beyond 2048: f32 x [30000, 4096]
+// 268 us, 4.6 TB/s, [30000, 6144] 377, 4.9, with the modulation ahead of the norm 265 and 497.  bf16 x with the modulation ahead of the norm is bound by
+// vector arithmetic (four sums a column; u and dn are formed in each of three passes over the row): [259200, 1536] 625 us, 3.8 TB/s, VALU busy 95 % of the cycles,
+// against 435 us, 71 %, with the modulation behind the norm.
 #include "common.h"
 #include "kernels.h"
 
@@ -435,8 +438,8 @@ int64_t segments_of(const aeris_norm_modulate_grad& a) { return (a.shift || a.sc
 
 // How a call is run: column groups of a lane, rows at a time, whether a row belongs to several waves.  One wave to a row of up to 2048
 // elements is the faster way (f32 x [259200, 1536] 803 against 834 us, [1036800, 1024] 2155 against 2216), but for many rows of bf16 x whose
-// modulation lies ahead of the norm: four sums a column leave one wave a SIMD, which then waits for its own arithmetic (bf16 [259200, 1536]
-// 830 -> 624 us with four waves to a row, [1036800, 1024] 1381 -> 1330 with two, [20000, 2048] 100 -> 92; [8192, 1536] 44 -> 54).
+// modulation lies ahead of the norm: four sums a column leave one wave a SIMD, whose arithmetic and memory nothing overlaps (bf16 [259200, 1536]
+// 830 -> 624 us with four waves to a row, of 3.2 waves a SIMD, [1036800, 1024] 1381 -> 1330 with two, [20000, 2048] 100 -> 92; [8192, 1536] 44 -> 54).
 struct Shape { int nv, slots, waves; };
 Shape shape_of(const aeris_norm_modulate_grad& a) {
   if (a.d <= 512) return {1, a.d <= 128 ? 16 : a.d <= 256 ? 8 : 4, 1};
