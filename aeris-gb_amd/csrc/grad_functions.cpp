@@ -107,7 +107,8 @@ void check_kept(const Tensor& t, const Tensor& dy, at::IntArrayRef sizes, at::Sc
 // those, and would leave the term out without a word.
 variable_list outgoing(variable_list grads, const Tensor& dy) {
   if (!at::GradMode::is_enabled()) return grads;
-  torch::autograd::edge_list behind = torch::autograd::get_current_node()->next_edges();
+  torch::autograd::edge_list behind;
+  if (const auto node = torch::autograd::get_current_node()) behind = node->next_edges();
   behind.push_back(torch::autograd::impl::gradient_edge(dy));
   const auto refusal = std::make_shared<torch::autograd::Error>("these operators are differentiable once", std::move(behind));
   for (const Tensor& t : grads)

@@ -340,3 +340,64 @@ def test_an_unknown_norm_is_the_operators_own_error(pkg):
             pkg.ops.norm_modulate_backward(x, x, x[0, 0], **kw)
     with pytest.raises(RuntimeError, match="GPU"):
         pkg.ops.norm_modulate_backward(x, x, x[0, 0])
+
+
+@pytest.mark.gpu
+def test_a_single_token_without_a_row(pkg, cuda):
+    """Inputs of one dimension: the bits of a matrix of one row."""
+    g, G = torch.Generator().manual_seed(6), pkg.grad
+    x, res = normal(g, 64, dtype=BF16).to(cuda), normal(g, 72, dtype=BF16).to(cuda)
+    w, w1, w2 = normal(g, 72, 64, dtype=BF16).to(cuda), normal(g, 96, 64, dtype=BF16).to(cuda), normal(g, 64, 48, dtype=BF16).to(cuda)
+    for f, *inputs in ((lambda x, r, w: G.linear(x, w, residual=r), x, res, w), (lambda x, r, w: G.linear(x, w, act="silu", residual=r), x, res, w), (G.feed_forward, x, w1, w2)):
+        flat = [t.clone().requires_grad_() for t in inputs]
+        rows = [(t[None] if t.dim() == 1 else t).clone().requires_grad_() for t in inputs]
+        y, want = f(*flat), f(*rows)
+        assert y.dim() == 1 and torch.equal(y, want[0])
+        dy = normal(g, *y.shape, dtype=BF16).to(cuda)
+        for a, b, t in zip(torch.autograd.grad(y, flat, dy), torch.autograd.grad(want, rows, dy[None]), flat):
+            assert a.shape == t.shape and torch.equal(a, b.view(a.shape))
+
+
+@pytest.mark.gpu
+def test_two_threads_at_once(pkg, cuda):
+    """Each on a stream and on leaves of its own, with the bits of calls alone."""
+    from concurrent.futures import ThreadPoolExecutor
+    both = [operators(pkg, cuda, seed) for seed in (7, 8)]
+    want = [{n: torch.autograd.grad(call().float().sum(), list(t.values())) for n, (call, t) in ops.items()} for ops in both]
+    torch.cuda.synchronize()
+
+    def work(ops):
+        got = []
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got.append({n: torch.autograd.grad(call().float().sum(), list(t.values())) for n, (call, t) in ops.items()})
+            torch.cuda.current_stream().synchronize()
+        return got
+    with ThreadPoolExecutor(2) as pool:
+        runs = list(pool.map(work, both))
+    for got, w in zip(runs, want):
+        for one in got:
+            assert all(torch.equal(a, b) for n in w for a, b in zip(one[n], w[n]))
+
+
+@pytest.mark.gpu
+def test_accumulated_gradients_in_a_captured_step(pkg, cuda):
+    """Forward and backward pass into ``.grad``, captured and replayed several times beside eager work: as many times the gradients of one pass, and
+    the residual's apart from the result's."""
+    g, G = torch.Generator().manual_seed(9), pkg.grad
+    a, w = torch.randint(-3, 4, (40, 64), generator=g).to(BF16).to(cuda), torch.randint(-3, 4, (16, 64), generator=g).to(BF16).to(cuda)
+    dy = torch.randint(-3, 4, (40, 16), generator=g).float().to(cuda)
+    kept = dy.clone()
+    leaf = {"w": w, "res": torch.zeros(40, 16, device=cuda)}
+    for t in leaf.values():
+        t.requires_grad_().grad = torch.zeros_like(t)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        G.linear(a, leaf["w"], residual=leaf["res"], out_dtype=F32).backward(dy)
+    for n in range(1, 4):
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = [t.detach().clone().requires_grad_() for t in leaf.values()]
+        once = torch.autograd.grad(G.linear(a, eager[0], residual=eager[1], out_dtype=F32), eager, dy)
+        assert torch.equal(dy, kept) and torch.equal(leaf["res"].grad, n * kept)
+        assert (leaf["w"].grad.float() - n * once[0].float()).abs().max() <= n * 2 ** -8 * leaf["w"].grad.float().abs().max()  # (a sum of n in bf16: a rounding each)
